@@ -476,6 +476,18 @@ hq_status run_gemm(const void* X, hq_dtype dtype, int64_t ldx, hq_format fmt, co
   return launch_plan(fmt, dtype, d, p, w, fault_ptr(s), s);
 }
 
+}  // namespace
+
+hq_status hq_internal_workspace(hipStream_t stream, size_t need, void** out) {
+  try {
+    return get_internal_ws(stream, need, need, out);
+  } catch (...) {
+    return fail(HQ_ERR_INTERNAL, "out of host memory");
+  }
+}
+
+namespace {
+
 // ---- the no-allocation entry point's scratch ----
 // A file-scope device array is the workspace of hq_gemm_fused_noalloc: each GPU the library
 // runs on holds its own copy, at its own address, until the process ends. Host code never
