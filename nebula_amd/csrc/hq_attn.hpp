@@ -42,7 +42,12 @@ struct AttnArgs {
 
 // How a call is split, from host-side sizes alone (the lengths stay on the device).
 struct AttnPlan {
-  size_t ws = 0;
+  bool tile = false, row = false;  // the kernels that run
+  bool prefix = false;             // the tile kernel over shared prefixes, the row kernel over the rest
+  uint32_t tile_grid = 0, tile_splits = 0, tile_keys = 0;
+  uint32_t row_grid = 0, row_splits = 0, row_keys = 0;
+  uint32_t slots = 0;              // parts of a row in the workspace (0: none, the kernels write O)
+  size_t o_offset = 0, ws = 0;
 };
 AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                    uint32_t dim, uint32_t max_keys, uint32_t max_prefix);
