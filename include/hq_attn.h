@@ -58,7 +58,7 @@ typedef struct hq_kv_cache {
     void* K;
     void* V;
     int64_t layer_stride, page_stride, head_stride, token_stride;
-    uint32_t layers, pages, kv_heads, page_tokens /* a power of two, at most 65536 */, head_dim;
+    uint32_t layers, pages, kv_heads, page_tokens /* a power of two, 16 to 65536 */, head_dim;
     hq_dtype dtype;
     int32_t* table;
     int64_t table_stride;
@@ -91,7 +91,7 @@ hq_status hq_describe_attn(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint
 /* Packed prompts. Sequence b's new tokens are rows [cu_q[b], cu_q[b + 1]) of Q, its keys rows
  * [cu_k[b], cu_k[b + 1]) of K and V (cu_k NULL: cu_q, the whole prompt). cu_*: int32 [seqs + 1],
  * not falling, cu_q[seqs] <= rows, cu_k[seqs] <= total_k (values outside are clamped). K: element (j, head, d)
- * at j * k_row + head * k_head + d, V likewise; strides multiples of 8, 16-byte aligned. max_k: no
+ * at j * k_row + head * k_head + d, V likewise; strides multiples of 8 (k_row, v_row at most 2^23), 16-byte aligned. max_k: no
  * sequence has more keys (0: total_k); it only chooses how the work is split. */
 hq_status hq_attn_prompt(const hq_attn_io* io, const void* K, int64_t k_row, int64_t k_head, const void* V,
                          int64_t v_row, int64_t v_head, uint32_t kv_heads, uint32_t total_k, const int32_t* cu_q,

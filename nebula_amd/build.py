@@ -28,6 +28,11 @@ SOURCES = ["hq_api.cpp", "hq_gguf.cpp", "hq_decode.hip", "hq_decode_ls.hip", "hq
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
+# Per source: the attention kernels' accumulators take part in vector arithmetic, so their MFMAs write
+# vector registers (with more than 256 registers a lane the compiler would move them to and fro: 380
+# moves a tile on heads of 256).
+SOURCE_FLAGS = {"hq_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 COMMON_FLAGS = [
     "-O3",
     "-std=c++17",
@@ -62,7 +67,7 @@ def build_library(verbose: bool = False) -> Path:
     for src in SOURCES:
         obj = BUILD / (src + ".o")
         lang = ["-x", "hip"]
-        cmd = [HIPCC, *lang, *COMMON_FLAGS, "-c", str(CSRC / src), "-o", str(obj)]
+        cmd = [HIPCC, *lang, *COMMON_FLAGS, *SOURCE_FLAGS.get(src, []), "-c", str(CSRC / src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd))
         procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))

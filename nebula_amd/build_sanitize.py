@@ -13,12 +13,12 @@ from __future__ import annotations
 import os
 from pathlib import Path
 
-from .build import ARCH, BUILD, COMMON_FLAGS, CSRC, HIPCC, LIBDIR, ORACLE_DIR, SOURCES, _run
+from .build import ARCH, BUILD, COMMON_FLAGS, CSRC, HIPCC, LIBDIR, ORACLE_DIR, SOURCE_FLAGS, SOURCES, _run
 
 SAN_LIB = LIBDIR / "libnebula_hq_san.so"
 SAN_HOST = ["-fsanitize=address", "-fsanitize=undefined", "-fno-sanitize-recover=undefined",
             "-fno-omit-frame-pointer", "-shared-libsan", "-g"]
-SAN_SOURCES = ["hq_api.cpp", "hq_gguf.cpp"]
+SAN_SOURCES = ["hq_api.cpp", "hq_gguf.cpp", "hq_attn_api.cpp"]
 LLVM = Path(os.environ.get("HQ_LLVM", "/opt/rocm/llvm"))
 
 
@@ -42,7 +42,7 @@ def build_sanitized() -> tuple[Path, Path]:
         else:
             obj = BUILD / (src + ".o")
             if not obj.exists():
-                _run([HIPCC, "-x", "hip", *COMMON_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
+                _run([HIPCC, "-x", "hip", *COMMON_FLAGS, *SOURCE_FLAGS.get(src, []), "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(obj)
     tmp = SAN_LIB.with_suffix(".so.tmp")
     _run([HIPCC, "-shared", "-fPIC", f"--offload-arch={ARCH}", *host, *map(str, objs), "-o", str(tmp)])

@@ -27,13 +27,6 @@
 
 namespace hq {
 
-typedef __attribute__((address_space(1))) const void* global_ptr_t;
-// 16 bytes per lane from any address straight into LDS: lane i writes lds + 16 i (lds wave-uniform). Not
-// inside a template: clang's host pass does not know the builtin.
-__device__ __forceinline__ void global_to_lds16(const void* p, void* lds) {
-  __builtin_amdgcn_global_load_lds((global_ptr_t)p, (lds_ptr_t)lds, 16, 0, 0);
-}
-
 namespace {
 
 typedef float f16x __attribute__((ext_vector_type(16)));
@@ -49,10 +42,47 @@ __device__ __forceinline__ f16x mfma32x32x16(u4 a, u4 b, f16x c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// Four rows of 16 elements, 8 bytes from each lane of 16: lane i gets column i.
-__device__ __forceinline__ u2 lds_read_tr(const unsigned char* p) {
-  typedef __attribute__((address_space(3))) s4* lds_s4;
-  return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)p));
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
+}
+// Transposing reads: four rows of 16 elements, 8 bytes from each lane of 16; lane i gets column i. N
+// fragments of two reads each, from at[i] + OFF and at[i] + OFF + NEXT. In asm, and waited for there,
+// because the compiler holds the builtin back until every copy into LDS under way has landed.
+template <int OFF, int NEXT>
+__device__ __forceinline__ void lds_read_tr(const uint32_t (&at)[2], u4 (&f)[2]) {
+  u2 a, b, c, d;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+      "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+      : "v"(at[0]), "v"(at[1]), "i"(OFF), "i"(OFF + NEXT));
+  f[0] = u4{a[0], a[1], b[0], b[1]};
+  f[1] = u4{c[0], c[1], d[0], d[1]};
+}
+template <int OFF, int NEXT>
+__device__ __forceinline__ void lds_read_tr(const uint32_t (&at)[4], u4 (&f)[4]) {
+  u2 a, b, c, d, e, g, h, i;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d), "=&v"(e), "=&v"(g), "=&v"(h), "=&v"(i)
+      : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "i"(OFF), "i"(OFF + NEXT));
+  f[0] = u4{a[0], a[1], b[0], b[1]};
+  f[1] = u4{c[0], c[1], d[0], d[1]};
+  f[2] = u4{e[0], e[1], g[0], g[1]};
+  f[3] = u4{h[0], h[1], i[0], i[1]};
+}
+template <int I>
+using Int = std::integral_constant<int, I>;
+// f(Int<0>) .. f(Int<N - 1>).
+template <int N, class F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(Int<N - 1>{});
+  }
 }
 
 // Two weights, each rounded to nearest in the activation type (it is the type of V, and the MFMA has
@@ -210,6 +240,48 @@ __device__ __forceinline__ uint32_t page_or_report(const AttnKeys& k, int32_t pa
   return 0;
 }
 
+// Pages of tiles of KEYS keys, held in registers a batch of 64 blocks of 16 keys ahead: lane j of a batch
+// holds block j, that is block j % (KEYS / 16) of the batch's tile j / (KEYS / 16); tile i of the wavefront
+// begins at key first + i * step. Pages hold 16 tokens or more, so a block lies in one.
+template <int KEYS>
+struct Pages {
+  static constexpr uint32_t kSub = KEYS / 16, kBatch = 64 / kSub;
+  const int32_t* table;
+  uint32_t first, step, nk;
+  int32_t now, next;
+
+  __device__ __forceinline__ int32_t load(const AttnKeys& k, uint32_t batch) const {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint64_t key = first + (uint64_t)(batch * kBatch + lane / kSub) * step + lane % kSub * 16;
+    return table[min((uint32_t)min(key >> k.page_shift, (uint64_t)k.max_pages - 1), k.max_pages - 1)];
+  }
+  // Pages of batch `batch` as numbers that can be followed.
+  __device__ __forceinline__ int32_t held(const AttnKeys& k, uint32_t batch, int32_t p) const {
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint64_t key = first + (uint64_t)(batch * kBatch + lane / kSub) * step + lane % kSub * 16;
+    return key < nk ? (int32_t)page_or_report(k, p) : 0;
+  }
+  __device__ __forceinline__ void start(const AttnKeys& k) {
+    now = load(k, 0);
+    next = load(k, 1);
+    now = held(k, 0, now);
+  }
+  // Before tile i's first use of of(): every tile in turn.
+  __device__ __forceinline__ void advance(const AttnKeys& k, uint32_t i) {
+    if (i % kBatch || i == 0) return;
+    now = held(k, i / kBatch, next);
+    next = load(k, i / kBatch + 1);
+  }
+  // Page of block `sub` of tile i.
+  __device__ __forceinline__ uint32_t page(uint32_t i, uint32_t sub) const {
+    return (uint32_t)__builtin_amdgcn_readlane(now, i % kBatch * kSub + sub);
+  }
+};
+
+// 16 keys of one head from `base` on (uniform). Rows are at most 2^24 bytes apart, so a lane's offset is 32-bit;
+// the descriptor is made anew for each block, since a pool or an operand may span more than 4 GiB.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint16_t* base) { return make_rsrc(base, 0x7FFFFFFFu); }
+
 // ---- parts of rows whose keys are split ----
 // Row (token t, head h) has `slots` places: fp32 O [D] (not divided by the sum), the maximum times c and
 // the sum; a place without weight has sum 0 and no O.
@@ -220,9 +292,8 @@ struct Parts {
 };
 
 struct TilePlan {
-  uint32_t splits, split_keys;  // workgroup s of a tile takes keys [s split_keys, (s + 1) split_keys), the last one all the rest
-  uint32_t prefix;              // rows are the sequences of a group, keys its shared prefix
-  uint32_t slot0;
+  uint32_t splits;  // workgroups that share a tile's keys, in equal runs of them
+  uint32_t prefix;  // rows are the sequences of a group, keys its shared prefix
   Parts parts;
 };
 
@@ -302,9 +373,8 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
     const int64_t n = (int64_t)((min(w.r0 + BR, w.R) - 1) / a.G) + nk - w.nq + 1;
     wg_lim = n < 0 ? 0u : (uint32_t)n;
   }
-  const uint32_t kbeg = split * pl.split_keys;
-  const uint32_t kend = split + 1 == pl.splits ? wg_lim : min(wg_lim, kbeg + pl.split_keys);
-  const uint32_t t0 = kbeg / kKeys, t1 = kend > kbeg ? (kend + kKeys - 1) / kKeys : t0;
+  const uint32_t tiles = (wg_lim + kKeys - 1) / kKeys, per = (tiles + pl.splits - 1) / pl.splits;
+  const uint32_t t0 = min(split * per, tiles), t1 = min(t0 + per, tiles);
 
   const uint16_t* const qp = a.Q + (int64_t)(w.q0 + token) * a.q_row + head * a.q_head + 8 * half;
   u4 q[kSteps];
@@ -318,24 +388,26 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   // Copies of tile t into a stage: load i of the wavefront brings rows kRowsPerLoad (i NW + wave) ...; a
   // lane's row and source chunk undo the swizzle. Keys past the last are copies of it (masked below).
   const uint32_t in_row = lane / (D / 8), in_chunk = lane % (D / 8);
-  auto issue = [&](uint32_t t, uint32_t stage) {
+  const uint32_t k_step = (uint32_t)a.k.k_row * 2, v_step = (uint32_t)a.k.v_row * 2, page_mask = (1u << a.k.page_shift) - 1;
+  Pages<kKeys> pages{table, t0 * kKeys, kKeys, nk, 0, 0};
+  auto issue = [&](uint32_t t, uint32_t stage) __attribute__((always_inline)) {
     unsigned char* const base = smem + stage * kStage;
+    const uint32_t left = nk - 1 - t * kKeys;  // last row with a key
+    if constexpr (PAGED) pages.advance(a.k, t - t0);
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; ++i) {
-      const uint32_t row = (i * NW + wave) * kRowsPerLoad + in_row;
-      const uint32_t key = min(t * kKeys + row, nk - 1);
+      const uint32_t row0 = (i * NW + wave) * kRowsPerLoad, row = row0 + in_row;
+      const uint32_t sub = min(row0 / 16, left / 16), in = min(row, left) - 16 * sub;
       int64_t ko, vo;
       if constexpr (PAGED) {
-        const uint32_t page = page_or_report(a.k, table[key >> a.k.page_shift]);
-        const int64_t in = page * a.k.page_stride + (key & ((1u << a.k.page_shift) - 1)) * a.k.k_row;
-        ko = vo = in;
+        ko = vo = pages.page(t - t0, sub) * a.k.page_stride + ((t * kKeys + 16 * sub) & page_mask) * a.k.k_row;
       } else {
-        ko = (w.key0 + key) * a.k.k_row;
-        vo = (w.key0 + key) * a.k.v_row;
+        ko = (w.key0 + t * kKeys + 16 * sub) * a.k.k_row;
+        vo = (w.key0 + t * kKeys + 16 * sub) * a.k.v_row;
       }
       unsigned char* const to = base + (i * NW + wave) * 1024;
-      global_to_lds16(Kh + ko + (in_chunk ^ swz_k<D>(row)) * 8, to);
-      global_to_lds16(Vh + vo + (in_chunk ^ swz_v<D>(row)) * 8, to + kVOff);
+      buffer_to_lds16(block_rsrc(Kh + ko), to, in * k_step + ((in_chunk ^ swz_k<D>(row)) << 4));
+      buffer_to_lds16(block_rsrc(Vh + vo), to + kVOff, in * v_step + ((in_chunk ^ swz_v<D>(row)) << 4));
     }
   };
 
@@ -348,13 +420,13 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   uint32_t v_at[kDims];
 #pragma unroll
   for (int dt = 0; dt < kDims; ++dt)
-    v_at[dt] = kVOff + v_row * kPitch + (((4 * dt + 2 * (l32 >> 4) + ((lane & 3u) >> 1)) ^ swz_v<D>(v_row)) << 4) + 8 * (lane & 1u);
+    v_at[dt] = lds_address(smem) + kVOff + v_row * kPitch + (((4 * dt + 2 * (l32 >> 4) + ((lane & 3u) >> 1)) ^ swz_v<D>(v_row)) << 4) + 8 * (lane & 1u);
 
   f16x o[kDims];
   float m, l;
   // Second pass (careful) only where a first one gave values that are not finite, or no weight at all:
   // values of V at keys a row may not see, times its weight 0, may have made them, or scores past 1e7.
-  auto pass = [&](auto mode) {
+  auto pass = [&](auto mode) __attribute__((always_inline)) {
     constexpr bool careful = decltype(mode)::value;
     m = kNone;
     l = 0.f;
@@ -362,6 +434,8 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
     for (int dt = 0; dt < kDims; ++dt) o[dt] = f16x{};
     uint32_t ts = t0;
     asm volatile("" : "+s"(ts));  // what one pass computes is not held for the other
+    if constexpr (PAGED)
+      if (t1 > ts) pages.start(a.k);
     if (t1 > ts) issue(ts, ts & 1u);
     for (uint32_t t = ts; t < t1; ++t) {
       __builtin_amdgcn_s_waitcnt(0);  // the wavefront's copies of tile t have landed, its reads of t - 1 are done
@@ -425,35 +499,36 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
         }
       l += sum;
 
-      auto v_frag = [&](int dt, int j, uint32_t from = 0) {
-        const u2 lo = lds_read_tr(st + from + v_at[dt] + 16 * j * kPitch), hi = lds_read_tr(st + from + v_at[dt] + (16 * j + 8) * kPitch);
-        return u4{lo[0], lo[1], hi[0], hi[1]};
-      };
-      if (careful && masked) {
-        uint32_t from = 0;
-        asm volatile("" : "+s"(from));  // these reads are not the other branch's: not all taken before it
+      // O^T += V^T P^T: 16 keys a step, fragments of as many groups of 32 dims as registers are taken for.
+      constexpr int kBlock = kDims < 4 ? kDims : 4;
+      const uint32_t stage_at = (t & 1u) * kStage;
+      each<4>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value;
 #pragma unroll
-        for (int dt = 0; dt < kDims; ++dt) {
-          f16x count = f16x{};
+        for (int d0 = 0; d0 < kDims; d0 += kBlock) {
+          uint32_t at[kBlock];
+          u4 f[kBlock];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            __builtin_amdgcn_sched_barrier(0);  // one fragment at a time in registers
+          for (int i = 0; i < kBlock; ++i) at[i] = stage_at + v_at[d0 + i];
+          lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
+          if (careful && masked) {
             const uint32_t key = t * kKeys + 16 * j + 4 * half;
             const u4 sees = {seen2<DT>(key, lim), seen2<DT>(key + 2, lim), seen2<DT>(key + 8, lim), seen2<DT>(key + 10, lim)};
-            u4 finite, code;
-            split_odd<DT>(v_frag(dt, j, from), finite, code);
-            o[dt] = mfma32x32x16<DT>(finite, p[j], o[dt]);
-            count = mfma32x32x16<DT>(code, sees, count);
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) {
+              u4 finite, code;
+              split_odd<DT>(f[i], finite, code);
+              o[d0 + i] = mfma32x32x16<DT>(finite, p[j], o[d0 + i]);
+              const f16x count = mfma32x32x16<DT>(code, sees, f16x{});
+#pragma unroll
+              for (int v = 0; v < 16; ++v) o[d0 + i][v] += odd_value(count[v]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) o[d0 + i] = mfma32x32x16<DT>(f[i], p[j], o[d0 + i]);
           }
-#pragma unroll
-          for (int v = 0; v < 16; ++v) o[dt][v] += odd_value(count[v]);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int dt = 0; dt < kDims; ++dt) o[dt] = mfma32x32x16<DT>(v_frag(dt, j), p[j], o[dt]);
-      }
+      });
     }
     {
       const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -471,7 +546,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   const uint32_t tok = w.q0 + token;
   const float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift;
   if (pl.parts.slots) {
-    const uint64_t at = ((uint64_t)tok * a.H + head) * pl.parts.slots + pl.slot0 + split;
+    const uint64_t at = ((uint64_t)tok * a.H + head) * pl.parts.slots + split;
     if (half == 0) pl.parts.ml[at] = f2{mc, l};
     if (l != 0.f)
 #pragma unroll
@@ -500,12 +575,14 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 constexpr int kRowKeys = 32;  // keys of a wavefront's tile
 
 struct RowPlan {
-  uint32_t splits, split_keys;
-  uint32_t slot0;
-  Parts parts;
+  uint32_t splits;     // workgroups that share the keys of 16 rows
+  uint32_t* cnt;       // arrivals of a tile's workgroups, zero between launches
+  float* o;            // their parts: [tile][kv head][splits][16][D], and the maxima and sums [..][16]
+  f2* ml;
+  Parts prefix;        // parts of the shared prefix, from the tile kernel (slots 0: none)
 };
 
-// As swz_k / swz_v, for this kernel's reads: V 16 rows of 32 bytes.
+// As swz_v, for this kernel's reads: 16 rows of 32 bytes.
 template <int D>
 __device__ __forceinline__ uint32_t swz_rv(uint32_t r) {
   return D == 64 ? ((r >> 1) & 3u) << 1 : (r & 7u) << 1;
@@ -515,15 +592,22 @@ template <int D>
 constexpr uint32_t row_waves() {
   return D == 256 ? 2u : 4u;
 }
+// Two stages of V per wavefront; the join of the wavefronts lies over them.
 template <int D>
 constexpr uint32_t row_lds_bytes() {
-  return row_waves<D>() * 2u * (2u * kRowKeys * D * 2u);
+  const uint32_t stages = row_waves<D>() * 2u * (kRowKeys * D * 2u), join = row_waves<D>() * 16u * ((D + 4u) * 4u + 8u);
+  return (stages > join ? stages : join) + 16u;
 }
+constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on other XCDs
 
+// Tiles of 32 keys go to the splits' wavefronts in turn, (round * splits + split) * NW + wavefront, so that
+// any lengths are shared evenly. A wavefront's K goes straight into the registers of its first product (a
+// lane's 16 bytes of a row are 8 consecutive dims, four lanes take 64 bytes), its V through LDS; both are a
+// tile ahead.
 template <int DT, int D, bool PAGED>
 __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnArgs a, RowPlan pl) {
   constexpr uint32_t NW = row_waves<D>();
-  constexpr uint32_t kPitch = 2 * D, kStage = 2 * kRowKeys * kPitch, kVOff = kStage / 2;
+  constexpr uint32_t kPitch = 2 * D, kStage = kRowKeys * kPitch;
   constexpr int kSteps = D / 32, kDims = D / 16;
   constexpr uint32_t kRowsPerLoad = 1024 / kPitch, kLoads = kRowKeys / kRowsPerLoad;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -549,16 +633,19 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
 
   const uint32_t r_mine = w.r0 + l16;
   const uint32_t r = min(r_mine, w.R - 1), token = r / a.G, head = kvh * a.G + (r - token * a.G);
-  uint32_t lim = nk, wg_lim = nk;
+  uint32_t lim = nk, end = nk, full = nk;  // keys of this lane's row, of any row, of every row
   if (a.causal) {
-    const int64_t n = (int64_t)token + nk - w.nq + 1, last = (int64_t)((min(w.r0 + 16, w.R) - 1) / a.G) + nk - w.nq + 1;
-    lim = n < 0 ? 0u : (uint32_t)n;
-    wg_lim = last < 0 ? 0u : (uint32_t)last;
+    auto limit = [&](uint32_t t) {
+      const int64_t n = (int64_t)t + nk - w.nq + 1;
+      return n < 0 ? 0u : (uint32_t)n;
+    };
+    lim = limit(token);
+    full = limit(w.r0 / a.G);
+    end = limit((min(w.r0 + 16, w.R) - 1) / a.G);
   }
-  const uint32_t kbeg = begin + split * pl.split_keys;
-  const uint32_t kend = split + 1 == pl.splits ? wg_lim : min(wg_lim, kbeg + pl.split_keys);
-  if (kend <= kbeg && split > 0) return;  // the join counts the parts by the lengths
-  const uint32_t tiles = kend > kbeg ? (kend - kbeg + kRowKeys - 1) / kRowKeys : 0u;
+  const uint32_t tiles = end > begin ? (end - begin + kRowKeys - 1) / kRowKeys : 0u;
+  const uint32_t active = max(1u, min(pl.splits, (tiles + NW - 1) / NW));
+  if (split >= active) return;
 
   const uint16_t* const qp = a.Q + (int64_t)(w.q0 + token) * a.q_row + head * a.q_head + 8 * quad;
   u4 q[kSteps];
@@ -570,126 +657,118 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   unsigned char* const mine = smem + wave * 2 * kStage;
 
   const uint32_t in_row = lane / (D / 8), in_chunk = lane % (D / 8);
-  auto page_of = [&](uint32_t t) -> int32_t {  // the page of key lane % 32 of tile t
-    if constexpr (PAGED) return table[min(kbeg + t * kRowKeys + (lane & 31u), nk - 1) >> a.k.page_shift];
-    else return 0;
+  const uint32_t stride = active * NW;
+  Pages<kRowKeys> pages{table, begin + (split * NW + wave) * kRowKeys, stride * kRowKeys, nk, 0, 0};
+  const uint32_t k_step = (uint32_t)a.k.k_row * 2, v_step = (uint32_t)a.k.v_row * 2, page_mask = (1u << a.k.page_shift) - 1;
+  // Elements from the head's first to block `sub` of tile n of this wavefront, which begins at key k0.
+  auto block_at = [&](uint32_t n, uint32_t k0, uint32_t sub, int64_t token_stride) __attribute__((always_inline)) -> int64_t {
+    if constexpr (PAGED) return pages.page(n, sub) * a.k.page_stride + ((k0 + 16 * sub) & page_mask) * token_stride;
+    else return (w.key0 + k0 + 16 * sub) * token_stride;
   };
-  auto issue = [&](uint32_t t, uint32_t stage, int32_t pages) {
-    if constexpr (PAGED) pages = (int32_t)page_or_report(a.k, pages);
+  // Rows past the last key are copies of its (masked below).
+  u4 kf[2][kSteps];
+  auto load_k = [&](uint32_t n, uint32_t k0) __attribute__((always_inline)) {
+    const uint32_t left = nk - 1 - k0;
+#pragma unroll
+    for (uint32_t kt = 0; kt < 2; ++kt) {
+      const uint32_t sub = min(kt, left / 16), at = (min(16 * kt + l16, left) - 16 * sub) * k_step + 16 * quad;
+      const __amdgpu_buffer_rsrc_t kr = block_rsrc(Kh + block_at(n, k0, sub, a.k.k_row));
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) kf[kt][s] = __builtin_amdgcn_raw_buffer_load_b128(kr, at + 64 * s, 0, 0);
+    }
+  };
+  auto copy_v = [&](uint32_t n, uint32_t k0) __attribute__((always_inline)) {
+    const uint32_t left = nk - 1 - k0;
 #pragma unroll
     for (uint32_t i = 0; i < kLoads; ++i) {
-      const uint32_t row = i * kRowsPerLoad + in_row, key = min(kbeg + t * kRowKeys + row, nk - 1);
-      int64_t ko, vo;
-      if constexpr (PAGED) {
-        const uint32_t page = (uint32_t)__shfl(pages, row);
-        ko = vo = page * a.k.page_stride + (key & ((1u << a.k.page_shift) - 1)) * a.k.k_row;
-      } else {
-        ko = (w.key0 + key) * a.k.k_row;
-        vo = (w.key0 + key) * a.k.v_row;
-      }
-      unsigned char* const to = mine + stage * kStage + i * 1024;
-      global_to_lds16(Kh + ko + (in_chunk ^ swz_k<D>(row)) * 8, to);
-      global_to_lds16(Vh + vo + (in_chunk ^ swz_rv<D>(row)) * 8, to + kVOff);
+      const uint32_t row = i * kRowsPerLoad + in_row, sub = min(i * kRowsPerLoad / 16, left / 16);
+      buffer_to_lds16(block_rsrc(Vh + block_at(n, k0, sub, a.k.v_row)), mine + (n & 1u) * kStage + i * 1024,
+                      (min(row, left) - 16 * sub) * v_step + ((in_chunk ^ swz_rv<D>(row)) << 4));
     }
   };
 
-  uint32_t k_at[kSteps], v_at[kDims];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) k_at[s] = l16 * kPitch + (((4 * s + quad) ^ swz_k<D>(l16)) << 4);
+  uint32_t v_at[kDims];
   const uint32_t v_row = 4 * quad + (l16 >> 2);
 #pragma unroll
   for (int dt = 0; dt < kDims; ++dt)
-    v_at[dt] = kVOff + v_row * kPitch + (((2 * dt + ((l16 & 3u) >> 1)) ^ swz_rv<D>(v_row)) << 4) + 8 * (l16 & 1u);
+    v_at[dt] = lds_address(mine) + v_row * kPitch + (((2 * dt + ((l16 & 3u) >> 1)) ^ swz_rv<D>(v_row)) << 4) + 8 * (l16 & 1u);
 
   f4 o[kDims];
   float m, l;
-  // Twice only where the first pass gave values that are not finite, as in the tile kernel.
-  auto pass = [&](auto mode) {
-    constexpr bool careful = decltype(mode)::value;
-#pragma unroll
-    for (int dt = 0; dt < kDims; ++dt) o[dt] = f4{};
-    m = kNone;
-    l = 0.f;
-    int32_t next = 0;
-    if (wave < tiles) {
-      issue(wave, 0, page_of(wave));
-      if (wave + NW < tiles) next = page_of(wave + NW);
+  const uint32_t t_first = split * NW + wave;
+  // Tile n of this wavefront, from key k0; its V and K are under way. kMore: the next tile's are asked for,
+  // V before and K after the first product (which frees the registers), so that every wait but the last
+  // leaves a tile in flight. The counts need paths without branches around the copies.
+  auto tile = [&](uint32_t n, uint32_t k0, auto mode, auto next) __attribute__((always_inline)) {
+    constexpr bool careful = decltype(mode)::value, more = decltype(next)::value;
+    if constexpr (more) {
+      if constexpr (PAGED) pages.advance(a.k, n + 1);
+      copy_v(n + 1, k0 + stride * kRowKeys);
     }
-    uint32_t stage = 0;
-    for (uint32_t t = wave; t < tiles; t += NW, stage ^= 1u) {
-      if (t + NW < tiles) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of the stage that is filled next
-        issue(t + NW, stage ^ 1u, next);
-        if (t + 2 * NW < tiles) {
-          next = page_of(t + 2 * NW);
-          __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads + (PAGED ? 1 : 0)));
-        } else {
-          __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * kLoads));
-        }
-      } else {
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
-      }
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      const unsigned char* const st = mine + stage * kStage;
-      f4 s[2] = {f4{}, f4{}};
+    f4 s[2] = {f4{}, f4{}};
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
+    for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-          s[kt] = mfma16x16x32<DT>(*reinterpret_cast<const u4*>(st + k_at[i] + kt * 16 * kPitch), q[i], s[kt]);
-      const uint32_t k0 = kbeg + t * kRowKeys;
-      const bool masked = k0 + kRowKeys > min(kend, uni(w.nq) == 1 ? kend : k0);
-      const uint32_t stop = min(lim, kend);
-      if (masked) {
+      for (int kt = 0; kt < 2; ++kt) s[kt] = mfma16x16x32<DT>(kf[kt][i], q[i], s[kt]);
+    // V of this tile was asked for before its K; only the next tile's copies may be left.
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(more ? kLoads : 0));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (more) load_k(n + 1, k0 + stride * kRowKeys);
+    const bool masked = k0 + kRowKeys > full;
+    if (masked) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (k0 + 16 * kt + 4 * quad + v >= stop) s[kt][v] = -INFINITY;
-      }
-      float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (__any((top - m) * c > Weights<DT>::kLag)) {
-        const float n = (top - m) * c > Weights<DT>::kLag ? top : m, al = __builtin_amdgcn_exp2f((m - n) * c);
-        m = n;
-        l *= al;
+        for (int v = 0; v < 4; ++v)
+          if (k0 + 16 * kt + 4 * quad + v >= lim) s[kt][v] = -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (__any((top - m) * c > Weights<DT>::kLag)) {
+      const float n = (top - m) * c > Weights<DT>::kLag ? top : m, al = __builtin_amdgcn_exp2f((m - n) * c);
+      m = n;
+      l *= al;
 #pragma unroll
-        for (int dt = 0; dt < kDims; ++dt) o[dt] *= al;
-      }
-      const float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift;
-      float p[8];
+      for (int dt = 0; dt < kDims; ++dt) o[dt] *= al;
+    }
+    const float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift;
+    float p[8];
 #pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        const float x = s[v / 4][v % 4];
-        p[v] = __builtin_amdgcn_exp2f(careful ? fmaf(x - m, c, Weights<DT>::kLift) : fmaf(x, c, -mc));
-        l += p[v];
-      }
-      const u4 pf = {pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
+    for (int v = 0; v < 8; ++v) {
+      const float x = s[v / 4][v % 4];
+      p[v] = __builtin_amdgcn_exp2f(careful ? fmaf(x - m, c, Weights<DT>::kLift) : fmaf(x, c, -mc));
+      l += p[v];
+    }
+    const u4 pf = {pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
+    const uint32_t stage_at = (n & 1u) * kStage;
+#pragma unroll
+    for (int d0 = 0; d0 < kDims; d0 += 4) {
+      uint32_t at[4];
+      u4 f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[i] = stage_at + v_at[d0 + i];
+      lds_read_tr<0, 16 * (int)kPitch>(at, f);
       if (careful && masked) {
-        uint32_t from = 0;
-        asm volatile("" : "+s"(from));
-        const u4 sees = {seen2<DT>(k0 + 4 * quad, stop), seen2<DT>(k0 + 4 * quad + 2, stop), seen2<DT>(k0 + 16 + 4 * quad, stop),
-                         seen2<DT>(k0 + 16 + 4 * quad + 2, stop)};
+        const u4 sees = {seen2<DT>(k0 + 4 * quad, lim), seen2<DT>(k0 + 4 * quad + 2, lim), seen2<DT>(k0 + 16 + 4 * quad, lim),
+                         seen2<DT>(k0 + 16 + 4 * quad + 2, lim)};
 #pragma unroll
-        for (int dt = 0; dt < kDims; ++dt) {
-          const u2 lo = lds_read_tr(st + from + v_at[dt]), hi = lds_read_tr(st + from + v_at[dt] + 16 * kPitch);
+        for (int i = 0; i < 4; ++i) {
           u4 finite, code;
-          split_odd<DT>(u4{lo[0], lo[1], hi[0], hi[1]}, finite, code);
-          o[dt] = mfma16x16x32<DT>(finite, pf, o[dt]);
+          split_odd<DT>(f[i], finite, code);
+          o[d0 + i] = mfma16x16x32<DT>(finite, pf, o[d0 + i]);
           const f4 count = mfma16x16x32<DT>(code, sees, f4{});
 #pragma unroll
-          for (int v = 0; v < 4; ++v) o[dt][v] += odd_value(count[v]);
+          for (int v = 0; v < 4; ++v) o[d0 + i][v] += odd_value(count[v]);
         }
-        continue;
-      }
+      } else {
 #pragma unroll
-      for (int dt = 0; dt < kDims; ++dt) {
-        const u2 lo = lds_read_tr(st + v_at[dt]), hi = lds_read_tr(st + v_at[dt] + 16 * kPitch);
-        o[dt] = mfma16x16x32<DT>(u4{lo[0], lo[1], hi[0], hi[1]}, pf, o[dt]);
+        for (int i = 0; i < 4; ++i) o[d0 + i] = mfma16x16x32<DT>(f[i], pf, o[d0 + i]);
       }
     }
+  };
+  auto finish = [&]() {
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     float bad = 0.f;
@@ -699,12 +778,43 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
       for (int v = 0; v < 4; ++v) bad = fmaf(o[dt][v], 0.f, bad);
     return __any(!(bad == 0.f) || (l == 0.f && m != kNone)) != 0;
   };
-  if (pass(std::false_type{})) pass(std::true_type{});
+  auto start = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int dt = 0; dt < kDims; ++dt) o[dt] = f4{};
+    m = kNone;
+    l = 0.f;
+    if constexpr (PAGED) pages.start(a.k);
+  };
+  if (t_first < tiles) {
+    uint32_t t = t_first, n = 0;
+    start();
+    copy_v(0, begin + t * kRowKeys);
+    load_k(0, begin + t * kRowKeys);
+    for (; t + stride < tiles; t += stride, ++n) tile(n, begin + t * kRowKeys, std::false_type{}, std::true_type{});
+    tile(n, begin + t * kRowKeys, std::false_type{}, std::false_type{});
+    // Again, tile by tile, where values are not finite or a row has no weight, as in the tile kernel.
+    if (finish()) {
+      start();
+      for (t = t_first, n = 0; t < tiles; t += stride, ++n) {
+        if constexpr (PAGED) pages.advance(a.k, n);
+        copy_v(n, begin + t * kRowKeys);
+        load_k(n, begin + t * kRowKeys);
+        tile(n, begin + t * kRowKeys, std::true_type{}, std::false_type{});
+      }
+      finish();
+    }
+  } else {
+#pragma unroll
+    for (int dt = 0; dt < kDims; ++dt) o[dt] = f4{};
+    m = kNone;
+    l = 0.f;
+  }
 
   // Join the wavefronts: each brings its sums to the common maximum, [wavefront][row][dim].
   __syncthreads();
   float* const red = reinterpret_cast<float*>(smem);
   f2* const stat = reinterpret_cast<f2*>(smem + NW * 16 * (D + 4) * 4);
+  uint32_t* const flag = reinterpret_cast<uint32_t*>(smem + row_lds_bytes<D>() - 16);
   if (quad == 0) stat[wave * 16 + l16] = f2{m, l};
   __syncthreads();
   float top = kNone;
@@ -715,100 +825,154 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   for (int dt = 0; dt < kDims; ++dt)
     *reinterpret_cast<f4*>(red + (wave * 16 + l16) * (D + 4) + 16 * dt + 4 * quad) = l == 0.f ? f4{} : o[dt] * al;
   __syncthreads();
-  for (uint32_t u = threadIdx.x; u < 16 * (D / 4); u += NW * 64) {
-    const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
-    const uint32_t rr = w.r0 + row;
-    if (rr >= w.R) continue;
-    const uint32_t tk = w.q0 + rr / a.G, hd = kvh * a.G + rr % a.G;
-    float mx = kNone, sum = 0.f;
+
+  const uint32_t rows = min(16u, w.R - w.r0), units = rows * (D / 4);
+  auto joined = [&](uint32_t row, uint32_t d, f4& v, float& mc, float& sum) {
+    float mx = kNone;
 #pragma unroll
     for (uint32_t i = 0; i < NW; ++i) mx = fmaxf(mx, stat[i * 16 + row][0]);
-    f4 v = f4{};
+    sum = 0.f;
+    v = f4{};
 #pragma unroll
     for (uint32_t i = 0; i < NW; ++i) {
       const f2 e = stat[i * 16 + row];
       if (e[1] != 0.f) sum += e[1] * __builtin_amdgcn_exp2f((e[0] - mx) * c);
       v += *reinterpret_cast<const f4*>(red + (i * 16 + row) * (D + 4) + d);
     }
-    const float mc = fmaxf(mx * c, kNone) - Weights<DT>::kLift;
-    if (pl.parts.slots) {
-      const uint64_t at = ((uint64_t)tk * a.H + hd) * pl.parts.slots + pl.slot0 + split;
-      if (d == 0) pl.parts.ml[at] = f2{mc, sum};
-      if (sum != 0.f) *reinterpret_cast<f4*>(pl.parts.o + at * D + d) = v;
-    } else {
-      const float inv = 1.f / sum;
-      if (sum == 0.f) v = f4{};
-      else v *= inv;
-      *reinterpret_cast<u2*>(a.O + (int64_t)tk * a.o_row + hd * a.o_head + d) = u2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-      if (a.lse && d == 0) a.lse[(uint64_t)tk * a.H + hd] = sum == 0.f ? -INFINITY : (mc + __log2f(sum)) * 0.69314718055994530942f;
+    mc = fmaxf(mx * c, kNone) - Weights<DT>::kLift;
+  };
+  auto store = [&](uint32_t row, uint32_t d, f4 v, float mc, float sum) {
+    const uint32_t rr = w.r0 + row, tk = w.q0 + rr / a.G, hd = kvh * a.G + rr % a.G;
+    if (sum == 0.f) v = f4{};
+    else v *= 1.f / sum;
+    *reinterpret_cast<u2*>(a.O + (int64_t)tk * a.o_row + hd * a.o_head + d) = u2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+    if (a.lse && d == 0) a.lse[(uint64_t)tk * a.H + hd] = sum == 0.f ? -INFINITY : (mc + __log2f(sum)) * 0.69314718055994530942f;
+  };
+  if (active == 1 && pl.prefix.slots == 0) {
+    for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
+      f4 v;
+      float mc, sum;
+      const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
+      joined(row, d, v, mc, sum);
+      store(row, d, v, mc, sum);
     }
+    return;
+  }
+  // Parts: the workgroup that arrives last joins them, in the order of their numbers.
+  const uint64_t first = (uint64_t)(idx * a.Hkv + kvh) * pl.splits;
+  const __amdgpu_buffer_rsrc_t po = make_rsrc(pl.o + first * 16 * D, pl.splits * 16 * D * 4);
+  const __amdgpu_buffer_rsrc_t pm = make_rsrc(pl.ml + first * 16, pl.splits * 16 * 8);
+  for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
+    f4 v;
+    float mc, sum;
+    const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
+    joined(row, d, v, mc, sum);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), po, ((split * 16 + row) * D + d) * 4, 0, kAgent);
+    if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, (f2{mc, sum})), pm, (split * 16 + row) * 8, 0, kAgent);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t* const cnt = pl.cnt + idx * a.Hkv + kvh;
+    const uint32_t last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
+    if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *flag = last;
+  }
+  __syncthreads();
+  if (!*flag) return;
+  for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
+    const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
+    const uint32_t rr = w.r0 + row;
+    const uint64_t pre = ((uint64_t)(w.q0 + rr / a.G) * a.H + kvh * a.G + rr % a.G) * pl.prefix.slots;
+    const uint32_t parts = pl.prefix.slots + active;
+    float mx = kNone, sum = 0.f;
+    f4 v = f4{};
+    constexpr uint32_t kBatch = 8;
+    for (uint32_t p0 = 0; p0 < parts; p0 += kBatch) {
+      f2 e[kBatch];
+      f4 x[kBatch];
+#pragma unroll
+      for (uint32_t i = 0; i < kBatch; ++i) {
+        const uint32_t p = p0 + i, s = p - pl.prefix.slots;
+        e[i] = f2{kNone, 0.f};
+        x[i] = f4{};
+        if (p < pl.prefix.slots) {
+          e[i] = pl.prefix.ml[pre + p];
+          x[i] = *reinterpret_cast<const f4*>(pl.prefix.o + (pre + p) * D + d);
+        } else if (p < parts) {
+          e[i] = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(pm, (s * 16 + row) * 8, 0, kAgent));
+          x[i] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(po, ((s * 16 + row) * D + d) * 4, 0, kAgent));
+        }
+      }
+      float n = mx;
+#pragma unroll
+      for (uint32_t i = 0; i < kBatch; ++i) n = e[i][1] != 0.f ? fmaxf(n, e[i][0]) : n;
+      const float f = __builtin_amdgcn_exp2f(mx - n);
+      mx = n;
+      sum *= f;
+      v *= f;
+#pragma unroll
+      for (uint32_t i = 0; i < kBatch; ++i) {
+        const float g = __builtin_amdgcn_exp2f(e[i][0] - n);
+        if (e[i][1] != 0.f) {  // a part without weight left its O unwritten
+          sum = fmaf(e[i][1], g, sum);
+          v += x[i] * g;
+        }
+      }
+    }
+    store(row, d, v, mx, sum);
   }
 }
 
-// ---- joining parts ----
-struct JoinPlan {
-  Parts parts;
-  uint32_t prefix_slots, prefix_keys;  // of a shared prefix, first
-  uint32_t own_slots, own_keys;        // of the rows' own keys (tile kernel: all written; row kernel: those with keys)
-  uint32_t all;                        // every place was written
-};
-
+// ---- joining the parts of the tile kernel ----
 template <int DT, int D>
-__global__ __launch_bounds__(256) void hq_attn_join_kernel(AttnArgs a, JoinPlan pl) {
+__global__ __launch_bounds__(256) void hq_attn_join_kernel(AttnArgs a, Parts parts) {
   constexpr int E = D / 64;
+  typedef float fe __attribute__((ext_vector_type(E == 1 ? 2 : E)));  // E = 1 uses the first
   const uint32_t lane = threadIdx.x & 63u;
   const uint64_t u = (uint64_t)blockIdx.x * 4 + uni(threadIdx.x >> 6);
   if (u >= (uint64_t)a.T * a.H) return;
   const uint32_t t = (uint32_t)(u / a.H), h = (uint32_t)(u % a.H);
-  uint32_t b = t, nq = 1, q0 = t;
   if (a.cu_q) {
-    uint32_t lo = 0, hi = a.B;
+    uint32_t lo = 0, hi = a.B, q0;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
       if (a.cu_q[mid] <= (int32_t)t) lo = mid;
       else hi = mid;
     }
-    b = lo;
-    nq = span(a.cu_q, b, a.T, q0);
+    const uint32_t nq = span(a.cu_q, lo, a.T, q0);
     if (t < q0 || t >= q0 + nq) return;  // of no sequence
   }
-  uint32_t own = pl.own_slots;
-  if (!pl.all) {
-    uint32_t nk, begin = 0, k0;
-    int32_t row;
-    if (a.k.table) {
-      nk = cached_len(a.k, b, row);
-      if (a.groups) begin = min(nk, shared_tokens(a, group_of(a, b)));
-    } else {
-      nk = span(a.k.cu_k, b, a.k.total_k, k0);
-    }
-    // The rows of a tile share its workgroups: the last row's keys count.
-    uint32_t last = nk;
-    if (a.causal) {
-      const uint32_t r = (t - q0) * a.G + h % a.G, end = min((r / 16 + 1) * 16, nq * a.G) - 1;
-      const int64_t n = (int64_t)(end / a.G) + nk - nq + 1;
-      last = n < 0 ? 0u : (uint32_t)n;
-    }
-    own = last > begin ? min(own, (last - begin + pl.own_keys - 1) / pl.own_keys) : 1u;
-  }
-  const uint64_t at = u * pl.parts.slots;
-  const uint32_t n = pl.prefix_slots + own;
-  float m = kNone;
-  for (uint32_t i = lane; i < n; i += 64) {
-    const f2 e = pl.parts.ml[at + i];
-    if (e[1] != 0.f) m = fmaxf(m, e[0]);
-  }
+  // Lane i weighs part i (at most 64).
+  const uint64_t at = u * parts.slots;
+  f2 e = {kNone, 0.f};
+  if (lane < parts.slots) e = parts.ml[at + lane];
+  float m = e[1] != 0.f ? e[0] : kNone;
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  float l = 0.f, o[E] = {};
-  for (uint32_t i = 0; i < n; ++i) {
-    const f2 e = pl.parts.ml[at + i];
-    if (e[1] == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(e[0] - m);
-    l = fmaf(e[1], f, l);
-    const float* p = pl.parts.o + (at + i) * D + lane * E;
+  const float f = e[1] != 0.f ? __builtin_amdgcn_exp2f(e[0] - m) : 0.f;
+  float l = e[1] * f;
 #pragma unroll
-    for (int k = 0; k < E; ++k) o[k] = fmaf(p[k], f, o[k]);
+  for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+  float o[E] = {};
+  const float* const src = parts.o + at * D + lane * E;
+  constexpr uint32_t kBatch = 8;
+  for (uint32_t p0 = 0; p0 < parts.slots; p0 += kBatch) {
+    fe x[kBatch];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) {
+      const float* const p = src + (uint64_t)min(p0 + i, parts.slots - 1) * D;
+      if constexpr (E == 1) x[i][0] = *p;
+      else x[i] = *reinterpret_cast<const fe*>(p);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) {
+      const bool has = p0 + i < parts.slots && __builtin_amdgcn_readlane(__float_as_int(e[1]), (p0 + i) & 63u) << 1 != 0;
+      const float g = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), (p0 + i) & 63u));
+      if (has)  // a part without weight left its O unwritten
+#pragma unroll
+        for (int k = 0; k < E; ++k) o[k] = fmaf(x[i][k], g, o[k]);
+    }
   }
   uint16_t* const out = a.O + (int64_t)t * a.o_row + h * a.o_head + lane * E;
 #pragma unroll
@@ -818,14 +982,15 @@ __global__ __launch_bounds__(256) void hq_attn_join_kernel(AttnArgs a, JoinPlan 
 
 template <int DT, int D, bool PAGED>
 hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_t s) {
-  Parts parts{};
-  if (p.slots) {
-    parts.slots = p.slots;
-    parts.ml = reinterpret_cast<f2*>(static_cast<unsigned char*>(ws) + kCounterBytes);
-    parts.o = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes + p.o_offset);
+  unsigned char* const w = static_cast<unsigned char*>(ws);
+  Parts parts{};  // of the tile kernel
+  if (p.tile_slots) {
+    parts.slots = p.tile_slots;
+    parts.ml = reinterpret_cast<f2*>(w + p.tile_ml);
+    parts.o = reinterpret_cast<float*>(w + p.tile_o);
   }
   if (p.tile) {
-    TilePlan t{p.tile_splits, p.tile_keys, p.prefix, 0, parts};
+    const TilePlan t{p.tile_splits, p.prefix, parts};
     auto k = hq_attn_tile_kernel<DT, D, 4, PAGED>;
     constexpr uint32_t lds = 2 * tile_stage_bytes<D>();
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -835,23 +1000,21 @@ hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
     if (e != hipSuccess) return e;
   }
   if (p.row) {
-    RowPlan r{p.row_splits, p.row_keys, p.prefix ? p.tile_splits : 0u, parts};
+    RowPlan r{};
+    r.splits = p.row_splits;
+    r.cnt = reinterpret_cast<uint32_t*>(w);
+    r.o = reinterpret_cast<float*>(w + p.row_o);
+    r.ml = reinterpret_cast<f2*>(w + p.row_ml);
+    if (p.prefix) r.prefix = parts;
     auto k = hq_attn_row_kernel<DT, D, PAGED>;
     constexpr uint32_t lds = row_lds_bytes<D>();
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (set != hipSuccess) return set;
     hipLaunchKernelGGL(k, dim3(p.row_grid), dim3(row_waves<D>() * 64), lds, s, a, r);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    return hipGetLastError();
   }
-  if (p.slots) {
-    JoinPlan j{};
-    j.parts = parts;
-    j.prefix_slots = p.prefix ? p.tile_splits : 0u;
-    j.own_slots = p.prefix || p.row ? p.row_splits : p.tile_splits;
-    j.own_keys = p.row_keys;
-    j.all = !p.row;
-    hipLaunchKernelGGL((hq_attn_join_kernel<DT, D>), dim3((uint32_t)(((uint64_t)a.T * a.H + 3) / 4)), dim3(256), 0, s, a, j);
+  if (p.tile_slots) {
+    hipLaunchKernelGGL((hq_attn_join_kernel<DT, D>), dim3((uint32_t)(((uint64_t)a.T * a.H + 3) / 4)), dim3(256), 0, s, a, parts);
     return hipGetLastError();
   }
   return hipSuccess;
@@ -880,37 +1043,47 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   p.row = p.prefix || all_rows <= 32ull * seqs;
   p.tile = p.prefix || !p.row;
   max_keys = std::max(max_keys, 1u);
+  size_t ws = kCounterBytes;
+  auto take = [&](size_t bytes) {
+    const size_t at = ws;
+    ws += (bytes + 255) / 256 * 256;
+    return at;
+  };
   if (p.tile) {
     const uint32_t keys = p.prefix ? std::max(max_prefix, 1u) : max_keys;
     const uint32_t tiles = up(all_rows, 128) + (p.prefix ? groups : seqs);
-    const uint32_t want = up(2 * cus, tiles * kv_heads);  // workgroups for two on each CU
-    p.tile_keys = std::max(256u, up(up(keys, want), kKeys) * kKeys);
-    p.tile_splits = std::max(1u, up(keys, p.tile_keys));
+    // Workgroups for two on each CU, of 256 keys at least.
+    p.tile_splits = std::min({64u, up(2 * cus, tiles * kv_heads), up(keys, 256)});
     p.tile_grid = tiles * kv_heads * p.tile_splits;
+    if (p.prefix || p.tile_splits > 1) {
+      p.tile_slots = p.tile_splits;
+      const size_t places = (size_t)rows * heads * p.tile_slots;
+      p.tile_ml = take(places * sizeof(f2));
+      p.tile_o = take(places * dim * sizeof(float));
+    }
   }
   if (p.row) {
-    const uint32_t waves = dim == 256 ? 2u : 4u, step = waves * kRowKeys;
-    const uint32_t per = up(G, 16), tiles = rows == seqs ? seqs * per : up(all_rows, 16) + seqs;
-    p.row_keys = std::max(step, up(up((uint64_t)tiles * kv_heads * max_keys, 8 * cus), step) * step);
-    p.row_splits = up(max_keys, p.row_keys);
+    const uint32_t step = (dim == 256 ? 2u : 4u) * kRowKeys;
+    const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
+    const uint32_t keys = p.prefix ? std::max(max_keys - std::min(max_prefix, max_keys), 1u) : max_keys;
+    p.row_splits = std::min({64u, up(8 * cus, tiles * kv_heads), up(keys, step)});
+    if ((uint64_t)tiles * kv_heads > kMaxCounters && !p.prefix) p.row_splits = 1;
     p.row_grid = tiles * kv_heads * p.row_splits;
+    if (p.prefix || p.row_splits > 1) {
+      const size_t places = (size_t)tiles * kv_heads * p.row_splits * 16;
+      p.row_ml = take(places * sizeof(f2));
+      p.row_o = take(places * dim * sizeof(float));
+    }
   }
-  if (p.prefix || p.tile_splits > 1 || p.row_splits > 1) {
-    p.slots = p.tile_splits + p.row_splits;
-    const size_t places = (size_t)rows * heads * p.slots;
-    p.o_offset = (places * sizeof(f2) + 255) / 256 * 256;
-    p.ws = kCounterBytes + p.o_offset + places * dim * sizeof(float);
-  }
+  p.ws = ws > kCounterBytes ? ws : 0;
   return p;
 }
 
-void describe_attn(int kind, const AttnPlan& p, char* buf, size_t len) {
+void describe_attn(const AttnPlan& p, char* buf, size_t len) {
   char t[160] = "", r[160] = "";
-  if (p.tile) std::snprintf(t, sizeof t, "hq_attn_tile_kernel%s grid=%u splits=%u of %u keys", p.prefix ? "<prefix>" : "", p.tile_grid,
-                            p.tile_splits, p.tile_keys);
-  if (p.row) std::snprintf(r, sizeof r, "hq_attn_row_kernel grid=%u splits=%u of %u keys", p.row_grid, p.row_splits, p.row_keys);
-  std::snprintf(buf, len, "%s%s%s%s ws=%zu", t, p.tile && p.row ? ", " : "", r, p.slots ? ", hq_attn_join_kernel" : "", p.ws);
-  (void)kind;
+  if (p.tile) std::snprintf(t, sizeof t, "hq_attn_tile_kernel%s grid=%u splits=%u", p.prefix ? "<prefix>" : "", p.tile_grid, p.tile_splits);
+  if (p.row) std::snprintf(r, sizeof r, "hq_attn_row_kernel grid=%u splits=%u", p.row_grid, p.row_splits);
+  std::snprintf(buf, len, "%s%s%s%s ws=%zu", t, p.tile && p.row ? ", " : "", r, p.tile_slots && !p.prefix ? ", hq_attn_join_kernel" : "", p.ws);
 }
 
 hipError_t launch_attn(int dtype, const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_t s) {

@@ -44,14 +44,14 @@ struct AttnArgs {
 struct AttnPlan {
   bool tile = false, row = false;  // the kernels that run
   bool prefix = false;             // the tile kernel over shared prefixes, the row kernel over the rest
-  uint32_t tile_grid = 0, tile_splits = 0, tile_keys = 0;
-  uint32_t row_grid = 0, row_splits = 0, row_keys = 0;
-  uint32_t slots = 0;              // parts of a row in the workspace (0: none, the kernels write O)
-  size_t o_offset = 0, ws = 0;
+  uint32_t tile_grid = 0, tile_splits = 0;
+  uint32_t row_grid = 0, row_splits = 0;
+  uint32_t tile_slots = 0;         // parts of a row that the tile kernel leaves (0: none, it writes O)
+  size_t tile_ml = 0, tile_o = 0, row_ml = 0, row_o = 0, ws = 0;  // workspace offsets, and its size
 };
 AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                    uint32_t dim, uint32_t max_keys, uint32_t max_prefix);
-void describe_attn(int kind, const AttnPlan& p, char* buf, size_t len);
+void describe_attn(const AttnPlan& p, char* buf, size_t len);
 hipError_t launch_attn(int dtype, const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_t stream);
 
 // A page of one layer, K or V, as `runs` pieces of `run` consecutive elements per token count:

@@ -27,6 +27,9 @@ bool misaligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>
 // Elements an operand may span, and the largest stride: far inside int64 byte offsets.
 constexpr int64_t kMaxSpan = (int64_t)1 << 46;
 
+// Rows of keys and values at most 2^23 elements apart: the kernels address 16 of them with 32-bit offsets.
+constexpr int64_t kMaxRow = (int64_t)1 << 23;
+
 // Row and head strides of an operand of `heads` heads of `dim`: either order, nothing overlapping.
 hq_status check_strides(const char* name, int64_t row, int64_t head, uint32_t rows, uint32_t heads, uint32_t dim) {
   if (row < 0 || head < 0 || row > kMaxSpan || head > kMaxSpan)
@@ -101,7 +104,9 @@ hq_status check_cache(const hq_kv_cache* c, hq::CacheArgs* out) {
     return fail(HQ_ERR_SHAPE, "cache: layers=%u, pages=%u, kv_heads=%u, rows=%u and max_pages=%u must be positive",
                 c->layers, c->pages, c->kv_heads, c->rows, c->max_pages);
   const uint32_t T = c->page_tokens;
-  if (T == 0 || T > 65536 || (T & (T - 1))) return fail(HQ_ERR_SHAPE, "cache: page_tokens=%u must be a power of two up to 65536", T);
+  if (T < 16 || T > 65536 || (T & (T - 1))) return fail(HQ_ERR_SHAPE, "cache: page_tokens=%u must be a power of two, 16 to 65536", T);
+  if ((uint64_t)c->kv_heads * c->head_dim > (uint64_t)kMaxRow)
+    return fail(HQ_ERR_SHAPE, "cache: kv_heads=%u times head_dim=%u above %lld", c->kv_heads, c->head_dim, (long long)kMaxRow);
   if (c->pages > (1u << 21) || c->layers > 4096 || c->kv_heads > 1024 || c->rows > (1u << 20) ||
       (uint64_t)c->max_pages * T > (1u << 30))
     return fail(HQ_ERR_SHAPE, "cache: layers=%u, pages=%u, kv_heads=%u, rows=%u, max_pages=%u: too many", c->layers, c->pages, c->kv_heads,
@@ -240,7 +245,7 @@ hq_status hq_describe_attn(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint
   if (!buf || buf_len == 0) return fail(HQ_ERR_INVALID_ARG, "buf is null or empty");
   const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim);
   if (st != HQ_OK) return st;
-  hq::describe_attn(kind, hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix), buf, buf_len);
+  hq::describe_attn(hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix), buf, buf_len);
   return hq_set_error(HQ_OK, "");
 }
 
@@ -259,6 +264,8 @@ hq_status hq_attn_prompt(const hq_attn_io* io, const void* K, int64_t k_row, int
   if ((st = check_strides("K", k_row, k_head, total_k, kv_heads, io->head_dim)) != HQ_OK ||
       (st = check_strides("V", v_row, v_head, total_k, kv_heads, io->head_dim)) != HQ_OK)
     return st;
+  if (k_row > kMaxRow || v_row > kMaxRow)
+    return fail(HQ_ERR_SHAPE, "K, V: row strides %lld, %lld above %lld elements", (long long)k_row, (long long)v_row, (long long)kMaxRow);
   a.cu_q = cu_q;
   a.causal = causal != 0;
   a.k.K = static_cast<const uint16_t*>(K);

@@ -87,7 +87,7 @@ def test_prompt_refuses_bad_keys(kw, status):
 BAD_CACHE = [
     (dict(K=0), hq.HQ_ERR_INVALID_ARG), (dict(table=0), hq.HQ_ERR_INVALID_ARG), (dict(status=0), hq.HQ_ERR_INVALID_ARG),
     (dict(dtype=0), hq.HQ_ERR_INVALID_ARG), (dict(head_dim=80), hq.HQ_ERR_UNSUPPORTED), (dict(pages=0), hq.HQ_ERR_SHAPE),
-    (dict(page_tokens=0), hq.HQ_ERR_SHAPE), (dict(page_tokens=48), hq.HQ_ERR_SHAPE), (dict(page_tokens=1 << 17), hq.HQ_ERR_SHAPE),
+    (dict(page_tokens=0), hq.HQ_ERR_SHAPE), (dict(page_tokens=48), hq.HQ_ERR_SHAPE), (dict(page_tokens=8), hq.HQ_ERR_SHAPE), (dict(page_tokens=1 << 17), hq.HQ_ERR_SHAPE),
     (dict(table_stride=31), hq.HQ_ERR_SHAPE), (dict(token_stride=256), hq.HQ_ERR_SHAPE), (dict(page_stride=65528), hq.HQ_ERR_SHAPE),
     (dict(page_stride=65540), hq.HQ_ERR_SHAPE), (dict(layer_stride=8), hq.HQ_ERR_SHAPE), (dict(V=P + 8), hq.HQ_ERR_ALIGNMENT),
     (dict(lens=P + 2), hq.HQ_ERR_ALIGNMENT), (dict(max_pages=1 << 25, table_stride=1 << 25), hq.HQ_ERR_SHAPE),

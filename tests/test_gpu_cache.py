@@ -48,9 +48,9 @@ def grow(c, h, rows, counts, rng, check=True):
         c.check()
 
 
-@pytest.mark.parametrize("kw", [dict(), dict(page=1, pages=300, max_pages=90), dict(page=64, D=128, dtype=torch.float16),
+@pytest.mark.parametrize("kw", [dict(), dict(page=16, pages=300, max_pages=90, Hkv=1), dict(page=64, D=128, dtype=torch.float16),
                                 dict(order="tokens", Hkv=3, gap=2), dict(Hkv=1, D=256, page=32), dict(page=16, Hkv=1, layers=1, order="tokens"),
-                                dict(pages=9000, page=4, Hkv=1, max_pages=30, layers=1)],
+                                dict(pages=9000, page=16, Hkv=1, max_pages=30, layers=1)],
                          ids=lambda kw: "-".join(f"{a}{b}" for a, b in kw.items()) or "plain")
 def test_a_life_of_sequences(cuda, kw):
     """Sequences that grow, fork, end and are compacted, in an order of their own."""
@@ -105,10 +105,10 @@ def test_compaction_of_large_pools(cuda, live):
     held = np.flatnonzero(refs)
     for i in range(3):
         table[i, :min(64, live)] = rng.permutation(held)[:64]
-    k = torch.arange(P, device="cuda").view(1, P, 1, 1, 1).expand(1, P, 1, 1, 64).to(torch.float16).contiguous()
+    k = torch.arange(P, device="cuda").view(1, P, 1, 1, 1).expand(1, P, 1, 16, 64).to(torch.float16).contiguous()
     v = (k + 0.5).contiguous()
-    h = A.Cache(k.cpu(), v.cpu(), table, [64] * 3, refs)
-    c = attn.KVCache(k, v, i32(table), i32([64] * 3), i32(refs))
+    h = A.Cache(k.cpu(), v.cpu(), table, [1024] * 3, refs)
+    c = attn.KVCache(k, v, i32(table), i32([1024] * 3), i32(refs))
     c.compact()
     h.compact()
     same(c, h)
@@ -169,9 +169,9 @@ def test_free_and_copy_report_and_skip(cuda):
 
 def test_many_sequences_at_once(cuda):
     n = attn.MAX_BATCH
-    c, h = fresh(page=4, pages=3 * n, rows=2 * n, max_pages=3, layers=1, Hkv=1)
+    c, h = fresh(page=16, pages=3 * n, rows=2 * n, max_pages=3, layers=1, Hkv=1)
     rng = np.random.default_rng(7)
-    rows, counts = rng.permutation(2 * n)[:n], rng.integers(0, 9, n)
+    rows, counts = rng.permutation(2 * n)[:n], rng.integers(0, 40, n)
     grow(c, h, list(rows), list(counts), rng)
     kids = np.setdiff1d(np.arange(2 * n), rows)
     c.fork(i32(rows), i32(kids))
@@ -185,7 +185,7 @@ def test_many_sequences_at_once(cuda):
 
 
 def test_strided_sources_and_single_tokens(cuda):
-    c, h = fresh(page=8, Hkv=4, D=128, dtype=torch.float16)
+    c, h = fresh(page=16, Hkv=4, D=128, dtype=torch.float16)
     rows = [2, 5, 0]
     c.reserve(i32(rows), i32([1, 1, 1]))
     h.reserve(rows, [1, 1, 1])
