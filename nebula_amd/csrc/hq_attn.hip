@@ -181,7 +181,7 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_
   const uint32_t lane = threadIdx.x & 63u;
   if (!cu) {  // one token each
     const uint32_t per = (G + rows - 1) / rows;
-    w.b = idx / per;
+    w.b = uni(idx / per);
     if (w.b >= n) return false;
     w.q0 = w.b;
     w.nq = 1;
@@ -278,9 +278,15 @@ struct Pages {
   }
 };
 
-// 16 keys of one head from `base` on (uniform). Rows are at most 2^24 bytes apart, so a lane's offset is 32-bit;
-// the descriptor is made anew for each block, since a pool or an operand may span more than 4 GiB.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const uint16_t* base) { return make_rsrc(base, 0x7FFFFFFFu); }
+// Keys from `base` (uniform) on, `rows` of them `step` bytes apart (at most 64 and 2^24): what lies past them
+// reads as 0. A lane's offset is 32-bit; the descriptor is made anew for each tile, since a pool or an
+// operand may span more than 4 GiB.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_rsrc(const uint16_t* base, uint32_t rows, uint32_t step) {
+  // Both are uniform; said so, because the compiler multiplies 64-bit numbers in vector registers.
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  const uint64_t q = (uint64_t)uni((uint32_t)(p >> 32)) << 32 | uni((uint32_t)p);
+  return make_rsrc(reinterpret_cast<const void*>(q), uni(rows * step));
+}
 
 // ---- parts of rows whose keys are split ----
 // Row (token t, head h) has `slots` places: fp32 O [D] (not divided by the sum), the maximum times c and
@@ -345,6 +351,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
     nk = span(a.k.cu_k, w.b, a.k.total_k, w.key0);
   }
   nk = uni(nk);
+  w.key0 = uni(w.key0);
 
   // This lane's row, and the keys it may see.
   const uint32_t r_mine = w.r0 + wave * 32 + l32;
@@ -386,29 +393,46 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   const uint16_t* const Vh = a.k.V + kvh * a.k.v_head;
 
   // Copies of tile t into a stage: load i of the wavefront brings rows kRowsPerLoad (i NW + wave) ...; a
-  // lane's row and source chunk undo the swizzle. Keys past the last are copies of it (masked below).
+  // lane's row and source chunk undo the swizzle. Keys past the last are 0 (masked below).
   const uint32_t in_row = lane / (D / 8), in_chunk = lane % (D / 8);
   const uint32_t k_step = (uint32_t)a.k.k_row * 2, v_step = (uint32_t)a.k.v_row * 2, page_mask = (1u << a.k.page_shift) - 1;
   Pages<kKeys> pages{table, t0 * kKeys, kKeys, nk, 0, 0};
-  auto issue = [&](uint32_t t, uint32_t stage) __attribute__((always_inline)) {
-    unsigned char* const base = smem + stage * kStage;
-    const uint32_t left = nk - 1 - t * kKeys;  // last row with a key
-    if constexpr (PAGED) pages.advance(a.k, t - t0);
+  const bool whole = !PAGED || a.k.page_shift >= 6;  // a tile lies in one page
+  // Offsets of load 0, and of load 1 less its rows: the swizzle of K goes with the row modulo 16, which later
+  // loads have in common with one of them.
+  uint32_t k_off[2], v_off[2];
 #pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i) {
-      const uint32_t row0 = (i * NW + wave) * kRowsPerLoad, row = row0 + in_row;
-      const uint32_t sub = min(row0 / 16, left / 16), in = min(row, left) - 16 * sub;
-      int64_t ko, vo;
-      if constexpr (PAGED) {
-        ko = vo = pages.page(t - t0, sub) * a.k.page_stride + ((t * kKeys + 16 * sub) & page_mask) * a.k.k_row;
-      } else {
-        ko = (w.key0 + t * kKeys + 16 * sub) * a.k.k_row;
-        vo = (w.key0 + t * kKeys + 16 * sub) * a.k.v_row;
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t row = (i * NW + wave) * kRowsPerLoad + in_row;
+    k_off[i] = (wave * kRowsPerLoad + in_row) * k_step + ((in_chunk ^ swz_k<D>(row)) << 4);
+    v_off[i] = (wave * kRowsPerLoad + in_row) * v_step + ((in_chunk ^ swz_v<D>(row)) << 4);
+  }
+  auto copy = [&](uint32_t t, const uint16_t* from, int64_t row_stride, uint32_t step, const uint32_t (&off)[2], unsigned char* to)
+                  __attribute__((always_inline)) {
+    const uint32_t key = t * kKeys, left = min(nk - key, (uint32_t)kKeys);
+    if (whole) {
+      int64_t at;
+      if constexpr (PAGED) at = pages.page(t - t0, 0) * a.k.page_stride + (key & page_mask) * row_stride;
+      else at = (int64_t)(w.key0 + key) * row_stride;
+      const __amdgpu_buffer_rsrc_t r = keys_rsrc(from + at, left, step);
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i)
+        buffer_to_lds16(r, to + (i * NW + wave) * 1024, off[i & 1] + i * NW * kRowsPerLoad * step);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < kLoads; ++i) {  // a block of 16 rows each
+        const uint32_t row0 = (i * NW + wave) * kRowsPerLoad, first = row0 & ~15u;
+        const int64_t at = pages.page(t - t0, row0 / 16) * a.k.page_stride + ((key + first) & page_mask) * row_stride;
+        buffer_to_lds16(keys_rsrc(from + at, left > first ? left - first : 0u, step), to + (i * NW + wave) * 1024,
+                        off[i & 1] + (row0 - first - wave * kRowsPerLoad) * step);
       }
-      unsigned char* const to = base + (i * NW + wave) * 1024;
-      buffer_to_lds16(block_rsrc(Kh + ko), to, in * k_step + ((in_chunk ^ swz_k<D>(row)) << 4));
-      buffer_to_lds16(block_rsrc(Vh + vo), to + kVOff, in * v_step + ((in_chunk ^ swz_v<D>(row)) << 4));
     }
+  };
+  auto copy_k = [&](uint32_t t) __attribute__((always_inline)) {
+    copy(t, Kh, a.k.k_row, k_step, k_off, smem + (t & 1u) * kStage);
+  };
+  auto copy_v = [&](uint32_t t) __attribute__((always_inline)) {
+    copy(t, Vh, a.k.v_row, v_step, v_off, smem + (t & 1u) * kStage + kVOff);
   };
 
   // LDS places of this lane's fragments. K^T: row l32 (+ 32), dims 16 s + 8 half: chunk 2 s + half.
@@ -424,83 +448,104 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 
   f16x o[kDims];
   float m, l;
-  // Second pass (careful) only where a first one gave values that are not finite, or no weight at all:
-  // values of V at keys a row may not see, times its weight 0, may have made them, or scores past 1e7.
-  auto pass = [&](auto mode) __attribute__((always_inline)) {
-    constexpr bool careful = decltype(mode)::value;
+  constexpr int kBlock = kDims < 4 ? kDims : 4;  // fragments of V^T in registers
+
+  auto scores = [&](uint32_t t, f16x (&s)[2], int i) __attribute__((always_inline)) {  // step i of S^T = K Q^T
+    const unsigned char* const st = smem + (t & 1u) * kStage;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+      s[kt] = mfma32x32x16<DT>(*reinterpret_cast<const u4*>(st + k_at[i] + kt * 32 * kPitch), q[i], i ? s[kt] : f16x{});
+  };
+  auto mask = [&](uint32_t t, f16x (&s)[2]) __attribute__((always_inline)) {
+    const uint32_t k0 = t * kKeys + 4 * half;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        if (k0 + 32 * kt + 8 * (v / 4) + v % 4 >= lim) s[kt][v] = -INFINITY;
+  };
+  auto both_halves = [&](float x, float y) {  // this lane's and the other half's
+    const auto e = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return f2{__uint_as_float(e[0]), __uint_as_float(e[1])};
+  };
+  // The maximum follows the scores only where it lags by more than kLag: each row by itself, so that its
+  // bits do not depend on its neighbours, and the sums are rescaled only where some row's moves.
+  auto follow = [&](float top) __attribute__((always_inline)) {
+    const f2 e = both_halves(top, top);
+    top = fmaxf(e[0], e[1]);
+    if (__any((top - m) * c > Weights<DT>::kLag)) {
+      const float n = (top - m) * c > Weights<DT>::kLag ? top : m, al = __builtin_amdgcn_exp2f((m - n) * c);
+      m = n;
+      l *= al;
+#pragma unroll
+      for (int dt = 0; dt < kDims; ++dt) o[dt] *= al;
+    }
+  };
+  auto meet = [&]() __attribute__((always_inline)) {  // the wavefronts' copies have landed, their reads are done
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto reset = [&]() __attribute__((always_inline)) {
     m = kNone;
     l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < kDims; ++dt) o[dt] = f16x{};
-    uint32_t ts = t0;
-    asm volatile("" : "+s"(ts));  // what one pass computes is not held for the other
     if constexpr (PAGED)
-      if (t1 > ts) pages.start(a.k);
-    if (t1 > ts) issue(ts, ts & 1u);
-    for (uint32_t t = ts; t < t1; ++t) {
-      __builtin_amdgcn_s_waitcnt(0);  // the wavefront's copies of tile t have landed, its reads of t - 1 are done
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      if (t + 1 < t1) issue(t + 1, (t + 1) & 1u);
-      if (t * kKeys >= lim_max) continue;
-      const unsigned char* const st = smem + (t & 1u) * kStage;
+      if (t1 > t0) pages.start(a.k);
+  };
 
-      f16x s[2] = {f16x{}, f16x{}};
+  // Tiles this wavefront computes: t0 .. tw - 1 (its rows see nothing of the others).
+  const uint32_t tw = min(t1, (lim_max + kKeys - 1) / kKeys);
+  reset();
+  if (t1 > t0) {
+    // The scores of a tile are computed while the weights of the one before are, and its maximum while that
+    // one's second product runs: the matrix and the vector pipes each have the other's work beside theirs.
+    f16x s[2];
+    copy_k(t0);
+    copy_v(t0);
+    if (t0 + 1 < t1) {
+      if constexpr (PAGED) pages.advance(a.k, 1);
+      copy_k(t0 + 1);
+    }
+    meet();
+    if (t0 < tw) {
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-          s[kt] = mfma32x32x16<DT>(*reinterpret_cast<const u4*>(st + k_at[i] + kt * 32 * kPitch), q[i], s[kt]);
-
-      const bool masked = t * kKeys + kKeys > lim_min;
-      if (masked) {
-        const uint32_t k0 = t * kKeys + 4 * half;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (k0 + 32 * kt + 8 * (v / 4) + v % 4 >= lim) s[kt][v] = -INFINITY;
-      }
+      for (int i = 0; i < kSteps; ++i) scores(t0, s, i);
+      if (t0 * kKeys + kKeys > lim_min) mask(t0, s);
       float top = s[0][0];
 #pragma unroll
       for (int v = 0; v < 16; ++v) top = fmaxf(fmaxf(top, s[0][v]), s[1][v]);
-      {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-      }
-      if (__any((top - m) * c > Weights<DT>::kLag)) {
-        const float n = (top - m) * c > Weights<DT>::kLag ? top : m, al = __builtin_amdgcn_exp2f((m - n) * c);
-        m = n;  // each row by itself, so that its bits do not depend on its neighbours
-        l *= al;
-#pragma unroll
-        for (int dt = 0; dt < kDims; ++dt) o[dt] *= al;
-      }
-      float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift, cs = c;
-      if constexpr (careful) {  // differences first: m c may be rounded by more than the exponential's range
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          s[0][v] = (s[0][v] - m) * c;
-          s[1][v] = (s[1][v] - m) * c;
-        }
-        mc = -Weights<DT>::kLift;
-        cs = 1.f;
-      }
+      follow(top);
+    }
+    auto tile = [&](uint32_t t, auto next) __attribute__((always_inline)) {
+      constexpr bool more = decltype(next)::value;  // the next tile is this wavefront's too
+      // With and without a next tile are two pieces of code: what they share is not taken out of them.
+      if constexpr (more) asm volatile("" : "+v"(s[0]), "+v"(s[1]));
+      const float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift;
       u4 p[4];
+      f16x ns[2];
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int i = 0; i < kSteps; ++i) {
+        if constexpr (more) scores(t + 1, ns, i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = 8 * (j & 1) + 2 * e;
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[j / 2][v], cs, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[j / 2][v + 1], cs, -mc));
+        for (int u = 16 * i / kSteps; u < 16 * (i + 1) / kSteps; ++u) {  // weights 2 u, 2 u + 1 of 32
+          const int v = 2 * (u & 7);
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[u / 8][v], c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[u / 8][v + 1], c, -mc));
           sum += x + y;
-          p[j][e] = pack2<DT>(x, y);
+          p[u / 4][u & 3] = pack2<DT>(x, y);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
       l += sum;
-
-      // O^T += V^T P^T: 16 keys a step, fragments of as many groups of 32 dims as registers are taken for.
-      constexpr int kBlock = kDims < 4 ? kDims : 4;
+      if constexpr (more) {
+        // Both stay above, in turn.
+        asm volatile("" : "+v"(ns[0]), "+v"(ns[1]), "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
+        if ((t + 1) * kKeys + kKeys > lim_min) mask(t + 1, ns);
+      }
+      float top = more ? ns[0][0] : 0.f;
       const uint32_t stage_at = (t & 1u) * kStage;
       each<4>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::value;
@@ -511,37 +556,96 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 #pragma unroll
           for (int i = 0; i < kBlock; ++i) at[i] = stage_at + v_at[d0 + i];
           lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
-          if (careful && masked) {
-            const uint32_t key = t * kKeys + 16 * j + 4 * half;
-            const u4 sees = {seen2<DT>(key, lim), seen2<DT>(key + 2, lim), seen2<DT>(key + 8, lim), seen2<DT>(key + 10, lim)};
 #pragma unroll
-            for (int i = 0; i < kBlock; ++i) {
-              u4 finite, code;
-              split_odd<DT>(f[i], finite, code);
-              o[d0 + i] = mfma32x32x16<DT>(finite, p[j], o[d0 + i]);
-              const f16x count = mfma32x32x16<DT>(code, sees, f16x{});
-#pragma unroll
-              for (int v = 0; v < 16; ++v) o[d0 + i][v] += odd_value(count[v]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < kBlock; ++i) o[d0 + i] = mfma32x32x16<DT>(f[i], p[j], o[d0 + i]);
-          }
+          for (int i = 0; i < kBlock; ++i) o[d0 + i] = mfma32x32x16<DT>(f[i], p[j], o[d0 + i]);
         }
+        if constexpr (more)
+#pragma unroll
+          for (int v = 4 * j; v < 4 * j + 4; ++v) top = fmaxf(fmaxf(top, ns[0][v]), ns[1][v]);
       });
+      if constexpr (more) {
+        follow(top);
+        s[0] = ns[0];
+        s[1] = ns[1];
+      }
+    };
+    for (uint32_t t = t0; t < t1; ++t) {
+      if (t > t0) meet();
+      else __builtin_amdgcn_s_barrier();  // every wavefront has its scores of t0: its K may be overwritten
+      if (t + 1 < t1) copy_v(t + 1);
+      if (t + 2 < t1) {
+        if constexpr (PAGED) pages.advance(a.k, t + 2 - t0);
+        copy_k(t + 2);
+      }
+      if (t + 1 < tw) tile(t, std::true_type{});
+      else if (t < tw) tile(t, std::false_type{});
     }
-    {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-      l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-    }
+  }
+  // Again where values are not finite, or a row has no weight: V at keys a row may not see, times its weight
+  // 0, may have made them, or scores past 1e7. Tile by tile, differences of scores before the factor (m c may
+  // be rounded by more than the exponential's range), and those values apart.
+  auto odd = [&]() {
+    const f2 e = both_halves(l, l);
+    l = e[0] + e[1];
     float bad = 0.f;
 #pragma unroll
     for (int dt = 0; dt < kDims; ++dt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) bad = fmaf(o[dt][v], 0.f, bad);
-    return __syncthreads_or(!(bad == 0.f) || (l == 0.f && m != kNone)) != 0;
+    return !(bad == 0.f) || (l == 0.f && m != kNone);
   };
-  if (pass(std::false_type{})) pass(std::true_type{});
+  if (__syncthreads_or(odd())) {
+    reset();
+    for (uint32_t t = t0; t < t1; ++t) {
+      meet();
+      if constexpr (PAGED) pages.advance(a.k, t - t0);
+      copy_k(t);
+      copy_v(t);
+      meet();
+      if (t >= tw) continue;
+      f16x s[2];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) scores(t, s, i);
+      const bool masked = t * kKeys + kKeys > lim_min;
+      if (masked) mask(t, s);
+      float top = s[0][0];
+#pragma unroll
+      for (int v = 0; v < 16; ++v) top = fmaxf(fmaxf(top, s[0][v]), s[1][v]);
+      follow(top);
+      u4 p[4];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        const int v = 2 * (u & 7);
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[u / 8][v] - m, c, Weights<DT>::kLift));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[u / 8][v + 1] - m, c, Weights<DT>::kLift));
+        l += x + y;
+        p[u / 4][u & 3] = pack2<DT>(x, y);
+      }
+      const uint32_t stage_at = (t & 1u) * kStage;
+      each<4>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value;
+        const uint32_t key = t * kKeys + 16 * j + 4 * half;
+        const u4 sees = {seen2<DT>(key, lim), seen2<DT>(key + 2, lim), seen2<DT>(key + 8, lim), seen2<DT>(key + 10, lim)};
+#pragma unroll
+        for (int d0 = 0; d0 < kDims; d0 += 2) {
+          const uint32_t at[2] = {stage_at + v_at[d0], stage_at + v_at[d0 + 1]};
+          u4 f[2];
+          lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            u4 finite, code;
+            split_odd<DT>(f[i], finite, code);
+            o[d0 + i] = mfma32x32x16<DT>(finite, p[j], o[d0 + i]);
+            const f16x count = mfma32x32x16<DT>(code, sees, f16x{});
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[d0 + i][v] += odd_value(count[v]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      });
+    }
+    odd();
+  }
   if (!live) return;
   const uint32_t tok = w.q0 + token;
   const float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift;
@@ -629,6 +733,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     nk = span(a.k.cu_k, w.b, a.k.total_k, w.key0);
   }
   nk = uni(nk);
+  w.key0 = uni(w.key0);
   begin = uni(begin);
 
   const uint32_t r_mine = w.r0 + l16;
@@ -660,30 +765,51 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   const uint32_t stride = active * NW;
   Pages<kRowKeys> pages{table, begin + (split * NW + wave) * kRowKeys, stride * kRowKeys, nk, 0, 0};
   const uint32_t k_step = (uint32_t)a.k.k_row * 2, v_step = (uint32_t)a.k.v_row * 2, page_mask = (1u << a.k.page_shift) - 1;
-  // Elements from the head's first to block `sub` of tile n of this wavefront, which begins at key k0.
-  auto block_at = [&](uint32_t n, uint32_t k0, uint32_t sub, int64_t token_stride) __attribute__((always_inline)) -> int64_t {
-    if constexpr (PAGED) return pages.page(n, sub) * a.k.page_stride + ((k0 + 16 * sub) & page_mask) * token_stride;
-    else return (w.key0 + k0 + 16 * sub) * token_stride;
-  };
-  // Rows past the last key are copies of its (masked below).
+  const bool whole = !PAGED || (a.k.page_shift >= 5 && begin % kRowKeys == 0);  // a tile lies in one page
+  // Offsets of the first loads of V, less their rows: the swizzle goes with the row modulo 8.
+  uint32_t v_off[4];
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) v_off[i] = in_row * v_step + ((in_chunk ^ swz_rv<D>(i * kRowsPerLoad + in_row)) << 4);
+  const uint32_t k_off = l16 * k_step + 16 * quad;
   u4 kf[2][kSteps];
+  // From here on: tile n of this wavefront, which begins at key k0. Keys past the last are 0 (masked below).
+  auto rsrc_at = [&](uint32_t n, uint32_t k0, uint32_t row, const uint16_t* from, int64_t row_stride, uint32_t step) __attribute__((always_inline)) {
+    int64_t at;
+    if constexpr (PAGED) at = pages.page(n, row / 16) * a.k.page_stride + ((k0 + row) & page_mask) * row_stride;
+    else at = (int64_t)(w.key0 + k0 + row) * row_stride;
+    const uint32_t left = min(nk - k0, (uint32_t)kRowKeys);
+    return keys_rsrc(from + at, left > row ? left - row : 0u, step);
+  };
   auto load_k = [&](uint32_t n, uint32_t k0) __attribute__((always_inline)) {
-    const uint32_t left = nk - 1 - k0;
+    if (whole) {
+      const __amdgpu_buffer_rsrc_t r = rsrc_at(n, k0, 0, Kh, a.k.k_row, k_step);
 #pragma unroll
-    for (uint32_t kt = 0; kt < 2; ++kt) {
-      const uint32_t sub = min(kt, left / 16), at = (min(16 * kt + l16, left) - 16 * sub) * k_step + 16 * quad;
-      const __amdgpu_buffer_rsrc_t kr = block_rsrc(Kh + block_at(n, k0, sub, a.k.k_row));
+      for (uint32_t kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) kf[kt][s] = __builtin_amdgcn_raw_buffer_load_b128(kr, at + 64 * s, 0, 0);
+        for (int s = 0; s < kSteps; ++s) kf[kt][s] = __builtin_amdgcn_raw_buffer_load_b128(r, k_off + 16 * kt * k_step + 64 * s, 0, 0);
+    } else {
+#pragma unroll
+      for (uint32_t kt = 0; kt < 2; ++kt) {
+        const __amdgpu_buffer_rsrc_t r = rsrc_at(n, k0, 16 * kt, Kh, a.k.k_row, k_step);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) kf[kt][s] = __builtin_amdgcn_raw_buffer_load_b128(r, k_off + 64 * s, 0, 0);
+      }
     }
   };
   auto copy_v = [&](uint32_t n, uint32_t k0) __attribute__((always_inline)) {
-    const uint32_t left = nk - 1 - k0;
+    unsigned char* const to = mine + (n & 1u) * kStage;
+    if (whole) {
+      const __amdgpu_buffer_rsrc_t r = rsrc_at(n, k0, 0, Vh, a.k.v_row, v_step);
 #pragma unroll
-    for (uint32_t i = 0; i < kLoads; ++i) {
-      const uint32_t row = i * kRowsPerLoad + in_row, sub = min(i * kRowsPerLoad / 16, left / 16);
-      buffer_to_lds16(block_rsrc(Vh + block_at(n, k0, sub, a.k.v_row)), mine + (n & 1u) * kStage + i * 1024,
-                      (min(row, left) - 16 * sub) * v_step + ((in_chunk ^ swz_rv<D>(row)) << 4));
+      for (uint32_t i = 0; i < kLoads; ++i) buffer_to_lds16(r, to + i * 1024, v_off[i & 3] + i * kRowsPerLoad * v_step);
+    } else {
+#pragma unroll
+      for (uint32_t sub = 0; sub < 2; ++sub) {
+        const __amdgpu_buffer_rsrc_t r = rsrc_at(n, k0, 16 * sub, Vh, a.k.v_row, v_step);
+#pragma unroll
+        for (uint32_t i = 0; i < kLoads / 2; ++i)
+          buffer_to_lds16(r, to + (sub * (kLoads / 2) + i) * 1024, v_off[(sub * (kLoads / 2) + i) & 3] + i * kRowsPerLoad * v_step);
+      }
     }
   };
 

@@ -270,9 +270,9 @@ hq_status hq_attn_prompt(const hq_attn_io* io, const void* K, int64_t k_row, int
   a.causal = causal != 0;
   a.k.K = static_cast<const uint16_t*>(K);
   a.k.V = static_cast<const uint16_t*>(V);
-  a.k.k_row = k_row;
+  a.k.k_row = total_k > 1 ? k_row : std::max<int64_t>(k_row, io->head_dim);  // a row's bytes bound its reads
   a.k.k_head = k_head;
-  a.k.v_row = v_row;
+  a.k.v_row = total_k > 1 ? v_row : std::max<int64_t>(v_row, io->head_dim);
   a.k.v_head = v_head;
   a.k.cu_k = cu_k ? cu_k : cu_q;
   a.k.total_k = total_k;
