@@ -146,25 +146,32 @@ __device__ __forceinline__ uint32_t clamp_u(int32_t v, uint32_t hi) { return v <
 __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
 // ---- sequences ----
-// What a tile works on: rows [r0, R) of a sequence (or of a group, for its shared prefix) whose first
-// token is q0, over keys [k0, k1) of n.
+// The loads that a workgroup starts with depend on each other (offsets, a row's number, its length, its
+// pages, its keys), and short calls last little longer than they do: what does not depend on the last
+// load's result is loaded beside it.
+
+// What a tile works on: rows [r0, R) of a sequence, or of a group for its shared prefix, whose first token
+// is q0 of nq.
 struct Work {
-  uint32_t b, q0, R, r0;
-  uint32_t nq, nk;       // new tokens, keys
-  uint32_t key0;         // packed: row of key 0 in K and V
-  int32_t row;           // paged: cache row
-  bool ok;
+  uint32_t b, q0, nq, R, r0;
+  uint32_t key0;  // packed: row of key 0 in K and V
 };
 
-// Cache row of sequence b and its length (0, reported, if there is no such row).
-__device__ __forceinline__ uint32_t cached_len(const AttnKeys& k, uint32_t b, int32_t& row) {
-  row = k.rows ? k.rows[b] : (int32_t)b;
-  if ((uint32_t)row >= k.cache_rows) {
+// Cache row of sequence b; a number out of range is reported where `ok` is asked, and stands for row 0.
+__device__ __forceinline__ int32_t row_number(const AttnKeys& k, uint32_t b) { return k.rows ? k.rows[b] : (int32_t)b; }
+__device__ __forceinline__ bool row_ok(const AttnKeys& k, int32_t row) { return (uint32_t)row < k.cache_rows; }
+__device__ __forceinline__ int32_t row_length(const AttnKeys& k, int32_t row) { return k.lens[row_ok(k, row) ? row : 0]; }
+__device__ __forceinline__ uint32_t length_or_report(const AttnKeys& k, int32_t row, int32_t len) {
+  if (!row_ok(k, row)) {
     report(k.status, HQ_CACHE_BAD_ROW);
-    row = 0;
     return 0;
   }
-  return clamp_u(k.lens[row], k.max_pages << k.page_shift);
+  return clamp_u(len, k.max_pages << k.page_shift);
+}
+// The tokens of a group's shared prefix that lie in whole pages: no more than its first row holds.
+__device__ __forceinline__ uint32_t whole_pages(const AttnKeys& k, int32_t first_row, int32_t first_len, int32_t prefix) {
+  const uint32_t len = row_ok(k, first_row) ? clamp_u(first_len, k.max_pages << k.page_shift) : 0u;
+  return min(len, clamp_u(prefix, 1u << 30)) >> k.page_shift << k.page_shift;
 }
 
 // Tokens of entry b of a list of offsets (queries of a sequence, sequences of a group), held to [0, most].
@@ -216,22 +223,20 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_
   return false;
 }
 
-// The group of sequence b, and the tokens of its prefix that lie in whole pages.
-__device__ __forceinline__ uint32_t shared_tokens(const AttnArgs& a, uint32_t g) {
-  const uint32_t first = clamp_u(a.starts[g], a.B);
-  if (first >= a.B) return 0;
-  int32_t row;
-  const uint32_t n = min(cached_len(a.k, first, row), clamp_u(a.prefix[g], 1u << 30));
-  return n >> a.k.page_shift << a.k.page_shift;
-}
-__device__ __forceinline__ uint32_t group_of(const AttnArgs& a, uint32_t b) {
-  uint32_t lo = 0, hi = a.groups;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.starts[mid] <= (int32_t)b) lo = mid;
-    else hi = mid;
+// The group of sequence b, the last one that starts at or before it, and where it starts.
+__device__ __forceinline__ uint32_t group_of(const AttnArgs& a, uint32_t b, uint32_t& first) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t g = 0;
+  first = 0;
+  for (uint32_t base = 0; base < a.groups; base += 64) {
+    const int32_t at = base + lane < a.groups ? a.starts[base + lane] : 0x7FFFFFFF;
+    const uint64_t before = __ballot(at <= (int32_t)b);
+    if (!before) break;
+    const int last = 63 - __builtin_clzll(before);
+    g = base + last;
+    first = clamp_u(__builtin_amdgcn_readlane(at, last), a.B - 1);
   }
-  return lo;
+  return g;
 }
 
 __device__ __forceinline__ uint32_t page_or_report(const AttnKeys& k, int32_t page) {
@@ -340,30 +345,37 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   const uint32_t split = rest % pl.splits, idx = rest / pl.splits;
   Work w{};
   if (!find_tile(pl.prefix ? a.starts : a.cu_q, pl.prefix ? a.groups : a.B, pl.prefix ? a.B : a.T, a.G, BR, idx, w)) return;
-  const int32_t* table = nullptr;
-  uint32_t nk;
-  if constexpr (PAGED) {
-    int32_t row;
-    nk = cached_len(a.k, pl.prefix ? w.q0 : w.b, row);
-    if (pl.prefix) nk = shared_tokens(a, w.b);
-    table = a.k.table + row * a.k.table_stride;
-  } else {
-    nk = span(a.k.cu_k, w.b, a.k.total_k, w.key0);
-  }
-  nk = uni(nk);
-  w.key0 = uni(w.key0);
-
-  // This lane's row, and the keys it may see.
+  // This lane's row.
   const uint32_t r_mine = w.r0 + wave * 32 + l32;
   const bool live = r_mine < w.R;
   const uint32_t r = min(r_mine, w.R - 1), token = r / a.G, head = kvh * a.G + (r - token * a.G);
-  uint32_t lim = nk;
-  if (pl.prefix) {
-    int32_t row;
-    lim = min(nk, cached_len(a.k, w.q0 + token, row));
-  } else if (a.causal) {
-    const int64_t n = (int64_t)token + nk - w.nq + 1;
-    lim = n < 0 ? 0u : (uint32_t)n;
+
+  const int32_t* table = nullptr;
+  uint32_t nk, lim = 0;  // keys of the sequence, and those below lim this lane's row may see
+  if constexpr (PAGED) {
+    const int32_t row = row_number(a.k, pl.prefix ? w.q0 : w.b);
+    table = a.k.table + (row_ok(a.k, row) ? row : 0) * a.k.table_stride;
+    if (pl.prefix) {
+      const int32_t own = row_number(a.k, w.q0 + token), prefix = a.prefix[w.b];
+      const int32_t len = row_length(a.k, row), own_len = row_length(a.k, own);
+      nk = uni(whole_pages(a.k, row, len, prefix));
+      lim = min(nk, length_or_report(a.k, own, own_len));
+    } else {
+      nk = uni(length_or_report(a.k, row, row_length(a.k, row)));
+    }
+  } else if (a.k.cu_k == a.cu_q && a.k.total_k >= a.T) {
+    nk = w.nq;
+    w.key0 = w.q0;
+  } else {
+    nk = uni(span(a.k.cu_k, w.b, a.k.total_k, w.key0));
+    w.key0 = uni(w.key0);
+  }
+  if (!pl.prefix) {
+    lim = nk;
+    if (a.causal) {
+      const int64_t n = (int64_t)token + nk - w.nq + 1;
+      lim = n < 0 ? 0u : (uint32_t)n;
+    }
   }
   uint32_t lim_min = lim, lim_max = lim;
 #pragma unroll
@@ -435,26 +447,26 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
     copy(t, Vh, a.k.v_row, v_step, v_off, smem + (t & 1u) * kStage + kVOff);
   };
 
-  // LDS places of this lane's fragments. K^T: row l32 (+ 32), dims 16 s + 8 half: chunk 2 s + half.
-  uint32_t k_at[kSteps];
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s) k_at[s] = l32 * kPitch + (((2 * s + half) ^ swz_k<D>(l32)) << 4);
-  // V^T: keys 4 half + (lane % 16) / 4 (+ 8, + 16 steps), dims 32 dt + 16 (l32 / 16) + 4 (lane % 4).
+  // LDS places of this lane's fragments. K^T: row l32 (+ 32), dims 16 s + 8 half, chunk 2 s + half: the place of
+  // step 0, s << 5 exclusive-or'ed. V^T: keys 4 half + (lane % 16) / 4 (+ 8, + 16 steps), dims 32 dt + 16
+  // (l32 / 16) + 4 (lane % 4): dt << 6 likewise. (Held apart they are 14 registers that the kernel has not.)
+  const uint32_t k_at = l32 * kPitch + ((half ^ swz_k<D>(l32)) << 4);
   const uint32_t v_row = 4 * half + ((lane & 15u) >> 2);
-  uint32_t v_at[kDims];
-#pragma unroll
-  for (int dt = 0; dt < kDims; ++dt)
-    v_at[dt] = lds_address(smem) + kVOff + v_row * kPitch + (((4 * dt + 2 * (l32 >> 4) + ((lane & 3u) >> 1)) ^ swz_v<D>(v_row)) << 4) + 8 * (lane & 1u);
+  const uint32_t v_at = lds_address(smem) + kVOff + v_row * kPitch + (((2 * (l32 >> 4) + ((lane & 3u) >> 1)) ^ swz_v<D>(v_row)) << 4) + 8 * (lane & 1u);
 
   f16x o[kDims];
   float m, l;
   constexpr int kBlock = kDims < 4 ? kDims : 4;  // fragments of V^T in registers
 
-  auto scores = [&](uint32_t t, f16x (&s)[2], int i) __attribute__((always_inline)) {  // step i of S^T = K Q^T
-    const unsigned char* const st = smem + (t & 1u) * kStage;
+  auto opaque = [](uint32_t v) __attribute__((always_inline)) {  // what is computed from it stays in its tile
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  auto scores = [&](uint32_t at, f16x (&s)[2], int i) __attribute__((always_inline)) {  // step i of S^T = K Q^T
+    const unsigned char* const p = smem + (at ^ (uint32_t)(i << 5));
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
-      s[kt] = mfma32x32x16<DT>(*reinterpret_cast<const u4*>(st + k_at[i] + kt * 32 * kPitch), q[i], i ? s[kt] : f16x{});
+      s[kt] = mfma32x32x16<DT>(*reinterpret_cast<const u4*>(p + kt * 32 * kPitch), q[i], i ? s[kt] : f16x{});
   };
   auto mask = [&](uint32_t t, f16x (&s)[2]) __attribute__((always_inline)) {
     const uint32_t k0 = t * kKeys + 4 * half;
@@ -511,8 +523,9 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
     }
     meet();
     if (t0 < tw) {
+      const uint32_t at = opaque(k_at + (t0 & 1u) * kStage);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) scores(t0, s, i);
+      for (int i = 0; i < kSteps; ++i) scores(at, s, i);
       if (t0 * kKeys + kKeys > lim_min) mask(t0, s);
       float top = s[0][0];
 #pragma unroll
@@ -527,9 +540,10 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
       u4 p[4];
       f16x ns[2];
       float sum = 0.f;
+      const uint32_t at = opaque(k_at + ((t + 1) & 1u) * kStage);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        if constexpr (more) scores(t + 1, ns, i);
+        if constexpr (more) scores(at, ns, i);
 #pragma unroll
         for (int u = 16 * i / kSteps; u < 16 * (i + 1) / kSteps; ++u) {  // weights 2 u, 2 u + 1 of 32
           const int v = 2 * (u & 7);
@@ -546,7 +560,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
         if ((t + 1) * kKeys + kKeys > lim_min) mask(t + 1, ns);
       }
       float top = more ? ns[0][0] : 0.f;
-      const uint32_t stage_at = (t & 1u) * kStage;
+      const uint32_t v0 = opaque(v_at + (t & 1u) * kStage);
       each<4>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::value;
 #pragma unroll
@@ -554,7 +568,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
           uint32_t at[kBlock];
           u4 f[kBlock];
 #pragma unroll
-          for (int i = 0; i < kBlock; ++i) at[i] = stage_at + v_at[d0 + i];
+          for (int i = 0; i < kBlock; ++i) at[i] = v0 ^ (uint32_t)((d0 + i) << 6);
           lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
 #pragma unroll
           for (int i = 0; i < kBlock; ++i) o[d0 + i] = mfma32x32x16<DT>(f[i], p[j], o[d0 + i]);
@@ -604,8 +618,9 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
       meet();
       if (t >= tw) continue;
       f16x s[2];
+      const uint32_t k0 = opaque(k_at + (t & 1u) * kStage), v0 = opaque(v_at + (t & 1u) * kStage);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) scores(t, s, i);
+      for (int i = 0; i < kSteps; ++i) scores(k0, s, i);
       const bool masked = t * kKeys + kKeys > lim_min;
       if (masked) mask(t, s);
       float top = s[0][0];
@@ -621,14 +636,13 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
         l += x + y;
         p[u / 4][u & 3] = pack2<DT>(x, y);
       }
-      const uint32_t stage_at = (t & 1u) * kStage;
       each<4>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::value;
         const uint32_t key = t * kKeys + 16 * j + 4 * half;
         const u4 sees = {seen2<DT>(key, lim), seen2<DT>(key + 2, lim), seen2<DT>(key + 8, lim), seen2<DT>(key + 10, lim)};
 #pragma unroll
         for (int d0 = 0; d0 < kDims; d0 += 2) {
-          const uint32_t at[2] = {stage_at + v_at[d0], stage_at + v_at[d0 + 1]};
+          const uint32_t at[2] = {v0 ^ (uint32_t)(d0 << 6), v0 ^ (uint32_t)((d0 + 1) << 6)};
           u4 f[2];
           lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
 #pragma unroll
@@ -679,7 +693,8 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 constexpr int kRowKeys = 32;  // keys of a wavefront's tile
 
 struct RowPlan {
-  uint32_t splits;     // workgroups that share the keys of 16 rows
+  uint32_t splits;     // workgroups that share the keys of 16 rows, at most
+  uint32_t least;      // tiles of a wavefront before one more takes part
   uint32_t* cnt;       // arrivals of a tile's workgroups, zero between launches
   float* o;            // their parts: [tile][kv head][splits][16][D], and the maxima and sums [..][16]
   f2* ml;
@@ -722,22 +737,34 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   const uint32_t split = rest % pl.splits, idx = rest / pl.splits;
   Work w{};
   if (!find_tile(a.cu_q, a.B, a.T, a.G, 16, idx, w)) return;
-  const int32_t* table = nullptr;
-  uint32_t nk, begin = 0;
-  if constexpr (PAGED) {
-    int32_t row;
-    nk = cached_len(a.k, w.b, row);
-    table = a.k.table + row * a.k.table_stride;
-    if (a.groups) begin = min(nk, shared_tokens(a, group_of(a, w.b)));
-  } else {
-    nk = span(a.k.cu_k, w.b, a.k.total_k, w.key0);
-  }
-  nk = uni(nk);
-  w.key0 = uni(w.key0);
-  begin = uni(begin);
-
   const uint32_t r_mine = w.r0 + l16;
   const uint32_t r = min(r_mine, w.R - 1), token = r / a.G, head = kvh * a.G + (r - token * a.G);
+  const uint32_t t_first = split * NW + wave;
+
+  const int32_t* table = nullptr;
+  uint32_t nk, begin = 0;
+  int32_t early = 0;  // pages of the first tile: lane j % 2 that of its block j
+  if constexpr (PAGED) {
+    uint32_t g = 0, first = 0;
+    if (a.groups) g = group_of(a, w.b, first);
+    const int32_t row = row_number(a.k, w.b);
+    table = a.k.table + (row_ok(a.k, row) ? row : 0) * a.k.table_stride;
+    if (a.groups) {
+      const int32_t first_row = row_number(a.k, first), prefix = a.prefix[g];
+      const int32_t len = row_length(a.k, row), first_len = row_length(a.k, first_row);
+      nk = uni(length_or_report(a.k, row, len));
+      begin = min(nk, uni(whole_pages(a.k, first_row, first_len, prefix)));
+    }
+    early = table[min((begin + t_first * kRowKeys + (lane & 1u) * 16) >> a.k.page_shift, a.k.max_pages - 1)];
+    if (!a.groups) nk = uni(length_or_report(a.k, row, row_length(a.k, row)));
+  } else if (a.k.cu_k == a.cu_q && a.k.total_k >= a.T) {
+    nk = w.nq;
+    w.key0 = w.q0;
+  } else {
+    nk = uni(span(a.k.cu_k, w.b, a.k.total_k, w.key0));
+    w.key0 = uni(w.key0);
+  }
+
   uint32_t lim = nk, end = nk, full = nk;  // keys of this lane's row, of any row, of every row
   if (a.causal) {
     auto limit = [&](uint32_t t) {
@@ -749,7 +776,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     end = limit((min(w.r0 + 16, w.R) - 1) / a.G);
   }
   const uint32_t tiles = end > begin ? (end - begin + kRowKeys - 1) / kRowKeys : 0u;
-  const uint32_t active = max(1u, min(pl.splits, (tiles + NW - 1) / NW));
+  const uint32_t active = max(1u, min(pl.splits, (tiles + NW * pl.least - 1) / (NW * pl.least)));
   if (split >= active) return;
 
   const uint16_t* const qp = a.Q + (int64_t)(w.q0 + token) * a.q_row + head * a.q_head + 8 * quad;
@@ -821,7 +848,6 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
 
   f4 o[kDims];
   float m, l;
-  const uint32_t t_first = split * NW + wave;
   // Tile n of this wavefront, from key k0; its V and K are under way. kMore: the next tile's are asked for,
   // V before and K after the first product (which frees the registers), so that every wait but the last
   // leaves a tile in flight. The counts need paths without branches around the copies.
@@ -909,18 +935,26 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     for (int dt = 0; dt < kDims; ++dt) o[dt] = f4{};
     m = kNone;
     l = 0.f;
-    if constexpr (PAGED) pages.start(a.k);
   };
   if (t_first < tiles) {
     uint32_t t = t_first, n = 0;
     start();
+    int32_t now = 0;
+    if constexpr (PAGED) {
+      now = pages.load(a.k, 0);
+      pages.next = pages.load(a.k, 1);
+      const uint32_t key = begin + t * kRowKeys + (lane & 1u) * 16;
+      pages.now = key < nk ? (int32_t)page_or_report(a.k, early) : 0;
+    }
     copy_v(0, begin + t * kRowKeys);
     load_k(0, begin + t * kRowKeys);
+    if constexpr (PAGED) pages.now = pages.held(a.k, 0, now);
     for (; t + stride < tiles; t += stride, ++n) tile(n, begin + t * kRowKeys, std::false_type{}, std::true_type{});
     tile(n, begin + t * kRowKeys, std::false_type{}, std::false_type{});
     // Again, tile by tile, where values are not finite or a row has no weight, as in the tile kernel.
     if (finish()) {
       start();
+      if constexpr (PAGED) pages.start(a.k);
       for (t = t_first, n = 0; t < tiles; t += stride, ++n) {
         if constexpr (PAGED) pages.advance(a.k, n);
         copy_v(n, begin + t * kRowKeys);
@@ -953,6 +987,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   __syncthreads();
 
   const uint32_t rows = min(16u, w.R - w.r0), units = rows * (D / 4);
+  __amdgpu_buffer_rsrc_t po = make_rsrc(pl.o, 0), pm = po;
   auto joined = [&](uint32_t row, uint32_t d, f4& v, float& mc, float& sum) {
     float mx = kNone;
 #pragma unroll
@@ -974,45 +1009,39 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     *reinterpret_cast<u2*>(a.O + (int64_t)tk * a.o_row + hd * a.o_head + d) = u2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
     if (a.lse && d == 0) a.lse[(uint64_t)tk * a.H + hd] = sum == 0.f ? -INFINITY : (mc + __log2f(sum)) * 0.69314718055994530942f;
   };
-  if (active == 1 && pl.prefix.slots == 0) {
+  if (active > 1) {
+    // Parts: the workgroup that arrives last joins them, in the order of their numbers.
+    const uint64_t at = (uint64_t)(idx * a.Hkv + kvh) * pl.splits;
+    po = make_rsrc(pl.o + at * 16 * D, pl.splits * 16 * D * 4);
+    pm = make_rsrc(pl.ml + at * 16, pl.splits * 16 * 8);
     for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
       f4 v;
       float mc, sum;
       const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
       joined(row, d, v, mc, sum);
-      store(row, d, v, mc, sum);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), po, ((split * 16 + row) * D + d) * 4, 0, kAgent);
+      if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, (f2{mc, sum})), pm, (split * 16 + row) * 8, 0, kAgent);
     }
-    return;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      uint32_t* const cnt = pl.cnt + idx * a.Hkv + kvh;
+      const uint32_t last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
+      if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      *flag = last;
+    }
+    __syncthreads();
+    if (!*flag) return;
   }
-  // Parts: the workgroup that arrives last joins them, in the order of their numbers.
-  const uint64_t first = (uint64_t)(idx * a.Hkv + kvh) * pl.splits;
-  const __amdgpu_buffer_rsrc_t po = make_rsrc(pl.o + first * 16 * D, pl.splits * 16 * D * 4);
-  const __amdgpu_buffer_rsrc_t pm = make_rsrc(pl.ml + first * 16, pl.splits * 16 * 8);
-  for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
-    f4 v;
-    float mc, sum;
-    const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
-    joined(row, d, v, mc, sum);
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), po, ((split * 16 + row) * D + d) * 4, 0, kAgent);
-    if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, (f2{mc, sum})), pm, (split * 16 + row) * 8, 0, kAgent);
-  }
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t* const cnt = pl.cnt + idx * a.Hkv + kvh;
-    const uint32_t last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
-    if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *flag = last;
-  }
-  __syncthreads();
-  if (!*flag) return;
+  const uint32_t parts = pl.prefix.slots + (active > 1 ? active : 0u);
   for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
     const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
     const uint32_t rr = w.r0 + row;
     const uint64_t pre = ((uint64_t)(w.q0 + rr / a.G) * a.H + kvh * a.G + rr % a.G) * pl.prefix.slots;
-    const uint32_t parts = pl.prefix.slots + active;
     float mx = kNone, sum = 0.f;
     f4 v = f4{};
+    if (active == 1) joined(row, d, v, mx, sum);
+    if (sum == 0.f) mx = kNone;
     constexpr uint32_t kBatch = 8;
     for (uint32_t p0 = 0; p0 < parts; p0 += kBatch) {
       f2 e[kBatch];
@@ -1128,6 +1157,7 @@ hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
   if (p.row) {
     RowPlan r{};
     r.splits = p.row_splits;
+    r.least = p.row_least;
     r.cnt = reinterpret_cast<uint32_t*>(w);
     r.o = reinterpret_cast<float*>(w + p.row_o);
     r.ml = reinterpret_cast<f2*>(w + p.row_ml);
@@ -1155,6 +1185,12 @@ hipError_t launch_dim(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
   return hipErrorInvalidValue;
 }
 
+#ifndef V_TW
+#define V_TW 2
+#define V_RW 8
+#define V_LT 4
+#endif
+constexpr uint32_t kTileWorkgroups = V_TW, kRowWorkgroups = V_RW, kLeastTiles = V_LT;
 uint32_t up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 }  // namespace
@@ -1179,7 +1215,7 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     const uint32_t keys = p.prefix ? std::max(max_prefix, 1u) : max_keys;
     const uint32_t tiles = up(all_rows, 128) + (p.prefix ? groups : seqs);
     // Workgroups for two on each CU, of 256 keys at least.
-    p.tile_splits = std::min({64u, up(2 * cus, tiles * kv_heads), up(keys, 256)});
+    p.tile_splits = std::min({64u, up(kTileWorkgroups * cus, tiles * kv_heads), up(keys, 256)});
     p.tile_grid = tiles * kv_heads * p.tile_splits;
     if (p.prefix || p.tile_splits > 1) {
       p.tile_slots = p.tile_splits;
@@ -1192,10 +1228,12 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     const uint32_t step = (dim == 256 ? 2u : 4u) * kRowKeys;
     const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
     const uint32_t keys = p.prefix ? std::max(max_keys - std::min(max_prefix, max_keys), 1u) : max_keys;
-    p.row_splits = std::min({64u, up(8 * cus, tiles * kv_heads), up(keys, step)});
-    if ((uint64_t)tiles * kv_heads > kMaxCounters && !p.prefix) p.row_splits = 1;
-    p.row_grid = tiles * kv_heads * p.row_splits;
-    if (p.prefix || p.row_splits > 1) {
+    const uint32_t all = tiles * kv_heads;
+    p.row_least = all >= cus ? kLeastTiles : 1;
+    p.row_splits = std::min({64u, up(kRowWorkgroups * cus, all), up(keys, step * p.row_least)});
+    if (all > kMaxCounters) p.row_splits = 1;
+    p.row_grid = all * p.row_splits;
+    if (p.row_splits > 1) {
       const size_t places = (size_t)tiles * kv_heads * p.row_splits * 16;
       p.row_ml = take(places * sizeof(f2));
       p.row_o = take(places * dim * sizeof(float));
