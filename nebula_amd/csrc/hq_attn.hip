@@ -1187,10 +1187,13 @@ hipError_t launch_dim(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
 
 #ifndef V_TW
 #define V_TW 2
-#define V_RW 8
+#define V_RW 4
 #define V_LT 4
+#define V_LS 2
+#define V_MK 512
 #endif
-constexpr uint32_t kTileWorkgroups = V_TW, kRowWorkgroups = V_RW, kLeastTiles = V_LT;
+constexpr uint32_t kSplitKeys = V_MK;
+constexpr uint32_t kRowWorkgroups = V_RW, kLeastTiles = V_LT;
 uint32_t up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 }  // namespace
@@ -1214,8 +1217,10 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   if (p.tile) {
     const uint32_t keys = p.prefix ? std::max(max_prefix, 1u) : max_keys;
     const uint32_t tiles = up(all_rows, 128) + (p.prefix ? groups : seqs);
-    // Workgroups for two on each CU, of 256 keys at least.
-    p.tile_splits = std::min({64u, up(kTileWorkgroups * cus, tiles * kv_heads), up(keys, 256)});
+    // Workgroups for two on each CU and no more (a third round would be nearly empty), of kSplitKeys at least.
+    const uint32_t n = p.prefix ? groups : seqs, likely = n * up(up(all_rows, n), 128);
+    const uint32_t room = (dim == 256 ? 1 : 2) * cus;
+    p.tile_splits = std::min({64u, std::max(1u, room / (likely * kv_heads)), up(keys, kSplitKeys)});
     p.tile_grid = tiles * kv_heads * p.tile_splits;
     if (p.prefix || p.tile_splits > 1) {
       p.tile_slots = p.tile_splits;
@@ -1229,7 +1234,7 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
     const uint32_t keys = p.prefix ? std::max(max_keys - std::min(max_prefix, max_keys), 1u) : max_keys;
     const uint32_t all = tiles * kv_heads;
-    p.row_least = all >= cus ? kLeastTiles : 1;
+    p.row_least = all >= cus ? kLeastTiles : V_LS;
     p.row_splits = std::min({64u, up(kRowWorkgroups * cus, all), up(keys, step * p.row_least)});
     if (all > kMaxCounters) p.row_splits = 1;
     p.row_grid = all * p.row_splits;
