@@ -45,20 +45,17 @@ __device__ __forceinline__ f16x mfma32x32x16(u4 a, u4 b, f16x c) {
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
 }
-// Transposing reads: four rows of 16 elements, 8 bytes from each lane of 16; lane i gets column i. N
-// fragments of two reads each, from at[i] + OFF and at[i] + OFF + NEXT. In asm, and waited for there,
-// because the compiler holds the builtin back until every copy into LDS under way has landed.
+// Transposing reads: four rows of 16 elements, 8 bytes from each lane of 16; lane i gets column i. A
+// fragment is two of them.
 template <int OFF, int NEXT>
-__device__ __forceinline__ void lds_read_tr(const uint32_t (&at)[2], u4 (&f)[2]) {
-  u2 a, b, c, d;
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
-      "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
-      : "v"(at[0]), "v"(at[1]), "i"(OFF), "i"(OFF + NEXT));
-  f[0] = u4{a[0], a[1], b[0], b[1]};
-  f[1] = u4{c[0], c[1], d[0], d[1]};
+__device__ __forceinline__ u4 lds_read_tr(uint32_t at) {
+  typedef __attribute__((address_space(3))) s4* lds_s4;
+  const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(at + OFF)));
+  const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(at + OFF + NEXT)));
+  return u4{a[0], a[1], b[0], b[1]};
 }
+// Several fragments, in asm and waited for there: the compiler holds the builtin back until every copy
+// into LDS that it knows to be under way has landed.
 template <int OFF, int NEXT>
 __device__ __forceinline__ void lds_read_tr(const uint32_t (&at)[4], u4 (&f)[4]) {
   u2 a, b, c, d, e, g, h, i;
@@ -286,11 +283,21 @@ struct Pages {
 // Keys from `base` (uniform) on, `rows` of them `step` bytes apart (at most 64 and 2^24): what lies past them
 // reads as 0. A lane's offset is 32-bit; the descriptor is made anew for each tile, since a pool or an
 // operand may span more than 4 GiB.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_rsrc(const uint16_t* base, uint32_t rows, uint32_t step) {
-  // Both are uniform; said so, because the compiler multiplies 64-bit numbers in vector registers.
+__device__ __forceinline__ u4 keys_words(const uint16_t* base, uint32_t rows, uint32_t step) {
+  // All are uniform; said so, because the compiler multiplies 64-bit numbers in vector registers.
   const uint64_t p = reinterpret_cast<uint64_t>(base);
-  const uint64_t q = (uint64_t)uni((uint32_t)(p >> 32)) << 32 | uni((uint32_t)p);
-  return make_rsrc(reinterpret_cast<const void*>(q), uni(rows * step));
+  return u4{uni((uint32_t)p), uni((uint32_t)(p >> 32)) & 0xFFFFu, uni(rows * step), (uint32_t)kBufferFlags};
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_rsrc(const uint16_t* base, uint32_t rows, uint32_t step) {
+  const u4 d = keys_words(base, rows, step);
+  return make_rsrc(reinterpret_cast<const void*>((uint64_t)d[1] << 32 | d[0]), d[2]);
+}
+// buffer_to_lds16 of such a descriptor, to LDS address `to` (uniform), unknown to the compiler's counts: it
+// would hold every transposing read back until all copies under way have landed. Whoever uses it waits for
+// its copies itself; the compiler's own waits for loads only become longer by it. It has no destination
+// register.
+__device__ __forceinline__ void copy_to_lds16(u4 d, uint32_t to, uint32_t offset) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "memory");
 }
 
 // ---- parts of rows whose keys are split ----
@@ -410,6 +417,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   const uint32_t k_step = (uint32_t)a.k.k_row * 2, v_step = (uint32_t)a.k.v_row * 2, page_mask = (1u << a.k.page_shift) - 1;
   Pages<kKeys> pages{table, t0 * kKeys, kKeys, nk, 0, 0};
   const bool whole = !PAGED || a.k.page_shift >= 6;  // a tile lies in one page
+  const uint32_t lds0 = uni(lds_address(smem)) + wave * 1024;
   // Offsets of load 0, and of load 1 less its rows: the swizzle of K goes with the row modulo 16, which later
   // loads have in common with one of them.
   uint32_t k_off[2], v_off[2];
@@ -419,32 +427,31 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
     k_off[i] = (wave * kRowsPerLoad + in_row) * k_step + ((in_chunk ^ swz_k<D>(row)) << 4);
     v_off[i] = (wave * kRowsPerLoad + in_row) * v_step + ((in_chunk ^ swz_v<D>(row)) << 4);
   }
-  auto copy = [&](uint32_t t, const uint16_t* from, int64_t row_stride, uint32_t step, const uint32_t (&off)[2], unsigned char* to)
+  auto copy = [&](uint32_t t, const uint16_t* from, int64_t row_stride, uint32_t step, const uint32_t (&off)[2], uint32_t to)
                   __attribute__((always_inline)) {
     const uint32_t key = t * kKeys, left = min(nk - key, (uint32_t)kKeys);
     if (whole) {
       int64_t at;
       if constexpr (PAGED) at = pages.page(t - t0, 0) * a.k.page_stride + (key & page_mask) * row_stride;
       else at = (int64_t)(w.key0 + key) * row_stride;
-      const __amdgpu_buffer_rsrc_t r = keys_rsrc(from + at, left, step);
+      const u4 r = keys_words(from + at, left, step);
 #pragma unroll
-      for (uint32_t i = 0; i < kLoads; ++i)
-        buffer_to_lds16(r, to + (i * NW + wave) * 1024, off[i & 1] + i * NW * kRowsPerLoad * step);
+      for (uint32_t i = 0; i < kLoads; ++i) copy_to_lds16(r, to + i * NW * 1024, off[i & 1] + i * NW * kRowsPerLoad * step);
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < kLoads; ++i) {  // a block of 16 rows each
         const uint32_t row0 = (i * NW + wave) * kRowsPerLoad, first = row0 & ~15u;
         const int64_t at = pages.page(t - t0, row0 / 16) * a.k.page_stride + ((key + first) & page_mask) * row_stride;
-        buffer_to_lds16(keys_rsrc(from + at, left > first ? left - first : 0u, step), to + (i * NW + wave) * 1024,
-                        off[i & 1] + (row0 - first - wave * kRowsPerLoad) * step);
+        copy_to_lds16(keys_words(from + at, left > first ? left - first : 0u, step), to + i * NW * 1024,
+                      off[i & 1] + (row0 - first - wave * kRowsPerLoad) * step);
       }
     }
   };
   auto copy_k = [&](uint32_t t) __attribute__((always_inline)) {
-    copy(t, Kh, a.k.k_row, k_step, k_off, smem + (t & 1u) * kStage);
+    copy(t, Kh, a.k.k_row, k_step, k_off, lds0 + (t & 1u) * kStage);
   };
   auto copy_v = [&](uint32_t t) __attribute__((always_inline)) {
-    copy(t, Vh, a.k.v_row, v_step, v_off, smem + (t & 1u) * kStage + kVOff);
+    copy(t, Vh, a.k.v_row, v_step, v_off, lds0 + (t & 1u) * kStage + kVOff);
   };
 
   // LDS places of this lane's fragments. K^T: row l32 (+ 32), dims 16 s + 8 half, chunk 2 s + half: the place of
@@ -456,7 +463,6 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 
   f16x o[kDims];
   float m, l;
-  constexpr int kBlock = kDims < 4 ? kDims : 4;  // fragments of V^T in registers
 
   auto opaque = [](uint32_t v) __attribute__((always_inline)) {  // what is computed from it stays in its tile
     asm volatile("" : "+v"(v));
@@ -564,15 +570,8 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
       each<4>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::value;
 #pragma unroll
-        for (int d0 = 0; d0 < kDims; d0 += kBlock) {
-          uint32_t at[kBlock];
-          u4 f[kBlock];
-#pragma unroll
-          for (int i = 0; i < kBlock; ++i) at[i] = v0 ^ (uint32_t)((d0 + i) << 6);
-          lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
-#pragma unroll
-          for (int i = 0; i < kBlock; ++i) o[d0 + i] = mfma32x32x16<DT>(f[i], p[j], o[d0 + i]);
-        }
+        for (int dt = 0; dt < kDims; ++dt)
+          o[dt] = mfma32x32x16<DT>(lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(v0 ^ (uint32_t)(dt << 6)), p[j], o[dt]);
         if constexpr (more)
 #pragma unroll
           for (int v = 4 * j; v < 4 * j + 4; ++v) top = fmaxf(fmaxf(top, ns[0][v]), ns[1][v]);
@@ -642,9 +641,9 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
         const u4 sees = {seen2<DT>(key, lim), seen2<DT>(key + 2, lim), seen2<DT>(key + 8, lim), seen2<DT>(key + 10, lim)};
 #pragma unroll
         for (int d0 = 0; d0 < kDims; d0 += 2) {
-          const uint32_t at[2] = {v0 ^ (uint32_t)(d0 << 6), v0 ^ (uint32_t)((d0 + 1) << 6)};
           u4 f[2];
-          lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(at, f);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) f[i] = lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(v0 ^ (uint32_t)((d0 + i) << 6));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             u4 finite, code;
