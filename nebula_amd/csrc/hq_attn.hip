@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 #include <cstdio>
 #include <type_traits>
 
@@ -693,7 +694,6 @@ constexpr int kRowKeys = 32;  // keys of a wavefront's tile
 
 struct RowPlan {
   uint32_t splits;     // workgroups that share the keys of 16 rows, at most
-  uint32_t least;      // tiles of a wavefront before one more takes part
   uint32_t* cnt;       // arrivals of a tile's workgroups, zero between launches
   float* o;            // their parts: [tile][kv head][splits][16][D], and the maxima and sums [..][16]
   f2* ml;
@@ -775,7 +775,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     end = limit((min(w.r0 + 16, w.R) - 1) / a.G);
   }
   const uint32_t tiles = end > begin ? (end - begin + kRowKeys - 1) / kRowKeys : 0u;
-  const uint32_t active = max(1u, min(pl.splits, (tiles + NW * pl.least - 1) / (NW * pl.least)));
+  const uint32_t active = max(1u, min(pl.splits, (tiles + NW - 1) / NW));
   if (split >= active) return;
 
   const uint16_t* const qp = a.Q + (int64_t)(w.q0 + token) * a.q_row + head * a.q_head + 8 * quad;
@@ -1156,7 +1156,6 @@ hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
   if (p.row) {
     RowPlan r{};
     r.splits = p.row_splits;
-    r.least = p.row_least;
     r.cnt = reinterpret_cast<uint32_t*>(w);
     r.o = reinterpret_cast<float*>(w + p.row_o);
     r.ml = reinterpret_cast<f2*>(w + p.row_ml);
@@ -1184,26 +1183,51 @@ hipError_t launch_dim(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
   return hipErrorInvalidValue;
 }
 
-#ifndef V_TW
-#define V_TW 2
-#define V_RW 4
-#define V_LT 4
-#define V_LS 2
-#define V_MK 512
-#endif
-constexpr uint32_t kSplitKeys = V_MK;
-constexpr uint32_t kRowWorkgroups = V_RW, kLeastTiles = V_LT;
 uint32_t up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+// Workgroups that share the keys of a tile of the tile kernel: the number of least time, in us of an MI355X.
+// A tile of 64 keys and 128 dims takes a workgroup 1.3 where it has its CU to itself and two of them 2.0
+// where they share one (heads of 256 never do); parts are written and read at 1 us to 4.5 MB, and the
+// join's launch is 6.5. On a chunk of 64 tokens after 6000, 24 tiles, 1 / 5 / 10 / 12 / 21 / 48 workgroups took
+// 117 / 38 / 30 / 34 / 32 / 54 us (10 chosen); on 512 tokens after 7488, 192 tiles, 1 / 2 / 5 / 8 / 16 took
+// 200 / 148 / 139 / 148 / 185 (5); on a prompt of 512, 1 / 2 / 4 took 18 / 35 / 38 (1).
+uint32_t tile_splits(uint64_t tiles, uint64_t rows, uint32_t dim, uint32_t keys, bool prefix) {
+  const uint32_t steps = up(keys, kKeys), cus = (uint32_t)cu_count();
+  uint32_t best = 1;
+  double least = 0;
+  for (uint32_t s = 1; s <= std::min(64u, steps); ++s) {
+    const uint64_t each = up(tiles * s, cus), pairs = dim == 256 ? 0 : each / 2;
+    double t = up(steps, s) * (dim / 128.) * (2.0 * pairs + 1.3 * (each - 2 * pairs));
+    if (prefix || s > 1) t += rows * s * dim * 4. / 4.5e6 + 6.5;
+    if (s == 1 || t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+// Workgroups that share the keys of a tile of the row kernel: no more than two a CU in one round (LDS holds
+// two), nor than pay for their parts, which the last of them reads alone: sqrt(keys / 32). Ragged rows up to
+// 8192 on heads of 256, 64 tiles: 4 / 8 / 10 / 16 took 53 / 35 / 43 / 40 us (8 chosen); 4 rows on 16384, 32
+// tiles, 4 / 8 / 16 / 32 took 58 / 51 / 54 / 62 (16); one row on 16384, 8 tiles, 8 / 16 / 24 / 48 took
+// 28 / 20 / 21 / 25 (23); 64 rows on 2048, 512 tiles, 1 / 2 / 4 took 94 / 101 / 105 (1).
+uint32_t row_splits(uint32_t tiles, uint32_t dim, uint32_t keys) {
+  const uint32_t step = (dim == 256 ? 2u : 4u) * kRowKeys;  // a tile for each wavefront
+  if (tiles > kMaxCounters) return 1;
+  return std::min({64u, std::max(1u, 2 * (uint32_t)cu_count() / tiles), up(keys, step), (uint32_t)std::ceil(std::sqrt(keys / 32.))});
+}
 
 }  // namespace
 
 AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                    uint32_t max_keys, uint32_t max_prefix) {
   AttnPlan p{};
-  const uint32_t G = heads / kv_heads, cus = (uint32_t)cu_count();
+  const uint32_t G = heads / kv_heads;
   const uint64_t all_rows = (uint64_t)rows * G;
   p.prefix = kind == HQ_ATTN_SHARED;
-  // Few rows a sequence: tiles of 16.
+  // Few rows a sequence: tiles of 16. 16 sequences of 48 rows on up to 3000 keys took 34 us in tiles of 128 and 49
+  // in tiles of 16, 8 of 24 rows 24 in both.
   p.row = p.prefix || all_rows <= 32ull * seqs;
   p.tile = p.prefix || !p.row;
   max_keys = std::max(max_keys, 1u);
@@ -1216,10 +1240,9 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   if (p.tile) {
     const uint32_t keys = p.prefix ? std::max(max_prefix, 1u) : max_keys;
     const uint32_t tiles = up(all_rows, 128) + (p.prefix ? groups : seqs);
-    // Workgroups for two on each CU and no more (a third round would be nearly empty), of kSplitKeys at least.
+    // The sequences' lengths are not known here: as if all were alike.
     const uint32_t n = p.prefix ? groups : seqs, likely = n * up(up(all_rows, n), 128);
-    const uint32_t room = (dim == 256 ? 1 : 2) * cus;
-    p.tile_splits = std::min({64u, std::max(1u, room / (likely * kv_heads)), up(keys, kSplitKeys)});
+    p.tile_splits = tile_splits((uint64_t)likely * kv_heads, (uint64_t)rows * heads, dim, keys, p.prefix);
     p.tile_grid = tiles * kv_heads * p.tile_splits;
     if (p.prefix || p.tile_splits > 1) {
       p.tile_slots = p.tile_splits;
@@ -1229,13 +1252,10 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     }
   }
   if (p.row) {
-    const uint32_t step = (dim == 256 ? 2u : 4u) * kRowKeys;
     const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
     const uint32_t keys = p.prefix ? std::max(max_keys - std::min(max_prefix, max_keys), 1u) : max_keys;
     const uint32_t all = tiles * kv_heads;
-    p.row_least = all >= cus ? kLeastTiles : V_LS;
-    p.row_splits = std::min({64u, up(kRowWorkgroups * cus, all), up(keys, step * p.row_least)});
-    if (all > kMaxCounters) p.row_splits = 1;
+    p.row_splits = row_splits(all, dim, keys);
     p.row_grid = all * p.row_splits;
     if (p.row_splits > 1) {
       const size_t places = (size_t)tiles * kv_heads * p.row_splits * 16;
