@@ -17,8 +17,11 @@ Rows are independent, so a step's rows may be any mix of decode tokens and prefi
 (the split-fuse batch of hydrogen/src/batcher/split_fuse.cpp:110-159: the decode streams'
 tokens first, then one prefill chunk); the library picks its streaming (decode) kernels for
 up to 80 rows and its prefill kernels above. `StepRows` builds such a batch's activation
-matrix and splits the outputs back per chunk. Normalisation, attention, the SSM step and SwiGLU stay with the
-caller: they are not projections.
+matrix and splits the outputs back per chunk. Between q | k | v and attn_output, `LayerProjections.attend`
+keeps the keys and values in a paged cache and computes the attention (nebula_amd.attn) of the step's
+decode tokens, over a shared prefix where they have one, and of its prefill chunk; `StepCache` holds what
+a step's layers have in common. Normalisation, rotation and gating of the query, the SSM step and SwiGLU stay
+with the caller.
 
 Activations are fp16 or bf16 (the reference's are fp32); the ternary weights and their
 per-block scales are kept exactly (group = 256, one scale per TQ1_0 block).
@@ -28,7 +31,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
-from . import hq
+from . import attn, hq
 
 # Dimensions of the reference's 27B model (hydrogen/include/native_decoder.hpp:180-188).
 EMBEDDING = 5120
@@ -36,6 +39,7 @@ FFN = 17408
 Q_OUT = 12288
 KV_OUT = 1024
 MIXER_IN = 6144      # attn_output / ssm_out input width
+HEADS, KV_HEADS, HEAD_DIM = 24, 4, 256   # MIXER_IN = 24 x 256, KV_OUT = 4 x 256; q holds the query and its gate
 SSM_GATE = 6144
 SSM_QKV = 10240
 TQ1_GROUP = 256
@@ -97,6 +101,37 @@ class LayerProjections:
         """attn_output or ssm_out (6144 -> 5120)."""
         return self._fused(FUSED_GROUPS[self.kind][1], y, None if out is None else [out], stream)[0]
 
+    def attend(self, x_norm, cache: "attn.KVCache", cache_layer: int, step: "StepCache", prepare=None, gate=None, stream=None):
+        """The attention mixer of one layer over a step's rows: mixer_in, the new keys and values to layer
+        cache_layer of the cache, attention of the decode rows and of the prefill chunks, mixer_out.
+
+        prepare(q_out, k, v) makes the query and key heads of the projections' outputs ([M, 12288], [M,
+        1024], [M, 1024]): q [M, 24, 256], k and v [M, 4, 256], normalised and rotated as the model has it
+        (default: the first half of q_out, k and v as they are). gate(y, q_out) is what goes to mixer_out in
+        y's place (default: y, [M, 6144]). step.reserve(cache) comes first, once for all layers."""
+        if self.kind != "attention":
+            raise ValueError(f"attend() is the attention mixer's, the layer's kind is {self.kind!r}")
+        M = step.M
+        if x_norm.shape[0] != M:
+            raise ValueError(f"x_norm has {x_norm.shape[0]} rows, the step {M}")
+        q_out, k, v = self.mixer_in(x_norm, stream=stream)
+        if prepare is None:
+            q = q_out[:, :MIXER_IN].unflatten(1, (HEADS, HEAD_DIM))
+            k, v = (t.unflatten(1, (KV_HEADS, HEAD_DIM)) for t in (k, v))
+        else:
+            q, k, v = prepare(q_out, k, v)
+        cache.append(cache_layer, k, v, step.rows, step.cu, stream=stream)
+        y = q.new_empty((M, HEADS, HEAD_DIM))
+        n = step.decodes
+        if n and step.prefix is not None:
+            attn.shared_prefix(q[:n], cache, cache_layer, step.decode_rows, *step.prefix, max_len=step.max_len, out=y[:n], stream=stream)
+        elif n:
+            attn.paged(q[:n], cache, cache_layer, step.decode_rows, max_len=step.max_len, out=y[:n], stream=stream)
+        if M > n:
+            attn.paged(q[n:], cache, cache_layer, step.chunk_rows, step.chunk_cu, max_len=step.max_len, out=y[n:], stream=stream)
+        y = y.flatten(1)
+        return self.mixer_out(y if gate is None else gate(y, q_out), stream=stream)
+
     def ffn_in(self, x_norm, outs=None, stream=None) -> List:
         """[gate, up] — one fused call."""
         return self._fused(FUSED_GROUPS["ffn"][0], x_norm, outs, stream)
@@ -148,6 +183,45 @@ class StepRows:
     def split(self, Y) -> Dict[int, object]:
         """Output rows back per request (views into Y)."""
         return {c.request_id: Y[o:o + c.num_tokens] for c, o in zip(self.chunks, self.offsets)}
+
+
+class StepCache:
+    """The cache rows of a step, made once and used by each of its layers. row_of[request_id] is a request's
+    row of the cache. groups: lists of the step's decode requests, in its order and all of them, with the
+    number of first tokens that each list's rows share (as cache.fork leaves them): [([request_id, ..],
+    prefix), ..]."""
+
+    def __init__(self, rows: StepRows, row_of: Dict[int, int], groups=None, device="cuda"):
+        import torch
+
+        counts = [c.num_tokens for c in rows.chunks]
+        self.M, self.decodes = rows.M, sum(not c.is_prefill for c in rows.chunks)
+        held = [row_of[c.request_id] for c in rows.chunks]
+        if len(set(held)) != len(held):
+            raise ValueError(f"two chunks of a step have the same cache row: {held}")
+        cu = rows.offsets + [rows.M]
+        self.max_len = max((c.start_token + c.num_tokens for c in rows.chunks), default=0)
+        self.prefix = None
+        starts, lens = [0], []
+        if groups is not None:
+            flat = [r for ids, _ in groups for r in ids]
+            if flat != [c.request_id for c in rows.chunks[:self.decodes]]:
+                raise ValueError(f"groups hold requests {flat}, the step decodes {[c.request_id for c in rows.chunks[:self.decodes]]}")
+            for ids, n in groups:
+                starts.append(starts[-1] + len(ids))
+                lens.append(n)
+        # One copy to the device for all lists.
+        chunk_cu = [c - self.decodes for c in cu[self.decodes:]]
+        parts = [held, counts, cu, chunk_cu, starts, lens]
+        both = torch.tensor([x for p in parts for x in p], dtype=torch.int32).to(device)
+        self.rows, self.counts, self.cu, self.chunk_cu, starts_t, lens_t = both.split([len(p) for p in parts])
+        self.decode_rows, self.chunk_rows = self.rows[:self.decodes], self.rows[self.decodes:]
+        if lens:
+            self.prefix = (starts_t, lens_t, max(lens))
+
+    def reserve(self, cache: "attn.KVCache", stream=None) -> None:
+        """Room in the cache for the step's tokens: once, before its first layer."""
+        cache.reserve(self.rows, self.counts, stream=stream)
 
 
 def random_tq1_0(K: int, N: int, generator=None, device="cuda"):
