@@ -141,7 +141,41 @@ __device__ __forceinline__ void report(uint32_t* status, uint32_t what) {
   __hip_atomic_fetch_or(status, what, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ uint32_t clamp_u(int32_t v, uint32_t hi) { return v < 0 ? 0u : min((uint32_t)v, hi); }
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// f over the lanes up to each one, by moves inside rows of 16 lanes and then from row to row: a shuffle through
+// LDS takes ten times as long, and a call begins with several of these one after the other.
+template <class F>
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t none, F f) {
+#define HQ_SCAN_STEP(CTRL, ROWS) x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xF, false))
+  HQ_SCAN_STEP(0x111, 0xF);  // from the lane 1, 2, 4, 8 below
+  HQ_SCAN_STEP(0x112, 0xF);
+  HQ_SCAN_STEP(0x114, 0xF);
+  HQ_SCAN_STEP(0x118, 0xF);
+  HQ_SCAN_STEP(0x142, 0xA);  // lane 15 of a row to the next one: rows 1 and 3
+  HQ_SCAN_STEP(0x143, 0xC);  // lane 31: rows 2 and 3
+#undef HQ_SCAN_STEP
+  return x;
+}
+__device__ __forceinline__ uint32_t scan_sum(uint32_t x) {
+  return scan(x, 0, [](uint32_t a, uint32_t b) { return a + b; });
+}
+__device__ __forceinline__ uint32_t sum_lanes(uint32_t x) { return lane_value(scan_sum(x), 63); }
+__device__ __forceinline__ uint32_t min_lanes(uint32_t x) {
+  return lane_value(scan(x, ~0u, [](uint32_t a, uint32_t b) { return min(a, b); }), 63);
+}
+__device__ __forceinline__ uint32_t max_lanes(uint32_t x) {
+  return lane_value(scan(x, 0, [](uint32_t a, uint32_t b) { return max(a, b); }), 63);
+}
+// f of the values of the lanes that are 16, 32 and 48 away.
+template <class F>
+__device__ __forceinline__ float over_quads(float x, F f) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // ---- sequences ----
 // The loads that a workgroup starts with depend on each other (offsets, a row's number, its length, its
@@ -200,23 +234,101 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_
     uint32_t first = 0, nq = 0;
     if (b < n) nq = span(cu, b, most, first);
     const uint32_t tiles = (nq * G + rows - 1) / rows;
-    uint32_t x = tiles;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-      const uint32_t y = __shfl_up(x, d);
-      if (lane >= d) x += y;
-    }
+    const uint32_t x = scan_sum(tiles);
     const uint64_t past = __ballot(before + x > idx);
     if (past) {
       const int at = __builtin_ctzll(past);
       w.b = base + at;
-      w.q0 = uni(__shfl(first, at));
-      w.nq = uni(__shfl(nq, at));
+      w.q0 = lane_value(first, at);
+      w.nq = lane_value(nq, at);
       w.R = w.nq * G;
-      w.r0 = (uni(__shfl(before + x, at)) - 1 - idx) * rows;
+      w.r0 = (before + lane_value(x, at) - 1 - idx) * rows;
       return true;
     }
-    before += uni(__shfl(x, 63));
+    before += lane_value(x, 63);
+  }
+  return false;
+}
+
+// Work of slot `slot` of `slots` where rows' keys are shared between workgroups (row kernel): the tiles of 16
+// rows get slots by the keys they have, so that a batch of long and short rows ends together. A share is
+// `unit` tiles of 32 keys, the least of three that the slots are enough for: sum / slots, where rounding up may
+// cost more than there are; sum / (slots - tiles), where it can't; their mean. No tile has more shares than
+// sqrt(its key tiles): the last workgroup reads the others' parts alone.
+struct Share {
+  uint32_t split, of;  // this workgroup's number among those of its tile
+  int32_t row, len;    // paged: cache row of the sequence, and its length as read
+};
+template <uint32_t WAVES, bool PAGED>
+__device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t slots, uint32_t like, uint32_t slot, Work& w, Share& sh) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t first, nq, tiles, keys;
+  int32_t row, len;
+  auto entry = [&](uint32_t b) __attribute__((always_inline)) {
+    first = nq = keys = 0;
+    row = len = 0;
+    if (b < a.B) {
+      if constexpr (PAGED) row = row_number(a.k, b);
+      if (a.cu_q) {
+        nq = span(a.cu_q, b, a.T, first);
+      } else {
+        first = b;
+        nq = 1;
+      }
+      if constexpr (PAGED) {
+        len = row_length(a.k, row);
+        keys = a.groups ? like : clamp_u(len, a.k.max_pages << a.k.page_shift);  // of a group: all alike
+      } else if (a.k.cu_k == a.cu_q && a.k.total_k >= a.T) {
+        keys = nq;
+      } else {
+        uint32_t k0;
+        keys = span(a.k.cu_k, b, a.k.total_k, k0);
+      }
+    }
+    tiles = (nq * a.G + 15) / 16;
+    keys = min((keys + 31) / 32, 1u << 22);  // tiles of them
+  };
+  auto shares = [&](uint32_t unit) __attribute__((always_inline)) {
+    const uint32_t most = (uint32_t)__builtin_ceilf(__builtin_amdgcn_sqrtf((float)keys));
+    return max(1u, min(min((keys + unit - 1) / unit, most), 64u));
+  };
+  uint32_t all = 0, work = 0;
+  for (uint32_t base = 0; base < a.B; base += 64) {
+    entry(base + lane);
+    all += sum_lanes(tiles);
+    work += sum_lanes(tiles * keys);
+  }
+  uint32_t unit = 1u << 22;  // lists that are not offsets may name more tiles than there can be: one share each
+  if (all < slots) {
+    const uint32_t lo = max((work + slots - 1) / slots, WAVES), hi = max((work + slots - all - 1) / (slots - all), lo), mid = (lo + hi) / 2;
+    uint32_t got = 0;
+    for (uint32_t base = 0; base < a.B; base += 64) {
+      if (a.B > 64) entry(base + lane);
+      got += sum_lanes(tiles * shares(lo) << 16 | tiles * shares(mid));
+    }
+    unit = got >> 16 <= slots ? lo : (got & 0xFFFFu) <= slots ? mid : hi;
+  }
+  uint32_t before = 0;
+  for (uint32_t base = 0; base < a.B; base += 64) {
+    if (a.B > 64) entry(base + lane);
+    const uint32_t each = shares(unit), mine = tiles * each;
+    const uint32_t x = scan_sum(mine);
+    const uint64_t past = __ballot(before + x > slot);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const uint32_t off = slot - before - lane_value(x - mine, at);
+      w.b = base + at;
+      w.q0 = lane_value(first, at);
+      w.nq = lane_value(nq, at);
+      w.R = w.nq * a.G;
+      sh.of = lane_value(each, at);
+      w.r0 = off / sh.of * 16;
+      sh.split = off % sh.of;
+      sh.row = (int32_t)lane_value((uint32_t)row, at);
+      sh.len = (int32_t)lane_value((uint32_t)len, at);
+      return true;
+    }
+    before += lane_value(x, 63);
   }
   return false;
 }
@@ -385,14 +497,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
       lim = n < 0 ? 0u : (uint32_t)n;
     }
   }
-  uint32_t lim_min = lim, lim_max = lim;
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    lim_min = min(lim_min, (uint32_t)__shfl_xor((int)lim_min, d));
-    lim_max = max(lim_max, (uint32_t)__shfl_xor((int)lim_max, d));
-  }
-  lim_min = uni(lim_min);
-  lim_max = w.r0 + wave * 32 < w.R ? uni(lim_max) : 0u;
+  const uint32_t lim_min = min_lanes(lim), lim_max = w.r0 + wave * 32 < w.R ? max_lanes(lim) : 0u;
 
   // Keys of this workgroup: up to the last that any of its rows sees.
   uint32_t wg_lim = nk;
@@ -693,9 +798,11 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 constexpr int kRowKeys = 32;  // keys of a wavefront's tile
 
 struct RowPlan {
-  uint32_t splits;     // workgroups that share the keys of 16 rows, at most
-  uint32_t* cnt;       // arrivals of a tile's workgroups, zero between launches
-  float* o;            // their parts: [tile][kv head][splits][16][D], and the maxima and sums [..][16]
+  uint32_t slots;      // workgroups of a kv head where they share rows' keys (0: a workgroup for each 16 rows)
+  uint32_t one;        // there is one tile, all slots are its shares
+  uint32_t like;       // keys past the prefix that a group's rows are taken to have
+  uint32_t* cnt;       // arrivals of a tile's workgroups, [kv head][its first slot], zero between launches
+  float* o;            // their parts: [kv head][slot][16][D], and the maxima and sums [..][16]
   f2* ml;
   Parts prefix;        // parts of the shared prefix, from the tile kernel (slots 0: none)
 };
@@ -706,14 +813,11 @@ __device__ __forceinline__ uint32_t swz_rv(uint32_t r) {
   return D == 64 ? ((r >> 1) & 3u) << 1 : (r & 7u) << 1;
 }
 
-template <int D>
-constexpr uint32_t row_waves() {
-  return D == 256 ? 2u : 4u;
-}
+constexpr uint32_t kRowWaves = 4;
 // Two stages of V per wavefront; the join of the wavefronts lies over them.
 template <int D>
 constexpr uint32_t row_lds_bytes() {
-  const uint32_t stages = row_waves<D>() * 2u * (kRowKeys * D * 2u), join = row_waves<D>() * 16u * ((D + 4u) * 4u + 8u);
+  const uint32_t stages = kRowWaves * 2u * (kRowKeys * D * 2u), join = kRowWaves * 16u * ((D + 4u) * 4u + 8u);
   return (stages > join ? stages : join) + 16u;
 }
 constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on other XCDs
@@ -723,8 +827,8 @@ constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on othe
 // lane's 16 bytes of a row are 8 consecutive dims, four lanes take 64 bytes), its V through LDS; both are a
 // tile ahead.
 template <int DT, int D, bool PAGED>
-__global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnArgs a, RowPlan pl) {
-  constexpr uint32_t NW = row_waves<D>();
+__global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a, RowPlan pl) {
+  constexpr uint32_t NW = kRowWaves;
   constexpr uint32_t kPitch = 2 * D, kStage = kRowKeys * kPitch;
   constexpr int kSteps = D / 32, kDims = D / 16;
   constexpr uint32_t kRowsPerLoad = 1024 / kPitch, kLoads = kRowKeys / kRowsPerLoad;
@@ -732,10 +836,21 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
 
   const uint32_t lane = threadIdx.x & 63u, wave = uni(threadIdx.x >> 6);
   const uint32_t l16 = lane & 15u, quad = lane >> 4;
-  const uint32_t kvh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
-  const uint32_t split = rest % pl.splits, idx = rest / pl.splits;
+  const uint32_t kvh = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
   Work w{};
-  if (!find_tile(a.cu_q, a.B, a.T, a.G, 16, idx, w)) return;
+  Share sh{0, 1, 0, 0};
+  const bool find = pl.slots && !pl.one;
+  if (find) {
+    if (!find_share<NW, PAGED>(a, pl.slots, pl.like, slot, w, sh)) return;
+  } else {
+    if (!find_tile(a.cu_q, a.B, a.T, a.G, 16, pl.one ? 0u : slot, w)) return;
+    if (pl.one) {
+      sh.split = slot;
+      sh.of = pl.slots;
+    }
+    if constexpr (PAGED) sh.row = row_number(a.k, w.b);
+  }
+  const uint32_t split = sh.split;
   const uint32_t r_mine = w.r0 + l16;
   const uint32_t r = min(r_mine, w.R - 1), token = r / a.G, head = kvh * a.G + (r - token * a.G);
   const uint32_t t_first = split * NW + wave;
@@ -746,16 +861,17 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   if constexpr (PAGED) {
     uint32_t g = 0, first = 0;
     if (a.groups) g = group_of(a, w.b, first);
-    const int32_t row = row_number(a.k, w.b);
+    const int32_t row = sh.row;
     table = a.k.table + (row_ok(a.k, row) ? row : 0) * a.k.table_stride;
+    if (!find) sh.len = row_length(a.k, row);
     if (a.groups) {
       const int32_t first_row = row_number(a.k, first), prefix = a.prefix[g];
-      const int32_t len = row_length(a.k, row), first_len = row_length(a.k, first_row);
-      nk = uni(length_or_report(a.k, row, len));
+      const int32_t first_len = row_length(a.k, first_row);
+      nk = uni(length_or_report(a.k, row, sh.len));
       begin = min(nk, uni(whole_pages(a.k, first_row, first_len, prefix)));
     }
     early = table[min((begin + t_first * kRowKeys + (lane & 1u) * 16) >> a.k.page_shift, a.k.max_pages - 1)];
-    if (!a.groups) nk = uni(length_or_report(a.k, row, row_length(a.k, row)));
+    if (!a.groups) nk = uni(length_or_report(a.k, row, sh.len));
   } else if (a.k.cu_k == a.cu_q && a.k.total_k >= a.T) {
     nk = w.nq;
     w.key0 = w.q0;
@@ -775,7 +891,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     end = limit((min(w.r0 + 16, w.R) - 1) / a.G);
   }
   const uint32_t tiles = end > begin ? (end - begin + kRowKeys - 1) / kRowKeys : 0u;
-  const uint32_t active = max(1u, min(pl.splits, (tiles + NW - 1) / NW));
+  const uint32_t active = max(1u, min(sh.of, (tiles + NW - 1) / NW));
   if (split >= active) return;
 
   const uint16_t* const qp = a.Q + (int64_t)(w.q0 + token) * a.q_row + head * a.q_head + 8 * quad;
@@ -875,8 +991,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
           if (k0 + 16 * kt + 4 * quad + v >= lim) s[kt][v] = -INFINITY;
     }
     float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = over_quads(top, [](float x, float y) { return fmaxf(x, y); });
     if (__any((top - m) * c > Weights<DT>::kLag)) {
       const float n = (top - m) * c > Weights<DT>::kLag ? top : m, al = __builtin_amdgcn_exp2f((m - n) * c);
       m = n;
@@ -920,8 +1035,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     }
   };
   auto finish = [&]() {
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = over_quads(l, [](float x, float y) { return x + y; });
     float bad = 0.f;
 #pragma unroll
     for (int dt = 0; dt < kDims; ++dt)
@@ -1010,9 +1124,9 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
   };
   if (active > 1) {
     // Parts: the workgroup that arrives last joins them, in the order of their numbers.
-    const uint64_t at = (uint64_t)(idx * a.Hkv + kvh) * pl.splits;
-    po = make_rsrc(pl.o + at * 16 * D, pl.splits * 16 * D * 4);
-    pm = make_rsrc(pl.ml + at * 16, pl.splits * 16 * 8);
+    const uint64_t at = kvh * pl.slots + slot - split;
+    po = make_rsrc(pl.o + at * 16 * D, sh.of * 16 * D * 4);
+    pm = make_rsrc(pl.ml + at * 16, sh.of * 16 * 8);
     for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
       f4 v;
       float mc, sum;
@@ -1024,7 +1138,7 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
-      uint32_t* const cnt = pl.cnt + idx * a.Hkv + kvh;
+      uint32_t* const cnt = pl.cnt + kvh * pl.slots + slot - split;
       const uint32_t last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
       if (last) __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       *flag = last;
@@ -1032,47 +1146,59 @@ __global__ __launch_bounds__(row_waves<D>() * 64) void hq_attn_row_kernel(AttnAr
     __syncthreads();
     if (!*flag) return;
   }
-  const uint32_t parts = pl.prefix.slots + (active > 1 ? active : 0u);
   for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
     const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
     const uint32_t rr = w.r0 + row;
-    const uint64_t pre = ((uint64_t)(w.q0 + rr / a.G) * a.H + kvh * a.G + rr % a.G) * pl.prefix.slots;
     float mx = kNone, sum = 0.f;
     f4 v = f4{};
     if (active == 1) joined(row, d, v, mx, sum);
     if (sum == 0.f) mx = kNone;
-    constexpr uint32_t kBatch = 8;
-    for (uint32_t p0 = 0; p0 < parts; p0 += kBatch) {
-      f2 e[kBatch];
-      f4 x[kBatch];
+    // N parts from number p on, of n: what lies past the last is read again and left out.
+    auto add = [&](auto batch, uint32_t p, uint32_t n, auto stat_of, auto o_of) __attribute__((always_inline)) {
+      constexpr int N = decltype(batch)::value;
+      f2 e[N];
+      f4 x[N];
 #pragma unroll
-      for (uint32_t i = 0; i < kBatch; ++i) {
-        const uint32_t p = p0 + i, s = p - pl.prefix.slots;
-        e[i] = f2{kNone, 0.f};
-        x[i] = f4{};
-        if (p < pl.prefix.slots) {
-          e[i] = pl.prefix.ml[pre + p];
-          x[i] = *reinterpret_cast<const f4*>(pl.prefix.o + (pre + p) * D + d);
-        } else if (p < parts) {
-          e[i] = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(pm, (s * 16 + row) * 8, 0, kAgent));
-          x[i] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(po, ((s * 16 + row) * D + d) * 4, 0, kAgent));
-        }
+      for (int i = 0; i < N; ++i) {
+        const uint32_t at = min(p + i, n - 1);
+        e[i] = stat_of(at);
+        x[i] = o_of(at);
       }
-      float n = mx;
+      float top = mx;
 #pragma unroll
-      for (uint32_t i = 0; i < kBatch; ++i) n = e[i][1] != 0.f ? fmaxf(n, e[i][0]) : n;
-      const float f = __builtin_amdgcn_exp2f(mx - n);
-      mx = n;
+      for (int i = 0; i < N; ++i) {
+        if (p + i >= n) e[i][1] = 0.f;
+        top = e[i][1] != 0.f ? fmaxf(top, e[i][0]) : top;
+      }
+      const float f = __builtin_amdgcn_exp2f(mx - top);
+      mx = top;
       sum *= f;
       v *= f;
 #pragma unroll
-      for (uint32_t i = 0; i < kBatch; ++i) {
-        const float g = __builtin_amdgcn_exp2f(e[i][0] - n);
+      for (int i = 0; i < N; ++i) {
+        const float g = __builtin_amdgcn_exp2f(e[i][0] - top);
         if (e[i][1] != 0.f) {  // a part without weight left its O unwritten
           sum = fmaf(e[i][1], g, sum);
           v += x[i] * g;
         }
       }
+    };
+    if (pl.prefix.slots) {
+      const uint64_t pre = ((uint64_t)(w.q0 + rr / a.G) * a.H + kvh * a.G + rr % a.G) * pl.prefix.slots;
+      for (uint32_t p = 0; p < pl.prefix.slots; p += 8)
+        add(Int<8>{}, p, pl.prefix.slots, [&](uint32_t i) { return pl.prefix.ml[pre + i]; },
+            [&](uint32_t i) { return *reinterpret_cast<const f4*>(pl.prefix.o + (pre + i) * D + d); });
+    }
+    if (active > 1) {
+      auto own_stat = [&](uint32_t i) {
+        return __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(pm, (i * 16 + row) * 8, 0, kAgent));
+      };
+      auto own_o = [&](uint32_t i) {
+        return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(po, ((i * 16 + row) * D + d) * 4, 0, kAgent));
+      };
+      if (active <= 8) add(Int<8>{}, 0, active, own_stat, own_o);
+      else
+        for (uint32_t p = 0; p < active; p += 16) add(Int<16>{}, p, active, own_stat, own_o);
     }
     store(row, d, v, mx, sum);
   }
@@ -1155,7 +1281,9 @@ hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
   }
   if (p.row) {
     RowPlan r{};
-    r.splits = p.row_splits;
+    r.slots = p.row_slots;
+    r.one = p.row_one;
+    r.like = p.row_like;
     r.cnt = reinterpret_cast<uint32_t*>(w);
     r.o = reinterpret_cast<float*>(w + p.row_o);
     r.ml = reinterpret_cast<f2*>(w + p.row_ml);
@@ -1164,7 +1292,7 @@ hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
     constexpr uint32_t lds = row_lds_bytes<D>();
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (set != hipSuccess) return set;
-    hipLaunchKernelGGL(k, dim3(p.row_grid), dim3(row_waves<D>() * 64), lds, s, a, r);
+    hipLaunchKernelGGL(k, dim3(p.row_grid), dim3(kRowWaves * 64), lds, s, a, r);
     return hipGetLastError();
   }
   if (p.tile_slots) {
@@ -1207,15 +1335,12 @@ uint32_t tile_splits(uint64_t tiles, uint64_t rows, uint32_t dim, uint32_t keys,
   return best;
 }
 
-// Workgroups that share the keys of a tile of the row kernel: no more than two a CU in one round (LDS holds
-// two), nor than pay for their parts, which the last of them reads alone: sqrt(keys / 32). Ragged rows up to
-// 8192 on heads of 256, 64 tiles: 4 / 8 / 10 / 16 took 53 / 35 / 43 / 40 us (8 chosen); 4 rows on 16384, 32
-// tiles, 4 / 8 / 16 / 32 took 58 / 51 / 54 / 62 (16); one row on 16384, 8 tiles, 8 / 16 / 24 / 48 took
-// 28 / 20 / 21 / 25 (23); 64 rows on 2048, 512 tiles, 1 / 2 / 4 took 94 / 101 / 105 (1).
-uint32_t row_splits(uint32_t tiles, uint32_t dim, uint32_t keys) {
-  const uint32_t step = (dim == 256 ? 2u : 4u) * kRowKeys;  // a tile for each wavefront
-  if (tiles > kMaxCounters) return 1;
-  return std::min({64u, std::max(1u, 2 * (uint32_t)cu_count() / tiles), up(keys, step), (uint32_t)std::ceil(std::sqrt(keys / 32.))});
+// Workgroups of a kv head that share rows' keys in the row kernel: as many as LDS holds in one round, no
+// more than pay for their parts (find_share). 0: a workgroup for each 16 rows.
+uint32_t row_slots(uint32_t tiles, uint32_t kv_heads, uint32_t dim, uint32_t keys) {
+  const uint64_t useful = (uint64_t)tiles * std::min(up(keys, kRowWaves * kRowKeys), (uint32_t)std::ceil(std::sqrt(up(keys, kRowKeys))));
+  const uint32_t slots = (uint32_t)std::min<uint64_t>(useful, (dim == 256 ? 1 : 2) * (uint32_t)cu_count() / kv_heads);
+  return slots > tiles && slots * kv_heads <= kMaxCounters ? slots : 0;
 }
 
 }  // namespace
@@ -1254,11 +1379,12 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   if (p.row) {
     const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
     const uint32_t keys = p.prefix ? std::max(max_keys - std::min(max_prefix, max_keys), 1u) : max_keys;
-    const uint32_t all = tiles * kv_heads;
-    p.row_splits = row_splits(all, dim, keys);
-    p.row_grid = all * p.row_splits;
-    if (p.row_splits > 1) {
-      const size_t places = (size_t)tiles * kv_heads * p.row_splits * 16;
+    p.row_slots = row_slots(tiles, kv_heads, dim, keys);
+    p.row_one = p.row_slots && tiles == 1;
+    p.row_like = keys;
+    p.row_grid = (p.row_slots ? p.row_slots : tiles) * kv_heads;
+    if (p.row_slots) {
+      const size_t places = (size_t)p.row_slots * kv_heads * 16;
       p.row_ml = take(places * sizeof(f2));
       p.row_o = take(places * dim * sizeof(float));
     }
@@ -1270,7 +1396,7 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
 void describe_attn(const AttnPlan& p, char* buf, size_t len) {
   char t[160] = "", r[160] = "";
   if (p.tile) std::snprintf(t, sizeof t, "hq_attn_tile_kernel%s grid=%u splits=%u", p.prefix ? "<prefix>" : "", p.tile_grid, p.tile_splits);
-  if (p.row) std::snprintf(r, sizeof r, "hq_attn_row_kernel grid=%u splits=%u", p.row_grid, p.row_splits);
+  if (p.row) std::snprintf(r, sizeof r, "hq_attn_row_kernel grid=%u%s", p.row_grid, p.row_slots ? " shared" : "");
   std::snprintf(buf, len, "%s%s%s%s ws=%zu", t, p.tile && p.row ? ", " : "", r, p.tile_slots && !p.prefix ? ", hq_attn_join_kernel" : "", p.ws);
 }
 

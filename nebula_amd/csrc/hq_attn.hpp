@@ -45,7 +45,8 @@ struct AttnPlan {
   bool tile = false, row = false;  // the kernels that run
   bool prefix = false;             // the tile kernel over shared prefixes, the row kernel over the rest
   uint32_t tile_grid = 0, tile_splits = 0;
-  uint32_t row_grid = 0, row_splits = 0;
+  uint32_t row_grid = 0;
+  uint32_t row_slots = 0, row_one = 0, row_like = 0;  // workgroups of a kv head that share rows' keys (0: none share), keys of a row past its prefix
   uint32_t tile_slots = 0;         // parts of a row that the tile kernel leaves (0: none, it writes O)
   size_t tile_ml = 0, tile_o = 0, row_ml = 0, row_o = 0, ws = 0;  // workspace offsets, and its size
 };
