@@ -449,7 +449,7 @@ constexpr uint32_t tile_stage_bytes() {
 }
 
 template <int DT, int D, int NW, bool PAGED>
-__global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel(AttnArgs a, TilePlan pl) {
+__device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl, uint32_t block) {
   constexpr uint32_t BR = NW * 32;
   constexpr uint32_t kPitch = 2 * D, kStage = tile_stage_bytes<D>(), kVOff = kStage / 2;
   constexpr int kSteps = D / 16, kDims = D / 32;
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
 
   // Heads run fastest: workgroups go to the XCDs in turn, so with eight key/value heads each XCD's L2
   // sees the keys of one.
-  const uint32_t kvh = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv;
+  const uint32_t kvh = block % a.Hkv, rest = block / a.Hkv;
   const uint32_t split = rest % pl.splits, idx = rest / pl.splits;
   Work w{};
   if (!find_tile(pl.prefix ? a.starts : a.cu_q, pl.prefix ? a.groups : a.B, pl.prefix ? a.B : a.T, a.G, BR, idx, w)) return;
@@ -794,6 +794,11 @@ __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel
   if (a.lse && half == 0) a.lse[(uint64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (mc + __log2f(l)) * 0.69314718055994530942f;
 }
 
+template <int DT, int D, int NW, bool PAGED>
+__global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel(AttnArgs a, TilePlan pl) {
+  tile_body<DT, D, NW, PAGED>(a, pl, blockIdx.x);
+}
+
 // ---- few rows ----
 constexpr int kRowKeys = 32;  // keys of a wavefront's tile
 
@@ -804,7 +809,7 @@ struct RowPlan {
   uint32_t* cnt;       // arrivals of a tile's workgroups, [kv head][its first slot], zero between launches
   float* o;            // their parts: [kv head][slot][16][D], and the maxima and sums [..][16]
   f2* ml;
-  Parts prefix;        // parts of the shared prefix, from the tile kernel (slots 0: none)
+  Parts to;            // where rows of a group leave their own keys' part, the last place (slots 0: rows are written out)
 };
 
 // As swz_v, for this kernel's reads: 16 rows of 32 bytes.
@@ -827,7 +832,7 @@ constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on othe
 // lane's 16 bytes of a row are 8 consecutive dims, four lanes take 64 bytes), its V through LDS; both are a
 // tile ahead.
 template <int DT, int D, bool PAGED>
-__global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a, RowPlan pl) {
+__device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, uint32_t block) {
   constexpr uint32_t NW = kRowWaves;
   constexpr uint32_t kPitch = 2 * D, kStage = kRowKeys * kPitch;
   constexpr int kSteps = D / 32, kDims = D / 16;
@@ -836,7 +841,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
 
   const uint32_t lane = threadIdx.x & 63u, wave = uni(threadIdx.x >> 6);
   const uint32_t l16 = lane & 15u, quad = lane >> 4;
-  const uint32_t kvh = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
+  const uint32_t kvh = block % a.Hkv, slot = block / a.Hkv;
   Work w{};
   Share sh{0, 1, 0, 0};
   const bool find = pl.slots && !pl.one;
@@ -1117,6 +1122,12 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
   };
   auto store = [&](uint32_t row, uint32_t d, f4 v, float mc, float sum) {
     const uint32_t rr = w.r0 + row, tk = w.q0 + rr / a.G, hd = kvh * a.G + rr % a.G;
+    if (pl.to.slots) {
+      const uint64_t at = ((uint64_t)tk * a.H + hd) * pl.to.slots + pl.to.slots - 1;
+      if (d == 0) pl.to.ml[at] = f2{mc, sum};
+      *reinterpret_cast<f4*>(pl.to.o + at * D + d) = v;
+      return;
+    }
     if (sum == 0.f) v = f4{};
     else v *= 1.f / sum;
     *reinterpret_cast<u2*>(a.O + (int64_t)tk * a.o_row + hd * a.o_head + d) = u2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
@@ -1148,7 +1159,6 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
   }
   for (uint32_t u = threadIdx.x; u < units; u += NW * 64) {
     const uint32_t row = u / (D / 4), d = (u % (D / 4)) * 4;
-    const uint32_t rr = w.r0 + row;
     float mx = kNone, sum = 0.f;
     f4 v = f4{};
     if (active == 1) joined(row, d, v, mx, sum);
@@ -1183,12 +1193,6 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
         }
       }
     };
-    if (pl.prefix.slots) {
-      const uint64_t pre = ((uint64_t)(w.q0 + rr / a.G) * a.H + kvh * a.G + rr % a.G) * pl.prefix.slots;
-      for (uint32_t p = 0; p < pl.prefix.slots; p += 8)
-        add(Int<8>{}, p, pl.prefix.slots, [&](uint32_t i) { return pl.prefix.ml[pre + i]; },
-            [&](uint32_t i) { return *reinterpret_cast<const f4*>(pl.prefix.o + (pre + i) * D + d); });
-    }
     if (active > 1) {
       auto own_stat = [&](uint32_t i) {
         return __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(pm, (i * 16 + row) * 8, 0, kAgent));
@@ -1204,7 +1208,21 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
   }
 }
 
-// ---- joining the parts of the tile kernel ----
+template <int DT, int D, bool PAGED>
+__global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a, RowPlan pl) {
+  row_body<DT, D, PAGED>(a, pl, blockIdx.x);
+}
+
+// ---- shared prefixes ----
+// Groups' prefixes in tiles of many rows and what their sequences have past them in tiles of few are one
+// launch: the first is bound by its products and the second by memory, and neither has workgroups enough.
+template <int DT, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void hq_attn_prefix_kernel(AttnArgs a, TilePlan t, RowPlan r, uint32_t tile_blocks) {
+  if (blockIdx.x < tile_blocks) tile_body<DT, D, 4, true>(a, t, blockIdx.x);
+  else row_body<DT, D, true>(a, r, blockIdx.x - tile_blocks);
+}
+
+// ---- joining parts ----
 template <int DT, int D>
 __global__ __launch_bounds__(256) void hq_attn_join_kernel(AttnArgs a, Parts parts) {
   constexpr int E = D / 64;
@@ -1260,46 +1278,53 @@ __global__ __launch_bounds__(256) void hq_attn_join_kernel(AttnArgs a, Parts par
   if (a.lse && lane == 0) a.lse[u] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f;
 }
 
+uint32_t up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+template <class K, class... Args>
+hipError_t launch_lds(K k, uint32_t grid, uint32_t lds, hipStream_t s, Args... args) {
+  hipLaunchKernelGGL(k, dim3(grid), dim3(256), lds, s, args...);
+  return hipGetLastError();
+}
+
 template <int DT, int D, bool PAGED>
 hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_t s) {
   unsigned char* const w = static_cast<unsigned char*>(ws);
-  Parts parts{};  // of the tile kernel
-  if (p.tile_slots) {
-    parts.slots = p.tile_slots;
-    parts.ml = reinterpret_cast<f2*>(w + p.tile_ml);
-    parts.o = reinterpret_cast<float*>(w + p.tile_o);
+  Parts parts{};
+  if (p.parts) {
+    parts.slots = p.parts;
+    parts.ml = reinterpret_cast<f2*>(w + p.part_ml);
+    parts.o = reinterpret_cast<float*>(w + p.part_o);
   }
-  if (p.tile) {
-    const TilePlan t{p.tile_splits, p.prefix, parts};
+  const TilePlan t{p.tile_splits, p.prefix, parts};
+  RowPlan r{};
+  r.slots = p.row_slots;
+  r.one = p.row_one;
+  r.like = p.row_like;
+  r.cnt = reinterpret_cast<uint32_t*>(w);
+  r.o = reinterpret_cast<float*>(w + p.row_o);
+  r.ml = reinterpret_cast<f2*>(w + p.row_ml);
+  if (p.prefix) r.to = parts;
+  constexpr uint32_t tile_lds = 2 * tile_stage_bytes<D>(), row_lds = row_lds_bytes<D>();
+  auto allow = [](const void* k, uint32_t lds) { return hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, lds); };
+  hipError_t e = hipSuccess;
+  if (p.prefix) {
+    if constexpr (PAGED) {
+      auto k = hq_attn_prefix_kernel<DT, D>;
+      constexpr uint32_t lds = std::max(tile_lds, row_lds);
+      static const hipError_t set = allow(reinterpret_cast<const void*>(k), lds);
+      e = set != hipSuccess ? set : launch_lds(k, p.tile_grid + p.row_grid, lds, s, a, t, r, p.tile_grid);
+    }
+  } else if (p.tile) {
     auto k = hq_attn_tile_kernel<DT, D, 4, PAGED>;
-    constexpr uint32_t lds = 2 * tile_stage_bytes<D>();
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (set != hipSuccess) return set;
-    hipLaunchKernelGGL(k, dim3(p.tile_grid), dim3(256), lds, s, a, t);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (p.row) {
-    RowPlan r{};
-    r.slots = p.row_slots;
-    r.one = p.row_one;
-    r.like = p.row_like;
-    r.cnt = reinterpret_cast<uint32_t*>(w);
-    r.o = reinterpret_cast<float*>(w + p.row_o);
-    r.ml = reinterpret_cast<f2*>(w + p.row_ml);
-    if (p.prefix) r.prefix = parts;
+    static const hipError_t set = allow(reinterpret_cast<const void*>(k), tile_lds);
+    e = set != hipSuccess ? set : launch_lds(k, p.tile_grid, tile_lds, s, a, t);
+  } else {
     auto k = hq_attn_row_kernel<DT, D, PAGED>;
-    constexpr uint32_t lds = row_lds_bytes<D>();
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (set != hipSuccess) return set;
-    hipLaunchKernelGGL(k, dim3(p.row_grid), dim3(kRowWaves * 64), lds, s, a, r);
-    return hipGetLastError();
+    static const hipError_t set = allow(reinterpret_cast<const void*>(k), row_lds);
+    e = set != hipSuccess ? set : launch_lds(k, p.row_grid, row_lds, s, a, r);
   }
-  if (p.tile_slots) {
-    hipLaunchKernelGGL((hq_attn_join_kernel<DT, D>), dim3((uint32_t)(((uint64_t)a.T * a.H + 3) / 4)), dim3(256), 0, s, a, parts);
-    return hipGetLastError();
-  }
-  return hipSuccess;
+  if (e == hipSuccess && p.parts) e = launch_lds(hq_attn_join_kernel<DT, D>, up((uint64_t)a.T * a.H, 4), 0, s, a, parts);
+  return e;
 }
 
 template <int DT>
@@ -1311,8 +1336,6 @@ hipError_t launch_dim(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
   return hipErrorInvalidValue;
 }
 
-uint32_t up(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
-
 // Workgroups that share the keys of a tile of the tile kernel: the number of least time, in us of an MI355X.
 // A tile of 64 keys and 128 dims takes a workgroup 1.3 where it has its CU to itself and two of them 2.0
 // where they share one (heads of 256 never do); parts are written and read at 1 us to 4.5 MB, and the
@@ -1323,7 +1346,7 @@ uint32_t tile_splits(uint64_t tiles, uint64_t rows, uint32_t dim, uint32_t keys,
   const uint32_t steps = up(keys, kKeys), cus = (uint32_t)cu_count();
   uint32_t best = 1;
   double least = 0;
-  for (uint32_t s = 1; s <= std::min(64u, steps); ++s) {
+  for (uint32_t s = 1; s <= std::min(63u, steps); ++s) {
     const uint64_t each = up(tiles * s, cus), pairs = dim == 256 ? 0 : each / 2;
     double t = up(steps, s) * (dim / 128.) * (2.0 * pairs + 1.3 * (each - 2 * pairs));
     if (prefix || s > 1) t += rows * s * dim * 4. / 4.5e6 + 6.5;
@@ -1370,10 +1393,10 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     p.tile_splits = tile_splits((uint64_t)likely * kv_heads, (uint64_t)rows * heads, dim, keys, p.prefix);
     p.tile_grid = tiles * kv_heads * p.tile_splits;
     if (p.prefix || p.tile_splits > 1) {
-      p.tile_slots = p.tile_splits;
-      const size_t places = (size_t)rows * heads * p.tile_slots;
-      p.tile_ml = take(places * sizeof(f2));
-      p.tile_o = take(places * dim * sizeof(float));
+      p.parts = p.tile_splits + (p.prefix ? 1 : 0);
+      const size_t places = (size_t)rows * heads * p.parts;
+      p.part_ml = take(places * sizeof(f2));
+      p.part_o = take(places * dim * sizeof(float));
     }
   }
   if (p.row) {
@@ -1394,10 +1417,13 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
 }
 
 void describe_attn(const AttnPlan& p, char* buf, size_t len) {
-  char t[160] = "", r[160] = "";
-  if (p.tile) std::snprintf(t, sizeof t, "hq_attn_tile_kernel%s grid=%u splits=%u", p.prefix ? "<prefix>" : "", p.tile_grid, p.tile_splits);
-  if (p.row) std::snprintf(r, sizeof r, "hq_attn_row_kernel grid=%u%s", p.row_grid, p.row_slots ? " shared" : "");
-  std::snprintf(buf, len, "%s%s%s%s ws=%zu", t, p.tile && p.row ? ", " : "", r, p.tile_slots && !p.prefix ? ", hq_attn_join_kernel" : "", p.ws);
+  const char* const shared = p.row_slots ? " shared" : "";
+  char k[200];
+  if (p.prefix)
+    std::snprintf(k, sizeof k, "hq_attn_prefix_kernel grid=%u+%u splits=%u%s", p.tile_grid, p.row_grid, p.tile_splits, shared);
+  else if (p.tile) std::snprintf(k, sizeof k, "hq_attn_tile_kernel grid=%u splits=%u", p.tile_grid, p.tile_splits);
+  else std::snprintf(k, sizeof k, "hq_attn_row_kernel grid=%u%s", p.row_grid, shared);
+  std::snprintf(buf, len, "%s%s ws=%zu", k, p.parts ? ", hq_attn_join_kernel" : "", p.ws);
 }
 
 hipError_t launch_attn(int dtype, const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_t s) {

@@ -43,12 +43,12 @@ struct AttnArgs {
 // How a call is split, from host-side sizes alone (the lengths stay on the device).
 struct AttnPlan {
   bool tile = false, row = false;  // the kernels that run
-  bool prefix = false;             // the tile kernel over shared prefixes, the row kernel over the rest
+  bool prefix = false;             // both in one launch: tiles of many rows over shared prefixes, of few over the rest
   uint32_t tile_grid = 0, tile_splits = 0;
   uint32_t row_grid = 0;
   uint32_t row_slots = 0, row_one = 0, row_like = 0;  // workgroups of a kv head that share rows' keys (0: none share), keys of a row past its prefix
-  uint32_t tile_slots = 0;         // parts of a row that the tile kernel leaves (0: none, it writes O)
-  size_t tile_ml = 0, tile_o = 0, row_ml = 0, row_o = 0, ws = 0;  // workspace offsets, and its size
+  uint32_t parts = 0;              // parts of a row that are joined by a launch of their own (0: rows are written out)
+  size_t part_ml = 0, part_o = 0, row_ml = 0, row_o = 0, ws = 0;  // workspace offsets, and its size
 };
 AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                    uint32_t dim, uint32_t max_keys, uint32_t max_prefix);
