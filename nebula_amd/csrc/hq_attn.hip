@@ -626,7 +626,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
   if (t1 > t0) {
     // The scores of a tile are computed while the weights of the one before are, and its maximum while that
     // one's second product runs: the matrix and the vector pipes each have the other's work beside theirs.
-    f16x s[2];
+    f16x s0[2], s1[2];  // of a tile and of the next, in turn
     copy_k(t0);
     copy_v(t0);
     if (t0 + 1 < t1) {
@@ -637,20 +637,19 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
     if (t0 < tw) {
       const uint32_t at = opaque(k_at + (t0 & 1u) * kStage);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) scores(at, s, i);
-      if (t0 * kKeys + kKeys > lim_min) mask(t0, s);
-      float top = s[0][0];
+      for (int i = 0; i < kSteps; ++i) scores(at, s0, i);
+      if (t0 * kKeys + kKeys > lim_min) mask(t0, s0);
+      float top = s0[0][0];
 #pragma unroll
-      for (int v = 0; v < 16; ++v) top = fmaxf(fmaxf(top, s[0][v]), s[1][v]);
+      for (int v = 0; v < 16; ++v) top = fmaxf(fmaxf(top, s0[0][v]), s0[1][v]);
       follow(top);
     }
-    auto tile = [&](uint32_t t, auto next) __attribute__((always_inline)) {
+    auto tile = [&](uint32_t t, auto next, f16x (&s)[2], f16x (&ns)[2]) __attribute__((always_inline)) {
       constexpr bool more = decltype(next)::value;  // the next tile is this wavefront's too
       // With and without a next tile are two pieces of code: what they share is not taken out of them.
       if constexpr (more) asm volatile("" : "+v"(s[0]), "+v"(s[1]));
       const float mc = fmaxf(m * c, kNone) - Weights<DT>::kLift;
       u4 p[4];
-      f16x ns[2];
       float sum = 0.f;
       const uint32_t at = opaque(k_at + ((t + 1) & 1u) * kStage);
 #pragma unroll
@@ -682,13 +681,9 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
 #pragma unroll
           for (int v = 4 * j; v < 4 * j + 4; ++v) top = fmaxf(fmaxf(top, ns[0][v]), ns[1][v]);
       });
-      if constexpr (more) {
-        follow(top);
-        s[0] = ns[0];
-        s[1] = ns[1];
-      }
+      if constexpr (more) follow(top);
     };
-    for (uint32_t t = t0; t < t1; ++t) {
+    auto ahead = [&](uint32_t t) __attribute__((always_inline)) {  // copies of the next tiles, before tile t
       if (t > t0) meet();
       else __builtin_amdgcn_s_barrier();  // every wavefront has its scores of t0: its K may be overwritten
       if (t + 1 < t1) copy_v(t + 1);
@@ -696,9 +691,26 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
         if constexpr (PAGED) pages.advance(a.k, t + 2 - t0);
         copy_k(t + 2);
       }
-      if (t + 1 < tw) tile(t, std::true_type{});
-      else if (t < tw) tile(t, std::false_type{});
+    };
+    uint32_t t = t0;
+    for (; t + 2 < tw; t += 2) {
+      ahead(t);
+      tile(t, std::true_type{}, s0, s1);
+      ahead(t + 1);
+      tile(t + 1, std::true_type{}, s1, s0);
     }
+    if (t + 1 < tw) {
+      ahead(t);
+      tile(t, std::true_type{}, s0, s1);
+      ahead(++t);
+      tile(t, std::false_type{}, s1, s0);
+      ++t;
+    } else if (t < tw) {
+      ahead(t);
+      tile(t, std::false_type{}, s0, s1);
+      ++t;
+    }
+    for (; t < t1; ++t) ahead(t);  // the others' tiles
   }
   // Again where values are not finite, or a row has no weight: V at keys a row may not see, times its weight
   // 0, may have made them, or scores past 1e7. Tile by tile, differences of scores before the factor (m c may
