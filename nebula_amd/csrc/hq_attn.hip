@@ -580,6 +580,11 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
     for (int kt = 0; kt < 2; ++kt)
       s[kt] = mfma32x32x16<DT>(*reinterpret_cast<const u4*>(p + kt * 32 * kPitch), q[i], i ? s[kt] : f16x{});
   };
+  auto k_read = [&](uint32_t at, u4 (&f)[2], int i) __attribute__((always_inline)) {
+    const unsigned char* const p = smem + (at ^ (uint32_t)(i << 5));
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) f[kt] = *reinterpret_cast<const u4*>(p + kt * 32 * kPitch);
+  };
   auto mask = [&](uint32_t t, f16x (&s)[2]) __attribute__((always_inline)) {
     const uint32_t k0 = t * kKeys + 4 * half;
 #pragma unroll
@@ -652,9 +657,15 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
       u4 p[4];
       float sum = 0.f;
       const uint32_t at = opaque(k_at + ((t + 1) & 1u) * kStage);
+      u4 kf[2][2];
+      if constexpr (more) k_read(at, kf[0], 0);
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        if constexpr (more) scores(at, ns, i);
+        if constexpr (more) {
+          if (i + 1 < kSteps) k_read(at, kf[(i + 1) & 1], i + 1);
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) ns[kt] = mfma32x32x16<DT>(kf[i & 1][kt], q[i], i ? ns[kt] : f16x{});
+        }
 #pragma unroll
         for (int u = 16 * i / kSteps; u < 16 * (i + 1) / kSteps; ++u) {  // weights 2 u, 2 u + 1 of 32
           const int v = 2 * (u & 7);
