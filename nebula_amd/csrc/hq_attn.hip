@@ -679,18 +679,28 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
       if constexpr (more) {
         // Both stay above, in turn.
         asm volatile("" : "+v"(ns[0]), "+v"(ns[1]), "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
-        if ((t + 1) * kKeys + kKeys > lim_min) mask(t + 1, ns);
       }
-      float top = more ? ns[0][0] : 0.f;
+      // Products of a fragment of V each, read two of them ahead.
+      constexpr int kAll = 4 * kDims, kAhead = 2;
       const uint32_t v0 = opaque(v_at + (t & 1u) * kStage);
-      each<4>([&](auto jc) __attribute__((always_inline)) {
-        constexpr int j = decltype(jc)::value;
-#pragma unroll
-        for (int dt = 0; dt < kDims; ++dt)
-          o[dt] = mfma32x32x16<DT>(lds_read_tr<16 * j * (int)kPitch, 8 * (int)kPitch>(v0 ^ (uint32_t)(dt << 6)), p[j], o[dt]);
+      u4 vf[kAhead];
+      auto v_read = [&](auto nc) __attribute__((always_inline)) {
+        constexpr int n = decltype(nc)::value;
+        vf[n % kAhead] = lds_read_tr<16 * (n / kDims) * (int)kPitch, 8 * (int)kPitch>(v0 ^ (uint32_t)(n % kDims << 6));
+      };
+      each<kAhead>(v_read);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (more)
+        if ((t + 1) * kKeys + kKeys > lim_min) mask(t + 1, ns);
+      float top = more ? ns[0][0] : 0.f;
+      each<kAll>([&](auto nc) __attribute__((always_inline)) {
+        constexpr int n = decltype(nc)::value;
+        o[n % kDims] = mfma32x32x16<DT>(vf[n % kAhead], p[n / kDims], o[n % kDims]);
+        if constexpr (n + kAhead < kAll) v_read(Int<n + kAhead>{});
         if constexpr (more)
 #pragma unroll
-          for (int v = 4 * j; v < 4 * j + 4; ++v) top = fmaxf(fmaxf(top, ns[0][v]), ns[1][v]);
+          for (int v = 16 * n / kAll; v < 16 * (n + 1) / kAll; ++v) top = fmaxf(fmaxf(top, ns[0][v]), ns[1][v]);
+        __builtin_amdgcn_sched_barrier(0);
       });
       if constexpr (more) follow(top);
     };
