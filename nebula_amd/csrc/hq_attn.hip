@@ -673,6 +673,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
           sum += x + y;
           p[u / 4][u & 3] = pack2<DT>(x, y);
         }
+        asm volatile("" : "+v"(sum));  // added here, not in a row afterwards
         __builtin_amdgcn_sched_barrier(0);
       }
       l += sum;
