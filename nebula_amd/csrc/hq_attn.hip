@@ -1371,19 +1371,20 @@ hipError_t launch_dim(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
 }
 
 // Workgroups that share the keys of a tile of the tile kernel: the number of least time, in us of an MI355X.
-// A tile of 64 keys and 128 dims takes a workgroup 1.3 where it has its CU to itself and two of them 2.0
-// where they share one (heads of 256 never do); parts are written and read at 1 us to 4.5 MB, and the
-// join's launch is 6.5. On a chunk of 64 tokens after 6000, 24 tiles, 1 / 5 / 10 / 12 / 21 / 48 workgroups took
-// 117 / 38 / 30 / 34 / 32 / 54 us (10 chosen); on 512 tokens after 7488, 192 tiles, 1 / 2 / 5 / 8 / 16 took
-// 200 / 148 / 139 / 148 / 185 (5); on a prompt of 512, 1 / 2 / 4 took 18 / 35 / 38 (1).
+// A tile of 64 keys and 128 dims takes a workgroup 1.2 where it has its CU to itself and two of them 1.9
+// where they share one (heads of 256 never do). Parts are written and read at 1 us to 4.5 MB, to 1.3 MB beside the
+// row workgroups of a shared prefix, and the join's launch is 6.5. On a chunk of 64 tokens after 6000, 24 tiles,
+// 1 / 5 / 10 / 12 / 21 / 48 workgroups took 110 / 37 / 29 / 33 / 31 / 52 us (10 chosen); on 512 tokens after 7488, 192
+// tiles, 1 / 2 / 4 / 8 / 16 took 195 / 146 / 139 / 142 / 184 (4); on a prompt of 512, 1 / 2 / 4 took 16 / 33 / 37 (1);
+// on a prefix of 2000 under 5 groups of 20 rows, 1 / 2 / 4 / 6 / 12 took 66 / 40 / 29 / 34 / 39 (4).
 uint32_t tile_splits(uint64_t tiles, uint64_t rows, uint32_t dim, uint32_t keys, bool prefix) {
   const uint32_t steps = up(keys, kKeys), cus = (uint32_t)cu_count();
   uint32_t best = 1;
   double least = 0;
   for (uint32_t s = 1; s <= std::min(63u, steps); ++s) {
     const uint64_t each = up(tiles * s, cus), pairs = dim == 256 ? 0 : each / 2;
-    double t = up(steps, s) * (dim / 128.) * (2.0 * pairs + 1.3 * (each - 2 * pairs));
-    if (prefix || s > 1) t += rows * s * dim * 4. / 4.5e6 + 6.5;
+    double t = up(steps, s) * (dim / 128.) * (1.9 * pairs + 1.2 * (each - 2 * pairs));
+    if (prefix || s > 1) t += rows * s * dim * 4. / (prefix ? 1.3e6 : 4.5e6) + 6.5;
     if (s == 1 || t < least) {
       least = t;
       best = s;
