@@ -13,7 +13,9 @@
 //   keys, copied into LDS one tile ahead.
 // hq_attn_row_kernel: few rows (16) over many keys, as in decode steps: each wavefront takes tiles of
 //   32 keys of its own, and the wavefronts' results are joined at the end.
+// hq_attn_prefix_kernel: both in one launch, for rows that share a prefix.
 // hq_attn_join_kernel: joins the parts of rows whose keys were split between workgroups.
+// Times in comments are an MI355X's, of calls replayed from a graph.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -251,7 +253,8 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_
 }
 
 // Work of slot `slot` of `slots` where rows' keys are shared between workgroups (row kernel): the tiles of 16
-// rows get slots by the keys they have, so that a batch of long and short rows ends together. A share is
+// rows get slots by the keys they have, so that a batch of long and short rows ends together (32 rows of 30 to 8000
+// tokens: 50 us, with equal shares 65; the search costs a uniform batch 0.5). A share is
 // `unit` tiles of 32 keys, the least of three that the slots are enough for: sum / slots, where rounding up may
 // cost more than there are; sum / (slots - tiles), where it can't; their mean. No tile has more shares than
 // sqrt(its key tiles): the last workgroup reads the others' parts alone.
@@ -441,6 +444,16 @@ __device__ __forceinline__ uint32_t swz_v(uint32_t r) {
 }
 
 // ---- many rows ----
+// 4 operations a score and dim: bound by the matrix pipe, and as much by what feeds it. A fragment of K or
+// V (1 KB from LDS) is one product of 32 rows, 32 cycles of LDS for the CU's four SIMDs and 32 of each
+// one's matrix pipe; 32 scores a lane are about as many cycles of the vector pipe as their 16 + 16 products at
+// 128 dims. So the three run side by side: the next tile's scores beside this one's exponentials, K fragments
+// read a step and V fragments two products ahead. 8192 tokens on 48/8 heads of 128, bf16: 777 us, 1062
+// TFLOP/s, matrix, LDS and vector pipes busy 62, 62 and 57% at the 1.6 GHz that the card holds under it, no bank
+// conflicts. Heads of 256 leave registers for one wavefront a SIMD (a workgroup a CU): 2048 + 1531 tokens on 24/4
+// heads 111 us, 724 TFLOP/s, matrix pipe 33%; tiles of 32 keys 10% slower there and everywhere, of 128 on heads
+// of 64 slower too. A workgroup alone on its CU takes 1.1 us a tile, 0.9 without its copies: the rest is issue and
+// latency, so short calls gain by sharing keys (tile_splits).
 constexpr int kKeys = 64;  // keys of a tile
 
 template <int D>
@@ -861,10 +874,11 @@ constexpr uint32_t row_lds_bytes() {
 }
 constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on other XCDs
 
-// Tiles of 32 keys go to the splits' wavefronts in turn, (round * splits + split) * NW + wavefront, so that
-// any lengths are shared evenly. A wavefront's K goes straight into the registers of its first product (a
-// lane's 16 bytes of a row are 8 consecutive dims, four lanes take 64 bytes), its V through LDS; both are a
-// tile ahead.
+// Tiles of 32 keys go to the shares' wavefronts in turn, (round * shares + share) * 4 + wavefront. A wavefront's
+// K goes straight into the registers of its first product (a lane's 16 bytes of a row are 8 consecutive dims,
+// four lanes take 64 bytes), its V through LDS; both are a tile ahead, 32 KB a CU and more in flight. Bound by memory:
+// 64 rows on 2048 tokens, 48/8 heads of 128, 94 us, 5.7 TB/s of keys and values; 16 rows on 37 to 8192, 24/4 heads of
+// 256, 27 us, 4.0 TB/s (two wavefronts a workgroup, twice the parts to join by half the threads: 41). One row on 777: 8 us of launch, first loads, parts and join.
 template <int DT, int D, bool PAGED>
 __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, uint32_t block) {
   constexpr uint32_t NW = kRowWaves;
@@ -1249,7 +1263,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
 
 // ---- shared prefixes ----
 // Groups' prefixes in tiles of many rows and what their sequences have past them in tiles of few are one
-// launch: the first is bound by its products and the second by memory, and neither has workgroups enough.
+// launch: the first is bound by its products and the second by memory, and neither has workgroups enough. In
+// two launches 64 rows after 4011 took 34.7 us for 31.6, 16 after 8192 28.8 for 22.7, 128 of 2 groups after 32768 165
+// for 158.
 template <int DT, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void hq_attn_prefix_kernel(AttnArgs a, TilePlan t, RowPlan r, uint32_t tile_blocks) {
   if (blockIdx.x < tile_blocks) tile_body<DT, D, 4, true>(a, t, blockIdx.x);
@@ -1257,6 +1273,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void hq_attn_prefix_kernel(A
 }
 
 // ---- joining parts ----
+// A wavefront a row and head, bound by the parts' way through memory: 15.7 MB in 5.6 us.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void hq_attn_join_kernel(AttnArgs a, Parts parts) {
   constexpr int E = D / 64;
