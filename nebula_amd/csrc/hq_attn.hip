@@ -719,8 +719,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
       if constexpr (more) follow(top);
     };
     auto ahead = [&](uint32_t t) __attribute__((always_inline)) {  // copies of the next tiles, before tile t
-      if (t > t0) meet();
-      else __builtin_amdgcn_s_barrier();  // every wavefront has its scores of t0: its K may be overwritten
+      meet();
       if (t + 1 < t1) copy_v(t + 1);
       if (t + 2 < t1) {
         if constexpr (PAGED) pages.advance(a.k, t + 2 - t0);
@@ -746,6 +745,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
       ++t;
     }
     for (; t < t1; ++t) ahead(t);  // the others' tiles
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the last one asked for none)
   }
   // Again where values are not finite, or a row has no weight: V at keys a row may not see, times its weight
   // 0, may have made them, or scores past 1e7. Tile by tile, differences of scores before the factor (m c may
