@@ -448,7 +448,7 @@ __device__ __forceinline__ uint32_t swz_v(uint32_t r) {
 // V (1 KB from LDS) is one product of 32 rows, 32 cycles of LDS for the CU's four SIMDs and 32 of each
 // one's matrix pipe; 32 scores a lane are about as many cycles of the vector pipe as their 16 + 16 products at
 // 128 dims. So the three run side by side: the next tile's scores beside this one's exponentials, K fragments
-// read a step and V fragments two products ahead. 8192 tokens on 48/8 heads of 128, bf16: 777 us, 1062
+// read a step and V fragments two products ahead. 8192 tokens on 48/8 heads of 128, bf16: 736 us, 1120
 // TFLOP/s, matrix, LDS and vector pipes busy 62, 62 and 57% at the 1.6 GHz that the card holds under it, no bank
 // conflicts. Heads of 256 leave registers for one wavefront a SIMD (a workgroup a CU): 2048 + 1531 tokens on 24/4
 // heads 111 us, 724 TFLOP/s, matrix pipe 33%; tiles of 32 keys 10% slower there and everywhere, of 128 on heads
@@ -670,6 +670,10 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
       u4 p[4];
       float sum = 0.f;
       const uint32_t at = opaque(k_at + ((t + 1) & 1u) * kStage);
+      // The SIMD's other wavefront yields to scores and exponentials, which use both pipes: 8192 tokens on heads of
+      // 128 752 -> 736 us, ragged prompts 38.4 -> 37.8. On heads of 64 it took 60.8 for 57.7 and 83.6 for
+      // 86.4; on heads of 256 there is no other.
+      if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
       u4 kf[2][2];
       if constexpr (more) k_read(at, kf[0], 0);
 #pragma unroll
@@ -689,6 +693,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
         asm volatile("" : "+v"(sum));  // added here, not in a row afterwards
         __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (D == 128) __builtin_amdgcn_s_setprio(0);
       l += sum;
       if constexpr (more) {
         // Both stay above, in turn.
