@@ -879,11 +879,12 @@ constexpr uint32_t row_lds_bytes() {
 }
 constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on other XCDs
 
-// Tiles of 32 keys go to the shares' wavefronts in turn, (round * shares + share) * 4 + wavefront. A wavefront's
-// K goes straight into the registers of its first product (a lane's 16 bytes of a row are 8 consecutive dims,
-// four lanes take 64 bytes), its V through LDS; both are a tile ahead, 32 KB a CU and more in flight. Bound by memory:
-// 64 rows on 2048 tokens, 48/8 heads of 128, 94 us, 5.7 TB/s of keys and values; 16 rows on 37 to 8192, 24/4 heads of
-// 256, 27 us, 4.0 TB/s (two wavefronts a workgroup, twice the parts to join by half the threads: 41). One row on 777: 8 us of launch, first loads, parts and join.
+// Tiles of 32 keys go to the shares' wavefronts in turn, (round * shares + share) * 4 + wavefront. A
+// wavefront's K goes straight into the registers of its first product (a lane's 16 bytes of a row are 8
+// consecutive dims, four lanes take 64 bytes), its V through LDS; both are a tile ahead, 32 KB a CU and more
+// in flight. Bound by memory: 64 rows on 2048 tokens, 48/8 heads of 128, 94 us, 5.7 TB/s of keys and values; 16
+// rows on 37 to 8192, 24/4 heads of 256, 27 us, 4.0 TB/s (two wavefronts a workgroup, twice the parts to join
+// by half the threads: 41). One row on 777: 8 us of launch, first loads, parts and join.
 template <int DT, int D, bool PAGED>
 __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, uint32_t block) {
   constexpr uint32_t NW = kRowWaves;

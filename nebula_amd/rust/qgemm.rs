@@ -160,7 +160,7 @@ pub struct QgemmError {
     pub message: String,
 }
 
-fn check(status: Status) -> Result<(), QgemmError> {
+pub(crate) fn check(status: Status) -> Result<(), QgemmError> {
     if status == 0 {
         return Ok(());
     }
