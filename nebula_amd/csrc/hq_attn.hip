@@ -146,23 +146,6 @@ __device__ __forceinline__ uint32_t clamp_u(int32_t v, uint32_t hi) { return v <
 __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 __device__ __forceinline__ uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
-// f over the lanes up to each one, by moves inside rows of 16 lanes and then from row to row: a shuffle through
-// LDS takes ten times as long, and a call begins with several of these one after the other.
-template <class F>
-__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t none, F f) {
-#define HQ_SCAN_STEP(CTRL, ROWS) x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xF, false))
-  HQ_SCAN_STEP(0x111, 0xF);  // from the lane 1, 2, 4, 8 below
-  HQ_SCAN_STEP(0x112, 0xF);
-  HQ_SCAN_STEP(0x114, 0xF);
-  HQ_SCAN_STEP(0x118, 0xF);
-  HQ_SCAN_STEP(0x142, 0xA);  // lane 15 of a row to the next one: rows 1 and 3
-  HQ_SCAN_STEP(0x143, 0xC);  // lane 31: rows 2 and 3
-#undef HQ_SCAN_STEP
-  return x;
-}
-__device__ __forceinline__ uint32_t scan_sum(uint32_t x) {
-  return scan(x, 0, [](uint32_t a, uint32_t b) { return a + b; });
-}
 __device__ __forceinline__ uint32_t sum_lanes(uint32_t x) { return lane_value(scan_sum(x), 63); }
 __device__ __forceinline__ uint32_t min_lanes(uint32_t x) {
   return lane_value(scan(x, ~0u, [](uint32_t a, uint32_t b) { return min(a, b); }), 63);

@@ -8,8 +8,8 @@
 // where compaction moves them) is one workgroup's work; pages are moved by a grid of their own.
 //
 // Bound by the bytes moved, read and written once. On an MI355X: append of 80 tokens to 8 heads of 128 3.4 us, of
-// which 2 the launch; a fork of 32 children (88 MB of part-filled pages) 6.5 us of planning and 15 to 17 of copies; compaction of
-// 1.1 GB 6 us of planning and 224 to 234 of copies, 4.8 TB/s, a large copy's rate.
+// which 2 the launch; a fork of 32 children (88 MB of part-filled pages) 5 us of planning and 15 to 17 of copies; compaction of
+// 1.1 GB 5 us of planning and 224 to 234 of copies, 4.8 TB/s, a large copy's rate.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -33,12 +33,7 @@ __device__ __forceinline__ void report(uint32_t* status, uint32_t what) {
 // so calls may follow each other.
 __device__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_t& total) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint32_t x = v;
-#pragma unroll
-  for (uint32_t d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+  const uint32_t x = scan_sum(v);
   __syncthreads();
   if (lane == 63) sh[wave] = x;
   __syncthreads();
@@ -58,38 +53,52 @@ __device__ __forceinline__ void four_refs(const int32_t* refs, uint32_t i, uint3
   for (uint32_t e = 0; e < 4; ++e) r[e] = 4 * i + e < pages ? refs[4 * i + e] : 1;
 }
 
-// Whether the pool has `need` free pages; stops as soon as it has.
-__device__ bool enough_free(const CacheArgs& c, uint32_t need, uint32_t* sh) {
-  uint32_t found = 0;
-  for (uint32_t base = 0; base < c.pages && found < need; base += 4 * kPlanThreads) {
-    int32_t r[4];
-    four_refs(c.refs, base / 4 + threadIdx.x, c.pages, r);
-    uint32_t n = 0, total;
-    for (int e = 0; e < 4; ++e) n += r[e] == 0;
-    block_scan(n, sh, total);
-    found += total;
-  }
-  return found >= need;
-}
+// The pool's free pages, the first 4096 pages' counts in registers: they are on their way while the call's
+// lists are checked, and most calls need no others. A fork's plan takes 5.1 us so, and took 6.8 with each load
+// after the last.
+struct FreePages {
+  int32_t r[4];
+  uint32_t rank, total;  // free pages below this thread's four, and among all of them
 
-// Calls give(rank, page) for the `need` lowest free pages.
-template <class F>
-__device__ void take_free(const CacheArgs& c, uint32_t need, uint32_t* sh, F give) {
-  uint32_t found = 0;
-  for (uint32_t base = 0; base < c.pages && found < need; base += 4 * kPlanThreads) {
-    int32_t r[4];
-    four_refs(c.refs, base / 4 + threadIdx.x, c.pages, r);
-    uint32_t n = 0, total;
-    for (int e = 0; e < 4; ++e) n += r[e] == 0;
-    uint32_t rank = found + block_scan(n, sh, total);
-    for (uint32_t e = 0; e < 4; ++e)
-      if (r[e] == 0) {
-        if (rank < need) give(rank, base + 4 * threadIdx.x + e);
-        ++rank;
-      }
-    found += total;
+  __device__ __forceinline__ void look(const CacheArgs& c) { four_refs(c.refs, threadIdx.x, c.pages, r); }
+  __device__ __forceinline__ static uint32_t free_of(const int32_t (&r)[4]) {
+    return (r[0] == 0) + (r[1] == 0) + (r[2] == 0) + (r[3] == 0);
   }
-}
+  // Whether there are `need`; stops as soon as there are.
+  __device__ bool enough(const CacheArgs& c, uint32_t need, uint32_t* sh) {
+    rank = block_scan(free_of(r), sh, total);
+    uint32_t found = total;
+    for (uint32_t base = 4 * kPlanThreads; base < c.pages && found < need; base += 4 * kPlanThreads) {
+      int32_t q[4];
+      four_refs(c.refs, base / 4 + threadIdx.x, c.pages, q);
+      uint32_t more;
+      block_scan(free_of(q), sh, more);
+      found += more;
+    }
+    return found >= need;
+  }
+  // Calls give(rank, page) for the `need` lowest; after enough().
+  template <class F>
+  __device__ void take(const CacheArgs& c, uint32_t need, uint32_t* sh, F give) const {
+    auto some = [&](const int32_t (&q)[4], uint32_t base, uint32_t at) {
+      for (uint32_t e = 0; e < 4; ++e)
+        if (q[e] == 0) {
+          if (at < need) give(at, base + 4 * threadIdx.x + e);
+          ++at;
+        }
+    };
+    some(r, 0, rank);
+    uint32_t found = total;
+    for (uint32_t base = 4 * kPlanThreads; base < c.pages && found < need; base += 4 * kPlanThreads) {
+      int32_t q[4];
+      four_refs(c.refs, base / 4 + threadIdx.x, c.pages, q);
+      uint32_t more;
+      const uint32_t at = block_scan(free_of(q), sh, more);
+      some(q, base, found + at);
+      found += more;
+    }
+  }
+};
 
 // off[i] <= r < off[i + 1], off not falling over n + 1 entries.
 __device__ __forceinline__ uint32_t owner(const uint32_t* off, uint32_t n, uint32_t r) {
@@ -121,12 +130,13 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_reserve_kernel(CacheArg
   const uint32_t i = threadIdx.x;
   if (i == 0) fault = 0;
   list[i] = i < n ? rows[i] : -1;
+  int32_t len = 0, more = i < n ? counts[i] : 0;
+  FreePages pool;
+  pool.look(c);
   __syncthreads();
   const int32_t row = list[i];
   uint32_t add = 0, bad = 0;
-  int32_t len = 0, more = 0;
   if (i < n) {
-    more = counts[i];
     if (row < 0 || row >= (int32_t)c.rows || more < 0 || repeated(list, i)) {
       bad = HQ_CACHE_BAD_ROW;
     } else {
@@ -148,12 +158,12 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_reserve_kernel(CacheArg
   if (i == 0) off[n] = need;
   __syncthreads();
   bad = fault;
-  if (!bad && !enough_free(c, need, sh)) bad = HQ_CACHE_NO_PAGES;
+  if (!bad && !pool.enough(c, need, sh)) bad = HQ_CACHE_NO_PAGES;
   if (bad) {
     if (i == 0) report(c.status, bad);
     return;
   }
-  take_free(c, need, sh, [&](uint32_t r, uint32_t page) {
+  pool.take(c, need, sh, [&](uint32_t r, uint32_t page) {
     const uint32_t j = owner(off, n, r);
     c.table[(int64_t)list[j] * c.table_stride + first[j] + (r - off[j])] = (int32_t)page;
     c.refs[page] = 1;
@@ -245,18 +255,20 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_fork_plan_kernel(CacheA
   __shared__ uint16_t who[HQ_CACHE_MAX_BATCH];
   const uint32_t i = threadIdx.x;
   if (i == 0) fault = 0;
-  list[i] = i < n ? children[i] : -1;
+  const int32_t k = i < n ? children[i] : -1, p = i < n ? parents[i] : -1;
+  const bool rows = p >= 0 && p < (int32_t)c.rows && k >= 0 && k < (int32_t)c.rows;
+  const int32_t len = rows ? c.lens[p] : 0, own = rows ? c.lens[k] : 0;
+  FreePages pool;
+  pool.look(c);
+  list[i] = k;
   __syncthreads();
   uint32_t part = 0, bad = 0;
   int32_t from = -1;
   if (i < n) {
-    const int32_t p = parents[i], k = list[i];
     bool both = false;  // the parent is some child: its row is not what it will be
     for (uint32_t j = 0; j < n; ++j) both |= list[j] == p;
-    if (p < 0 || p >= (int32_t)c.rows || k < 0 || k >= (int32_t)c.rows || both || repeated(list, i)) bad = HQ_CACHE_BAD_ROW;
-    else if (c.lens[k] != 0 || c.lens[p] < 0) bad = HQ_CACHE_BAD_ROW;
+    if (!rows || both || repeated(list, i) || own != 0 || len < 0) bad = HQ_CACHE_BAD_ROW;
     else {
-      const int32_t len = c.lens[p];
       if (pages_of(len, c.page_shift) > c.max_pages) bad = HQ_CACHE_BAD_ROW;
       else if (len & ((1 << c.page_shift) - 1)) {
         part = 1;
@@ -272,13 +284,13 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_fork_plan_kernel(CacheA
   if (i < n) plan->tail[i] = make_int2(from, -1);
   __syncthreads();
   bad = fault;
-  if (!bad && !enough_free(c, need, sh)) bad = HQ_CACHE_NO_PAGES;
+  if (!bad && !pool.enough(c, need, sh)) bad = HQ_CACHE_NO_PAGES;
   if (i == 0) plan->ok = !bad;
   if (bad) {
     if (i == 0) report(c.status, bad);
     return;
   }
-  take_free(c, need, sh, [&](uint32_t r, uint32_t page) {
+  pool.take(c, need, sh, [&](uint32_t r, uint32_t page) {
     plan->tail[who[r]].y = (int32_t)page;
     c.refs[page] = 1;
   });

@@ -211,4 +211,22 @@ __device__ __forceinline__ uint16_t f32_to_out(float v) {
   }
 }
 
+// f over the lanes up to each one, by moves inside rows of 16 lanes and then from row to row: a shuffle through
+// LDS takes ten times as long, and a call begins with several of these one after the other.
+template <class F>
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t none, F f) {
+#define HQ_SCAN_STEP(CTRL, ROWS) x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xF, false))
+  HQ_SCAN_STEP(0x111, 0xF);  // from the lane 1, 2, 4, 8 below
+  HQ_SCAN_STEP(0x112, 0xF);
+  HQ_SCAN_STEP(0x114, 0xF);
+  HQ_SCAN_STEP(0x118, 0xF);
+  HQ_SCAN_STEP(0x142, 0xA);  // lane 15 of a row to the next one: rows 1 and 3
+  HQ_SCAN_STEP(0x143, 0xC);  // lane 31: rows 2 and 3
+#undef HQ_SCAN_STEP
+  return x;
+}
+__device__ __forceinline__ uint32_t scan_sum(uint32_t x) {
+  return scan(x, 0, [](uint32_t a, uint32_t b) { return a + b; });
+}
+
 }  // namespace hq
