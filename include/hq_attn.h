@@ -53,7 +53,9 @@ typedef struct hq_attn_io {
  * Sequence r holds lens[r] tokens, token j of it at slot j % page_tokens of page
  * table[r * table_stride + j / page_tokens]; entries past them are -1. refs[p] counts the sequences
  * that hold page p; 0: free. A part-filled page has one holder. status: one word, to which calls
- * OR the HQ_CACHE_* faults that they meet on the device (the caller clears it). */
+ * OR the HQ_CACHE_* faults that they meet on the device (the caller clears it). refused[r]: zero at
+ * first; not zero from an hq_cache_reserve that was refused room for row r to the next one that was
+ * not: hq_cache_append writes nothing to such a row (both calls need it, the others do not read it). */
 typedef struct hq_kv_cache {
     void* K;
     void* V;
@@ -66,12 +68,13 @@ typedef struct hq_kv_cache {
     int32_t* lens;
     int32_t* refs;
     uint32_t* status;
+    int32_t* refused;
 } hq_kv_cache;
 
 #define HQ_CACHE_BAD_ROW 1u      /* a row number out of range, repeated, or not as the call needs it */
 #define HQ_CACHE_NO_PAGES 2u     /* too few free pages: the call changed nothing */
 #define HQ_CACHE_ROW_FULL 4u     /* a sequence would pass max_pages: the call changed nothing */
-#define HQ_CACHE_BAD_PAGE 8u     /* a page number out of range, or a count below zero; it was not followed */
+#define HQ_CACHE_BAD_PAGE 8u     /* a page number out of range, a count below zero, an append to a page of several rows; it was not followed */
 #define HQ_CACHE_MAX_BATCH 1024u /* sequences of one hq_cache_* call */
 
 /* ---- attention ---- */
@@ -122,12 +125,14 @@ hq_status hq_attn_shared_prefix(const hq_attn_io* io, const hq_kv_cache* cache, 
 /* Workspace of hq_cache_fork and hq_cache_compact on this cache. */
 hq_status hq_cache_workspace_bytes(const hq_kv_cache* cache, size_t* bytes);
 /* Room for counts[i] (>= 0) more tokens of row rows[i]: pages for them, lens[rows[i]] += counts[i].
- * All rows or, with a fault in `status`, none. */
+ * All rows or, with a fault in `status`, none; the appends of a refused call's rows then write nothing, so
+ * a step can be enqueued whole and its fault be met at the end. */
 hq_status hq_cache_reserve(const hq_kv_cache* cache, const int32_t* rows, const int32_t* counts, uint32_t n,
                            hq_stream stream);
 /* Writes the keys and values of the last cu[i + 1] - cu[i] tokens of each row (cu NULL: of the last
- * one; then tokens = n) into one layer: source row cu[i] + t. Strides as in hq_attn_prompt. Call it
- * after hq_cache_reserve has made room. */
+ * one; then tokens = n) into one layer: source row cu[i] + t; a row appears once. Strides as in
+ * hq_attn_prompt. Call it after hq_cache_reserve has made room. Rows that it was refused for (BAD_ROW), and
+ * tokens on a page that several rows hold (BAD_PAGE), are skipped and reported. */
 hq_status hq_cache_append(const hq_kv_cache* cache, uint32_t layer, const void* K, int64_t k_row, int64_t k_head,
                           const void* V, int64_t v_row, int64_t v_head, uint32_t tokens, const int32_t* rows,
                           const int32_t* cu, uint32_t n, hq_stream stream);

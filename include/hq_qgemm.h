@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define HQ_ABI_VERSION 2
+#define HQ_ABI_VERSION 3
 
 /* The enums are int-sized. C++ gives them int as their underlying type, so that any value a C
  * caller passes (including invalid ones, which are rejected) is a valid enum value there. */

@@ -28,7 +28,8 @@ HEAD_DIMS = (64, 128, 256)
 BAD_ROW, NO_PAGES, ROW_FULL, BAD_PAGE = 1, 2, 4, 8
 MAX_BATCH = 1024
 FAULTS = {BAD_ROW: "a row number out of range, repeated, or not as the call needs it", NO_PAGES: "too few free pages",
-          ROW_FULL: "a sequence would pass its row of the table", BAD_PAGE: "a page number out of range"}
+          ROW_FULL: "a sequence would pass its row of the table",
+          BAD_PAGE: "a page number out of range, or tokens for a page that several rows hold"}
 
 # Every symbol include/hq_attn.h declares.
 EXPORTS = (
@@ -52,7 +53,7 @@ class KVCacheDesc(ctypes.Structure):
                 ("page_tokens", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("dtype", ctypes.c_int),
                 ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("rows", ctypes.c_uint32),
                 ("max_pages", ctypes.c_uint32), ("lens", ctypes.c_void_p), ("refs", ctypes.c_void_p),
-                ("status", ctypes.c_void_p)]
+                ("status", ctypes.c_void_p), ("refused", ctypes.c_void_p)]
 
 
 # hq_attn_io as bytes, packed by every call.
@@ -172,9 +173,12 @@ class KVCache:
     k, v: [layers, pages, kv_heads, page_tokens, head_dim] float16 or bfloat16 (or a view of it whose
     pages hold tokens before heads, k.transpose(2, 3) of a [.., page_tokens, kv_heads, ..] tensor).
     table: int32 [rows, max_pages], -1 past a row's tokens; lens: int32 [rows]; refs: int32 [pages],
-    holders of each page, 0: free; status: int32 [1], zero, made if not given."""
+    holders of each page, 0: free; status: int32 [1] and refused: int32 [rows], zero, made if not given.
 
-    def __init__(self, k, v, table, lens, refs, status=None):
+    Where reserve() is refused (check() will raise), nothing has changed, and append() to its rows changes
+    nothing either until a later reserve() of them goes through: a step can be enqueued whole."""
+
+    def __init__(self, k, v, table, lens, refs, status=None, refused=None):
         import torch
 
         if k.dim() != 5 or v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype or v.device != k.device:
@@ -187,12 +191,14 @@ class KVCache:
         if not (table.is_cuda and table.get_device() == dev and table.dtype == torch.int32 and table.dim() == 2 and
                 (table.stride(1) == 1 or table.shape[1] == 1) and (table.stride(0) >= table.shape[1] or table.shape[0] == 1)):
             raise ValueError("table must be an int32 [rows, max_pages] tensor on k's device with unit stride along its rows")
-        if status is None:
-            status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        if status is None or refused is None:
+            words = torch.zeros(1 + table.shape[0], dtype=torch.int32, device=k.device)
+            status, refused = words[:1] if status is None else status, words[1:] if refused is None else refused
         _ints("lens", lens, table.shape[0], dev)
         _ints("refs", refs, pages, dev)
         _ints("status", status, 1, dev)
-        self.k, self.v, self.table, self.lens, self.refs, self.status = k, v, table, lens, refs, status
+        _ints("refused", refused, table.shape[0], dev)
+        self.k, self.v, self.table, self.lens, self.refs, self.status, self.refused = k, v, table, lens, refs, status, refused
         self.layers, self.pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
         self.rows, self.max_pages = table.shape
         self.device_index = dev
@@ -205,7 +211,7 @@ class KVCache:
         self._desc = KVCacheDesc(k.data_ptr(), v.data_ptr(), sl if layers > 1 else dense * pages, sp if pages > 1 else dense, sh, st,
                                  layers, pages, heads, tokens, dim, dt, table.data_ptr(),
                                  table.stride(0) if table.shape[0] > 1 else table.shape[1], self.rows, self.max_pages,
-                                 lens.data_ptr(), refs.data_ptr(), status.data_ptr())
+                                 lens.data_ptr(), refs.data_ptr(), status.data_ptr(), refused.data_ptr())
         self._ref = ctypes.byref(self._desc)
 
     @classmethod
@@ -233,14 +239,15 @@ class KVCache:
             raise ValueError(f"{name} must be [tokens, {self.kv_heads}, {self.head_dim}], got {tuple(t.shape)}")
 
     def reserve(self, rows, counts, stream=None) -> None:
-        """Room for counts[i] more tokens of rows[i]: pages for them, and lens grows by as many."""
+        """Room for counts[i] more tokens of rows[i]: pages for them, and lens grows by as many. All rows or none."""
         n = rows.numel()
         hq.check((_bound or _lib()).hq_cache_reserve(self._ref, self._list("rows", rows), self._list("counts", counts, n), n,
                                                      hq._stream_ptr(stream)))
 
     def append(self, layer: int, k, v, rows, cu_seqlens=None, stream=None) -> None:
         """Writes k and v [tokens, kv_heads, head_dim] as the last tokens of each row: tokens
-        [cu_seqlens[i], cu_seqlens[i + 1]) are rows[i]'s (None: one token a row)."""
+        [cu_seqlens[i], cu_seqlens[i + 1]) are rows[i]'s (None: one token a row). Rows whose reserve() was
+        refused, and pages that several rows hold, are left as they are."""
         self._new("k", k)
         self._new("v", v, k.shape[0])
         n = rows.numel()

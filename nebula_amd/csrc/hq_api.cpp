@@ -610,7 +610,7 @@ hq_status check_int8_shape(uint32_t K, uint32_t N) {
 
 extern "C" {
 
-const char* hq_version(void) { return "nebula-hq 0.2.0 (gfx950, ABI 2)"; }
+const char* hq_version(void) { return "nebula-hq 0.2.0 (gfx950, ABI 3)"; }
 
 const char* hq_last_error(void) { return g_last_error.c_str(); }
 

@@ -75,6 +75,7 @@ struct CacheArgs {
   int32_t* lens;
   int32_t* refs;
   uint32_t* status;
+  int32_t* refused;  // rows that the last reserve was refused for
   PageShape shape;
 };
 

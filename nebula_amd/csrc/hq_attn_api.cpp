@@ -124,8 +124,8 @@ hq_status check_cache(const hq_kv_cache* c, hq::CacheArgs* out) {
     return fail(HQ_ERR_SHAPE, "cache: page_stride=%lld, layer_stride=%lld must be multiples of 8 and at least a page (%lld)",
                 (long long)c->page_stride, (long long)c->layer_stride, (long long)dense);
   if (misaligned(c->K, 16) || misaligned(c->V, 16)) return fail(HQ_ERR_ALIGNMENT, "cache: K and V must be 16-byte aligned");
-  if (misaligned(c->table, 4) || misaligned(c->lens, 4) || misaligned(c->refs, 4) || misaligned(c->status, 4))
-    return fail(HQ_ERR_ALIGNMENT, "cache: table, lens, refs and status must be 4-byte aligned");
+  if (misaligned(c->table, 4) || misaligned(c->lens, 4) || misaligned(c->refs, 4) || misaligned(c->status, 4) || misaligned(c->refused, 4))
+    return fail(HQ_ERR_ALIGNMENT, "cache: table, lens, refs, status and refused must be 4-byte aligned");
   hq::CacheArgs a{};
   a.K = static_cast<uint16_t*>(c->K);
   a.V = static_cast<uint16_t*>(c->V);
@@ -145,6 +145,7 @@ hq_status check_cache(const hq_kv_cache* c, hq::CacheArgs* out) {
   a.lens = c->lens;
   a.refs = c->refs;
   a.status = c->status;
+  a.refused = c->refused;
   a.shape.runs = heads_first ? c->kv_heads : 1u;
   a.shape.per_token = heads_first ? c->head_dim : c->kv_heads * c->head_dim;
   a.shape.run_stride = heads_first ? c->head_stride : 0;
@@ -324,6 +325,7 @@ hq_status hq_cache_reserve(const hq_kv_cache* cache, const int32_t* rows, const 
   if ((st = check_cache(cache, &c)) != HQ_OK || (st = check_batch(n)) != HQ_OK || (st = check_list("rows", rows)) != HQ_OK ||
       (st = check_list("counts", counts)) != HQ_OK)
     return st;
+  if (!c.refused) return fail(HQ_ERR_INVALID_ARG, "cache: refused is null");
   return from_hip(hq::launch_cache_reserve(c, rows, counts, n, reinterpret_cast<hipStream_t>(stream)), "reserve launch");
 }
 
@@ -342,6 +344,7 @@ hq_status hq_cache_append(const hq_kv_cache* cache, uint32_t layer, const void* 
   if ((st = check_strides("K", k_row, k_head, tokens, c.kv_heads, c.dim)) != HQ_OK ||
       (st = check_strides("V", v_row, v_head, tokens, c.kv_heads, c.dim)) != HQ_OK)
     return st;
+  if (!c.refused) return fail(HQ_ERR_INVALID_ARG, "cache: refused is null");
   return from_hip(hq::launch_cache_append(c, layer, static_cast<const uint16_t*>(K), k_row, k_head, static_cast<const uint16_t*>(V), v_row,
                                           v_head, tokens, rows, cu, n, reinterpret_cast<hipStream_t>(stream)),
                   "append launch");

@@ -161,6 +161,8 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_reserve_kernel(CacheArg
   if (!bad && !pool.enough(c, need, sh)) bad = HQ_CACHE_NO_PAGES;
   if (bad) {
     if (i == 0) report(c.status, bad);
+    // What is appended to these rows before a reserve goes through would lie over their last tokens.
+    if (i < n && row >= 0 && row < (int32_t)c.rows) c.refused[row] = 1;
     return;
   }
   pool.take(c, need, sh, [&](uint32_t r, uint32_t page) {
@@ -168,7 +170,10 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_reserve_kernel(CacheArg
     c.table[(int64_t)list[j] * c.table_stride + first[j] + (r - off[j])] = (int32_t)page;
     c.refs[page] = 1;
   });
-  if (i < n) c.lens[row] = len + more;
+  if (i < n) {
+    c.lens[row] = len + more;
+    c.refused[row] = 0;
+  }
 }
 
 // One 16-byte piece per thread: (token, head, piece of the head).
@@ -180,6 +185,9 @@ __global__ __launch_bounds__(kCopyThreads) void hq_cache_append_kernel(CacheArgs
   const uint64_t u = (uint64_t)blockIdx.x * kCopyThreads + threadIdx.x;
   const uint32_t t = (uint32_t)(u / per_token), p = (uint32_t)(u % per_token);
   if (t >= tokens) return;
+  // The source is on its way beside the chain list - row - length - page - holders.
+  const uint32_t h = p / per_head, e = (p % per_head) * 8;
+  const u4 k = *reinterpret_cast<const u4*>(K + t * k_row + h * k_head + e), v = *reinterpret_cast<const u4*>(V + t * v_row + h * v_head + e);
   uint32_t i = t, back = 1;  // sequence, tokens from its end
   if (cu) {
     // The last sequence that begins at or before t; it holds t if it does not end before it.
@@ -200,19 +208,18 @@ __global__ __launch_bounds__(kCopyThreads) void hq_cache_append_kernel(CacheArgs
     return;
   }
   const int64_t at = (int64_t)c.lens[row] - back;
-  if (at < 0 || at >= (int64_t)c.max_pages << c.page_shift) {
+  if (c.refused[row] || at < 0 || at >= (int64_t)c.max_pages << c.page_shift) {
     report(c.status, HQ_CACHE_BAD_ROW);
     return;
   }
   const uint32_t page = (uint32_t)c.table[row * c.table_stride + (at >> c.page_shift)];
-  if (page >= c.pages) {
+  if (page >= c.pages || c.refs[page] > 1) {
     report(c.status, HQ_CACHE_BAD_PAGE);
     return;
   }
-  const uint32_t h = p / per_head, e = (p % per_head) * 8;
   const int64_t to = page * c.page_stride + h * c.head_stride + (at & ((1 << c.page_shift) - 1)) * c.token_stride + e;
-  *reinterpret_cast<u4*>(c.K + to) = *reinterpret_cast<const u4*>(K + t * k_row + h * k_head + e);
-  *reinterpret_cast<u4*>(c.V + to) = *reinterpret_cast<const u4*>(V + t * v_row + h * v_head + e);
+  *reinterpret_cast<u4*>(c.K + to) = k;
+  *reinterpret_cast<u4*>(c.V + to) = v;
 }
 
 // Units of kUnitBytes that `tokens` tokens of a page hold.

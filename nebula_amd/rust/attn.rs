@@ -61,8 +61,9 @@ pub struct KvCache {
     pub lens: *mut i32,
     pub refs: *mut i32,
     pub status: *mut u32,
+    pub refused: *mut i32,
 }
-const _: () = assert!(std::mem::size_of::<KvCache>() == 120);
+const _: () = assert!(std::mem::size_of::<KvCache>() == 128);
 
 /// Faults that calls report in the cache's status word.
 pub const CACHE_BAD_ROW: u32 = 1;
