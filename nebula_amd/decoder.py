@@ -108,29 +108,38 @@ class LayerProjections:
         prepare(q_out, k, v) makes the query and key heads of the projections' outputs ([M, 12288], [M,
         1024], [M, 1024]): q [M, 24, 256], k and v [M, 4, 256], normalised and rotated as the model has it
         (default: the first half of q_out, k and v as they are). gate(y, q_out) is what goes to mixer_out in
-        y's place (default: y, [M, 6144]). step.reserve(cache) comes first, once for all layers."""
+        y's place (default: y, [M, 6144]). step.reserve(cache) comes first, once for all layers.
+
+        With a stream (torch's), everything runs on it, prepare and gate too, and it is the current one while
+        they do: the layer's tensors are its own. The caller orders it after what made x_norm, and orders
+        others after it."""
+        if stream is not None:
+            import torch
+
+            with torch.cuda.stream(stream):
+                return self.attend(x_norm, cache, cache_layer, step, prepare, gate)
         if self.kind != "attention":
             raise ValueError(f"attend() is the attention mixer's, the layer's kind is {self.kind!r}")
         M = step.M
         if x_norm.shape[0] != M:
             raise ValueError(f"x_norm has {x_norm.shape[0]} rows, the step {M}")
-        q_out, k, v = self.mixer_in(x_norm, stream=stream)
+        q_out, k, v = self.mixer_in(x_norm)
         if prepare is None:
             q = q_out[:, :MIXER_IN].unflatten(1, (HEADS, HEAD_DIM))
             k, v = (t.unflatten(1, (KV_HEADS, HEAD_DIM)) for t in (k, v))
         else:
             q, k, v = prepare(q_out, k, v)
-        cache.append(cache_layer, k, v, step.rows, step.cu, stream=stream)
+        cache.append(cache_layer, k, v, step.rows, step.cu)
         y = q.new_empty((M, HEADS, HEAD_DIM))
         n = step.decodes
         if n and step.prefix is not None:
-            attn.shared_prefix(q[:n], cache, cache_layer, step.decode_rows, *step.prefix, max_len=step.max_len, out=y[:n], stream=stream)
+            attn.shared_prefix(q[:n], cache, cache_layer, step.decode_rows, *step.prefix, max_len=step.max_len, out=y[:n])
         elif n:
-            attn.paged(q[:n], cache, cache_layer, step.decode_rows, max_len=step.max_len, out=y[:n], stream=stream)
+            attn.paged(q[:n], cache, cache_layer, step.decode_rows, max_len=step.max_len, out=y[:n])
         if M > n:
-            attn.paged(q[n:], cache, cache_layer, step.chunk_rows, step.chunk_cu, max_len=step.max_len, out=y[n:], stream=stream)
+            attn.paged(q[n:], cache, cache_layer, step.chunk_rows, step.chunk_cu, max_len=step.max_len, out=y[n:])
         y = y.flatten(1)
-        return self.mixer_out(y if gate is None else gate(y, q_out), stream=stream)
+        return self.mixer_out(y if gate is None else gate(y, q_out))
 
     def ffn_in(self, x_norm, outs=None, stream=None) -> List:
         """[gate, up] — one fused call."""
