@@ -81,12 +81,14 @@ typedef struct hq_kv_cache {
 typedef HQ_ENUM(hq_attn_kind) { HQ_ATTN_PROMPT = 1, HQ_ATTN_PAGED = 2, HQ_ATTN_SHARED = 3 } hq_attn_kind;
 
 /* Workspace of one attention call on the current device (0: none), as hq_workspace_bytes: seqs
- * sequences (groups of them for HQ_ATTN_SHARED), rows tokens, max_keys (and max_prefix) as in the
- * call. The buffer obeys the rules there and can be the same one. */
+ * sequences (groups of them for HQ_ATTN_SHARED), rows tokens, max_keys the call's max_k or max_len, or
+ * where that is 0 what it stands for (0 is refused here), max_prefix as in the call. The size does not fall as
+ * max_keys and max_prefix grow: one taken at the largest serves every call of as many rows and
+ * sequences on fewer keys, which may use less of it. The buffer obeys the rules there and can be the same one. */
 hq_status hq_attn_workspace_bytes(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups,
                                   uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_keys,
                                   uint32_t max_prefix, size_t* bytes);
-/* The kernels and the splits such a call runs, as text. */
+/* The kernels and the splits such a call runs and the workspace that it uses, as text. */
 hq_status hq_describe_attn(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads,
                            uint32_t kv_heads, uint32_t head_dim, uint32_t max_keys, uint32_t max_prefix,
                            char* buf, size_t buf_len);

@@ -307,7 +307,8 @@ class KVCache:
 # ---------------------------------------------------------------- attention
 def workspace_bytes(kind: int, rows: int, seqs: int, heads: int, kv_heads: int, head_dim: int, max_keys: int, groups: int = 1,
                     max_prefix: int = 0) -> int:
-    """Workspace of one call (KIND_*) on the current device."""
+    """Workspace of one call (KIND_*) on the current device, and of every call of as many rows and sequences on
+    fewer keys (and a shorter prefix): it does not fall as max_keys and max_prefix grow. max_keys is a bound, 0 is refused."""
     b = ctypes.c_size_t(0)
     hq.check(_lib().hq_attn_workspace_bytes(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix, ctypes.byref(b)))
     return int(b.value)

@@ -478,9 +478,9 @@ hq_status run_gemm(const void* X, hq_dtype dtype, int64_t ldx, hq_format fmt, co
 
 }  // namespace
 
-hq_status hq_internal_workspace(hipStream_t stream, size_t need, void** out) {
+hq_status hq_internal_workspace(hipStream_t stream, size_t use, size_t need, void** out) {
   try {
-    return get_internal_ws(stream, need, need, out);
+    return get_internal_ws(stream, use, need, out);
   } catch (...) {
     return fail(HQ_ERR_INTERNAL, "out of host memory");
   }

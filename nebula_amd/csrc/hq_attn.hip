@@ -1381,16 +1381,37 @@ hipError_t launch_dim(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
 // where they share one (heads of 256 never do). Parts are written and read at 1 us to 4.5 MB, to 1.3 MB beside the
 // row workgroups of a shared prefix, and the join's launch is 6.5. On a chunk of 64 tokens after 6000, 24 tiles,
 // 1 / 5 / 10 / 12 / 21 / 48 workgroups took 110 / 37 / 29 / 33 / 31 / 52 us (10 chosen); on 512 tokens after 7488, 192
-// tiles, 1 / 2 / 4 / 8 / 16 took 195 / 146 / 139 / 142 / 184 (4); on a prompt of 512, 1 / 2 / 4 took 16 / 33 / 37 (1);
+// tiles, 1 / 2 / 4 / 8 / 16 took 195 / 146 / 139 / 142 / 184 (5); on a prompt of 512, 1 / 2 / 4 took 16 / 33 / 37 (1);
 // on a prefix of 2000 under 5 groups of 20 rows, 1 / 2 / 4 / 6 / 12 took 66 / 40 / 29 / 34 / 39 (4).
-uint32_t tile_splits(uint64_t tiles, uint64_t rows, uint32_t dim, uint32_t keys, bool prefix) {
+//
+// No more than `most`, which does not fall as the keys grow, so that a workspace for long keys holds what any shorter
+// ones ask for: the best number for half as many keys again, in shares that need not be whole tiles. That
+// one's times are lines over the keys, the more workgroups the flatter and the higher where they begin; the lowest of
+// such lines is a flatter one the further out. Over 3000 shapes of 1 to 2000 tiles, each on up to 131,000 keys, the bound
+// moves 1.7% of the choices, whose times by the same cost are 0.02% more over all of them and 14% more at the worst.
+uint32_t tile_splits(uint64_t tiles, uint64_t rows, uint32_t dim, uint32_t keys, bool prefix, uint32_t& most) {
   const uint32_t steps = up(keys, kKeys), cus = (uint32_t)cu_count();
-  uint32_t best = 1;
+  struct Cost {
+    double step, parts;  // us of a key tile in all workgroups, of their parts
+  } cost[64];
   double least = 0;
-  for (uint32_t s = 1; s <= std::min(63u, steps); ++s) {
+  uint32_t n = 0;  // numbers whose parts alone do not cost more
+  most = 1;
+  for (uint32_t s = 1; s <= 63; ++s) {
     const uint64_t each = up(tiles * s, cus), pairs = dim == 256 ? 0 : each / 2;
-    double t = up(steps, s) * (dim / 128.) * (1.9 * pairs + 1.2 * (each - 2 * pairs));
-    if (prefix || s > 1) t += rows * s * dim * 4. / (prefix ? 1.3e6 : 4.5e6) + 6.5;
+    const double parts = prefix || s > 1 ? rows * s * dim * 4. / (prefix ? 1.3e6 : 4.5e6) + 6.5 : 0.;
+    const double step = (dim / 128.) * (1.9 * pairs + 1.2 * (each - 2 * pairs)), t = 1.5 * steps / s * step + parts;
+    if (s > 1 && parts >= least) break;
+    cost[n++] = Cost{step, parts};
+    if (s == 1 || t < least) {
+      least = t;
+      most = s;
+    }
+  }
+  most = std::min(most, steps);
+  uint32_t best = 1;
+  for (uint32_t s = 1; s <= most; ++s) {
+    const double t = up(steps, s) * cost[s - 1].step + cost[s - 1].parts;
     if (s == 1 || t < least) {
       least = t;
       best = s;
@@ -1420,10 +1441,12 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   p.row = p.prefix || all_rows <= 32ull * seqs;
   p.tile = p.prefix || !p.row;
   max_keys = std::max(max_keys, 1u);
-  size_t ws = kCounterBytes;
-  auto take = [&](size_t bytes) {
+  // What the plan writes, and what it and every plan of fewer keys need at most.
+  size_t ws = kCounterBytes, need = kCounterBytes;
+  auto take = [&](size_t bytes, size_t most) {
     const size_t at = ws;
     ws += (bytes + 255) / 256 * 256;
+    need += (most + 255) / 256 * 256;
     return at;
   };
   if (p.tile) {
@@ -1431,14 +1454,13 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     const uint32_t tiles = up(all_rows, 128) + (p.prefix ? groups : seqs);
     // The sequences' lengths are not known here: as if all were alike.
     const uint32_t n = p.prefix ? groups : seqs, likely = n * up(up(all_rows, n), 128);
-    p.tile_splits = tile_splits((uint64_t)likely * kv_heads, (uint64_t)rows * heads, dim, keys, p.prefix);
+    uint32_t most;
+    p.tile_splits = tile_splits((uint64_t)likely * kv_heads, (uint64_t)rows * heads, dim, keys, p.prefix, most);
     p.tile_grid = tiles * kv_heads * p.tile_splits;
-    if (p.prefix || p.tile_splits > 1) {
-      p.parts = p.tile_splits + (p.prefix ? 1 : 0);
-      const size_t places = (size_t)rows * heads * p.parts;
-      p.part_ml = take(places * sizeof(f2));
-      p.part_o = take(places * dim * sizeof(float));
-    }
+    if (p.prefix || p.tile_splits > 1) p.parts = p.tile_splits + (p.prefix ? 1 : 0);
+    const size_t all = (size_t)rows * heads, places = all * p.parts, held = p.prefix || most > 1 ? all * (most + (p.prefix ? 1 : 0)) : 0;
+    p.part_ml = take(places * sizeof(f2), held * sizeof(f2));
+    p.part_o = take(places * dim * sizeof(float), held * dim * sizeof(float));
   }
   if (p.row) {
     const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
@@ -1447,13 +1469,13 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     p.row_one = p.row_slots && tiles == 1;
     p.row_like = keys;
     p.row_grid = (p.row_slots ? p.row_slots : tiles) * kv_heads;
-    if (p.row_slots) {
-      const size_t places = (size_t)p.row_slots * kv_heads * 16;
-      p.row_ml = take(places * sizeof(f2));
-      p.row_o = take(places * dim * sizeof(float));
-    }
+    // More keys have no fewer slots; those past a prefix are most where there is none.
+    const size_t place = (size_t)kv_heads * 16, places = p.row_slots * place, held = row_slots(tiles, kv_heads, dim, max_keys) * place;
+    p.row_ml = take(places * sizeof(f2), held * sizeof(f2));
+    p.row_o = take(places * dim * sizeof(float), held * dim * sizeof(float));
   }
   p.ws = ws > kCounterBytes ? ws : 0;
+  p.need = need > kCounterBytes ? need : 0;
   return p;
 }
 

@@ -164,12 +164,12 @@ hq_status check_list(const char* name, const int32_t* p) {
   return HQ_OK;
 }
 
-// The caller's workspace after its checks, or the library's own; null where the call needs none.
-hq_status workspace(void* ws, size_t bytes, size_t need, hipStream_t s, void** out) {
+// The caller's workspace after its checks, or the library's own, which grows to `need`; null where the call uses none.
+hq_status workspace(void* ws, size_t bytes, size_t use, size_t need, hipStream_t s, void** out) {
   *out = nullptr;
-  if (need == 0) return HQ_OK;
-  if (!ws) return hq_internal_workspace(s, need, out);
-  if (bytes < need) return fail(HQ_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu this call needs", bytes, need);
+  if (need == 0 || (ws && use == 0)) return HQ_OK;
+  if (!ws) return hq_internal_workspace(s, use, need, out);
+  if (bytes < use) return fail(HQ_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu this call needs", bytes, use);
   if (misaligned(ws, 256)) return fail(HQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
   *out = ws;
   return HQ_OK;
@@ -180,7 +180,7 @@ hq_status run_attn(const hq::AttnArgs& a, int kind, int dtype, uint32_t max_keys
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hq::AttnPlan p = hq::plan_attn(kind, a.T, a.B, a.groups, a.H, a.Hkv, a.D, max_keys, max_prefix);
   void* w = nullptr;
-  const hq_status st = workspace(ws, bytes, p.ws, s, &w);
+  const hq_status st = workspace(ws, bytes, p.ws, p.need, s, &w);
   if (st != HQ_OK) return st;
   return from_hip(hq::launch_attn(dtype, a, p, w, s), "attention launch");
 }
@@ -219,8 +219,9 @@ hq_status cache_keys(const hq_attn_io* io, const hq_kv_cache* cache, uint32_t la
 uint32_t capacity(const hq_kv_cache* c) { return c->max_pages * c->page_tokens; }
 
 hq_status check_query(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
-                      uint32_t dim) {
+                      uint32_t dim, uint32_t max_keys) {
   if (kind < HQ_ATTN_PROMPT || kind > HQ_ATTN_SHARED) return fail(HQ_ERR_INVALID_ARG, "unknown kind %d", (int)kind);
+  if (max_keys == 0) return fail(HQ_ERR_SHAPE, "max_keys=0: a query needs the bound that 0 stands for in a call (total_k, a row's capacity)");
   hq_status st;
   if ((st = check_dim(dim)) != HQ_OK || (st = check_counts(rows, seqs, heads, kv_heads)) != HQ_OK) return st;
   if (kind == HQ_ATTN_SHARED && (groups == 0 || groups > seqs || rows != seqs))
@@ -235,16 +236,16 @@ extern "C" {
 hq_status hq_attn_workspace_bytes(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads,
                                   uint32_t kv_heads, uint32_t head_dim, uint32_t max_keys, uint32_t max_prefix, size_t* bytes) {
   if (!bytes) return fail(HQ_ERR_INVALID_ARG, "bytes is null");
-  const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim);
+  const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys);
   if (st != HQ_OK) return st;
-  *bytes = hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix).ws;
+  *bytes = hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix).need;
   return hq_set_error(HQ_OK, "");
 }
 
 hq_status hq_describe_attn(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim, uint32_t max_keys, uint32_t max_prefix, char* buf, size_t buf_len) {
   if (!buf || buf_len == 0) return fail(HQ_ERR_INVALID_ARG, "buf is null or empty");
-  const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim);
+  const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys);
   if (st != HQ_OK) return st;
   hq::describe_attn(hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix), buf, buf_len);
   return hq_set_error(HQ_OK, "");
@@ -359,7 +360,7 @@ hq_status hq_cache_fork(const hq_kv_cache* cache, const int32_t* parents, const 
     return st;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   void* w = nullptr;
-  if ((st = workspace(ws, ws_bytes, hq::cache_fork_bytes(), s, &w)) != HQ_OK) return st;
+  if ((st = workspace(ws, ws_bytes, hq::cache_fork_bytes(), hq::cache_fork_bytes(), s, &w)) != HQ_OK) return st;
   return from_hip(hq::launch_cache_fork(c, parents, children, n, w, s), "fork launch");
 }
 
@@ -391,7 +392,8 @@ hq_status hq_cache_compact(const hq_kv_cache* cache, int32_t* out_table, int64_t
   if (out_table == c.table && out_stride != c.table_stride) return fail(HQ_ERR_SHAPE, "out_table is the cache's own with another stride");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   void* w = nullptr;
-  if ((st = workspace(ws, ws_bytes, hq::cache_compact_bytes(c.pages), s, &w)) != HQ_OK) return st;
+  const size_t need = hq::cache_compact_bytes(c.pages);
+  if ((st = workspace(ws, ws_bytes, need, need, s, &w)) != HQ_OK) return st;
   return from_hip(hq::launch_cache_compact(c, out_table, out_stride, out_refs, w, s), "compact launch");
 }
 

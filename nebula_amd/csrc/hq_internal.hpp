@@ -8,10 +8,11 @@
 // Sets the calling thread's hq_last_error message (cleared for HQ_OK) and returns s.
 hq_status hq_set_error(hq_status s, const char* fmt, ...);
 
-// The library's own workspace of the current device and `stream`, at least `need` bytes, as the GEMM
-// calls without a workspace use it: its counter area (kCounterBytes) is zero between calls. Fails
-// with HQ_ERR_WORKSPACE where it would have to grow while the stream is capturing.
-hq_status hq_internal_workspace(hipStream_t stream, size_t need, void** out);
+// The library's own workspace of the current device and `stream`, as the GEMM calls without a
+// workspace use it: its counter area (kCounterBytes) is zero between calls. It has at least `use` bytes, and
+// `need` (no less) where it can grow. Fails with HQ_ERR_WORKSPACE where it would have to grow to `use` while
+// the stream is capturing.
+hq_status hq_internal_workspace(hipStream_t stream, size_t use, size_t need, void** out);
 
 namespace hq {
 
