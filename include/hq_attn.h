@@ -114,7 +114,7 @@ hq_status hq_attn_paged(const hq_attn_io* io, const hq_kv_cache* cache, uint32_t
  * their first prefix_lens[g] tokens (starts: int32 [groups + 1], from 0 to seqs, not falling). The
  * whole pages among those tokens are read once for the group, from its first sequence's table (after
  * hq_cache_fork every table of the group names the same ones); all later tokens from each sequence's
- * own pages. max_prefix: no prefix_lens is larger (0: max_len), as max_len only a bound for the split. */
+ * own pages. max_prefix: no prefix_lens is larger (0: not known), as max_len only a bound for the split. */
 hq_status hq_attn_shared_prefix(const hq_attn_io* io, const hq_kv_cache* cache, uint32_t layer,
                                 const int32_t* rows, uint32_t seqs, const int32_t* starts,
                                 const int32_t* prefix_lens, uint32_t groups, uint32_t max_prefix, uint32_t max_len,

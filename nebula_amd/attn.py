@@ -375,7 +375,8 @@ def shared_prefix(q, cache: KVCache, layer: int, rows, starts, prefix_lens, max_
                   scale: Optional[float] = None, out=None, lse=None, with_lse: bool = False, stream=None, workspace=None):
     """paged() with one token a row, for a batch in which sequences [starts[g], starts[g + 1]) share their
     first prefix_lens[g] tokens (as cache.fork leaves them): the whole pages of a prefix are read once
-    for its group. starts: int32 [groups + 1], prefix_lens: int32 [groups]."""
+    for its group. starts: int32 [groups + 1], prefix_lens: int32 [groups]. max_prefix: no prefix is longer (a
+    hint as max_len; 0: not known)."""
     _check_cached(q, cache)
     dev = cache.device_index
     seqs, groups = q.shape[0], prefix_lens.numel()

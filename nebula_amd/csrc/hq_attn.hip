@@ -1441,6 +1441,7 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   p.row = p.prefix || all_rows <= 32ull * seqs;
   p.tile = p.prefix || !p.row;
   max_keys = std::max(max_keys, 1u);
+  max_prefix = std::min(max_prefix, max_keys);
   // What the plan writes, and what it and every plan of fewer keys need at most.
   size_t ws = kCounterBytes, need = kCounterBytes;
   auto take = [&](size_t bytes, size_t most) {
@@ -1450,7 +1451,7 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     return at;
   };
   if (p.tile) {
-    const uint32_t keys = p.prefix ? std::max(max_prefix, 1u) : max_keys;
+    const uint32_t keys = p.prefix && max_prefix ? max_prefix : max_keys;
     const uint32_t tiles = up(all_rows, 128) + (p.prefix ? groups : seqs);
     // The sequences' lengths are not known here: as if all were alike.
     const uint32_t n = p.prefix ? groups : seqs, likely = n * up(up(all_rows, n), 128);
@@ -1464,7 +1465,9 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   }
   if (p.row) {
     const uint32_t tiles = rows == seqs ? seqs * up(G, 16) : up(all_rows, 16) + seqs;
-    const uint32_t keys = p.prefix ? std::max(max_keys - std::min(max_prefix, max_keys), 1u) : max_keys;
+    // Where the prefixes are not known (0), all keys may lie in them, and all past them: 4 rows of 8192 keys of their own on
+    // 48/8 heads of 128 took 94 us with one key taken to be past the prefix, and take 33.
+    const uint32_t keys = p.prefix ? std::max(max_keys - max_prefix, 1u) : max_keys;
     p.row_slots = row_slots(tiles, kv_heads, dim, keys);
     p.row_one = p.row_slots && tiles == 1;
     p.row_like = keys;

@@ -51,6 +51,7 @@ struct AttnPlan {
   size_t part_ml = 0, part_o = 0, row_ml = 0, row_o = 0, ws = 0;  // workspace offsets, and its size
   size_t need = 0;                 // not falling in the keys: what calls of fewer keys need at most, and this one
 };
+// max_prefix: 0, where it is not known.
 AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                    uint32_t dim, uint32_t max_keys, uint32_t max_prefix);
 void describe_attn(const AttnPlan& p, char* buf, size_t len);

@@ -308,7 +308,7 @@ hq_status hq_attn_shared_prefix(const hq_attn_io* io, const hq_kv_cache* cache, 
   a.prefix = prefix_lens;
   a.groups = groups;
   const uint32_t cap = capacity(cache), most = max_len && max_len < cap ? max_len : cap;
-  return run_attn(a, HQ_ATTN_SHARED, io->dtype, most, max_prefix && max_prefix < most ? max_prefix : most, ws, ws_bytes, stream);
+  return run_attn(a, HQ_ATTN_SHARED, io->dtype, most, max_prefix, ws, ws_bytes, stream);
 }
 
 hq_status hq_cache_workspace_bytes(const hq_kv_cache* cache, size_t* bytes) {

@@ -132,7 +132,7 @@ class LayerProjections:
         cache.append(cache_layer, k, v, step.rows, step.cu)
         y = q.new_empty((M, HEADS, HEAD_DIM))
         n = step.decodes
-        if n and step.prefix is not None:
+        if n and step.prefix is not None and step.prefix[2] >= cache.page_tokens:  # whole pages are shared
             attn.shared_prefix(q[:n], cache, cache_layer, step.decode_rows, *step.prefix, max_len=step.max_len, out=y[:n])
         elif n:
             attn.paged(q[:n], cache, cache_layer, step.decode_rows, max_len=step.max_len, out=y[:n])
