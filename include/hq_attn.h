@@ -30,7 +30,7 @@ extern "C" {
 #endif
 
 /* Queries and outputs of a call: element (t, h, d) of Q at t * q_row + h * q_head + d, of O
- * likewise. Strides are in elements and multiples of 8, Q and O 16-byte aligned. lse: NULL, or
+ * likewise, no two of O in one place. Strides are in elements and multiples of 8, Q and O 16-byte aligned. lse: NULL, or
  * fp32 [rows][heads]. head_dim: 64, 128 or 256. scale: positive and finite. */
 typedef struct hq_attn_io {
     const void* Q;

@@ -30,7 +30,7 @@ constexpr int64_t kMaxSpan = (int64_t)1 << 46;
 // Rows of keys and values at most 2^23 elements apart: the kernels address 16 of them with 32-bit offsets.
 constexpr int64_t kMaxRow = (int64_t)1 << 23;
 
-// Row and head strides of an operand of `heads` heads of `dim`: either order, nothing overlapping.
+// Row and head strides of an operand of `heads` heads of `dim`, in either order.
 hq_status check_strides(const char* name, int64_t row, int64_t head, uint32_t rows, uint32_t heads, uint32_t dim) {
   if (row < 0 || head < 0 || row > kMaxSpan || head > kMaxSpan)
     return fail(HQ_ERR_SHAPE, "%s: strides %lld, %lld out of range", name, (long long)row, (long long)head);
@@ -42,6 +42,17 @@ hq_status check_strides(const char* name, int64_t row, int64_t head, uint32_t ro
   if ((double)row * rows + (double)head * heads > (double)kMaxSpan)
     return fail(HQ_ERR_SHAPE, "%s: the operand spans too much", name);
   return HQ_OK;
+}
+
+// Whether elements of different rows or heads share memory (strides as check_strides accepts them).
+bool overlaps(int64_t row, int64_t head, uint32_t rows, uint32_t heads, uint32_t dim) {
+  if (rows == 1 || heads == 1) return false;
+  if (row >= (heads - 1) * head + dim || head >= (rows - 1) * row + dim) return false;
+  for (uint32_t h = 1; h < heads; ++h) {  // head h of row 0 among head 0 of the rows on either side
+    const int64_t at = h * head, t = at / row;
+    if ((t < rows && at - t * row < dim) || (t + 1 < rows && (t + 1) * row - at < dim)) return true;
+  }
+  return false;
 }
 
 hq_status check_dim(uint32_t D) {
@@ -76,6 +87,8 @@ hq_status check_io(const hq_attn_io* io, uint32_t seqs, uint32_t kv_heads, hq::A
   if ((st = check_strides("Q", io->q_row, io->q_head, io->rows, io->heads, io->head_dim)) != HQ_OK ||
       (st = check_strides("O", io->o_row, io->o_head, io->rows, io->heads, io->head_dim)) != HQ_OK)
     return st;
+  if (overlaps(io->o_row, io->o_head, io->rows, io->heads, io->head_dim))
+    return fail(HQ_ERR_SHAPE, "O: strides %lld, %lld make rows or heads overlap", (long long)io->o_row, (long long)io->o_head);
   *a = hq::AttnArgs{};
   a->Q = static_cast<const uint16_t*>(io->Q);
   a->O = static_cast<uint16_t*>(io->O);
