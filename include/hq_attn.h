@@ -111,7 +111,8 @@ hq_status hq_attn_paged(const hq_attn_io* io, const hq_kv_cache* cache, uint32_t
                         size_t workspace_bytes, hq_stream stream);
 
 /* One new token of each sequence, where the sequences [starts[g], starts[g + 1]) of the batch share
- * their first prefix_lens[g] tokens (starts: int32 [groups + 1], from 0 to seqs, not falling). The
+ * their first prefix_lens[g] tokens (starts: int32 [groups + 1], from 0 to seqs, not falling; where they are
+ * not that, HQ_CACHE_BAD_ROW is reported and every sequence reads all its keys from its own pages). The
  * whole pages among those tokens are read once for the group, from its first sequence's table (after
  * hq_cache_fork every table of the group names the same ones); all later tokens from each sequence's
  * own pages. max_prefix: no prefix_lens is larger (0: not known), as max_len only a bound for the split. */

@@ -319,6 +319,28 @@ __device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t slots, ui
   return false;
 }
 
+// Whether the groups hold each sequence once: starts from 0 to B, not falling. Where they don't, every workgroup
+// finds so, none works on a prefix and all keys of a row are its own. The first 64 are loaded beside what a
+// workgroup starts with and looked at after it.
+struct Groups {
+  int32_t first, end;
+  __device__ __forceinline__ void load(const AttnArgs& a, uint32_t base) {
+    const uint32_t g = min(base + (threadIdx.x & 63u), a.groups - 1);
+    first = a.starts[g];
+    end = a.starts[g + 1];
+  }
+  __device__ __forceinline__ bool ok(const AttnArgs& a) {
+    bool good = true;
+    for (uint32_t base = 0;;) {
+      const uint32_t g = min(base + (threadIdx.x & 63u), a.groups - 1);
+      good = good && first <= end && (g > 0 || first == 0) && (g + 1 < a.groups || end == (int32_t)a.B);
+      base += 64;
+      if (base >= a.groups) return __all(good);
+      load(a, base);
+    }
+  }
+};
+
 // The group of sequence b, the last one that starts at or before it, and where it starts.
 __device__ __forceinline__ uint32_t group_of(const AttnArgs& a, uint32_t b, uint32_t& first) {
   const uint32_t lane = threadIdx.x & 63u;
@@ -460,6 +482,8 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
   const uint32_t kvh = block % a.Hkv, rest = block / a.Hkv;
   const uint32_t split = rest % pl.splits, idx = rest / pl.splits;
   Work w{};
+  Groups groups{};
+  if (PAGED && pl.prefix) groups.load(a, 0);
   if (!find_tile(pl.prefix ? a.starts : a.cu_q, pl.prefix ? a.groups : a.B, pl.prefix ? a.B : a.T, a.G, BR, idx, w)) return;
   // This lane's row.
   const uint32_t r_mine = w.r0 + wave * 32 + l32;
@@ -474,6 +498,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
     if (pl.prefix) {
       const int32_t own = row_number(a.k, w.q0 + token), prefix = a.prefix[w.b];
       const int32_t len = row_length(a.k, row), own_len = row_length(a.k, own);
+      if (!groups.ok(a)) return;
       nk = uni(whole_pages(a.k, row, len, prefix));
       lim = min(nk, length_or_report(a.k, own, own_len));
     } else {
@@ -900,9 +925,14 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
   const int32_t* table = nullptr;
   uint32_t nk, begin = 0;
   int32_t early = 0;  // pages of the first tile: lane j % 2 that of its block j
+  bool grouped = true;
   if constexpr (PAGED) {
     uint32_t g = 0, first = 0;
-    if (a.groups) g = group_of(a, w.b, first);
+    Groups groups{};
+    if (a.groups) {
+      groups.load(a, 0);
+      g = group_of(a, w.b, first);
+    }
     const int32_t row = sh.row;
     table = a.k.table + (row_ok(a.k, row) ? row : 0) * a.k.table_stride;
     if (!find) sh.len = row_length(a.k, row);
@@ -910,7 +940,9 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
       const int32_t first_row = row_number(a.k, first), prefix = a.prefix[g];
       const int32_t first_len = row_length(a.k, first_row);
       nk = uni(length_or_report(a.k, row, sh.len));
-      begin = min(nk, uni(whole_pages(a.k, first_row, first_len, prefix)));
+      grouped = groups.ok(a);
+      begin = grouped ? min(nk, uni(whole_pages(a.k, first_row, first_len, prefix))) : 0u;
+      if (!grouped) report(a.k.status, HQ_CACHE_BAD_ROW);
     }
     early = table[min((begin + t_first * kRowKeys + (lane & 1u) * 16) >> a.k.page_shift, a.k.max_pages - 1)];
     if (!a.groups) nk = uni(length_or_report(a.k, row, sh.len));
@@ -1161,7 +1193,11 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
     const uint32_t rr = w.r0 + row, tk = w.q0 + rr / a.G, hd = kvh * a.G + rr % a.G;
     if (pl.to.slots) {
       const uint64_t at = ((uint64_t)tk * a.H + hd) * pl.to.slots + pl.to.slots - 1;
-      if (d == 0) pl.to.ml[at] = f2{mc, sum};
+      if (d == 0) {
+        pl.to.ml[at] = f2{mc, sum};
+        if (!grouped)  // no workgroup has the other places
+          for (uint32_t i = 1; i < pl.to.slots; ++i) pl.to.ml[at - i] = f2{kNone, 0.f};
+      }
       *reinterpret_cast<f4*>(pl.to.o + at * D + d) = v;
       return;
     }
