@@ -125,7 +125,7 @@ hq_status hq_attn_shared_prefix(const hq_attn_io* io, const hq_kv_cache* cache, 
  * n is at most HQ_CACHE_MAX_BATCH; the rows, counts and lists are device int32 arrays. New pages are
  * the lowest free numbers, in the order of the list. */
 
-/* Workspace of hq_cache_fork and hq_cache_compact on this cache. */
+/* Workspace of hq_cache_fork and hq_cache_compact on this cache, by the same rules (zero before its first use). */
 hq_status hq_cache_workspace_bytes(const hq_kv_cache* cache, size_t* bytes);
 /* Room for counts[i] (>= 0) more tokens of row rows[i]: pages for them, lens[rows[i]] += counts[i].
  * All rows or, with a fault in `status`, none; the appends of a refused call's rows then write nothing, so

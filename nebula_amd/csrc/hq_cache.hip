@@ -249,14 +249,36 @@ __device__ __forceinline__ void copy_unit(uint16_t* base, const CacheArgs& c, ui
     if (o[k] >= 0) *reinterpret_cast<u4*>(d + o[k]) = v[k];
 }
 
-// What fork decided: `ok`, then per child the page of its part-filled end (or -1) and the parent's.
+// What fork decided, then per child the page of its part-filled end (or -1) and the parent's.
+enum : uint32_t { kForkNone = 0, kForkAll = 1, kForkUndo = 2 };  // kForkUndo: some full page is bad, pages were taken
 struct ForkPlan {
   uint32_t ok, pad[3];
   int2 tail[HQ_CACHE_MAX_BATCH];  // (from, to), (-1, -1): the parent ends with a full page
 };
 
+// Workgroup 0 plans; 1 + i looks over the full pages of parents[i] beside it (in the planning workgroup they took 3 us of 24
+// at 32 children of 4 parents). cnt: their arrivals, 2^16 for each that met a bad number, 2^28 for a plan that
+// refuses; the last one has the answer. Zero between calls.
+__device__ __forceinline__ void fork_arrive(ForkPlan* plan, uint32_t* cnt, uint32_t add, uint32_t n) {
+  const uint32_t sum = __hip_atomic_fetch_add(cnt, add + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + add + 1;
+  if ((sum & 0xFFFFu) != n + 1) return;
+  plan->ok = sum >> 28 ? kForkNone : sum >> 16 ? kForkUndo : kForkAll;
+  __hip_atomic_store(cnt, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 __global__ __launch_bounds__(kPlanThreads) void hq_cache_fork_plan_kernel(CacheArgs c, const int32_t* parents, const int32_t* children,
-                                                                          uint32_t n, ForkPlan* plan) {
+                                                                          uint32_t n, ForkPlan* plan, uint32_t* cnt) {
+  if (blockIdx.x > 0) {
+    const int32_t row = parents[blockIdx.x - 1];
+    bool odd = false;
+    if (row >= 0 && row < (int32_t)c.rows) {
+      const int32_t len = c.lens[row];
+      const uint32_t full = len > 0 ? min((uint32_t)len >> c.page_shift, c.max_pages) : 0u;
+      for (uint32_t j = threadIdx.x; j < full; j += kPlanThreads) odd |= (uint32_t)c.table[row * c.table_stride + j] >= c.pages;
+    }
+    odd = __syncthreads_or(odd);
+    if (threadIdx.x == 0) fork_arrive(plan, cnt, odd ? 1u << 16 : 0u, n);
+    return;
+  }
   __shared__ uint32_t sh[kPlanThreads / 64 + 1], fault;
   __shared__ int32_t list[HQ_CACHE_MAX_BATCH];
   __shared__ uint16_t who[HQ_CACHE_MAX_BATCH];
@@ -292,7 +314,7 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_fork_plan_kernel(CacheA
   __syncthreads();
   bad = fault;
   if (!bad && !pool.enough(c, need, sh)) bad = HQ_CACHE_NO_PAGES;
-  if (i == 0) plan->ok = !bad;
+  if (i == 0) fork_arrive(plan, cnt, bad ? 1u << 28 : 0u, n);
   if (bad) {
     if (i == 0) report(c.status, bad);
     return;
@@ -307,26 +329,30 @@ __global__ __launch_bounds__(kPlanThreads) void hq_cache_fork_plan_kernel(CacheA
 // others the part-filled page, a unit of one layer of one pool each.
 __global__ __launch_bounds__(kCopyThreads) void hq_cache_fork_kernel(CacheArgs c, const int32_t* parents, const int32_t* children,
                                                                      const ForkPlan* plan, uint32_t units) {
-  if (!plan->ok) return;
-  const uint32_t i = blockIdx.y;
+  const uint32_t i = blockIdx.y, ok = plan->ok;
+  if (ok == kForkNone) return;
   const int32_t p = parents[i], k = children[i], len = c.lens[p];
   const int2 tail = plan->tail[i];
   if (blockIdx.x == 0) {
+    if (ok == kForkUndo) {  // (here and not before the loads: stores ahead of them made the copies 1 us slower)
+      if (threadIdx.x == 0) {
+        if (tail.y >= 0) c.refs[tail.y] = 0;
+        if (i == 0) report(c.status, HQ_CACHE_BAD_PAGE);
+      }
+      return;
+    }
     const uint32_t full = (uint32_t)len >> c.page_shift;
     const int32_t* from = c.table + p * c.table_stride;
     int32_t* to = c.table + k * c.table_stride;
     for (uint32_t j = threadIdx.x; j < c.max_pages; j += kCopyThreads) {
       int32_t page = j < full ? from[j] : j == full ? tail.y : -1;
-      if (j < full) {
-        if ((uint32_t)page < c.pages) atomicAdd(c.refs + page, 1);
-        else report(c.status, HQ_CACHE_BAD_PAGE);
-      }
+      if (j < full) atomicAdd(c.refs + page, 1);
       to[j] = page;
     }
     if (threadIdx.x == 0) c.lens[k] = len;
     return;
   }
-  if (tail.x < 0) return;
+  if (tail.x < 0 || ok == kForkUndo) return;
   const uint32_t tokens = (uint32_t)len & ((1u << c.page_shift) - 1);
   const uint32_t x = blockIdx.x - 1, u = x % units, l = x / units;  // l: layer, then pool
   if (u >= units_of(c.shape, tokens)) return;
@@ -474,7 +500,8 @@ hipError_t launch_cache_append(const CacheArgs& c, uint32_t layer, const uint16_
 
 hipError_t launch_cache_fork(const CacheArgs& c, const int32_t* parents, const int32_t* children, uint32_t n, void* ws, hipStream_t s) {
   ForkPlan* plan = static_cast<ForkPlan*>(scratch(ws));
-  hipLaunchKernelGGL(hq_cache_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, c, parents, children, n, plan);
+  hipLaunchKernelGGL(hq_cache_fork_plan_kernel, dim3(1 + n), dim3(kPlanThreads), 0, s, c, parents, children, n, plan,
+                     static_cast<uint32_t*>(ws));
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const uint32_t units = units_of(c.shape, 1u << c.page_shift);
