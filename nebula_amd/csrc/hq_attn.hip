@@ -417,9 +417,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t keys_rsrc(const uint16_t* base
 // would hold every transposing read back until all copies under way have landed. Whoever uses it waits for
 // its copies itself; the compiler's own waits for loads only become longer by it. It has no destination
 // register.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // it warns that m0, its own, is not saved; named, it knows that what it put there is gone
 __device__ __forceinline__ void copy_to_lds16(u4 d, uint32_t to, uint32_t offset) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(d) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // ---- parts of rows whose keys are split ----
 // Row (token t, head h) has `slots` places: fp32 O [D] (not divided by the sum), the maximum times c and
