@@ -297,7 +297,10 @@ class KVCache:
         return int(b.value)
 
     def check(self) -> None:
-        """Waits for the device and raises HQError if a call met a fault there since the last check."""
+        """Waits for the device, all its streams, and raises HQError if a call met a fault there since the last check."""
+        import torch
+
+        torch.cuda.synchronize(self.device_index)
         got = int(self.status.item())
         if got:
             self.status.zero_()
