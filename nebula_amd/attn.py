@@ -304,6 +304,7 @@ class KVCache:
         got = int(self.status.item())
         if got:
             self.status.zero_()
+            torch.cuda.synchronize(self.device_index)  # not after what a call on another stream reports next
             raise hq.HQError(hq.HQ_ERR_DEVICE, "cache: " + "; ".join(text for bit, text in FAULTS.items() if got & bit))
 
 

@@ -19,3 +19,28 @@ def test_a_fault_on_another_stream_is_met(cuda):
     with pytest.raises(hq.HQError, match="free pages"):
         c.check()
     c.check()
+
+
+def test_the_next_fault_on_another_stream_is_kept(cuda):
+    """The word is clear when check() raises, and not some time after."""
+    c, _ = fresh(pages=2)
+    rows, counts, status = i32([0]), i32([100]), c.status
+    side = torch.cuda.Stream()
+
+    class Slow:
+        def item(self):
+            return status.item()
+
+        def zero_(self):
+            torch.cuda._sleep(200_000_000)
+            status.zero_()
+
+    c.reserve(rows, counts)
+    c.status = Slow()
+    with pytest.raises(hq.HQError, match="free pages"):
+        c.check()
+    c.reserve(rows, counts, stream=side)
+    torch.cuda.synchronize()
+    c.status = status
+    with pytest.raises(hq.HQError, match="free pages"):
+        c.check()
