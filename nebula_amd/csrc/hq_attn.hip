@@ -137,6 +137,10 @@ __device__ __forceinline__ uint32_t seen2(uint32_t key, uint32_t lim) {
   return (key < lim ? one : 0u) | (key + 1 < lim ? one << 16 : 0u);
 }
 
+// Weights are exp2(c s - fl(c m)): past 2^22 the product's rounding is more than 1/4 of a power of two, at 2^28 16
+// powers and fp16's weights lose bits or vanish, at 2^31 fp32's do. Rows whose maximum is past it are computed
+// again from c (s - m).
+constexpr float kFar = 4194304.f;
 constexpr float kNone = -FLT_MAX;  // the maximum of no score: finite, so that differences with it are no NaN
 
 __device__ __forceinline__ void report(uint32_t* status, uint32_t what) {
@@ -763,9 +767,8 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
     for (; t < t1; ++t) ahead(t);  // the others' tiles
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the last one asked for none)
   }
-  // Again where values are not finite, or a row has no weight: V at keys a row may not see, times its weight
-  // 0, may have made them, or scores past 1e7. Tile by tile, differences of scores before the factor (m c may
-  // be rounded by more than the exponential's range), and those values apart.
+  // Again where values are not finite (V at keys a row may not see, times its weight 0, may have made them), or
+  // scores are far (kFar). Tile by tile, differences of scores before the factor, and those values apart.
   auto odd = [&]() {
     const f2 e = both_halves(l, l);
     l = e[0] + e[1];
@@ -774,7 +777,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
     for (int dt = 0; dt < kDims; ++dt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) bad = fmaf(o[dt][v], 0.f, bad);
-    return !(bad == 0.f) || (l == 0.f && m != kNone);
+    return !(bad == 0.f) || (m != kNone && fabsf(m * c) > kFar);
   };
   if (__syncthreads_or(odd())) {
     reset();
@@ -1118,7 +1121,7 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
     for (int dt = 0; dt < kDims; ++dt)
 #pragma unroll
       for (int v = 0; v < 4; ++v) bad = fmaf(o[dt][v], 0.f, bad);
-    return __any(!(bad == 0.f) || (l == 0.f && m != kNone)) != 0;
+    return __any(!(bad == 0.f) || (m != kNone && fabsf(m * c) > kFar)) != 0;
   };
   auto start = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -1141,7 +1144,7 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
     if constexpr (PAGED) pages.now = pages.held(a.k, 0, now);
     for (; t + stride < tiles; t += stride, ++n) tile(n, begin + t * kRowKeys, std::false_type{}, std::true_type{});
     tile(n, begin + t * kRowKeys, std::false_type{}, std::false_type{});
-    // Again, tile by tile, where values are not finite or a row has no weight, as in the tile kernel.
+    // Again, tile by tile, where values are not finite or scores are far, as in the tile kernel.
     if (finish()) {
       start();
       if constexpr (PAGED) pages.start(a.k);
