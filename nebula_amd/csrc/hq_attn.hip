@@ -1096,7 +1096,7 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
 #pragma unroll
       for (int i = 0; i < 4; ++i) at[i] = stage_at + v_at[d0 + i];
       lds_read_tr<0, 16 * (int)kPitch>(at, f);
-      if (careful && masked) {
+      if constexpr (careful) {
         const u4 sees = {seen2<DT>(k0 + 4 * quad, lim), seen2<DT>(k0 + 4 * quad + 2, lim), seen2<DT>(k0 + 16 + 4 * quad, lim),
                          seen2<DT>(k0 + 16 + 4 * quad + 2, lim)};
 #pragma unroll
