@@ -1499,7 +1499,8 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     const uint32_t n = p.prefix ? groups : seqs, likely = n * up(up(all_rows, n), 128);
     uint32_t most;
     p.tile_splits = tile_splits((uint64_t)likely * kv_heads, (uint64_t)rows * heads, dim, keys, p.prefix, most);
-    p.tile_grid = tiles * kv_heads * p.tile_splits;
+    p.largest = (uint64_t)tiles * kv_heads * p.tile_splits;
+    p.tile_grid = (uint32_t)p.largest;
     if (p.prefix || p.tile_splits > 1) p.parts = p.tile_splits + (p.prefix ? 1 : 0);
     const size_t all = (size_t)rows * heads, places = all * p.parts, held = p.prefix || most > 1 ? all * (most + (p.prefix ? 1 : 0)) : 0;
     p.part_ml = take(places * sizeof(f2), held * sizeof(f2));
@@ -1514,11 +1515,13 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     p.row_one = p.row_slots && tiles == 1;
     p.row_like = keys;
     p.row_grid = (p.row_slots ? p.row_slots : tiles) * kv_heads;
+    p.largest += (uint64_t)(p.row_slots ? p.row_slots : tiles) * kv_heads;
     // More keys have no fewer slots; those past a prefix are most where there is none.
     const size_t place = (size_t)kv_heads * 16, places = p.row_slots * place, held = row_slots(tiles, kv_heads, dim, max_keys) * place;
     p.row_ml = take(places * sizeof(f2), held * sizeof(f2));
     p.row_o = take(places * dim * sizeof(float), held * dim * sizeof(float));
   }
+  if (p.parts) p.largest = std::max(p.largest, ((uint64_t)rows * heads + 3) / 4);
   p.ws = ws > kCounterBytes ? ws : 0;
   p.need = need > kCounterBytes ? need : 0;
   return p;

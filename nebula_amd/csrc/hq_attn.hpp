@@ -49,8 +49,11 @@ struct AttnPlan {
   uint32_t row_slots = 0, row_one = 0, row_like = 0;  // workgroups of a kv head that share rows' keys (0: none share), keys of a row past its prefix
   uint32_t parts = 0;              // parts of a row that are joined by a launch of their own (0: rows are written out)
   size_t part_ml = 0, part_o = 0, row_ml = 0, row_o = 0, ws = 0;  // workspace offsets, and its size
+  uint64_t largest = 0;            // workgroups of its largest launch
   size_t need = 0;                 // not falling in the keys: what calls of fewer keys need at most, and this one
 };
+// A launch has fewer than 2^32 threads in a grid's dimension; all here have 256 a workgroup.
+constexpr uint64_t kMaxGrid = 0xFFFFFFFFu / 256u;
 // max_prefix: 0, where it is not known.
 AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                    uint32_t dim, uint32_t max_keys, uint32_t max_prefix);

@@ -136,6 +136,9 @@ hq_status check_cache(const hq_kv_cache* c, hq::CacheArgs* out) {
       (c->layers > 1 && c->layer_stride < dense) || c->layer_stride < 0 || c->layer_stride > kMaxSpan)
     return fail(HQ_ERR_SHAPE, "cache: page_stride=%lld, layer_stride=%lld must be multiples of 8 and at least a page (%lld)",
                 (long long)c->page_stride, (long long)c->layer_stride, (long long)dense);
+  // fork and copy_pages move it by one launch (16 KB a workgroup).
+  if ((uint64_t)dense * c->layers * 4 > (1ull << 37))
+    return fail(HQ_ERR_SHAPE, "cache: a page of %u layers has %lld bytes a layer: above 128 GiB", c->layers, (long long)dense * 4);
   if (misaligned(c->K, 16) || misaligned(c->V, 16)) return fail(HQ_ERR_ALIGNMENT, "cache: K and V must be 16-byte aligned");
   if (misaligned(c->table, 4) || misaligned(c->lens, 4) || misaligned(c->refs, 4) || misaligned(c->status, 4) || misaligned(c->refused, 4))
     return fail(HQ_ERR_ALIGNMENT, "cache: table, lens, refs, status and refused must be 4-byte aligned");
@@ -188,13 +191,18 @@ hq_status workspace(void* ws, size_t bytes, size_t use, size_t need, hipStream_t
   return HQ_OK;
 }
 
+hq_status check_plan(const hq::AttnPlan& p) {
+  if (p.largest > hq::kMaxGrid) return fail(HQ_ERR_SHAPE, "%llu workgroups: too many rows and heads for one call", (unsigned long long)p.largest);
+  return HQ_OK;
+}
+
 hq_status run_attn(const hq::AttnArgs& a, int kind, int dtype, uint32_t max_keys, uint32_t max_prefix, void* ws, size_t bytes,
                    hq_stream stream) {
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const hq::AttnPlan p = hq::plan_attn(kind, a.T, a.B, a.groups, a.H, a.Hkv, a.D, max_keys, max_prefix);
   void* w = nullptr;
-  const hq_status st = workspace(ws, bytes, p.ws, p.need, s, &w);
-  if (st != HQ_OK) return st;
+  hq_status st = check_plan(p);
+  if (st != HQ_OK || (st = workspace(ws, bytes, p.ws, p.need, s, &w)) != HQ_OK) return st;
   return from_hip(hq::launch_attn(dtype, a, p, w, s), "attention launch");
 }
 
@@ -249,18 +257,22 @@ extern "C" {
 hq_status hq_attn_workspace_bytes(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads,
                                   uint32_t kv_heads, uint32_t head_dim, uint32_t max_keys, uint32_t max_prefix, size_t* bytes) {
   if (!bytes) return fail(HQ_ERR_INVALID_ARG, "bytes is null");
-  const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys);
+  hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys);
   if (st != HQ_OK) return st;
-  *bytes = hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix).need;
+  const hq::AttnPlan p = hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix);
+  if ((st = check_plan(p)) != HQ_OK) return st;
+  *bytes = p.need;
   return hq_set_error(HQ_OK, "");
 }
 
 hq_status hq_describe_attn(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim, uint32_t max_keys, uint32_t max_prefix, char* buf, size_t buf_len) {
   if (!buf || buf_len == 0) return fail(HQ_ERR_INVALID_ARG, "buf is null or empty");
-  const hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys);
+  hq_status st = check_query(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys);
   if (st != HQ_OK) return st;
-  hq::describe_attn(hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix), buf, buf_len);
+  const hq::AttnPlan p = hq::plan_attn(kind, rows, seqs, groups, heads, kv_heads, head_dim, max_keys, max_prefix);
+  if ((st = check_plan(p)) != HQ_OK) return st;
+  hq::describe_attn(p, buf, buf_len);
   return hq_set_error(HQ_OK, "");
 }
 
@@ -358,6 +370,8 @@ hq_status hq_cache_append(const hq_kv_cache* cache, uint32_t layer, const void* 
   if ((st = check_strides("K", k_row, k_head, tokens, c.kv_heads, c.dim)) != HQ_OK ||
       (st = check_strides("V", v_row, v_head, tokens, c.kv_heads, c.dim)) != HQ_OK)
     return st;
+  if ((uint64_t)tokens * c.kv_heads * (c.dim / 8) > 256 * hq::kMaxGrid)
+    return fail(HQ_ERR_SHAPE, "tokens=%u of %u heads of %u: too many for one call", tokens, c.kv_heads, c.dim);
   if (!c.refused) return fail(HQ_ERR_INVALID_ARG, "cache: refused is null");
   return from_hip(hq::launch_cache_append(c, layer, static_cast<const uint16_t*>(K), k_row, k_head, static_cast<const uint16_t*>(V), v_row,
                                           v_head, tokens, rows, cu, n, reinterpret_cast<hipStream_t>(stream)),
