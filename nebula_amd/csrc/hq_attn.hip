@@ -1517,7 +1517,8 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
     p.row_grid = (p.row_slots ? p.row_slots : tiles) * kv_heads;
     p.largest += (uint64_t)(p.row_slots ? p.row_slots : tiles) * kv_heads;
     // More keys have no fewer slots; those past a prefix are most where there is none.
-    const size_t place = (size_t)kv_heads * 16, places = p.row_slots * place, held = row_slots(tiles, kv_heads, dim, max_keys) * place;
+    const uint32_t most = keys == max_keys ? p.row_slots : row_slots(tiles, kv_heads, dim, max_keys);
+    const size_t place = (size_t)kv_heads * 16, places = p.row_slots * place, held = most * place;
     p.row_ml = take(places * sizeof(f2), held * sizeof(f2));
     p.row_o = take(places * dim * sizeof(float), held * dim * sizeof(float));
   }
