@@ -105,7 +105,8 @@ hq_status hq_attn_prompt(const hq_attn_io* io, const void* K, int64_t k_row, int
 
 /* New tokens over a layer of the cache, causal. Sequence b is row rows[b] of the cache (rows NULL:
  * row b); its lens tokens are the keys, and the last cu_q[b + 1] - cu_q[b] of them (cu_q NULL: the
- * last one; then io->rows = seqs) are those of Q. max_len as max_k above (0: what a row can hold). */
+ * last one; then io->rows = seqs) are those of Q. max_len as max_k above (0: what a row can hold). The kernel
+ * is chosen by the mean number of new tokens: single tokens and a long chunk are faster as two calls. */
 hq_status hq_attn_paged(const hq_attn_io* io, const hq_kv_cache* cache, uint32_t layer, const int32_t* rows,
                         const int32_t* cu_q, uint32_t seqs, uint32_t max_len, void* workspace,
                         size_t workspace_bytes, hq_stream stream);

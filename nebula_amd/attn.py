@@ -361,7 +361,8 @@ def paged(q, cache: KVCache, layer: int, rows=None, cu_seqlens=None, max_len: in
           with_lse: bool = False, stream=None, workspace=None):
     """Causal attention of new tokens over a layer of the cache, theirs among it: tokens
     [cu_seqlens[b], cu_seqlens[b + 1]) of q are the last ones of cache row rows[b] (cu_seqlens None: one
-    token a row; rows None: row b). max_len: no row is longer (a hint for the split)."""
+    token a row; rows None: row b). max_len: no row is longer (a hint for the split). Single tokens and a long
+    chunk are faster as two calls: the mean number of new tokens chooses the kernel."""
     _check_cached(q, cache)
     dev = cache.device_index
     seqs = q.shape[0] if cu_seqlens is None else max(cu_seqlens.numel() - 1, 0)

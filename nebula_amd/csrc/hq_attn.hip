@@ -86,7 +86,8 @@ __device__ __forceinline__ void each(F f) {
 }
 
 // Two weights, each rounded to nearest in the activation type (it is the type of V, and the MFMA has
-// one for both operands).
+// one for both operands): outputs are off by 1.1 to 1.4 times what they are with fp32 weights (relative to their
+// norm, bf16 0.0019 to 0.0023 for 0.0015 to 0.0017, fp16 0.00019 to 0.00029 for 0.00017 to 0.00021).
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (DT == HQ_DTYPE_F16) return h2_bits(__builtin_convertvector((f2{a, b}), h2));
@@ -460,11 +461,12 @@ __device__ __forceinline__ uint32_t swz_v(uint32_t r) {
 // V (1 KB from LDS) is one product of 32 rows, 32 cycles of LDS for the CU's four SIMDs and 32 of each
 // one's matrix pipe; 32 scores a lane are about as many cycles of the vector pipe as their 16 + 16 products at
 // 128 dims. So the three run side by side: the next tile's scores beside this one's exponentials, K fragments
-// read a step and V fragments two products ahead. 8192 tokens on 48/8 heads of 128, bf16: 736 us, 1120
-// TFLOP/s, matrix, LDS and vector pipes busy 62, 62 and 57% at the 1.6 GHz that the card holds under it, no bank
-// conflicts. Heads of 256 leave registers for one wavefront a SIMD (a workgroup a CU): 2048 + 1531 tokens on 24/4
-// heads 111 us, 724 TFLOP/s, matrix pipe 33%; tiles of 32 keys 10% slower there and everywhere, of 128 on heads
-// of 64 slower too. A workgroup alone on its CU takes 1.1 us a tile, 0.9 without its copies: the rest is issue and
+// read a step and V fragments two products ahead. 8192 tokens on 48/8 heads of 128, bf16: 721 us in the trace of the
+// counters, 1143 TFLOP/s, matrix pipe busy 67% (LDS as much, by its bytes) and vector pipe 61% at the 1.65 GHz that the card
+// holds under it, no bank conflicts (718 to 760 us over boxes). Heads of 256 leave registers for one wavefront a SIMD (a workgroup
+// a CU): 2048 + 1531 tokens on 24/4 heads 113 us, 711 TFLOP/s, matrix pipe 33%; tiles of 32 keys 10% slower there and
+// everywhere, of 128 on heads of 64 slower too. Heads of 64 have twice the exponentials a product: 4096 tokens on 32/4 heads
+// 84 us, 816 TFLOP/s, vector pipe 71%, matrix pipe 42%. A workgroup alone on its CU takes 1.1 us a tile, 0.9 without its copies: the rest is issue and
 // latency, so short calls gain by sharing keys (tile_splits).
 constexpr int kKeys = 64;  // keys of a tile
 
@@ -896,8 +898,8 @@ constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on othe
 // Tiles of 32 keys go to the shares' wavefronts in turn, (round * shares + share) * 4 + wavefront. A
 // wavefront's K goes straight into the registers of its first product (a lane's 16 bytes of a row are 8
 // consecutive dims, four lanes take 64 bytes), its V through LDS; both are a tile ahead, 32 KB a CU and more
-// in flight. Bound by memory: 64 rows on 2048 tokens, 48/8 heads of 128, 94 us, 5.7 TB/s of keys and values; 16
-// rows on 37 to 8192, 24/4 heads of 256, 27 us, 4.0 TB/s (two wavefronts a workgroup, twice the parts to join
+// in flight. Bound by memory: 64 rows on 2048 tokens, 48/8 heads of 128, 91 us, 5.9 TB/s of keys and values (97 where
+// pages hold tokens before heads); 16 rows on 37 to 8192, 24/4 heads of 256, 27 us, 4.0 TB/s (two wavefronts a workgroup, twice the parts to join
 // by half the threads: 41). One row on 777: 8 us of launch, first loads, parts and join.
 template <int DT, int D, bool PAGED>
 __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, uint32_t block) {
@@ -1479,7 +1481,9 @@ AttnPlan plan_attn(int kind, uint32_t rows, uint32_t seqs, uint32_t groups, uint
   const uint64_t all_rows = (uint64_t)rows * G;
   p.prefix = kind == HQ_ATTN_SHARED;
   // Few rows a sequence: tiles of 16. 16 sequences of 48 rows on up to 3000 keys took 34 us in tiles of 128 and 49
-  // in tiles of 16, 8 of 24 rows 24 in both.
+  // in tiles of 16, 8 of 24 rows 24 in both. It is the mean that counts, for the lengths are on the device: 16 single tokens on
+  // 200 to 4096 keys and 64 tokens after 6000, 48/8 heads of 128, take 85 us in one call, in tiles of 16, and 52 in two
+  // calls of a kind each, as a decoder's step makes them.
   p.row = p.prefix || all_rows <= 32ull * seqs;
   p.tile = p.prefix || !p.row;
   max_keys = std::max(max_keys, 1u);
