@@ -196,6 +196,20 @@ __device__ __forceinline__ uint32_t whole_pages(const AttnKeys& k, int32_t first
   return min(len, clamp_u(prefix, 1u << 30)) >> k.page_shift << k.page_shift;
 }
 
+// Whether the groups hold each of B sequences once: starts from 0 to B, not falling. Where they don't, every workgroup finds
+// so, none works on a prefix and all keys of a row are its own. Of entry b, and of entries base .. n - 1.
+__device__ __forceinline__ bool entry_ok(int32_t first, int32_t end, uint32_t b, uint32_t n, uint32_t B) {
+  return first <= end && (b > 0 || first == 0) && (b + 1 < n || end == (int32_t)B);
+}
+__device__ __forceinline__ bool entries_ok(const int32_t* starts, uint32_t base, uint32_t n, uint32_t B) {
+  bool good = true;
+  for (; base < n; base += 64) {
+    const uint32_t b = min(base + (threadIdx.x & 63u), n - 1);
+    good = good && entry_ok(starts[b], starts[b + 1], b, n, B);
+  }
+  return __ballot(!good) == 0;
+}
+
 // Tokens of entry b of a list of offsets (queries of a sequence, sequences of a group), held to [0, most].
 __device__ __forceinline__ uint32_t span(const int32_t* cu, uint32_t b, uint32_t most, uint32_t& first) {
   first = clamp_u(cu[b], most);
@@ -205,6 +219,7 @@ __device__ __forceinline__ uint32_t span(const int32_t* cu, uint32_t b, uint32_t
 
 // The idx-th tile of `rows` rows over all entries, by one wavefront: the entries' tiles are counted 64
 // at a time. Inside an entry the last tile comes first: under the causal mask it has the most keys.
+template <bool GROUPS>
 __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_t most, uint32_t G, uint32_t rows, uint32_t idx,
                                           Work& w) {
   const uint32_t lane = threadIdx.x & 63u;
@@ -222,7 +237,15 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_
   for (uint32_t base = 0; base < n; base += 64) {
     const uint32_t b = base + lane;
     uint32_t first = 0, nq = 0;
-    if (b < n) nq = span(cu, b, most, first);
+    if constexpr (GROUPS) {
+      const uint32_t at = min(b, n - 1);
+      const int32_t lo = cu[at], hi = cu[at + 1];
+      if (__ballot(!entry_ok(lo, hi, at, n, most))) return false;
+      first = (uint32_t)lo;
+      nq = b < n ? (uint32_t)(hi - lo) : 0u;
+    } else {
+      if (b < n) nq = span(cu, b, most, first);
+    }
     const uint32_t tiles = (nq * G + rows - 1) / rows;
     const uint32_t x = scan_sum(tiles);
     const uint64_t past = __ballot(before + x > idx);
@@ -233,7 +256,7 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, uint32_t n, uint32_
       w.nq = lane_value(nq, at);
       w.R = w.nq * G;
       w.r0 = (before + lane_value(x, at) - 1 - idx) * rows;
-      return true;
+      return !GROUPS || entries_ok(cu, base + 64, n, most);
     }
     before += lane_value(x, 63);
   }
@@ -250,7 +273,7 @@ struct Share {
   uint32_t split, of;  // this workgroup's number among those of its tile
   int32_t row, len;    // paged: cache row of the sequence, and its length as read
 };
-template <uint32_t WAVES, bool PAGED>
+template <uint32_t WAVES, bool PAGED, bool GROUPS>
 __device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t slots, uint32_t like, uint32_t slot, Work& w, Share& sh) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t first, nq, tiles, keys;
@@ -268,7 +291,7 @@ __device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t slots, ui
       }
       if constexpr (PAGED) {
         len = row_length(a.k, row);
-        keys = a.groups ? like : clamp_u(len, a.k.max_pages << a.k.page_shift);  // of a group: all alike
+        keys = GROUPS ? like : clamp_u(len, a.k.max_pages << a.k.page_shift);  // of a group: all alike
       } else if (a.k.cu_k == a.cu_q && a.k.total_k >= a.T) {
         keys = nq;
       } else {
@@ -324,41 +347,25 @@ __device__ __forceinline__ bool find_share(const AttnArgs& a, uint32_t slots, ui
   return false;
 }
 
-// Whether the groups hold each sequence once: starts from 0 to B, not falling. Where they don't, every workgroup
-// finds so, none works on a prefix and all keys of a row are its own. The first 64 are loaded beside what a
-// workgroup starts with and looked at after it.
-struct Groups {
-  int32_t first, end;
-  __device__ __forceinline__ void load(const AttnArgs& a, uint32_t base) {
-    const uint32_t g = min(base + (threadIdx.x & 63u), a.groups - 1);
-    first = a.starts[g];
-    end = a.starts[g + 1];
-  }
-  __device__ __forceinline__ bool ok(const AttnArgs& a) {
-    bool good = true;
-    for (uint32_t base = 0;;) {
-      const uint32_t g = min(base + (threadIdx.x & 63u), a.groups - 1);
-      good = good && first <= end && (g > 0 || first == 0) && (g + 1 < a.groups || end == (int32_t)a.B);
-      base += 64;
-      if (base >= a.groups) return __all(good);
-      load(a, base);
-    }
-  }
-};
-
-// The group of sequence b, the last one that starts at or before it, and where it starts.
-__device__ __forceinline__ uint32_t group_of(const AttnArgs& a, uint32_t b, uint32_t& first) {
+// The group of sequence b, the last one that starts at or before it, where it starts, and whether all are sound (looked at
+// here, with the entries at hand: in a pass of its own it took 0.4 us of 28).
+__device__ __forceinline__ uint32_t group_of(const AttnArgs& a, uint32_t b, uint32_t& first, bool& ok) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t g = 0;
+  bool good = true;
   first = 0;
   for (uint32_t base = 0; base < a.groups; base += 64) {
-    const int32_t at = base + lane < a.groups ? a.starts[base + lane] : 0x7FFFFFFF;
-    const uint64_t before = __ballot(at <= (int32_t)b);
-    if (!before) break;
-    const int last = 63 - __builtin_clzll(before);
-    g = base + last;
-    first = clamp_u(__builtin_amdgcn_readlane(at, last), a.B - 1);
+    const uint32_t i = min(base + lane, a.groups - 1);
+    const int32_t at = a.starts[i], end = a.starts[i + 1];
+    good = good && entry_ok(at, end, i, a.groups, a.B);
+    const uint64_t before = __ballot(at <= (int32_t)b && base + lane < a.groups);
+    if (before) {
+      const int last = 63 - __builtin_clzll(before);
+      g = base + last;
+      first = clamp_u(__builtin_amdgcn_readlane(at, last), a.B - 1);
+    }
   }
+  ok = __ballot(!good) == 0;
   return g;
 }
 
@@ -440,7 +447,6 @@ struct Parts {
 
 struct TilePlan {
   uint32_t splits;  // workgroups that share a tile's keys, in equal runs of them
-  uint32_t prefix;  // rows are the sequences of a group, keys its shared prefix
   Parts parts;
 };
 
@@ -475,7 +481,7 @@ constexpr uint32_t tile_stage_bytes() {
   return 2u * kKeys * D * 2u;
 }
 
-template <int DT, int D, int NW, bool PAGED>
+template <int DT, int D, int NW, bool PAGED, bool PREFIX>
 __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl, uint32_t block) {
   constexpr uint32_t BR = NW * 32;
   constexpr uint32_t kPitch = 2 * D, kStage = tile_stage_bytes<D>(), kVOff = kStage / 2;
@@ -491,9 +497,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
   const uint32_t kvh = block % a.Hkv, rest = block / a.Hkv;
   const uint32_t split = rest % pl.splits, idx = rest / pl.splits;
   Work w{};
-  Groups groups{};
-  if (PAGED && pl.prefix) groups.load(a, 0);
-  if (!find_tile(pl.prefix ? a.starts : a.cu_q, pl.prefix ? a.groups : a.B, pl.prefix ? a.B : a.T, a.G, BR, idx, w)) return;
+  if (!find_tile<PREFIX>(PREFIX ? a.starts : a.cu_q, PREFIX ? a.groups : a.B, PREFIX ? a.B : a.T, a.G, BR, idx, w)) return;
   // This lane's row.
   const uint32_t r_mine = w.r0 + wave * 32 + l32;
   const bool live = r_mine < w.R;
@@ -502,12 +506,11 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
   const int32_t* table = nullptr;
   uint32_t nk, lim = 0;  // keys of the sequence, and those below lim this lane's row may see
   if constexpr (PAGED) {
-    const int32_t row = row_number(a.k, pl.prefix ? w.q0 : w.b);
+    const int32_t row = row_number(a.k, PREFIX ? w.q0 : w.b);
     table = a.k.table + (row_ok(a.k, row) ? row : 0) * a.k.table_stride;
-    if (pl.prefix) {
+    if constexpr (PREFIX) {
       const int32_t own = row_number(a.k, w.q0 + token), prefix = a.prefix[w.b];
       const int32_t len = row_length(a.k, row), own_len = row_length(a.k, own);
-      if (!groups.ok(a)) return;
       nk = uni(whole_pages(a.k, row, len, prefix));
       lim = min(nk, length_or_report(a.k, own, own_len));
     } else {
@@ -520,7 +523,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
     nk = uni(span(a.k.cu_k, w.b, a.k.total_k, w.key0));
     w.key0 = uni(w.key0);
   }
-  if (!pl.prefix) {
+  if constexpr (!PREFIX) {
     lim = nk;
     if (a.causal) {
       const int64_t n = (int64_t)token + nk - w.nq + 1;
@@ -531,7 +534,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
 
   // Keys of this workgroup: up to the last that any of its rows sees.
   uint32_t wg_lim = nk;
-  if (!pl.prefix && a.causal) {
+  if (!PREFIX && a.causal) {
     const int64_t n = (int64_t)((min(w.r0 + BR, w.R) - 1) / a.G) + nk - w.nq + 1;
     wg_lim = n < 0 ? 0u : (uint32_t)n;
   }
@@ -864,7 +867,7 @@ __device__ __forceinline__ void tile_body(const AttnArgs& a, const TilePlan& pl,
 
 template <int DT, int D, int NW, bool PAGED>
 __global__ __launch_bounds__(NW * 64, D == 256 ? 1 : 2) void hq_attn_tile_kernel(AttnArgs a, TilePlan pl) {
-  tile_body<DT, D, NW, PAGED>(a, pl, blockIdx.x);
+  tile_body<DT, D, NW, PAGED, false>(a, pl, blockIdx.x);
 }
 
 // ---- few rows ----
@@ -901,7 +904,7 @@ constexpr int kAgent = 16;  // cache policy of parts: seen by workgroups on othe
 // in flight. Bound by memory: 64 rows on 2048 tokens, 48/8 heads of 128, 91 us, 5.9 TB/s of keys and values (97 where
 // pages hold tokens before heads); 16 rows on 37 to 8192, 24/4 heads of 256, 27 us, 4.0 TB/s (two wavefronts a workgroup, twice the parts to join
 // by half the threads: 41). One row on 777: 8 us of launch, first loads, parts and join.
-template <int DT, int D, bool PAGED>
+template <int DT, int D, bool PAGED, bool GROUPS>
 __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, uint32_t block) {
   constexpr uint32_t NW = kRowWaves;
   constexpr uint32_t kPitch = 2 * D, kStage = kRowKeys * kPitch;
@@ -916,9 +919,9 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
   Share sh{0, 1, 0, 0};
   const bool find = pl.slots && !pl.one;
   if (find) {
-    if (!find_share<NW, PAGED>(a, pl.slots, pl.like, slot, w, sh)) return;
+    if (!find_share<NW, PAGED, GROUPS>(a, pl.slots, pl.like, slot, w, sh)) return;
   } else {
-    if (!find_tile(a.cu_q, a.B, a.T, a.G, 16, pl.one ? 0u : slot, w)) return;
+    if (!find_tile<false>(a.cu_q, a.B, a.T, a.G, 16, pl.one ? 0u : slot, w)) return;
     if (pl.one) {
       sh.split = slot;
       sh.of = pl.slots;
@@ -936,24 +939,19 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
   bool grouped = true;
   if constexpr (PAGED) {
     uint32_t g = 0, first = 0;
-    Groups groups{};
-    if (a.groups) {
-      groups.load(a, 0);
-      g = group_of(a, w.b, first);
-    }
+    if constexpr (GROUPS) g = group_of(a, w.b, first, grouped);
     const int32_t row = sh.row;
     table = a.k.table + (row_ok(a.k, row) ? row : 0) * a.k.table_stride;
     if (!find) sh.len = row_length(a.k, row);
-    if (a.groups) {
+    if constexpr (GROUPS) {
       const int32_t first_row = row_number(a.k, first), prefix = a.prefix[g];
       const int32_t first_len = row_length(a.k, first_row);
       nk = uni(length_or_report(a.k, row, sh.len));
-      grouped = groups.ok(a);
       begin = grouped ? min(nk, uni(whole_pages(a.k, first_row, first_len, prefix))) : 0u;
       if (!grouped) report(a.k.status, HQ_CACHE_BAD_ROW);
     }
     early = table[min((begin + t_first * kRowKeys + (lane & 1u) * 16) >> a.k.page_shift, a.k.max_pages - 1)];
-    if (!a.groups) nk = uni(length_or_report(a.k, row, sh.len));
+    if constexpr (!GROUPS) nk = uni(length_or_report(a.k, row, sh.len));
   } else if (a.k.cu_k == a.cu_q && a.k.total_k >= a.T) {
     nk = w.nq;
     w.key0 = w.q0;
@@ -1199,7 +1197,7 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
   };
   auto store = [&](uint32_t row, uint32_t d, f4 v, float mc, float sum) {
     const uint32_t rr = w.r0 + row, tk = w.q0 + rr / a.G, hd = kvh * a.G + rr % a.G;
-    if (pl.to.slots) {
+    if (GROUPS) {
       const uint64_t at = ((uint64_t)tk * a.H + hd) * pl.to.slots + pl.to.slots - 1;
       if (d == 0) {
         pl.to.ml[at] = f2{mc, sum};
@@ -1291,7 +1289,7 @@ __device__ __forceinline__ void row_body(const AttnArgs& a, const RowPlan& pl, u
 
 template <int DT, int D, bool PAGED>
 __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a, RowPlan pl) {
-  row_body<DT, D, PAGED>(a, pl, blockIdx.x);
+  row_body<DT, D, PAGED, false>(a, pl, blockIdx.x);
 }
 
 // ---- shared prefixes ----
@@ -1301,8 +1299,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void hq_attn_row_kernel(AttnArgs a,
 // for 158.
 template <int DT, int D>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void hq_attn_prefix_kernel(AttnArgs a, TilePlan t, RowPlan r, uint32_t tile_blocks) {
-  if (blockIdx.x < tile_blocks) tile_body<DT, D, 4, true>(a, t, blockIdx.x);
-  else row_body<DT, D, true>(a, r, blockIdx.x - tile_blocks);
+  if (blockIdx.x < tile_blocks) tile_body<DT, D, 4, true, true>(a, t, blockIdx.x);
+  else row_body<DT, D, true, true>(a, r, blockIdx.x - tile_blocks);
 }
 
 // ---- joining parts ----
@@ -1379,7 +1377,7 @@ hipError_t launch_all(const AttnArgs& a, const AttnPlan& p, void* ws, hipStream_
     parts.ml = reinterpret_cast<f2*>(w + p.part_ml);
     parts.o = reinterpret_cast<float*>(w + p.part_o);
   }
-  const TilePlan t{p.tile_splits, p.prefix, parts};
+  const TilePlan t{p.tile_splits, parts};
   RowPlan r{};
   r.slots = p.row_slots;
   r.one = p.row_one;
