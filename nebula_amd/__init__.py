@@ -3,6 +3,6 @@
 The compute lives in libnebula_hq.so (HIP, built by nebula_amd.build); this package
 holds its ctypes bindings (nebula_amd.hq, nebula_amd.attn) and the build recipe.
 """
-from . import attn, hq  # noqa: F401
+from . import attn, hq, rotary, ssm  # noqa: F401
 
-__all__ = ["attn", "hq"]
+__all__ = ["attn", "hq", "rotary", "ssm"]

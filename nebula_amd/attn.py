@@ -4,7 +4,7 @@ layer's q | k | v projections (nebula_amd.hq, nebula_amd.decoder) and its output
     cache = KVCache.create(layers, pages, page_tokens, kv_heads, head_dim, rows, max_pages, dtype)
     cache.reserve(rows, counts)                    # once a step: room for its new tokens
     for each layer:
-        cache.append(layer, k, v, rows, cu)        # the layer's new keys and values
+        cache.append(layer, k, v, rows, cu)        # the layer's new keys and values (append_rotated: normed and rotated)
         y = paged(q, cache, layer, rows, cu)       # or prompt(...), shared_prefix(...)
     cache.fork(parents, children); cache.free(rows); cache.compact()
 
@@ -167,6 +167,18 @@ def _scale(scale: Optional[float], D: int) -> float:
 
 
 # ---------------------------------------------------------------- the cache
+_rotary_module = None
+
+
+def _rotary():
+    global _rotary_module
+    if _rotary_module is None:
+        from . import rotary
+
+        _rotary_module = rotary
+    return _rotary_module
+
+
 class KVCache:
     """A paged key/value cache over the caller's tensors.
 
@@ -257,6 +269,13 @@ class KVCache:
                                                 hq._stream_ptr(stream))
         if st:
             hq.check(st)
+
+    def append_rotated(self, layer: int, rotary, q, k, v, rows, cu_seqlens=None, q_weight=None, k_weight=None, eps: float = 1e-6,
+                       out=None, stream=None):
+        """append() with k normed and rotated (nebula_amd.rotary) on its way into the pages by its tokens' places in their
+        rows, and q [tokens, heads, head_dim] (None: none) likewise to out: one launch. Returns q's output, which may be q.
+        Where append() skips a token, its q is written all the same."""
+        return _rotary().append(self, layer, rotary, q, k, v, rows, cu_seqlens, q_weight, k_weight, eps, out, stream)
 
     def fork(self, parents, children, stream=None, workspace=None) -> None:
         """children[i], an empty row, becomes a copy of parents[i]: full pages shared, a part-filled one copied."""

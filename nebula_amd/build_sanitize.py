@@ -18,7 +18,7 @@ from .build import ARCH, BUILD, COMMON_FLAGS, CSRC, HIPCC, LIBDIR, ORACLE_DIR, S
 SAN_LIB = LIBDIR / "libnebula_hq_san.so"
 SAN_HOST = ["-fsanitize=address", "-fsanitize=undefined", "-fno-sanitize-recover=undefined",
             "-fno-omit-frame-pointer", "-shared-libsan", "-g"]
-SAN_SOURCES = ["hq_api.cpp", "hq_gguf.cpp", "hq_attn_api.cpp"]
+SAN_SOURCES = ["hq_api.cpp", "hq_gguf.cpp", "hq_attn_api.cpp", "hq_ssm_api.cpp"]
 LLVM = Path(os.environ.get("HQ_LLVM", "/opt/rocm/llvm"))
 
 

@@ -1,5 +1,5 @@
-// hq_attn_api.cpp — the attention and cache entry points of the C ABI (include/hq_attn.h):
-// argument validation, workspaces and launches. No exception crosses the ABI.
+// hq_attn_api.cpp — the attention, cache and rotary entry points of the C ABI (include/hq_attn.h,
+// include/hq_rotary.h): argument validation, workspaces and launches. No exception crosses the ABI.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -7,63 +7,21 @@
 #include <cstdio>
 
 #include "hq_attn.hpp"
+#include "hq_checks.hpp"
 #include "hq_internal.hpp"
+#include "hq_rotary.hpp"
 
 namespace {
 
-template <class... A>
-hq_status fail(hq_status s, const char* fmt, A... a) {
-  return hq_set_error(s, fmt, a...);
-}
-hq_status fail(hq_status s, const char* msg) { return hq_set_error(s, "%s", msg); }
-
-hq_status from_hip(hipError_t e, const char* what) {
-  if (e == hipSuccess) return hq_set_error(HQ_OK, "");
-  return fail(HQ_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
-}
-
-bool misaligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
-
-// Elements an operand may span, and the largest stride: far inside int64 byte offsets.
-constexpr int64_t kMaxSpan = (int64_t)1 << 46;
+using namespace hq::checks;
 
 // Rows of keys and values at most 2^23 elements apart: the kernels address 16 of them with 32-bit offsets.
 constexpr int64_t kMaxRow = (int64_t)1 << 23;
-
-// Row and head strides of an operand of `heads` heads of `dim`, in either order.
-hq_status check_strides(const char* name, int64_t row, int64_t head, uint32_t rows, uint32_t heads, uint32_t dim) {
-  if (row < 0 || head < 0 || row > kMaxSpan || head > kMaxSpan)
-    return fail(HQ_ERR_SHAPE, "%s: strides %lld, %lld out of range", name, (long long)row, (long long)head);
-  if (row % 8 || head % 8)
-    return fail(HQ_ERR_ALIGNMENT, "%s: strides %lld, %lld must be multiples of 8 elements", name, (long long)row,
-                (long long)head);
-  if ((rows > 1 && row < (int64_t)dim) || (heads > 1 && head < (int64_t)dim))
-    return fail(HQ_ERR_SHAPE, "%s: strides %lld, %lld below head_dim=%u", name, (long long)row, (long long)head, dim);
-  if ((double)row * rows + (double)head * heads > (double)kMaxSpan)
-    return fail(HQ_ERR_SHAPE, "%s: the operand spans too much", name);
-  return HQ_OK;
-}
-
-// Whether elements of different rows or heads share memory (strides as check_strides accepts them).
-bool overlaps(int64_t row, int64_t head, uint32_t rows, uint32_t heads, uint32_t dim) {
-  if (rows == 1 || heads == 1) return false;
-  if (row >= (heads - 1) * head + dim || head >= (rows - 1) * row + dim) return false;
-  for (uint32_t h = 1; h < heads; ++h) {  // head h of row 0 among head 0 of the rows on either side
-    const int64_t at = h * head, t = at / row;
-    if ((t < rows && at - t * row < dim) || (t + 1 < rows && (t + 1) * row - at < dim)) return true;
-  }
-  return false;
-}
 
 hq_status check_dim(uint32_t D) {
   if (D != 64 && D != 128 && D != 256) return fail(HQ_ERR_UNSUPPORTED, "head_dim=%u must be 64, 128 or 256", D);
   return HQ_OK;
 }
-hq_status check_dtype(int d) {
-  if (d != HQ_DTYPE_F16 && d != HQ_DTYPE_BF16) return fail(HQ_ERR_INVALID_ARG, "unknown dtype %d", d);
-  return HQ_OK;
-}
-
 // Tokens and heads of a call: row numbers t * G + g and grid sizes are 32-bit.
 hq_status check_counts(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads) {
   if (rows == 0 || seqs == 0) return fail(HQ_ERR_SHAPE, "rows=%u and seqs=%u must be positive", rows, seqs);
@@ -174,23 +132,6 @@ hq_status check_batch(uint32_t n) {
   return HQ_OK;
 }
 
-hq_status check_list(const char* name, const int32_t* p) {
-  if (!p) return fail(HQ_ERR_INVALID_ARG, "%s is null", name);
-  if (misaligned(p, 4)) return fail(HQ_ERR_ALIGNMENT, "%s must be 4-byte aligned", name);
-  return HQ_OK;
-}
-
-// The caller's workspace after its checks, or the library's own, which grows to `need`; null where the call uses none.
-hq_status workspace(void* ws, size_t bytes, size_t use, size_t need, hipStream_t s, void** out) {
-  *out = nullptr;
-  if (need == 0 || (ws && use == 0)) return HQ_OK;
-  if (!ws) return hq_internal_workspace(s, use, need, out);
-  if (bytes < use) return fail(HQ_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu this call needs", bytes, use);
-  if (misaligned(ws, 256)) return fail(HQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
-  *out = ws;
-  return HQ_OK;
-}
-
 hq_status check_plan(const hq::AttnPlan& p) {
   if (p.largest > hq::kMaxGrid) return fail(HQ_ERR_SHAPE, "%llu workgroups: too many rows and heads for one call", (unsigned long long)p.largest);
   return HQ_OK;
@@ -247,6 +188,46 @@ hq_status check_query(hq_attn_kind kind, uint32_t rows, uint32_t seqs, uint32_t 
   if ((st = check_dim(dim)) != HQ_OK || (st = check_counts(rows, seqs, heads, kv_heads)) != HQ_OK) return st;
   if (kind == HQ_ATTN_SHARED && (groups == 0 || groups > seqs || rows != seqs))
     return fail(HQ_ERR_SHAPE, "groups=%u, rows=%u: need 1..seqs=%u groups and a row for each sequence", groups, rows, seqs);
+  return HQ_OK;
+}
+
+hq_status check_rotary(const hq_rotary* r, uint32_t head_dim, hq::RotaryArgs* a) {
+  if (!r) return fail(HQ_ERR_INVALID_ARG, "rotary is null");
+  if (!r->turns) return fail(HQ_ERR_INVALID_ARG, "rotary: turns is null");
+  if (misaligned(r->turns, 8)) return fail(HQ_ERR_ALIGNMENT, "rotary: turns must be 8-byte aligned");
+  if (r->layout != HQ_ROTARY_HALF && r->layout != HQ_ROTARY_INTERLEAVED) return fail(HQ_ERR_INVALID_ARG, "rotary: unknown layout %d", (int)r->layout);
+  if (r->dim == 0 || r->dim % 16 || r->dim > head_dim)
+    return fail(HQ_ERR_SHAPE, "rotary: dim=%u must be a multiple of 16, 16 to head_dim=%u", r->dim, head_dim);
+  if (!(r->scale > 0.f) || !std::isfinite(r->scale)) return fail(HQ_ERR_INVALID_ARG, "rotary: scale=%g must be positive and finite", (double)r->scale);
+  a->turns = r->turns;
+  a->R = r->dim;
+  a->scale = r->scale;
+  return HQ_OK;
+}
+
+// One operand of a rotation; `out`: whether it is written to its Out.
+hq_status check_heads(const char* name, const hq_rotary_heads* h, uint32_t tokens, uint32_t dim, bool out, hq::RotaryHeads* to) {
+  if (!h->In || (out && !h->Out)) return fail(HQ_ERR_INVALID_ARG, "%s: In or Out is null", name);
+  if (h->heads == 0 || h->heads > 1024) return fail(HQ_ERR_SHAPE, "%s: heads=%u must be 1..1024", name, h->heads);
+  if (misaligned(h->In, 16) || (out && misaligned(h->Out, 16))) return fail(HQ_ERR_ALIGNMENT, "%s: In and Out must be 16-byte aligned", name);
+  if (misaligned(h->weight, 16)) return fail(HQ_ERR_ALIGNMENT, "%s: weight must be 16-byte aligned", name);
+  if (h->weight && (!(h->eps >= 0.f) || !std::isfinite(h->eps))) return fail(HQ_ERR_INVALID_ARG, "%s: eps=%g must not be negative, and finite", name, (double)h->eps);
+  hq_status st;
+  if ((st = check_strides(name, h->in_row, h->in_head, tokens, h->heads, dim)) != HQ_OK) return st;
+  if (out) {
+    if ((st = check_strides(name, h->out_row, h->out_head, tokens, h->heads, dim)) != HQ_OK) return st;
+    if (overlaps(h->out_row, h->out_head, tokens, h->heads, dim))
+      return fail(HQ_ERR_SHAPE, "%s: strides %lld, %lld make rows or heads of Out overlap", name, (long long)h->out_row, (long long)h->out_head);
+    if (h->Out == h->In && ((tokens > 1 && h->out_row != h->in_row) || (h->heads > 1 && h->out_head != h->in_head)))
+      return fail(HQ_ERR_SHAPE, "%s: Out is In with other strides", name);
+  }
+  *to = {static_cast<const uint16_t*>(h->In), static_cast<uint16_t*>(h->Out), h->in_row, h->in_head, h->out_row, h->out_head, h->weight, h->heads, h->eps};
+  return HQ_OK;
+}
+
+hq_status check_rotated(uint32_t tokens, const hq::RotaryArgs& a) {
+  if (tokens == 0 || tokens > (1u << 24) || (uint64_t)tokens * a.all > (1u << 30))
+    return fail(HQ_ERR_SHAPE, "tokens=%u of %u heads: out of range for one call", tokens, a.all);
   return HQ_OK;
 }
 
@@ -422,6 +403,56 @@ hq_status hq_cache_compact(const hq_kv_cache* cache, int32_t* out_table, int64_t
   const size_t need = hq::cache_compact_bytes(c.pages);
   if ((st = workspace(ws, ws_bytes, need, need, s, &w)) != HQ_OK) return st;
   return from_hip(hq::launch_cache_compact(c, out_table, out_stride, out_refs, w, s), "compact launch");
+}
+
+hq_status hq_rotate(const hq_rotary* rotary, const hq_rotary_heads* q, const hq_rotary_heads* k, uint32_t tokens, uint32_t head_dim,
+                    hq_dtype dtype, const int32_t* positions, hq_stream stream) {
+  hq::RotaryArgs a{};
+  hq_status st;
+  if (!q) return fail(HQ_ERR_INVALID_ARG, "q is null");
+  if ((st = check_dtype(dtype)) != HQ_OK || (st = check_dim(head_dim)) != HQ_OK || (st = check_rotary(rotary, head_dim, &a)) != HQ_OK ||
+      (st = check_heads("q", q, tokens, head_dim, true, &a.q)) != HQ_OK ||
+      (k && (st = check_heads("k", k, tokens, head_dim, true, &a.k)) != HQ_OK) || (st = check_list("positions", positions)) != HQ_OK)
+    return st;
+  a.T = tokens;
+  a.D = head_dim;
+  a.all = a.q.heads + a.k.heads;
+  a.pos = positions;
+  if ((st = check_rotated(tokens, a)) != HQ_OK) return st;
+  return from_hip(hq::launch_rotate(dtype, rotary->layout, a, nullptr, reinterpret_cast<hipStream_t>(stream)), "rotation launch");
+}
+
+hq_status hq_cache_append_rotated(const hq_kv_cache* cache, uint32_t layer, const hq_rotary* rotary, const hq_rotary_heads* q,
+                                  const hq_rotary_heads* k, const void* V, int64_t v_row, int64_t v_head, uint32_t tokens,
+                                  const int32_t* rows, const int32_t* cu, uint32_t n, hq_stream stream) {
+  hq::CacheArgs c;
+  hq::RotaryArgs a{};
+  hq_status st;
+  if ((st = check_cache(cache, &c)) != HQ_OK || (st = check_batch(n)) != HQ_OK || (st = check_list("rows", rows)) != HQ_OK) return st;
+  if (misaligned(cu, 4)) return fail(HQ_ERR_ALIGNMENT, "cu must be 4-byte aligned");
+  if (!k || !V) return fail(HQ_ERR_INVALID_ARG, "k or V is null");
+  if (misaligned(V, 16)) return fail(HQ_ERR_ALIGNMENT, "V must be 16-byte aligned");
+  if (layer >= c.layers) return fail(HQ_ERR_SHAPE, "layer=%u of %u", layer, c.layers);
+  if (!cu && tokens != n) return fail(HQ_ERR_SHAPE, "tokens=%u: without cu there is one for each of the %u rows", tokens, n);
+  if (!c.refused) return fail(HQ_ERR_INVALID_ARG, "cache: refused is null");
+  if ((st = check_rotary(rotary, c.dim, &a)) != HQ_OK || (q && (st = check_heads("q", q, tokens, c.dim, true, &a.q)) != HQ_OK) ||
+      (st = check_heads("k", k, tokens, c.dim, false, &a.k)) != HQ_OK ||
+      (st = check_strides("V", v_row, v_head, tokens, c.kv_heads, c.dim)) != HQ_OK)
+    return st;
+  if (k->heads != c.kv_heads) return fail(HQ_ERR_SHAPE, "k has %u heads, the cache %u", k->heads, c.kv_heads);
+  a.V = static_cast<const uint16_t*>(V);
+  a.v_row = v_row;
+  a.v_head = v_head;
+  a.T = tokens;
+  a.D = c.dim;
+  a.all = a.q.heads + 2 * a.k.heads;
+  a.rows = rows;
+  a.cu = cu;
+  a.n = n;
+  if ((st = check_rotated(tokens, a)) != HQ_OK) return st;
+  c.K += layer * c.layer_stride;
+  c.V += layer * c.layer_stride;
+  return from_hip(hq::launch_rotate(cache->dtype, rotary->layout, a, &c, reinterpret_cast<hipStream_t>(stream)), "rotated append launch");
 }
 
 }  // extern "C"

@@ -211,6 +211,26 @@ __device__ __forceinline__ uint16_t f32_to_out(float v) {
   }
 }
 
+// Two elements of an activation word as fp32, and back, rounded to nearest.
+template <int DT>
+__device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
+  if constexpr (DT == HQ_DTYPE_F16) {
+    const h2 v = bits_h2(w);
+    a = (float)v[0];
+    b = (float)v[1];
+  } else {
+    a = __uint_as_float(w << 16);
+    b = __uint_as_float(w & 0xFFFF0000u);
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == HQ_DTYPE_F16) return h2_bits(__builtin_convertvector((f2{a, b}), h2));
+  else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+}
+
 // f over the lanes up to each one, by moves inside rows of 16 lanes and then from row to row: a shuffle through
 // LDS takes ten times as long, and a call begins with several of these one after the other.
 template <class F>

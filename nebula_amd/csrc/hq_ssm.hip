@@ -1,0 +1,252 @@
+// hq_ssm.hip — the short causal convolution and the scan token by token (include/hq_ssm.h).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdio>
+
+#include "hq_internal.hpp"
+#include "hq_ssm_device.hpp"
+
+namespace hq {
+namespace {
+
+// ---- the convolution ----
+// Bound by the bytes moved, inputs and outputs once. A lane holds 8 channels of a run of TT tokens: the run's inputs and the
+// W - 1 before it are loaded side by side, and each is W products' operand in registers.
+//
+// A sequence's first W - 1 tokens read the row's kept inputs, and its last ones replace them: whoever reads them
+// writes them. So those first tokens are all the work of the run that the sequence begins in, up to W - 2 tokens past
+// its end, and a run leaves out the first tokens of a sequence that begins before it.
+constexpr uint32_t kRuns = 4;  // wavefronts, and runs, of a workgroup
+
+template <int DT>
+__device__ __forceinline__ void unpack8(u4 v, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack_pair<DT>(v[i], f[2 * i], f[2 * i + 1]);
+}
+
+template <int DT, int W, int TT>
+__global__ __launch_bounds__(64 * kRuns) void hq_ssm_conv_kernel(ConvArgs a) {
+  constexpr int kLoads = TT + 2 * W - 3;  // tokens t0 - (W - 1) .. t0 + TT + W - 3
+  const uint32_t c = (blockIdx.x * 64 + (threadIdx.x & 63u)) * 8;
+  const uint32_t t0 = uni((blockIdx.y * kRuns + (threadIdx.x >> 6)) * TT);
+  if (t0 >= a.s.T) return;  // (wavefronts share nothing)
+  const bool some = c < a.C;
+  const uint32_t cc = some ? c : 0u;
+  u4 x[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int64_t t = (int64_t)t0 + i - (W - 1);
+    x[i] = u4{0, 0, 0, 0};
+    if (t >= 0 && t < a.s.T) x[i] = *reinterpret_cast<const u4*>(a.X + t * a.ldx + cc);
+  }
+  float w[8 * W], bias[8];
+#pragma unroll
+  for (int i = 0; i < 2 * W; ++i) {
+    const f4 v = *reinterpret_cast<const f4*>(a.W + (size_t)cc * W + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bias[i] = a.bias ? a.bias[cc + i] : 0.f;
+
+  uint32_t b = uni(seq_of(a.s, t0));
+  uint32_t begin = a.s.cu ? clamp_to(a.s.cu[b], a.s.T) : b, end = a.s.cu ? clamp_to(a.s.cu[b + 1], a.s.T) : b + 1;
+  u4 old[W - 1];  // the kept inputs of the sequence that begins in this run
+#pragma unroll
+  for (int i = 0; i < W - 1; ++i) old[i] = u4{0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < TT + W - 2; ++i) {
+    const uint32_t t = t0 + i;
+    // The sequence of token t: sequences that end at or before it are left behind.
+    while (t >= end && b + 1 < a.s.n) {
+      ++b;
+      begin = a.s.cu ? clamp_to(a.s.cu[b], a.s.T) : b;
+      end = a.s.cu ? clamp_to(a.s.cu[b + 1], a.s.T) : b + 1;
+    }
+    const bool mine = t >= begin && t < end &&
+                      (i < TT ? begin >= t0 || t - begin >= W - 1u : begin >= t0 && begin < t0 + TT && t - begin < W - 1u);
+    if (mine) {
+      if (t == begin) {
+        const Seq q = find_seq(a.s, b, c == 0);
+        uint16_t* kept = a.state + q.row * a.row_stride + cc;
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) {
+          old[j] = u4{0, 0, 0, 0};
+          if (q.read) old[j] = *reinterpret_cast<const u4*>(kept + (size_t)j * a.C);
+        }
+        // What is kept: inputs len - (W - 1) .. len - 1 of the sequence, those below 0 the old ones.
+        const uint32_t len = end - begin;
+        u4 now[W - 1];
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) {
+          if (len + j >= W - 1) now[j] = *reinterpret_cast<const u4*>(a.X + (int64_t)(begin + len + j - (W - 1)) * a.ldx + cc);
+          else {
+            now[j] = old[0];
+#pragma unroll
+            for (int k = 1; k < W - 1; ++k)
+              if (len + j == (uint32_t)k) now[j] = old[k];
+          }
+        }
+        if (q.keep && some) {
+#pragma unroll
+          for (int j = 0; j < W - 1; ++j) *reinterpret_cast<u4*>(kept + (size_t)j * a.C) = now[j];
+        }
+      }
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = bias[e];
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        // Input t - (W - 1) + j: of the sequence, or one of the kept ones.
+        u4 in = x[i + j];
+        const uint32_t k = t - begin + j;  // its place, W - 1 added
+        if (j < W - 1 && k < W - 1u) {
+          in = old[j];
+#pragma unroll
+          for (int o = j + 1; o < W - 1; ++o)
+            if (k == (uint32_t)o) in = old[o];
+        }
+        float f[8];
+        unpack8<DT>(in, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(w[e * W + j], f[e], y[e]);
+      }
+      if (a.silu) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = silu(y[e]);
+      }
+      if (some) *reinterpret_cast<u4*>(a.Y + t * a.ldy + c) = u4{pack_pair<DT>(y[0], y[1]), pack_pair<DT>(y[2], y[3]), pack_pair<DT>(y[4], y[5]), pack_pair<DT>(y[6], y[7])};
+    }
+  }
+}
+
+template <int DT, int W>
+hipError_t launch_conv(const ConvArgs& a, hipStream_t s) {
+  // Runs of 16 tokens read 1.3 times what they write; single tokens and short sequences, whose runs would wait for one row of
+  // the states after the other, go one a wavefront.
+  const bool run = a.s.cu && a.s.T >= 32ull * a.s.n;
+  const uint32_t tile = run ? 16 : 1, per = tile * kRuns;
+  const dim3 grid((a.C / 8 + 63) / 64, (a.s.T + per - 1) / per);
+  if (run) hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, 16>), grid, dim3(64 * kRuns), 0, s, a);
+  else hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, 1>), grid, dim3(64 * kRuns), 0, s, a);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_conv_type(const ConvArgs& a, hipStream_t s) {
+  switch (a.width) {
+    case 2: return launch_conv<DT, 2>(a, s);
+    case 3: return launch_conv<DT, 3>(a, s);
+    default: return launch_conv<DT, 4>(a, s);
+  }
+}
+
+// ---- the scan, token by token ----
+// Bound by the states' bytes, read and written once: a wavefront holds 8 rows of a head's state (32 a workgroup), every lane
+// 4 elements of a row as one 16-byte piece, so that a load is 1 KB of memory in one piece. The sum over a row is
+// one over the lanes that hold it, by moves between lanes.
+constexpr uint32_t kStepRows = 32;  // of a workgroup of four wavefronts
+
+// Sum over aligned groups of NL lanes (16, 32 or 64), in every lane of the group.
+template <int NL>
+__device__ __forceinline__ float lanes_sum(float x) {
+#define HQ_ADD(CTRL) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, true))
+  HQ_ADD(0xB1);   // the neighbour
+  HQ_ADD(0x4E);   // the other pair of four
+  HQ_ADD(0x141);  // the other four of eight
+  HQ_ADD(0x140);  // the other eight of sixteen
+#undef HQ_ADD
+  if constexpr (NL >= 32) {
+    const auto v = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(v[0]) + __uint_as_float(v[1]);
+  }
+  if constexpr (NL >= 64) {
+    const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(v[0]) + __uint_as_float(v[1]);
+  }
+  return x;
+}
+
+template <int DT, int N>
+__global__ __launch_bounds__(256) void hq_ssm_step_kernel(ScanArgs a) {
+  constexpr uint32_t kLanes = N / 4, kAtOnce = 64 / kLanes, kLoads = 8 / kAtOnce;  // lanes of a row, rows of a load
+  const uint32_t parts = a.P / kStepRows, h = blockIdx.x / parts, part = blockIdx.x - h * parts;
+  const uint32_t lane = threadIdx.x & 63u, n = lane % kLanes * 4, g = h / (a.H / a.G);
+  const uint32_t p0 = part * kStepRows + (threadIdx.x >> 6) * 8 + lane / kLanes;  // row of load i: p0 + i * kAtOnce
+  const Seq q = find_seq(a.s, blockIdx.y, blockIdx.x == 0 && threadIdx.x < 64);
+  if (q.a >= q.e) return;
+  float* state = a.state + q.row * a.row_stride + (size_t)h * a.P * N + n;
+  f4 s[kLoads];
+#pragma unroll
+  for (uint32_t i = 0; i < kLoads; ++i) {
+    s[i] = f4{0, 0, 0, 0};
+    if (q.read) s[i] = *reinterpret_cast<const f4*>(state + (size_t)(p0 + i * kAtOnce) * N);
+  }
+  const float A = a.A[h], D = a.D ? a.D[h] : 0.f, dt0 = a.dt_bias ? a.dt_bias[h] : 0.f;
+  const uint32_t mine = min(lane % kLanes, kLoads - 1), p = p0 + mine * kAtOnce;  // the row whose output this lane writes
+  for (uint32_t t = q.a; t < q.e; ++t) {
+    const float dt = step_of(load_dt(a, t, h, DT) + dt0, a.softplus);
+    const u2 bw = *reinterpret_cast<const u2*>(a.B + t * a.b_row + g * a.b_group + n);
+    const u2 cw = *reinterpret_cast<const u2*>(a.C + t * a.c_row + g * a.c_group + n);
+    const uint16_t* x = a.X + t * a.x_row + h * a.x_head;
+    float z = 0;
+    if (a.Z) z = to_f32<DT>(a.Z[t * a.z_row + h * a.z_head + p]);
+    float b[4], c[4], xs[kLoads], y[kLoads];
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) xs[i] = to_f32<DT>(x[p0 + i * kAtOnce]);
+    unpack_pair<DT>(bw[0], b[0], b[1]);
+    unpack_pair<DT>(bw[1], b[2], b[3]);
+    unpack_pair<DT>(cw[0], c[0], c[1]);
+    unpack_pair<DT>(cw[1], c[2], c[3]);
+    const float keep = expf(dt * A);
+    float out = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) {
+      const float dx = dt * xs[i];
+      y[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i][e] = fmaf(s[i][e], keep, dx * b[e]);
+        y[i] = fmaf(s[i][e], c[e], y[i]);
+      }
+      y[i] = lanes_sum<kLanes>(y[i]);
+      if (mine == i) out = fmaf(D, xs[i], y[i]);
+    }
+    if (lane % kLanes < kLoads) {
+      if (a.Z) out *= silu(z);
+      a.Y[t * a.y_row + h * a.y_head + p] = f32_to_out<DT>(out);
+    }
+  }
+  if (q.keep) {
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) *reinterpret_cast<f4*>(state + (size_t)(p0 + i * kAtOnce) * N) = s[i];
+  }
+}
+
+template <int DT>
+hipError_t launch_step(const ScanArgs& a, hipStream_t s) {
+  const dim3 grid(a.H * (a.P / kStepRows), a.s.n);
+  switch (a.N) {
+    case 64: hipLaunchKernelGGL((hq_ssm_step_kernel<DT, 64>), grid, dim3(256), 0, s, a); break;
+    case 128: hipLaunchKernelGGL((hq_ssm_step_kernel<DT, 128>), grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL((hq_ssm_step_kernel<DT, 256>), grid, dim3(256), 0, s, a); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_ssm_conv(int dtype, const ConvArgs& a, hipStream_t s) {
+  return dtype == HQ_DTYPE_F16 ? launch_conv_type<HQ_DTYPE_F16>(a, s) : launch_conv_type<HQ_DTYPE_BF16>(a, s);
+}
+
+ScanPlan plan_scan(uint32_t, uint32_t, bool, uint32_t, uint32_t, uint32_t, uint32_t) { return {}; }
+
+void describe_scan(const ScanPlan& p, char* buf, size_t len) { snprintf(buf, len, "hq_ssm_step_kernel ws=%zu", p.ws); }
+
+hipError_t launch_ssm_scan(int dtype, const ScanArgs& a, const ScanPlan&, void*, hipStream_t s) {
+  return dtype == HQ_DTYPE_F16 ? launch_step<HQ_DTYPE_F16>(a, s) : launch_step<HQ_DTYPE_BF16>(a, s);
+}
+
+}  // namespace hq
