@@ -56,7 +56,7 @@ hq_status hq_ssm_conv(const hq_state_cache* cache, uint32_t layer, const void* X
 
 /* Inputs and outputs of a scan, strides in elements: X, Y, Z (NULL: no gate) [tokens][heads][head_dim], B, C
  * [tokens][groups][state_dim], dt [tokens][heads] with its heads side by side, fp32 (dt_f32) or of the activations' type.
- * X, B, C, Y, Z: 16-byte aligned, strides multiples of 8. A, D (NULL: 0), dt_bias (NULL: 0): fp32 [heads], A not
+ * X, B, C, Y, Z: 16-byte aligned, strides multiples of 8 (rows of X, B and C at most 2^23, heads of 64 of X 2^29). A, D (NULL: 0), dt_bias (NULL: 0): fp32 [heads], A not
  * positive. heads: a multiple of groups. Y may be Z with the same strides (in place), else it is apart from all inputs. */
 typedef struct hq_ssm_io {
     const void* X;
@@ -74,12 +74,12 @@ typedef struct hq_ssm_io {
 } hq_ssm_io;
 
 /* Workspace of one hq_ssm_scan call on the current device (0: none), as hq_workspace_bytes; cu: whether the call has one.
- * The size does not fall as tokens, n and max_len grow. */
-hq_status hq_ssm_workspace_bytes(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t head_dim, uint32_t state_dim,
-                                 uint32_t max_len, size_t* bytes);
+ * The size does not fall as tokens and max_len grow: one taken at the largest serves every call of as many sequences. */
+hq_status hq_ssm_workspace_bytes(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t groups, uint32_t head_dim,
+                                 uint32_t state_dim, uint32_t max_len, size_t* bytes);
 /* The kernels that such a call runs and the workspace that it uses, as text. */
-hq_status hq_describe_ssm(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t head_dim, uint32_t state_dim, uint32_t max_len,
-                          char* buf, size_t buf_len);
+hq_status hq_describe_ssm(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim,
+                          uint32_t max_len, char* buf, size_t buf_len);
 /* Scan. max_len: no sequence has more new tokens (0: tokens); it only chooses how the work is split, as does the mean
  * number of tokens: single tokens and a long chunk are faster as two calls. */
 hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_io* io, const int32_t* rows, const int32_t* held,

@@ -25,14 +25,14 @@ ORACLE_DIR = ROOT / "oracle"
 
 SOURCES = ["hq_api.cpp", "hq_gguf.cpp", "hq_decode.hip", "hq_decode_ls.hip", "hq_rows.hip", "hq_prefill.hip", "hq_repack.hip", "hq_int8.hip",
            "hq_attn_api.cpp", "hq_attn.hip", "hq_cache.hip", "hq_rotary.hip", "hq_ssm_api.cpp",
-           "hq_ssm.hip"]
+           "hq_ssm.hip", "hq_ssm_chunk.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-# Per source: the attention kernels' accumulators take part in vector arithmetic, so their MFMAs write
+# Per source: the attention and the chunked scan kernels' accumulators take part in vector arithmetic, so their MFMAs write
 # vector registers (with more than 256 registers a lane the compiler would move them to and fro: 380
 # moves a tile on heads of 256).
-SOURCE_FLAGS = {"hq_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("hq_attn.hip", "hq_ssm_chunk.hip")}
 
 COMMON_FLAGS = [
     "-O3",

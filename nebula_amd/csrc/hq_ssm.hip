@@ -146,6 +146,7 @@ hipError_t launch_conv_type(const ConvArgs& a, hipStream_t s) {
 // Bound by the states' bytes, read and written once: a wavefront holds 8 rows of a head's state (32 a workgroup), every lane
 // 4 elements of a row as one 16-byte piece, so that a load is 1 KB of memory in one piece. The sum over a row is
 // one over the lanes that hold it, by moves between lanes.
+constexpr uint32_t kColumnsOfRun = 128;  // channels of a workgroup of the chunk kernel
 constexpr uint32_t kStepRows = 32;  // of a workgroup of four wavefronts
 
 // Sum over aligned groups of NL lanes (16, 32 or 64), in every lane of the group.
@@ -241,11 +242,48 @@ hipError_t launch_ssm_conv(int dtype, const ConvArgs& a, hipStream_t s) {
   return dtype == HQ_DTYPE_F16 ? launch_conv_type<HQ_DTYPE_F16>(a, s) : launch_conv_type<HQ_DTYPE_BF16>(a, s);
 }
 
-ScanPlan plan_scan(uint32_t, uint32_t, bool, uint32_t, uint32_t, uint32_t, uint32_t) { return {}; }
+// Which kernel, and how many tokens a run has, by a cost in time (us of an MI355X).
+ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim, uint32_t max_len) {
+  ScanPlan p;
+  p.largest = (uint64_t)heads * (head_dim / kStepRows) * n;
+  if (!cu || tokens < 8ull * n) return p;
+  p.chunk = true;
+  const uint32_t L = state_dim == 256 ? 32 : 64, two = 128 / head_dim, slots = (uint32_t)cu_count() * (state_dim == 256 ? 1 : 2);
+  p.units = groups * ((heads / groups + two - 1) / two);
+  const uint32_t longest = ((max_len && max_len < tokens ? max_len : tokens) + L - 1) / L;
+  // Runs there may be: two rounds of workgroups and one a sequence.
+  const uint32_t most = 2 * slots / p.units + n;
+  uint32_t chunks = longest;
+  if ((uint64_t)n * p.units < 2 * slots && longest > 1) {
+    float best = 0;
+    for (uint32_t k = 1; k <= std::min(longest, 64u); ++k) {
+      const uint32_t c = (longest + k - 1) / k, runs = tokens / (c * L) + n;
+      if (k > 1 && runs > most) break;
+      const uint64_t groups_of = (uint64_t)(k == 1 ? n : runs) * p.units, rounds = (groups_of + slots - 1) / slots;
+      const float cost = rounds * c * (groups_of * 2 > slots ? 4.f : 2.5f) * (k > 1 ? 1.6f : 1.f) + (k > 1 ? 8.f + k : 0.f);
+      if (k == 1 || cost < best) {
+        best = cost;
+        chunks = c;
+      }
+    }
+    const size_t run_bytes = (size_t)p.units * (kColumnsOfRun * state_dim + two) * 4;
+    p.need = kCounterBytes + std::min((tokens + L - 1) / L + n, most) * run_bytes;
+    p.split = chunks < longest;
+    if (p.split) p.ws = kCounterBytes + (tokens / (chunks * L) + n) * run_bytes;
+  }
+  p.run_tokens = chunks * L;
+  p.runs = p.split ? tokens / p.run_tokens + n : n;
+  p.largest = (uint64_t)p.runs * p.units + 8;
+  return p;
+}
 
-void describe_scan(const ScanPlan& p, char* buf, size_t len) { snprintf(buf, len, "hq_ssm_step_kernel ws=%zu", p.ws); }
+void describe_scan(const ScanPlan& p, char* buf, size_t len) {
+  if (!p.chunk) snprintf(buf, len, "hq_ssm_step_kernel ws=%zu", p.ws);
+  else snprintf(buf, len, "hq_ssm_chunk_kernel%s runs of %u tokens, grid=%u x %u ws=%zu", p.split ? " twice," : "", p.run_tokens, p.runs, p.units, p.ws);
+}
 
-hipError_t launch_ssm_scan(int dtype, const ScanArgs& a, const ScanPlan&, void*, hipStream_t s) {
+hipError_t launch_ssm_scan(int dtype, const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s) {
+  if (p.chunk) return launch_ssm_chunks(dtype, a, p, ws, s);
   return dtype == HQ_DTYPE_F16 ? launch_step<HQ_DTYPE_F16>(a, s) : launch_step<HQ_DTYPE_BF16>(a, s);
 }
 

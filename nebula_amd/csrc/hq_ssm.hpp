@@ -52,11 +52,15 @@ struct ScanArgs {
 
 // How a scan is split, from host-side sizes alone (the lengths stay on the device).
 struct ScanPlan {
+  bool chunk = false;       // in chunks, else token by token
+  bool split = false;       // sequences are cut into runs: a launch for what they add to the state comes first
+  uint32_t run_tokens = 0, units = 0, runs = 0;  // tokens of a run, workgroups of one, runs of the call at most
   uint64_t largest = 0;     // workgroups of its largest launch
   size_t ws = 0, need = 0;  // workspace that is used, and that is asked for: it does not fall as sizes grow
 };
-ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_t head_dim, uint32_t state_dim, uint32_t max_len);
+ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim, uint32_t max_len);
 void describe_scan(const ScanPlan& p, char* buf, size_t len);
 hipError_t launch_ssm_scan(int dtype, const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s);
+hipError_t launch_ssm_chunks(int dtype, const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s);
 
 }  // namespace hq

@@ -13,10 +13,17 @@ namespace {
 
 using namespace hq::checks;
 
+constexpr int64_t kMaxRow = (int64_t)1 << 23;
+
 hq_status check_sizes(uint32_t heads, uint32_t head_dim, uint32_t state_dim) {
   if (head_dim != 64 && head_dim != 128) return fail(HQ_ERR_UNSUPPORTED, "head_dim=%u must be 64 or 128", head_dim);
   if (state_dim != 64 && state_dim != 128 && state_dim != 256) return fail(HQ_ERR_UNSUPPORTED, "state_dim=%u must be 64, 128 or 256", state_dim);
   if (heads == 0 || heads > 1024) return fail(HQ_ERR_SHAPE, "heads=%u must be 1..1024", heads);
+  return HQ_OK;
+}
+
+hq_status check_groups(uint32_t H, uint32_t G) {
+  if (G == 0 || H % G) return fail(HQ_ERR_SHAPE, "heads=%u must be a positive multiple of groups=%u", H, G);
   return HQ_OK;
 }
 
@@ -61,9 +68,9 @@ hq_status check_plan(const hq::ScanPlan& p) {
   return HQ_OK;
 }
 
-hq_status check_query(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t head_dim, uint32_t state_dim) {
+hq_status check_query(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim) {
   hq_status st;
-  if ((st = check_sizes(heads, head_dim, state_dim)) != HQ_OK) return st;
+  if ((st = check_sizes(heads, head_dim, state_dim)) != HQ_OK || (st = check_groups(heads, groups)) != HQ_OK) return st;
   return check_tokens(tokens, n, cu != 0);
 }
 
@@ -102,23 +109,23 @@ hq_status hq_ssm_conv(const hq_state_cache* cache, uint32_t layer, const void* X
   return from_hip(hq::launch_ssm_conv(cache->dtype, a, reinterpret_cast<hipStream_t>(stream)), "convolution launch");
 }
 
-hq_status hq_ssm_workspace_bytes(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t head_dim, uint32_t state_dim,
+hq_status hq_ssm_workspace_bytes(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim,
                                  uint32_t max_len, size_t* bytes) {
   if (!bytes) return fail(HQ_ERR_INVALID_ARG, "bytes is null");
-  hq_status st = check_query(tokens, n, cu, heads, head_dim, state_dim);
+  hq_status st = check_query(tokens, n, cu, heads, groups, head_dim, state_dim);
   if (st != HQ_OK) return st;
-  const hq::ScanPlan p = hq::plan_scan(tokens, n, cu != 0, heads, head_dim, state_dim, max_len);
+  const hq::ScanPlan p = hq::plan_scan(tokens, n, cu != 0, heads, groups, head_dim, state_dim, max_len);
   if ((st = check_plan(p)) != HQ_OK) return st;
   *bytes = p.need;
   return hq_set_error(HQ_OK, "");
 }
 
-hq_status hq_describe_ssm(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t head_dim, uint32_t state_dim, uint32_t max_len,
+hq_status hq_describe_ssm(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim, uint32_t max_len,
                           char* buf, size_t buf_len) {
   if (!buf || buf_len == 0) return fail(HQ_ERR_INVALID_ARG, "buf is null or empty");
-  hq_status st = check_query(tokens, n, cu, heads, head_dim, state_dim);
+  hq_status st = check_query(tokens, n, cu, heads, groups, head_dim, state_dim);
   if (st != HQ_OK) return st;
-  const hq::ScanPlan p = hq::plan_scan(tokens, n, cu != 0, heads, head_dim, state_dim, max_len);
+  const hq::ScanPlan p = hq::plan_scan(tokens, n, cu != 0, heads, groups, head_dim, state_dim, max_len);
   if ((st = check_plan(p)) != HQ_OK) return st;
   hq::describe_scan(p, buf, buf_len);
   return hq_set_error(HQ_OK, "");
@@ -136,7 +143,7 @@ hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_
   if (!cache->ssm) return fail(HQ_ERR_INVALID_ARG, "cache: ssm is null");
   if (misaligned(cache->ssm, 16)) return fail(HQ_ERR_ALIGNMENT, "cache: ssm must be 16-byte aligned");
   if ((st = check_pool("ssm", cache->ssm_layer, cache->ssm_row, cache->layers, cache->rows, (int64_t)H * P * N, 4)) != HQ_OK) return st;
-  if (G == 0 || H % G) return fail(HQ_ERR_SHAPE, "heads=%u must be a positive multiple of groups=%u", H, G);
+  if ((st = check_groups(H, G)) != HQ_OK) return st;
   if ((uint64_t)T * H > (1u << 30)) return fail(HQ_ERR_SHAPE, "tokens=%u of %u heads: too many for one call", T, H);
   if (!io->X || !io->B || !io->C || !io->dt || !io->Y || !io->A) return fail(HQ_ERR_INVALID_ARG, "X, B, C, dt, Y or A is null");
   if (io->Y == io->X || io->Y == io->B || io->Y == io->C || io->Y == io->dt) return fail(HQ_ERR_INVALID_ARG, "Y is an input that others read");
@@ -148,6 +155,10 @@ hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_
       (st = check_strides("C", io->c_row, io->c_group, T, G, N)) != HQ_OK || (st = check_strides("Y", io->y_row, io->y_head, T, H, P)) != HQ_OK ||
       (io->Z && (st = check_strides("Z", io->z_row, io->z_head, T, H, P)) != HQ_OK))
     return st;
+  // The chunk kernel reaches 64 tokens, and two heads of 64, with 32-bit offsets.
+  if (io->x_row > kMaxRow || io->b_row > kMaxRow || io->c_row > kMaxRow || (P == 64 && H > 1 && io->x_head > 64 * kMaxRow))
+    return fail(HQ_ERR_SHAPE, "X, B, C: row strides %lld, %lld, %lld above %lld elements, or X's head stride %lld too large", (long long)io->x_row,
+                (long long)io->b_row, (long long)io->c_row, (long long)kMaxRow, (long long)io->x_head);
   if (overlaps(io->y_row, io->y_head, T, H, P)) return fail(HQ_ERR_SHAPE, "Y: strides %lld, %lld make rows or heads overlap", (long long)io->y_row, (long long)io->y_head);
   if (io->Y == io->Z && ((T > 1 && io->y_row != io->z_row) || (H > 1 && io->y_head != io->z_head))) return fail(HQ_ERR_SHAPE, "Y is Z with other strides");
   if (io->dt_row < 0 || io->dt_row > kMaxSpan || (T > 1 && io->dt_row < (int64_t)H) || (double)io->dt_row * T > (double)kMaxSpan)
@@ -181,7 +192,7 @@ hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_
   a.dt_f32 = io->dt_f32 != 0;
   a.softplus = io->softplus != 0;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const hq::ScanPlan p = hq::plan_scan(T, n, cu != nullptr, H, P, N, max_len);
+  const hq::ScanPlan p = hq::plan_scan(T, n, cu != nullptr, H, G, P, N, max_len);
   void* w = nullptr;
   if ((st = check_plan(p)) != HQ_OK || (st = workspace(ws, ws_bytes, p.ws, p.need, s, &w)) != HQ_OK) return st;
   return from_hip(hq::launch_ssm_scan(cache->dtype, a, p, w, s), "scan launch");

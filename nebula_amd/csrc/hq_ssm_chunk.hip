@@ -1,0 +1,652 @@
+// hq_ssm_chunk.hip — the selective scan of prompts in chunks of tokens, on matrix products (include/hq_ssm.h).
+//
+// Inside a chunk of L tokens with c_t = sum_{s <= t} A dt_s, a head's recursion is
+//   y_t = exp(c_t) S_in C_t + sum_{s <= t} M_ts x_s + D x_t,   M_ts = exp(c_t - c_s) dt_s (B_s . C_t)
+//   S_out = exp(c_end) S_in + sum_s w_s x_s B_s^T,             w_s = exp(c_end - c_s) dt_s
+// so a token costs 4 N + 4 L operations a channel in place of 6 N on the vector units, and the state is touched once a
+// chunk. A workgroup walks a run of chunks of one head (two heads of 64 of one group) with the state in the accumulators
+// of four wavefronts, 32 channels each:
+//   S^T [n][p] as products of 32 x 32: a lane holds one channel p and eight states n side by side, which is the next
+//   product's operand as it stands (its rows, the columns of B in LDS, are taken in the order that makes them so);
+//   y^T [p][t] = S C^T and x^T M^T, whose operand x^T is the one that the state's sum takes with its weights.
+// B, C and x go through LDS, the next chunk's in registers meanwhile; M is computed once by the head's wavefronts and
+// goes through LDS to all of them.
+//
+// Sums are fp32 throughout. What a matrix product's operands round away:
+//   the state's terms w x (fp32 times 16 bits) are kept as three bf16 parts, or in fp16 as two parts of values scaled by a
+//   power of two (22 bits of them either way), because the state is fp32 and goes on for the whole sequence;
+//   S as an operand, and M, are kept as two parts (16 bits, fp16: 22 of S): with one, outputs would be off by 1.4
+//   times their own rounding.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdio>
+
+#include "hq_internal.hpp"
+#include "hq_ssm_device.hpp"
+
+namespace hq {
+namespace {
+
+typedef float f16x __attribute__((ext_vector_type(16)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ f16x mfma32(u4 a, u4 b, f16x c) {
+  if constexpr (DT == HQ_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+constexpr int BF = HQ_DTYPE_BF16;
+constexpr uint32_t kChunkThreads = 256;
+constexpr uint32_t kColumns = 128;  // of a chunk's x: four wavefronts of 32 channels
+
+// Tokens of a chunk: the state of 256 leaves registers and LDS for 32.
+template <int N>
+constexpr int chunk_tokens() {
+  return N == 256 ? 32 : 64;
+}
+
+// 16-byte pieces of a row of LDS: piece c of row r lies at c ^ swizzle(r), so that reads of one piece of 16 rows, and
+// transposing reads of four pieces of four rows, meet in different banks (64 of 4 bytes).
+template <int BYTES>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
+  if constexpr (BYTES >= 256) return (r & 3u) << 2 | (r >> 2 & 3u);
+  else if constexpr (BYTES == 128) return (r >> 1 & 1u) << 2 | (r >> 2 & 3u);
+  else return r >> 2 & 3u;  // rows of 64 bytes: four side by side
+}
+template <int BYTES>
+__device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) {
+  return r * BYTES + ((c ^ swizzle<BYTES>(r)) << 4);
+}
+
+// A part of M in LDS, [token][earlier token]: 32 tokens with 32 earlier ones, then the 32 behind them with 64.
+template <int L>
+constexpr uint32_t m_bytes() {
+  return L == 64 ? 32 * 64 + 32 * 128 : 32 * 64;
+}
+template <int L>
+__device__ __forceinline__ uint32_t m_place(uint32_t block, uint32_t r, uint32_t c) {
+  return L == 64 && block ? 32 * 64 + piece_at<128>(r, c) : piece_at<64>(r, c);
+}
+
+// A fragment of the transposed tile [tokens][columns]: columns 32 c32 .., tokens 16 ks ..; lane: column (SWAP: the middle
+// fours of 16 exchanged), eight tokens. `at`: what tr_place gives.
+template <int BYTES, bool SWAP>
+__device__ __forceinline__ void tr_place(uint32_t lane, uint32_t c32, uint32_t (&at)[2]) {
+  const uint32_t j = lane & 3u, row = 8 * (lane >> 5) + (lane >> 2 & 3u);
+  const uint32_t piece = 4 * c32 + 2 * (lane >> 4 & 1u) + (SWAP ? j & 1u : j >> 1), byte = 8 * (SWAP ? j >> 1 : j & 1u);
+  at[0] = piece_at<BYTES>(row, piece) + byte;
+  at[1] = piece_at<BYTES>(row + 4, piece) + byte;
+}
+__device__ __forceinline__ u4 tr_read(const unsigned char* p0, const unsigned char* p1) {
+  typedef __attribute__((address_space(3))) s4* lds_s4;
+  const u2 a = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p0));
+  const u2 b = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(uintptr_t)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p1));
+  return u4{a[0], a[1], b[0], b[1]};
+}
+
+__device__ __forceinline__ float scan_add(float x) {
+  return __uint_as_float(scan(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+__device__ __forceinline__ float max_of_lanes(float x) {
+  return __int_as_float(__builtin_amdgcn_readlane(
+      (int)scan(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }), 63));
+}
+
+// 2^k that brings a maximum m to 2^14..2^15, and 2^-k: fp16 then holds 11 bits of a value and as many of the rest, down to
+// 2^-39 of the maximum. No values, infinities or NaN: as they are.
+__device__ __forceinline__ void range_scale(float m, float& up, float& down) {
+  const uint32_t e = __float_as_uint(m) >> 23 & 255u;
+  const uint32_t k = m == 0.f || e == 255u ? 127u : min(268u - e, 247u);  // 141 - e + 127
+  up = __uint_as_float(k << 23);
+  down = __uint_as_float((254u - k) << 23);
+}
+
+// The rest that one rounding of two values leaves, and the rounded ones.
+template <int DT>
+__device__ __forceinline__ uint32_t take_part(float& a, float& b) {
+  const uint32_t w = pack_pair<DT>(a, b);
+  float x, y;
+  unpack_pair<DT>(w, x, y);
+  a -= x;
+  b -= y;
+  return w;
+}
+
+template <int DT, int K>
+__device__ __forceinline__ bool any_odd(const u4 (&x)[K]) {
+  constexpr uint32_t kExp = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;
+  bool odd = false;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd |= (x[k][i] & kExp) == kExp || (x[k][i] >> 16 & kExp) == kExp;
+  return odd;
+}
+
+// A place in LDS as the compiler has it: what is computed from it stays in its chunk. (Held from chunk to chunk, the places
+// of all fragments are more registers than there are.)
+__device__ __forceinline__ uint32_t opaque(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// Which run of chunks a workgroup works on.
+struct Run {
+  Seq q;
+  uint32_t t0, t1;      // tokens
+  uint32_t first, idx, last;  // runs of the whole call: the sequence's first, this one, the sequence's last
+};
+
+__device__ __forceinline__ bool find_run(const SeqArgs& s, uint32_t run_tokens, uint32_t idx, bool tell, Run& r) {
+  uint32_t before = 0;
+  for (uint32_t i = 0; i < s.n; i += 64) {
+    const uint32_t b = i + (threadIdx.x & 63u);
+    uint32_t runs = 0;
+    if (b < s.n) {
+      const uint32_t a = s.cu ? clamp_to(s.cu[b], s.T) : b, e = s.cu ? clamp_to(s.cu[b + 1], s.T) : b + 1;
+      runs = e > a ? (e - a + run_tokens - 1) / run_tokens : 0u;
+    }
+    const uint32_t upto = scan_sum(runs) + before, all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    if (idx < all) {
+      const uint64_t past = __ballot(upto > idx);  // some lane: the last one is
+      const int lane = __builtin_ctzll(past);
+      const uint32_t mine = (uint32_t)__builtin_amdgcn_readlane((int)runs, lane);
+      r.last = (uint32_t)__builtin_amdgcn_readlane((int)upto, lane) - 1;
+      r.first = r.last + 1 - mine;
+      r.idx = idx;
+      r.q = find_seq(s, i + lane, tell);
+      r.t0 = r.q.a + (idx - r.first) * run_tokens;
+      r.t1 = min(r.t0 + run_tokens, r.q.e);
+      return true;
+    }
+    before = all;
+  }
+  return false;
+}
+
+struct ChunkArgs {
+  uint32_t run_tokens, units, runs, blocks;  // tokens of a run; workgroups of a run; runs, workgroups of the launch less the padding
+  float* states;                       // [runs][units][register quads][threads] f4: what a run adds to the state
+  float* totals;                       // [runs][heads]: its whole decay's exponent
+};
+
+template <int N>
+constexpr uint32_t vec_bytes() {
+  return 4 * 4 * chunk_tokens<N>() * 4;
+}
+template <int N, bool CARRY>
+constexpr uint32_t chunk_lds(uint32_t heads) {
+  constexpr uint32_t L = chunk_tokens<N>();
+  return (CARRY ? 1 : 2) * L * N * 2 + L * kColumns * 2 + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>());
+}
+
+// CARRY: the state alone, of all runs but a sequence's last, for the runs behind them.
+template <int DT, int P, int N, bool CARRY>
+__global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_kernel(ScanArgs a, ChunkArgs pl) {
+  constexpr int L = chunk_tokens<N>(), kHeads = kColumns / P, kWaves = P / 32;  // heads, wavefronts of a head
+  constexpr int kTB = L / 32, kTS = L / 16, kNT = N / 32, kNS = N / 16;
+  constexpr int kRow = 2 * N, kXRow = 2 * kColumns;
+  extern __shared__ __align__(16) unsigned char smem[];
+  unsigned char* const sB = smem;
+  unsigned char* const sX = sB + L * kRow;
+  float* const vec = reinterpret_cast<float*>(sX + L * kXRow);
+  unsigned char* const sC = reinterpret_cast<unsigned char*>(vec) + vec_bytes<N>();
+  unsigned char* const sM = sC + L * kRow;
+
+  // Workgroups go to the eight XCDs in turn: a run of neighbouring ones, which share B and C, goes to one.
+  const uint32_t block = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (block >= pl.blocks) return;
+  const uint32_t idx = block / pl.units, unit = block - idx * pl.units;
+  const uint32_t of_group = a.H / a.G, per_group = (of_group + kHeads - 1) / kHeads;
+  const uint32_t g = unit / per_group, head0 = (unit - g * per_group) * kHeads;  // the first head, in its group
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uni(tid >> 6), l32 = lane & 31u, half = lane >> 5;
+  const uint32_t mine = wave / kWaves, part = wave % kWaves;  // this wavefront's head and 32 channels of it
+  const bool live = head0 + mine < of_group;                  // (an odd group's last head is alone)
+  const uint32_t h = g * of_group + min(head0 + mine, of_group - 1);
+
+  Run run;
+  if (!find_run(a.s, pl.run_tokens, idx, unit == 0 && tid < 64, run)) return;
+  if (CARRY && run.idx == run.last) return;
+  if (run.last >= pl.runs) {  // offsets that fall hold more tokens than there are: no room for the sequence's runs
+    if (unit == 0 && tid == 0) __hip_atomic_fetch_or(a.s.status, HQ_CACHE_BAD_ROW, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return;
+  }
+
+  const float A = a.A[h] * 1.44269504f, D = !CARRY && a.D ? a.D[h] : 0.f, dt0 = a.dt_bias ? a.dt_bias[h] : 0.f;
+
+  // ---- a chunk's inputs, on their way in registers ----
+  constexpr int kPieces = N / 8, kRows = kChunkThreads / kPieces, kLoads = L / kRows, kXLoads = L / 16;
+  u4 rb[kLoads], rc[CARRY ? 1 : kLoads], rx[kXLoads];
+  float rdt = 0;
+  const uint32_t row = tid / kPieces, piece = tid % kPieces, xrow = tid / 16, xpiece = tid % 16;
+  const bool xlive = head0 + xpiece / (P / 8) < of_group;
+  // 32-bit offsets from the chunk's first token; a place past any operand reads as 0 without touching memory.
+  const uint32_t b_off = (row * (uint32_t)a.b_row + piece * 8) * 2, c_off = (row * (uint32_t)a.c_row + piece * 8) * 2;
+  const uint32_t x_off = (xrow * (uint32_t)a.x_row + (xpiece / (P / 8)) * (uint32_t)a.x_head + xpiece % (P / 8) * 8) * 2;
+  auto load = [&](uint32_t t) __attribute__((always_inline)) {  // of the chunk at token t; zeros from the run's end on
+    const uint32_t n = run.t1 - t;
+    const __amdgpu_buffer_rsrc_t bb = make_rsrc(a.B + t * a.b_row + g * a.b_group, kOutOfRange - 1);
+    const __amdgpu_buffer_rsrc_t bc = make_rsrc(a.C + t * a.c_row + g * a.c_group, kOutOfRange - 1);
+    const __amdgpu_buffer_rsrc_t bx = make_rsrc(a.X + t * a.x_row + (g * of_group + head0) * a.x_head, kOutOfRange - 1);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool some = row + i * kRows < n;
+      rb[i] = __builtin_amdgcn_raw_buffer_load_b128(bb, some ? b_off + i * kRows * (uint32_t)a.b_row * 2 : kOutOfRange, 0, 0);
+      if constexpr (!CARRY) rc[i] = __builtin_amdgcn_raw_buffer_load_b128(bc, some ? c_off + i * kRows * (uint32_t)a.c_row * 2 : kOutOfRange, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kXLoads; ++i)
+      rx[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, xlive && xrow + i * 16 < n ? x_off + i * 16 * (uint32_t)a.x_row * 2 : kOutOfRange, 0, 0);
+    rdt = lane < min(n, (uint32_t)L) ? load_dt(a, t + lane, h, DT) : 0.f;
+  };
+  auto put = [&]() __attribute__((always_inline)) {
+    const uint32_t r = opaque(row), xr = opaque(xrow);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t at = piece_at<kRow>(r + i * kRows, piece);
+      *reinterpret_cast<u4*>(sB + at) = rb[i];
+      if constexpr (!CARRY) *reinterpret_cast<u4*>(sC + at) = rc[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kXLoads; ++i) *reinterpret_cast<u4*>(sX + piece_at<kXRow>(xr, xpiece) + i * 16 * kXRow) = rx[i];
+  };
+  load(run.t0);
+
+  // ---- the state: s[nt][r] is channel l32, state 32 nt + 16 (r / 8) + 8 half + r % 8 ----
+  f16x s[kNT];
+  float* const kept = a.state + run.q.row * a.row_stride + ((size_t)h * P + part * 32 + l32) * N + 8 * half;
+  auto place = [&](uint32_t i) { return pl.states + (((size_t)i * pl.units + unit) * (kNT * 4) * kChunkThreads + tid) * 4; };
+  auto fetch = [&](const float* p, size_t quad, f4 (&v)[kNT * 4]) {
+#pragma unroll
+    for (int i = 0; i < kNT * 4; ++i) v[i] = *reinterpret_cast<const f4*>(p + i * quad);
+  };
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) s[i] = f16x{};
+  if (CARRY ? run.idx == run.first : run.first == run.last) {
+    if (run.q.read) {
+#pragma unroll
+      for (int i = 0; i < kNT * 4; ++i) {
+        const f4 v = *reinterpret_cast<const f4*>(kept + 16 * (i / 2) + 4 * (i & 1));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[i / 4][(i & 3) * 4 + e] = v[e];
+      }
+    }
+    // A sequence's first run reads its state here for both launches: its last one, whose place is free, will have
+    // replaced it when the second launch's first one begins.
+    if constexpr (CARRY) {
+      float* const p = place(run.last);
+#pragma unroll
+      for (int i = 0; i < kNT * 4; ++i)
+        *reinterpret_cast<f4*>(p + i * 4 * kChunkThreads) = f4{s[i / 4][(i & 3) * 4], s[i / 4][(i & 3) * 4 + 1], s[i / 4][(i & 3) * 4 + 2], s[i / 4][(i & 3) * 4 + 3]};
+    }
+  } else if constexpr (!CARRY) {
+    // What the runs before this one leave: each adds its own to what it decays.
+    for (uint32_t i = run.first; i < max(run.idx, run.first + 1); ++i) {
+      f4 v[kNT * 4];
+      fetch(place(run.idx == run.first ? run.last : i), 4 * kChunkThreads, v);
+      const float d = i == run.first ? 0.f : __builtin_amdgcn_exp2f(pl.totals[(size_t)i * a.H + h]);
+#pragma unroll
+      for (int j = 0; j < kNT * 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j / 4][(j & 3) * 4 + e] = i == run.first ? v[j][e] : fmaf(s[j / 4][(j & 3) * 4 + e], d, v[j][e]);
+    }
+  }
+
+  float* const cum = vec + wave * 4 * L;  // of this wavefront's head: exponents (of 2), steps, weights, decays
+  float *const steps = cum + L, *const weights = steps + L, *const decays = weights + L;
+  unsigned char* const m0 = sM + mine * 2 * m_bytes<L>();  // M's parts
+  if constexpr (!CARRY) {
+    // The tiles of 16 x 16 right of the diagonal that products of 32 tokens take in stay zero.
+    for (uint32_t i = tid; i < kHeads * 2 * m_bytes<L>() / 16; i += kChunkThreads) *reinterpret_cast<u4*>(sM + i * 16) = u4{0, 0, 0, 0};
+  }
+  // Places of this lane's fragments; a step of products further is an exclusive or, 16 or 32 rows a sum.
+  uint32_t tr_b[2], at_x[2];
+  tr_place<kRow, true>(lane, 0, tr_b);
+  tr_place<kXRow, false>(lane, wave, at_x);
+  const uint32_t row_c = piece_at<kRow>(l32, half), tile_bc = piece_at<kRow>(lane & 15u, lane >> 4);
+  const uint32_t row_m0 = m_place<L>(0, l32, half), row_m1 = m_place<L>(1, l32, half);
+
+  put();
+  float total = 0;
+  for (uint32_t t = run.t0; t < run.t1; t += L) {
+    __syncthreads();
+    const uint32_t n = min(run.t1 - t, (uint32_t)L);
+    // Steps and their sums, a token a lane: from the chunk's beginning, and from its end for the state's weights.
+    const float dt = lane < n ? step_of(rdt + dt0, a.softplus) : 0.f;
+    // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it.)
+    const float e = lane < n ? fmaxf(dt * A, -200.f) : 0.f;
+    const float up = scan_add(e);
+    const float back = scan_add(__shfl(e, 63 - lane));
+    const float after = __shfl(back, (62 - lane) & 63);
+    const float whole = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(up), 63));
+    if (lane < L) {
+      cum[lane] = up;
+      steps[lane] = dt;
+      weights[lane] = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt;
+      decays[lane] = __builtin_amdgcn_exp2f(up);
+    }
+    total += whole;
+    if (t + L < run.t1) load(t + L);
+    __builtin_amdgcn_sched_barrier(0);
+
+    u4 x[kTS];  // x^T: channel l32, tokens 16 i + 8 half ..
+    auto read_x = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < kTS; ++i) x[i] = tr_read(sX + at_x[0] + i * 16 * kXRow, sX + at_x[1] + i * 16 * kXRow);
+    };
+    if constexpr (CARRY) read_x();
+
+    if constexpr (!CARRY) {
+      // M in tiles of 16 x 16, dealt to the head's wavefronts: B_s . C_t, a lane one t and four s.
+      constexpr int kT16 = L / 16, kTiles = kT16 * (kT16 + 1) / 2;
+#pragma unroll
+      for (int k = 0; k < (kTiles + kWaves - 1) / kWaves; ++k) {
+        const uint32_t tile = k * kWaves + part;
+        if (tile < kTiles) {
+          const uint32_t ti = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, si = tile - ti * (ti + 1) / 2;
+          const uint32_t l16 = lane & 15u, quad = lane >> 4;
+          const uint32_t at = opaque(tile_bc);
+          f4 m = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < N / 32; ++j) {
+            const u4 fb = *reinterpret_cast<const u4*>(sB + 16 * si * kRow + (at ^ (uint32_t)(j << 6)));
+            const u4 fc = *reinterpret_cast<const u4*>(sC + 16 * ti * kRow + (at ^ (uint32_t)(j << 6)));
+            m = mfma16x16x32<DT>(fb, fc, m);
+          }
+          const uint32_t tt = 16 * ti + l16, ss = 16 * si + 4 * quad;
+          const float ct = cum[tt];
+          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
+          float w[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[v];
+            if (ss + v == tt) w[v] += D;
+            if (ss + v > tt) w[v] = 0.f;
+          }
+          const uint32_t to = m_place<L>(ti / 2, tt & 31u, ss / 8) + (ss & 4u) * 2;
+          u2 hi, lo;
+          hi[0] = take_part<BF>(w[0], w[1]);
+          hi[1] = take_part<BF>(w[2], w[3]);
+          lo[0] = pack_pair<BF>(w[0], w[1]);
+          lo[1] = pack_pair<BF>(w[2], w[3]);
+          *reinterpret_cast<u2*>(m0 + to) = hi;
+          *reinterpret_cast<u2*>(m0 + m_bytes<L>() + to) = lo;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __syncthreads();
+
+      // y^T: what the state gives, decayed, and the chunk's own.
+      f16x y[kTB];
+      float up2 = 1.f, down2 = 1.f;
+      if constexpr (DT == HQ_DTYPE_F16) {
+        float m = 0;
+#pragma unroll
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(s[i][r]));
+        range_scale(max_of_lanes(m), up2, down2);
+      }
+      auto from_state = [&](float up) __attribute__((always_inline)) {
+        const uint32_t at_c = opaque(row_c);
+        // C's fragments are read a step ahead; their order is held, or all of them would be in registers at once.
+        u4 c[2][kTB];
+        auto read_c = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+          for (int b = 0; b < kTB; ++b) c[k & 1][b] = *reinterpret_cast<const u4*>(sC + (at_c ^ (uint32_t)(k << 5)) + 32 * b * kRow);
+        };
+        read_c(0);
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) y[b] = f16x{};
+#pragma unroll
+        for (int k = 0; k < kNS; ++k) {
+          if (k + 1 < kNS) read_c(k + 1);
+          u4 hi, lo;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float u = s[k / 2][(k & 1) * 8 + 2 * i], v = s[k / 2][(k & 1) * 8 + 2 * i + 1];
+            u *= up;
+            v *= up;
+            hi[i] = take_part<DT>(u, v);
+            lo[i] = pack_pair<DT>(u, v);
+          }
+#pragma unroll
+          for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(hi, c[k & 1][b], y[b]);
+#pragma unroll
+          for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(lo, c[k & 1][b], y[b]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) {
+          const float d = decays[32 * b + l32] * down2;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[b][r] *= d;
+        }
+      };
+      from_state(up2);
+      read_x();
+      const uint32_t at_m[2] = {opaque(row_m0), opaque(row_m1)};
+#pragma unroll
+      for (int k = 0; k < kTS; ++k) {
+        u4 v = x[k], rest = u4{0, 0, 0, 0};
+        if constexpr (DT == HQ_DTYPE_F16) {  // 11 bits are two bf16 parts, exactly
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float p, q;
+            unpack_pair<DT>(v[i], p, q);
+            v[i] = take_part<BF>(p, q);
+            rest[i] = pack_pair<BF>(p, q);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) {
+          if (k > 2 * b + 1) continue;
+          const unsigned char* const p = m0 + (at_m[b] ^ (uint32_t)(k << 5));
+          const u4 hi = *reinterpret_cast<const u4*>(p), lo = *reinterpret_cast<const u4*>(p + m_bytes<L>());
+          y[b] = mfma32<BF>(v, hi, y[b]);
+          y[b] = mfma32<BF>(v, lo, y[b]);
+          if constexpr (DT == HQ_DTYPE_F16) y[b] = mfma32<BF>(rest, hi, y[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // An infinite or NaN x_s reaches the tokens before it as 0 times itself. The last tokens' sums hold every x, were
+      // it times 0: where they are not finite and an x is not, once more with the finite ones, and NaN from the others on.
+      float sum = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += y[kTB - 1][r];
+      if (__builtin_expect(__any(!(fabsf(sum) < INFINITY)) && __any(any_odd<DT>(x)), 0)) {
+        from_state(__uint_as_float(opaque(__float_as_uint(up2))));  // (or all parts of the state are kept for this)
+        const uint32_t m_at[2] = {opaque(row_m0), opaque(row_m1)};
+#pragma unroll
+        for (int b = 0; b < kTB; ++b) {
+          f16x odd = {};
+#pragma unroll 1
+          for (int k = 0; k < 2 * b + 2; ++k) {
+            u4 v = tr_read(sX + at_x[0] + k * 16 * kXRow, sX + at_x[1] + k * 16 * kXRow), rest = u4{0, 0, 0, 0}, code, seen;
+            constexpr uint32_t kExp = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;
+            const uint32_t s0 = 16 * k + 8 * half, tt = 32 * b + l32;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool o0 = (v[i] & kExp) == kExp, o1 = (v[i] >> 16 & kExp) == kExp;
+              code[i] = (o0 ? 0x3F80u : 0u) | (o1 ? 0x3F800000u : 0u);  // 1 in bf16
+              seen[i] = (s0 + 2 * i <= tt ? 0x3F80u : 0u) | (s0 + 2 * i + 1 <= tt ? 0x3F800000u : 0u);
+              v[i] &= (o0 ? 0u : 0xFFFFu) | (o1 ? 0u : 0xFFFF0000u);
+              if constexpr (DT == HQ_DTYPE_F16) {
+                float p, q;
+                unpack_pair<DT>(v[i], p, q);
+                v[i] = take_part<BF>(p, q);
+                rest[i] = pack_pair<BF>(p, q);
+              }
+            }
+            const unsigned char* const p = m0 + (m_at[b] ^ (uint32_t)(k << 5));
+            const u4 hi = *reinterpret_cast<const u4*>(p), lo = *reinterpret_cast<const u4*>(p + m_bytes<L>());
+            y[b] = mfma32<BF>(v, hi, y[b]);
+            y[b] = mfma32<BF>(v, lo, y[b]);
+            if constexpr (DT == HQ_DTYPE_F16) y[b] = mfma32<BF>(rest, hi, y[b]);
+            odd = mfma32<BF>(code, seen, odd);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (odd[r] != 0.f) y[b][r] = NAN;
+        }
+        read_x();
+      }
+
+      // Out: this lane's token (and the one 32 on), four channels side by side.
+#pragma unroll
+      for (int b = 0; b < kTB; ++b) {
+        const uint32_t tt = 32 * b + l32;
+        if (tt < n && live) {
+          const uint32_t p0 = part * 32 + 4 * half;
+          uint16_t* const to = a.Y + (t + tt) * a.y_row + h * a.y_head + p0;
+          const uint16_t* const zp = a.Z + (t + tt) * a.z_row + h * a.z_head + p0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v[4];
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) v[e2] = y[b][4 * i + e2];
+            if (a.Z) {
+              const u2 zw = *reinterpret_cast<const u2*>(zp + 8 * i);
+              float z[4];
+              unpack_pair<DT>(zw[0], z[0], z[1]);
+              unpack_pair<DT>(zw[1], z[2], z[3]);
+#pragma unroll
+              for (int e2 = 0; e2 < 4; ++e2) v[e2] *= silu(z[e2]);
+            }
+            *reinterpret_cast<u2*>(to + 8 * i) = u2{pack_pair<DT>(v[0], v[1]), pack_pair<DT>(v[2], v[3])};
+          }
+        }
+      }
+    }
+
+    // The state: decayed, and the chunk's terms.
+    const float keep = __builtin_amdgcn_exp2f(whole);
+    const uint32_t at_b[2] = {opaque(tr_b[0]), opaque(tr_b[1])};
+    if constexpr (DT == HQ_DTYPE_F16) {
+      float m = 0, xw[kTS][8], up3, down3;
+#pragma unroll
+      for (int k = 0; k < kTS; ++k) {
+        const f4 w0 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half), w1 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          unpack_pair<DT>(x[k][i], xw[k][2 * i], xw[k][2 * i + 1]);
+          xw[k][2 * i] *= i < 2 ? w0[(2 * i) & 3] : w1[(2 * i) & 3];
+          xw[k][2 * i + 1] *= i < 2 ? w0[(2 * i + 1) & 3] : w1[(2 * i + 1) & 3];
+          m = fmaxf(m, fmaxf(fabsf(xw[k][2 * i]), fabsf(xw[k][2 * i + 1])));
+        }
+      }
+      range_scale(max_of_lanes(m), up3, down3);
+      u4 hi[kTS], lo[kTS];
+#pragma unroll
+      for (int k = 0; k < kTS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float u = xw[k][2 * i] * up3, v = xw[k][2 * i + 1] * up3;
+          hi[k][i] = take_part<DT>(u, v);
+          lo[k][i] = pack_pair<DT>(u, v);
+        }
+#pragma unroll
+      for (int i = 0; i < kNT; ++i) {
+        f16x acc = {};
+#pragma unroll
+        for (int k = 0; k < kTS; ++k) {
+          const u4 b = tr_read(sB + (at_b[0] ^ (uint32_t)(i << 6)) + k * 16 * kRow, sB + (at_b[1] ^ (uint32_t)(i << 6)) + k * 16 * kRow);
+          acc = mfma32<DT>(b, hi[k], acc);
+          acc = mfma32<DT>(b, lo[k], acc);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], keep, acc[r] * down3);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kNT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] *= keep;
+#pragma unroll
+      for (int k = 0; k < kTS; ++k) {
+        const f4 w0 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half), w1 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half + 4);
+        u4 p0, p1, p2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float u, v;
+          unpack_pair<DT>(x[k][i], u, v);
+          u *= i < 2 ? w0[(2 * i) & 3] : w1[(2 * i) & 3];
+          v *= i < 2 ? w0[(2 * i + 1) & 3] : w1[(2 * i + 1) & 3];
+          p0[i] = take_part<DT>(u, v);
+          p1[i] = take_part<DT>(u, v);
+          p2[i] = pack_pair<DT>(u, v);
+        }
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) {
+          const u4 b = tr_read(sB + (at_b[0] ^ (uint32_t)(i << 6)) + k * 16 * kRow, sB + (at_b[1] ^ (uint32_t)(i << 6)) + k * 16 * kRow);
+          s[i] = mfma32<DT>(b, p0, s[i]);
+          s[i] = mfma32<DT>(b, p1, s[i]);
+          s[i] = mfma32<DT>(b, p2, s[i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();
+    if (t + L < run.t1) put();
+  }
+
+  if constexpr (CARRY) {
+    float* const p = place(run.idx);
+#pragma unroll
+    for (int i = 0; i < kNT * 4; ++i)
+      *reinterpret_cast<f4*>(p + i * 4 * kChunkThreads) = f4{s[i / 4][(i & 3) * 4], s[i / 4][(i & 3) * 4 + 1], s[i / 4][(i & 3) * 4 + 2], s[i / 4][(i & 3) * 4 + 3]};
+    if (live && part == 0 && lane == 0) pl.totals[(size_t)run.idx * a.H + h] = total;
+  } else if (run.idx == run.last && run.q.keep && live) {
+#pragma unroll
+    for (int i = 0; i < kNT * 4; ++i)
+      *reinterpret_cast<f4*>(kept + 16 * (i / 2) + 4 * (i & 1)) =
+          f4{s[i / 4][(i & 3) * 4], s[i / 4][(i & 3) * 4 + 1], s[i / 4][(i & 3) * 4 + 2], s[i / 4][(i & 3) * 4 + 3]};
+  }
+}
+
+template <int DT, int P, int N, bool CARRY>
+hipError_t launch_one(const ScanArgs& a, const ChunkArgs& c, hipStream_t s) {
+  auto k = hq_ssm_chunk_kernel<DT, P, N, CARRY>;
+  constexpr uint32_t lds = chunk_lds<N, CARRY>(kColumns / P);
+  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (set != hipSuccess) return set;
+  hipLaunchKernelGGL(k, dim3((c.blocks + 7) / 8 * 8), dim3(kChunkThreads), lds, s, a, c);
+  return hipGetLastError();
+}
+
+template <int DT, int P, int N>
+hipError_t launch(const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s) {
+  ChunkArgs c{p.run_tokens, p.units, p.runs, p.runs * p.units, nullptr, nullptr};
+  if (p.split) {
+    c.states = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes);
+    c.totals = c.states + (size_t)c.blocks * kColumns * N;
+    const hipError_t e = launch_one<DT, P, N, true>(a, c, s);
+    if (e != hipSuccess) return e;
+  }
+  return launch_one<DT, P, N, false>(a, c, s);
+}
+
+template <int DT>
+hipError_t launch_type(const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s) {
+  switch (a.P * 1024 + a.N) {
+    case 64 * 1024 + 64: return launch<DT, 64, 64>(a, p, ws, s);
+    case 64 * 1024 + 128: return launch<DT, 64, 128>(a, p, ws, s);
+    case 64 * 1024 + 256: return launch<DT, 64, 256>(a, p, ws, s);
+    case 128 * 1024 + 64: return launch<DT, 128, 64>(a, p, ws, s);
+    case 128 * 1024 + 128: return launch<DT, 128, 128>(a, p, ws, s);
+    default: return launch<DT, 128, 256>(a, p, ws, s);
+  }
+}
+
+}  // namespace
+
+hipError_t launch_ssm_chunks(int dtype, const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s) {
+  return dtype == HQ_DTYPE_F16 ? launch_type<HQ_DTYPE_F16>(a, p, ws, s) : launch_type<HQ_DTYPE_BF16>(a, p, ws, s);
+}
+
+}  // namespace hq

@@ -57,8 +57,8 @@ def _lib() -> ctypes.CDLL:
     cache = ctypes.POINTER(StateCacheDesc)
     args = {
         "hq_ssm_conv": [cache, u32, vp, i64, vp, i64, vp, vp, i32, u32, vp, vp, vp, u32, vp],
-        "hq_ssm_workspace_bytes": [u32, u32, i32, u32, u32, u32, u32, ctypes.POINTER(sz)],
-        "hq_describe_ssm": [u32, u32, i32, u32, u32, u32, u32, ctypes.c_char_p, sz],
+        "hq_ssm_workspace_bytes": [u32, u32, i32, u32, u32, u32, u32, u32, ctypes.POINTER(sz)],
+        "hq_describe_ssm": [u32, u32, i32, u32, u32, u32, u32, u32, ctypes.c_char_p, sz],
         "hq_ssm_scan": [cache, u32, ctypes.c_char_p, vp, vp, vp, u32, u32, vp, sz, vp],
     }
     for name, types in args.items():
@@ -221,15 +221,16 @@ class StateCache:
             raise hq.HQError(hq.HQ_ERR_DEVICE, "states: " + "; ".join(text for bit, text in attn.FAULTS.items() if got & bit))
 
 
-def workspace_bytes(tokens: int, sequences: int, heads: int, head_dim: int, state_dim: int, max_len: int = 0, single: bool = False) -> int:
-    """Workspace of one scan on the current device (single: one without cu_seqlens). It does not fall as its sizes grow."""
+def workspace_bytes(tokens: int, sequences: int, heads: int, groups: int, head_dim: int, state_dim: int, max_len: int = 0, single: bool = False) -> int:
+    """Workspace of one scan on the current device (single: one without cu_seqlens), and of every one of as many sequences with
+    fewer tokens: it does not fall as tokens and max_len grow."""
     b = ctypes.c_size_t(0)
-    hq.check(_lib().hq_ssm_workspace_bytes(tokens, sequences, int(not single), heads, head_dim, state_dim, max_len, ctypes.byref(b)))
+    hq.check(_lib().hq_ssm_workspace_bytes(tokens, sequences, int(not single), heads, groups, head_dim, state_dim, max_len, ctypes.byref(b)))
     return int(b.value)
 
 
-def describe(tokens: int, sequences: int, heads: int, head_dim: int, state_dim: int, max_len: int = 0, single: bool = False) -> str:
+def describe(tokens: int, sequences: int, heads: int, groups: int, head_dim: int, state_dim: int, max_len: int = 0, single: bool = False) -> str:
     """The kernels such a scan runs."""
     buf = ctypes.create_string_buffer(512)
-    hq.check(_lib().hq_describe_ssm(tokens, sequences, int(not single), heads, head_dim, state_dim, max_len, buf, len(buf)))
+    hq.check(_lib().hq_describe_ssm(tokens, sequences, int(not single), heads, groups, head_dim, state_dim, max_len, buf, len(buf)))
     return buf.value.decode()

@@ -95,7 +95,8 @@ def scan(x, dt, A, B, C, state, rows, cu=None, D=None, z=None, dt_bias=None, sof
     In chunks of 64 (chunk), decays are exponentials of sums of up to 64 exponents: a sum of magnitude at most a = the largest
     sum over 64 tokens is off by 12 a U32 (scans of 6 steps, both ways) beside the steps' own, and terms beyond a decay
     of e^-88 vanish; the state's terms are products of parts that keep 2^-22 of them (three of 8 bits, two of 11), its 64
-    sums and those of the chunk's halves 70 U32; the output's weights and states are in two parts, 2^-15 of them at most."""
+    sums and those of the chunk's halves 70 U32, and up to 16 runs' states that are joined 4 U32 each; the output's weights and
+    states are in two parts, 2^-15 of them at most."""
     dtype = x.dtype
     T, H, P = x.shape
     N, R = B.shape[2], H // B.shape[1]
@@ -127,7 +128,7 @@ def scan(x, dt, A, B, C, state, rows, cu=None, D=None, z=None, dt_bias=None, sof
             M = k * M + term.abs()
             E = E + 2 * U32 * M
             if chunk:
-                extra = 1.1 * (2.0 ** -22 + (70 + 13 * most) * U32) / 64  # of M, spread over the chunk's tokens
+                extra = 1.1 * (2.0 ** -22 + (134 + 13 * most) * U32) / 64  # of M, spread over the chunk's tokens
                 E = E + extra * M
             out[t] = (S * Cs[t][:, None, :]).sum(-1)
             y_mag = (M * Cs[t][:, None, :].abs()).sum(-1)

@@ -117,14 +117,14 @@ def run(c, layer, p, rows=None, cu=None, held=None, **kw):
     return c.scan(layer, p["x"], p["dt"], p["A"], p["B"], p["C"], D=p["D"], z=p["z"], dt_bias=p["dt_bias"], **lists, **kw)
 
 
-def in_chunks(T, n, cu, H, P, N):
-    return "chunk" in ssm.describe(T, n, H, P, N, single=cu is None)
+def in_chunks(T, n, cu, H, G, P, N):
+    return "chunk" in ssm.describe(T, n, H, G, P, N, single=cu is None)
 
 
 def compare(c, got, p, state, rows, cu, held, label="", **kw):
     T, H, P = p["x"].shape
-    N = p["B"].shape[2]
-    chunk = in_chunks(T, len(rows), cu, H, P, N)
+    G, N = p["B"].shape[1:]
+    chunk = in_chunks(T, len(rows), cu, H, G, P, N)
     want, bound, S, off = M.scan(p["x"], p["dt"], p["A"], p["B"], p["C"], state, rows, cu, p["D"], p["z"], p["dt_bias"], held=held, chunk=chunk, **kw)
     a = M.check(got, want, bound, label + " outputs")
     b = M.check(c.ssm_state[-1], S, off, label + " states")
@@ -155,6 +155,29 @@ def test_scan(cuda, dtype, lens, H, G, P, N):
         c.check()
         compare(c, got, p, state[1], rows, cu, hold, f"{lens}")
         assert torch.equal(c.ssm_state[0], state[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,G,P,N,lens", [(8, 4, 128, 128, [700]), (8, 4, 128, 128, [3, 1, 1000, 500]), (3, 1, 64, 64, [1029]), (4, 4, 64, 256, [600, 40]),
+                                          (2, 1, 128, 256, [513])])
+def test_scan_of_sequences_in_runs(cuda, dtype, H, G, P, N, lens):
+    """Long sequences whose tokens are dealt to several workgroups, some that continue and some that begin."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    cu, T, n = offsets(lens), sum(lens), len(lens)
+    assert "twice" in ssm.describe(T, n, H, G, P, N)
+    p = problem(gen, dtype, T, H, G, P, N)
+    p["A"] /= 30  # states that last from run to run
+    state = 0.1 * randn(gen, torch.float32, 1, n + 1, H, P, N)
+    for held in (None, [i % 2 for i in range(n)]):
+        c = ssm.StateCache(ssm=state.clone())
+        rows = list(range(n))[::-1]
+        got = run(c, 0, p, rows, cu, held)
+        compare(c, got, p, state[0], rows, cu, held)
+        d = ssm.StateCache(ssm=state.clone())  # a workspace of the caller's
+        ws = torch.zeros(ssm.workspace_bytes(T, n, H, G, P, N), dtype=torch.uint8, device="cuda")
+        assert torch.equal(run(d, 0, p, rows, cu, held, workspace=ws), got) and torch.equal(c.ssm_state, d.ssm_state)
+        d = ssm.StateCache(ssm=state.clone())  # (another split, other roundings)
+        compare(d, run(d, 0, p, rows, cu, held, workspace=ws, max_len=max(lens)), p, state[0], rows, cu, held)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -216,7 +239,7 @@ def test_scan_rows_that_are_not_kept(cuda, lens):
     c.check()
     padded = torch.cat([state[0], torch.zeros(3, H, P, N, device="cuda")])
     padded[0] = 0
-    chunk = in_chunks(T, n, cu, H, P, N)
+    chunk = in_chunks(T, n, cu, H, 1, P, N)
     want, bound, S, off = M.scan(p["x"], p["dt"], p["A"], p["B"], p["C"], padded, [3, 8, 5, 9, 10, 0], cu, p["D"], p["z"], p["dt_bias"], held=held,
                                  chunk=chunk)
     M.check(out, want, bound)
@@ -261,7 +284,7 @@ def test_scan_in_pieces(cuda, dtype):
         cu = None if n == 1 else [0, n]
         got = run(c, 0, part, [1], cu, [at])
         want, bound, S, off = M.scan(part["x"], part["dt"], part["A"], part["B"], part["C"], before, [1], cu, part["D"], part["z"], part["dt_bias"],
-                                     held=[at], chunk=in_chunks(n, 1, cu, H, P, N))
+                                     held=[at], chunk=in_chunks(n, 1, cu, H, G, P, N))
         M.check(got, want, bound, f"{at}")
         M.check(c.ssm_state[0, 1], S[1], off[1], f"{at} states")
         at += n
@@ -307,6 +330,20 @@ def test_streams_and_graphs(cuda):
             torch.cuda.synchronize()
             assert torch.equal(y, want) and torch.equal(a.ssm_state, b.ssm_state) and torch.equal(a.conv_state, b.conv_state)
         b.check()
+
+
+def test_offsets_that_fall(cuda):
+    """Offsets that are not what they should be are clamped: whatever comes out, nothing is touched but the call's own."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    H, P, N, T, dtype = 2, 64, 64, 900, torch.float16
+    p = problem(gen, dtype, T, H, 1, P, N)
+    for cu in ([0, T, 0, T, -5, 10 * T, 3], [T, T, T, T, T, T, T], [-9, -8, -7, 100, 50, 60, T + 1]):
+        c = ssm.StateCache.create(1, 8, 64, 4, H, P, N, dtype)
+        out = torch.full((T + 64, H, P), 7.0, dtype=dtype, device="cuda")
+        run(c, 0, p, list(range(6)), cu, out=out[:T])
+        c.conv(0, p["x"][:, 0].contiguous(), randn(gen, torch.float32, P, 4), i32(*range(6)), i32(*cu))
+        torch.cuda.synchronize()
+        assert (out[T:] == 7).all() and not c.ssm_state[0, 6:].any() and not c.conv_state[0, 6:].any()
 
 
 def test_results_are_the_same_every_time(cuda):

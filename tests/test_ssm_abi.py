@@ -82,7 +82,8 @@ def test_bad_conv(kw, status):
 @pytest.mark.parametrize("kw,status", [
     (dict(c=cache(ssm=0)), hq.HQ_ERR_INVALID_ARG), (dict(c=cache(ssm=P + 4)), hq.HQ_ERR_ALIGNMENT), (dict(c=cache(head_dim=96)), hq.HQ_ERR_UNSUPPORTED),
     (dict(c=cache(state_dim=16)), hq.HQ_ERR_UNSUPPORTED), (dict(c=cache(heads=0)), hq.HQ_ERR_SHAPE), (dict(c=cache(heads=1025)), hq.HQ_ERR_SHAPE),
-    (dict(c=cache(ssm_row=65532)), hq.HQ_ERR_SHAPE), (dict(c=cache(ssm_row=65538)), hq.HQ_ERR_ALIGNMENT), (dict(c=cache(ssm_layer=65540)), hq.HQ_ERR_SHAPE)])
+    (dict(c=cache(ssm_row=65532)), hq.HQ_ERR_SHAPE), (dict(c=cache(ssm_row=65538)), hq.HQ_ERR_ALIGNMENT), (dict(c=cache(ssm_layer=65540)), hq.HQ_ERR_SHAPE),
+    (dict(ws=P + 128, wsb=1 << 40, n=1, cu=P, i=io(tokens=1 << 16)), hq.HQ_ERR_ALIGNMENT), (dict(ws=P, wsb=8, n=1, cu=P, i=io(tokens=1 << 16)), hq.HQ_ERR_WORKSPACE)])
 def test_bad_scan(kw, status):
     assert scan(**kw) == status
     assert ssm._lib().hq_ssm_scan(cache(), 0, None, P, None, None, 4, 0, None, 0, None) == hq.HQ_ERR_INVALID_ARG
@@ -97,7 +98,7 @@ def test_bad_scan(kw, status):
     (dict(x_head=64), hq.HQ_ERR_SHAPE), (dict(b_group=64), hq.HQ_ERR_SHAPE), (dict(c_row=-8), hq.HQ_ERR_SHAPE), (dict(y_row=256), hq.HQ_ERR_SHAPE),
     (dict(Z=P, z_head=100), hq.HQ_ERR_ALIGNMENT), (dict(Z=P + 4096, z_row=1024), hq.HQ_ERR_SHAPE), (dict(dt_row=3), hq.HQ_ERR_SHAPE),
     (dict(dt_row=-4), hq.HQ_ERR_SHAPE), (dict(dt_row=1 << 50), hq.HQ_ERR_SHAPE), (dict(tokens=0), hq.HQ_ERR_SHAPE), (dict(tokens=5), hq.HQ_ERR_SHAPE),
-    (dict(y_row=128, y_head=256), hq.HQ_ERR_SHAPE)])
+    (dict(y_row=128, y_head=256), hq.HQ_ERR_SHAPE), (dict(x_row=(1 << 23) + 8), hq.HQ_ERR_SHAPE), (dict(b_row=1 << 24), hq.HQ_ERR_SHAPE)])
 def test_bad_io(kw, status):
     assert scan(i=io(**kw)) == status
 
@@ -108,17 +109,18 @@ def workspace(*a):
 
 
 def test_workspace_query():
-    assert workspace(4, 4, 0, 48, 128, 128, 0) == (hq.HQ_OK, 0)
-    for bad, status in (((0, 1, 1, 48, 128, 128, 0), hq.HQ_ERR_SHAPE), ((5, 4, 0, 48, 128, 128, 0), hq.HQ_ERR_SHAPE), ((5, 0, 1, 48, 128, 128, 0), hq.HQ_ERR_SHAPE),
-                        ((5, 1, 1, 0, 128, 128, 0), hq.HQ_ERR_SHAPE), ((5, 1, 1, 48, 32, 128, 0), hq.HQ_ERR_UNSUPPORTED),
-                        ((5, 1, 1, 48, 128, 512, 0), hq.HQ_ERR_UNSUPPORTED)):
+    assert workspace(4, 4, 0, 48, 16, 128, 128, 0) == (hq.HQ_OK, 0)
+    for bad, status in (((0, 1, 1, 48, 16, 128, 128, 0), hq.HQ_ERR_SHAPE), ((5, 4, 0, 48, 16, 128, 128, 0), hq.HQ_ERR_SHAPE),
+                        ((5, 0, 1, 48, 16, 128, 128, 0), hq.HQ_ERR_SHAPE), ((5, 1, 1, 0, 16, 128, 128, 0), hq.HQ_ERR_SHAPE),
+                        ((5, 1, 1, 48, 7, 128, 128, 0), hq.HQ_ERR_SHAPE), ((5, 1, 1, 48, 0, 128, 128, 0), hq.HQ_ERR_SHAPE),
+                        ((5, 1, 1, 48, 16, 32, 128, 0), hq.HQ_ERR_UNSUPPORTED), ((5, 1, 1, 48, 16, 128, 512, 0), hq.HQ_ERR_UNSUPPORTED)):
         assert workspace(*bad)[0] == status
-    assert ssm._lib().hq_ssm_workspace_bytes(4, 4, 0, 48, 128, 128, 0, None) == hq.HQ_ERR_INVALID_ARG
-    assert "hq_ssm" in ssm.describe(4, 4, 48, 128, 128, single=True)
+    assert ssm._lib().hq_ssm_workspace_bytes(4, 4, 0, 48, 16, 128, 128, 0, None) == hq.HQ_ERR_INVALID_ARG
+    assert "hq_ssm" in ssm.describe(4, 4, 48, 16, 128, 128, single=True)
     for n in (1, 3, 16):
         for H in (1, 8, 48, 128):
             last = 0
             for T in [16, 64, 65, 100, 128, 200, 500, 640, 1000, 1600, 2000, 4096, 6000, 8192, 20000, 65536, 1 << 20]:
-                size = ssm.workspace_bytes(T, n, H, 128, 128)
+                size = ssm.workspace_bytes(T, n, H, 1, 128, 128)
                 assert size >= last, (n, H, T)
                 last = size
