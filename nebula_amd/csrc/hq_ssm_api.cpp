@@ -155,10 +155,10 @@ hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_
       (st = check_strides("C", io->c_row, io->c_group, T, G, N)) != HQ_OK || (st = check_strides("Y", io->y_row, io->y_head, T, H, P)) != HQ_OK ||
       (io->Z && (st = check_strides("Z", io->z_row, io->z_head, T, H, P)) != HQ_OK))
     return st;
-  // The chunk kernel reaches 64 tokens, and two heads of 64, with 32-bit offsets.
-  if (io->x_row > kMaxRow || io->b_row > kMaxRow || io->c_row > kMaxRow || (P == 64 && H > 1 && io->x_head > 64 * kMaxRow))
-    return fail(HQ_ERR_SHAPE, "X, B, C: row strides %lld, %lld, %lld above %lld elements, or X's head stride %lld too large", (long long)io->x_row,
-                (long long)io->b_row, (long long)io->c_row, (long long)kMaxRow, (long long)io->x_head);
+  // The chunk kernel reaches 64 tokens with 32-bit offsets.
+  if (io->x_row > kMaxRow || io->b_row > kMaxRow || io->c_row > kMaxRow || io->y_row > kMaxRow || (io->Z && io->z_row > kMaxRow))
+    return fail(HQ_ERR_SHAPE, "X, B, C, Y, Z: row strides %lld, %lld, %lld, %lld, %lld above %lld elements", (long long)io->x_row,
+                (long long)io->b_row, (long long)io->c_row, (long long)io->y_row, (long long)io->z_row, (long long)kMaxRow);
   if (overlaps(io->y_row, io->y_head, T, H, P)) return fail(HQ_ERR_SHAPE, "Y: strides %lld, %lld make rows or heads overlap", (long long)io->y_row, (long long)io->y_head);
   if (io->Y == io->Z && ((T > 1 && io->y_row != io->z_row) || (H > 1 && io->y_head != io->z_head))) return fail(HQ_ERR_SHAPE, "Y is Z with other strides");
   if (io->dt_row < 0 || io->dt_row > kMaxSpan || (T > 1 && io->dt_row < (int64_t)H) || (double)io->dt_row * T > (double)kMaxSpan)

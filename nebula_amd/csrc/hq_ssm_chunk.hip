@@ -41,7 +41,7 @@ __device__ __forceinline__ f16x mfma32(u4 a, u4 b, f16x c) {
 
 constexpr int BF = HQ_DTYPE_BF16;
 constexpr uint32_t kChunkThreads = 256;
-constexpr uint32_t kColumns = 128;  // of a chunk's x: four wavefronts of 32 channels
+constexpr uint32_t kColumns = 128;  // channels of a workgroup, four wavefronts of 32
 
 // Tokens of a chunk: the state of 256 leaves registers and LDS for 32.
 template <int N>
@@ -116,15 +116,17 @@ __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
   return w;
 }
 
+// The largest exponents (of both halves) of 16-byte pieces of activations; an infinity or NaN has the type's largest.
 template <int DT, int K>
-__device__ __forceinline__ bool any_odd(const u4 (&x)[K]) {
-  constexpr uint32_t kExp = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;
-  bool odd = false;
+__device__ __forceinline__ uint32_t exponents(const u4 (&x)[K]) {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kMask = DT == HQ_DTYPE_F16 ? 0x7C007C00u : 0x7F807F80u;
+  us2 m = {0, 0};
 #pragma unroll
   for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) odd |= (x[k][i] & kExp) == kExp || (x[k][i] >> 16 & kExp) == kExp;
-  return odd;
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, x[k][i] & kMask));
+  return max((uint32_t)m[0], (uint32_t)m[1]);
 }
 
 // A place in LDS as the compiler has it: what is computed from it stays in its chunk. (Held from chunk to chunk, the places
@@ -132,6 +134,17 @@ __device__ __forceinline__ bool any_odd(const u4 (&x)[K]) {
 __device__ __forceinline__ uint32_t opaque(uint32_t v) {
   asm volatile("" : "+v"(v));
   return v;
+}
+
+// The order of a step: a product, then VALU other instructions and READS reads of LDS, N times.
+template <int N, int VALU, int READS>
+__device__ __forceinline__ void between() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, VALU, 0);
+  }
 }
 
 // Which run of chunks a workgroup works on.
@@ -181,19 +194,23 @@ constexpr uint32_t vec_bytes() {
 template <int N, bool CARRY>
 constexpr uint32_t chunk_lds(uint32_t heads) {
   constexpr uint32_t L = chunk_tokens<N>();
-  return (CARRY ? 1 : 2) * L * N * 2 + L * kColumns * 2 + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>());
+  return (CARRY ? 1 : 2) * L * N * 2 + L * kColumns * 2 + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>()) + 16;
 }
 
-// CARRY: the state alone, of all runs but a sequence's last, for the runs behind them.
-template <int DT, int P, int N, bool CARRY>
+// What a launch computes: outputs, outputs through a gate, or the state alone, of all runs but a sequence's last, for the runs
+// behind them.
+enum Kind : int { kPlain, kGated, kCarry };
+
+template <int DT, int P, int N, int KIND>
 __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_kernel(ScanArgs a, ChunkArgs pl) {
+  constexpr bool CARRY = KIND == kCarry, GATED = KIND == kGated;
   constexpr int L = chunk_tokens<N>(), kHeads = kColumns / P, kWaves = P / 32;  // heads, wavefronts of a head
   constexpr int kTB = L / 32, kTS = L / 16, kNT = N / 32, kNS = N / 16;
-  constexpr int kRow = 2 * N, kXRow = 2 * kColumns;
+  constexpr int kRow = 2 * N, kXRow = 64;
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char* const sB = smem;
   unsigned char* const sX = sB + L * kRow;
-  float* const vec = reinterpret_cast<float*>(sX + L * kXRow);
+  float* const vec = reinterpret_cast<float*>(sX + 4 * L * kXRow);
   unsigned char* const sC = reinterpret_cast<unsigned char*>(vec) + vec_bytes<N>();
   unsigned char* const sM = sC + L * kRow;
 
@@ -222,37 +239,54 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   constexpr int kPieces = N / 8, kRows = kChunkThreads / kPieces, kLoads = L / kRows, kXLoads = L / 16;
   u4 rb[kLoads], rc[CARRY ? 1 : kLoads], rx[kXLoads];
   float rdt = 0;
-  const uint32_t row = tid / kPieces, piece = tid % kPieces, xrow = tid / 16, xpiece = tid % 16;
-  const bool xlive = head0 + xpiece / (P / 8) < of_group;
-  // 32-bit offsets from the chunk's first token; a place past any operand reads as 0 without touching memory.
-  const uint32_t b_off = (row * (uint32_t)a.b_row + piece * 8) * 2, c_off = (row * (uint32_t)a.c_row + piece * 8) * 2;
-  const uint32_t x_off = (xrow * (uint32_t)a.x_row + (xpiece / (P / 8)) * (uint32_t)a.x_head + xpiece % (P / 8) * 8) * 2;
+  // 32-bit offsets from the chunk's first token, made anew for each chunk; a place past any operand reads as 0 without
+  // touching memory.
   auto load = [&](uint32_t t) __attribute__((always_inline)) {  // of the chunk at token t; zeros from the run's end on
+    const uint32_t id = opaque(tid), row = id / kPieces, piece = id % kPieces, xrow = (id & 63u) / 4, xpiece = id % 4;  // x: the wavefront's channels
+    const uint32_t b_off = (row * (uint32_t)a.b_row + piece * 8) * 2, c_off = (row * (uint32_t)a.c_row + piece * 8) * 2;
+    const uint32_t x_off = (xrow * (uint32_t)a.x_row + xpiece * 8) * 2;
     const uint32_t n = run.t1 - t;
     const __amdgpu_buffer_rsrc_t bb = make_rsrc(a.B + t * a.b_row + g * a.b_group, kOutOfRange - 1);
     const __amdgpu_buffer_rsrc_t bc = make_rsrc(a.C + t * a.c_row + g * a.c_group, kOutOfRange - 1);
-    const __amdgpu_buffer_rsrc_t bx = make_rsrc(a.X + t * a.x_row + (g * of_group + head0) * a.x_head, kOutOfRange - 1);
+    const __amdgpu_buffer_rsrc_t bx = make_rsrc(a.X + t * a.x_row + h * a.x_head + part * 32, kOutOfRange - 1);
+    auto place = [&](uint32_t off, uint32_t r) __attribute__((always_inline)) { return off | (r < n ? 0u : kOutOfRange); };
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const bool some = row + i * kRows < n;
-      rb[i] = __builtin_amdgcn_raw_buffer_load_b128(bb, some ? b_off + i * kRows * (uint32_t)a.b_row * 2 : kOutOfRange, 0, 0);
-      if constexpr (!CARRY) rc[i] = __builtin_amdgcn_raw_buffer_load_b128(bc, some ? c_off + i * kRows * (uint32_t)a.c_row * 2 : kOutOfRange, 0, 0);
+      rb[i] = __builtin_amdgcn_raw_buffer_load_b128(bb, place(b_off + i * kRows * (uint32_t)a.b_row * 2, row + i * kRows), 0, 0);
+      if constexpr (!CARRY) rc[i] = __builtin_amdgcn_raw_buffer_load_b128(bc, place(c_off + i * kRows * (uint32_t)a.c_row * 2, row + i * kRows), 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < kXLoads; ++i)
-      rx[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, xlive && xrow + i * 16 < n ? x_off + i * 16 * (uint32_t)a.x_row * 2 : kOutOfRange, 0, 0);
+    for (int i = 0; i < kXLoads; ++i) rx[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, place(x_off + i * 16 * (uint32_t)a.x_row * 2, xrow + i * 16), 0, 0);
     rdt = lane < min(n, (uint32_t)L) ? load_dt(a, t + lane, h, DT) : 0.f;
   };
   auto put = [&]() __attribute__((always_inline)) {
-    const uint32_t r = opaque(row), xr = opaque(xrow);
+    const uint32_t id = opaque(tid);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint32_t at = piece_at<kRow>(r + i * kRows, piece);
+      const uint32_t at = piece_at<kRow>(id / kPieces + i * kRows, id % kPieces);
       *reinterpret_cast<u4*>(sB + at) = rb[i];
       if constexpr (!CARRY) *reinterpret_cast<u4*>(sC + at) = rc[i];
     }
+  };
+  // x goes through LDS for its order alone, to the wavefront that brought it.
+  unsigned char* const own = sX + wave * L * kXRow;
+  constexpr uint32_t kOdd = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;  // the exponent of infinities and NaN
+  float x_most = 0;  // fp16: a power of two above the next chunk's x
+  auto put_x = [&](uint32_t* odd) __attribute__((always_inline)) {
+    const uint32_t id = opaque(lane), xrow = id / 4, at = piece_at<kXRow>(xrow, id % 4), most = exponents<DT>(rx);
 #pragma unroll
-    for (int i = 0; i < kXLoads; ++i) *reinterpret_cast<u4*>(sX + piece_at<kXRow>(xr, xpiece) + i * 16 * kXRow) = rx[i];
+    for (int i = 0; i < kXLoads; ++i) *reinterpret_cast<u4*>(own + at + i * 16 * kXRow) = rx[i];
+    if (__builtin_expect(most == kOdd, 0)) {
+#pragma unroll
+      for (int i = kXLoads - 1; i >= 0; --i) {
+        const u4 one[1] = {rx[i]};
+        if (exponents<DT>(one) == kOdd) atomicMin(odd, xrow + i * 16);
+      }
+    }
+    if constexpr (DT == HQ_DTYPE_F16) {
+      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)scan(most, 0, [](uint32_t p, uint32_t q) { return max(p, q); }), 63);
+      x_most = __uint_as_float(((all >> 10) + 113u) << 23);  // 2^(e - 15 + 1), for exponent e
+    }
   };
   load(run.t0);
 
@@ -306,15 +340,29 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   // Places of this lane's fragments; a step of products further is an exclusive or, 16 or 32 rows a sum.
   uint32_t tr_b[2], at_x[2];
   tr_place<kRow, true>(lane, 0, tr_b);
-  tr_place<kXRow, false>(lane, wave, at_x);
-  const uint32_t row_c = piece_at<kRow>(l32, half), tile_bc = piece_at<kRow>(lane & 15u, lane >> 4);
-  const uint32_t row_m0 = m_place<L>(0, l32, half), row_m1 = m_place<L>(1, l32, half);
+  tr_place<kXRow, false>(lane, 0, at_x);
 
+  // odd[i]: the first token of a chunk (the i-th, modulo 2) with an x that is not finite.
+  uint32_t* const odd = reinterpret_cast<uint32_t*>(smem + chunk_lds<N, CARRY>(kHeads) - 8);
+  if (tid < 2) odd[tid] = L;
+  __syncthreads();
   put();
+  put_x(odd);
   float total = 0;
-  for (uint32_t t = run.t0; t < run.t1; t += L) {
+  uint32_t n, turn = 0;
+  for (uint32_t t = run.t0; t < run.t1; t += n, turn ^= 1u) {
     __syncthreads();
-    const uint32_t n = min(run.t1 - t, (uint32_t)L);
+    n = min(run.t1 - t, (uint32_t)L);
+    // 0 times an infinity is no 0: the tokens before an x that is not finite, and it alone, are chunks of their own. What
+    // lies past them in LDS is cleared.
+    const uint32_t first = uni(odd[turn]);
+    if (__builtin_expect(first < n, 0)) {
+      n = max(first, 1u);
+      for (uint32_t i = tid; i < (L - n) * kPieces; i += kChunkThreads) *reinterpret_cast<u4*>(sB + n * kRow + i * 16) = u4{0, 0, 0, 0};
+      for (uint32_t i = lane; i < (L - n) * 4; i += 64) *reinterpret_cast<u4*>(own + n * kXRow + i * 16) = u4{0, 0, 0, 0};
+      __syncthreads();
+    }
+    if (tid == 0) odd[turn ^ 1u] = L;
     // Steps and their sums, a token a lane: from the chunk's beginning, and from its end for the state's weights.
     const float dt = lane < n ? step_of(rdt + dt0, a.softplus) : 0.f;
     // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it.)
@@ -323,23 +371,28 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     const float back = scan_add(__shfl(e, 63 - lane));
     const float after = __shfl(back, (62 - lane) & 63);
     const float whole = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(up), 63));
+    const float weight = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt;
+    float up3 = 1.f, down3 = 1.f;
+    if constexpr (DT == HQ_DTYPE_F16) range_scale(max_of_lanes(fabsf(weight)) * x_most, up3, down3);
     if (lane < L) {
       cum[lane] = up;
       steps[lane] = dt;
-      weights[lane] = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt;
+      weights[lane] = weight * up3;
       decays[lane] = __builtin_amdgcn_exp2f(up);
     }
     total += whole;
-    if (t + L < run.t1) load(t + L);
+    if (t + n < run.t1) load(t + n);
     __builtin_amdgcn_sched_barrier(0);
 
     u4 x[kTS];  // x^T: channel l32, tokens 16 i + 8 half ..
     auto read_x = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < kTS; ++i) x[i] = tr_read(sX + at_x[0] + i * 16 * kXRow, sX + at_x[1] + i * 16 * kXRow);
+      for (int i = 0; i < kTS; ++i) x[i] = tr_read(own + at_x[0] + i * 16 * kXRow, own + at_x[1] + i * 16 * kXRow);
     };
     if constexpr (CARRY) read_x();
 
+    f16x y[kTB];
+    u2 zr[kTB][4];  // the gates
     if constexpr (!CARRY) {
       // M in tiles of 16 x 16, dealt to the head's wavefronts: B_s . C_t, a lane one t and four s.
       constexpr int kT16 = L / 16, kTiles = kT16 * (kT16 + 1) / 2;
@@ -348,8 +401,8 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         const uint32_t tile = k * kWaves + part;
         if (tile < kTiles) {
           const uint32_t ti = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, si = tile - ti * (ti + 1) / 2;
-          const uint32_t l16 = lane & 15u, quad = lane >> 4;
-          const uint32_t at = opaque(tile_bc);
+          // (Opaque: places and masks of all tiles are not to be kept from chunk to chunk.)
+          const uint32_t id = opaque(lane), l16 = id & 15u, quad = id >> 4, at = piece_at<kRow>(l16, quad);
           f4 m = {0, 0, 0, 0};
 #pragma unroll
           for (int j = 0; j < N / 32; ++j) {
@@ -362,10 +415,11 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
           const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
           float w[4];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[v];
-            if (ss + v == tt) w[v] += D;
-            if (ss + v > tt) w[v] = 0.f;
+          for (int v = 0; v < 4; ++v) w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[v];
+          if (ti == si) {
+            const int32_t past = (int32_t)l16 - 4 * (int32_t)quad;  // tokens from the lane's first one to its own
+#pragma unroll
+            for (int v = 0; v < 4; ++v) w[v] = v < past ? w[v] : v == past ? w[v] + D : 0.f;
           }
           const uint32_t to = m_place<L>(ti / 2, tt & 31u, ss / 8) + (ss & 4u) * 2;
           u2 hi, lo;
@@ -381,7 +435,6 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
       __syncthreads();
 
       // y^T: what the state gives, decayed, and the chunk's own.
-      f16x y[kTB];
       float up2 = 1.f, down2 = 1.f;
       if constexpr (DT == HQ_DTYPE_F16) {
         float m = 0;
@@ -392,32 +445,33 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         range_scale(max_of_lanes(m), up2, down2);
       }
       auto from_state = [&](float up) __attribute__((always_inline)) {
-        const uint32_t at_c = opaque(row_c);
-        // C's fragments are read a step ahead; their order is held, or all of them would be in registers at once.
-        u4 c[2][kTB];
-        auto read_c = [&](int k) __attribute__((always_inline)) {
+        const uint32_t id = opaque(lane), at_c = piece_at<kRow>(id & 31u, id >> 5);
+        // A step's parts of the state are made, and C's fragments read, between the products of the step before it.
+        u4 c[2][kTB], hi[2], lo[2];
+        auto ready = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
           for (int b = 0; b < kTB; ++b) c[k & 1][b] = *reinterpret_cast<const u4*>(sC + (at_c ^ (uint32_t)(k << 5)) + 32 * b * kRow);
-        };
-        read_c(0);
-#pragma unroll
-        for (int b = 0; b < kTB; ++b) y[b] = f16x{};
-#pragma unroll
-        for (int k = 0; k < kNS; ++k) {
-          if (k + 1 < kNS) read_c(k + 1);
-          u4 hi, lo;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float u = s[k / 2][(k & 1) * 8 + 2 * i], v = s[k / 2][(k & 1) * 8 + 2 * i + 1];
-            u *= up;
-            v *= up;
-            hi[i] = take_part<DT>(u, v);
-            lo[i] = pack_pair<DT>(u, v);
+            if constexpr (DT == HQ_DTYPE_F16) {
+              u *= up;
+              v *= up;
+            }
+            hi[k & 1][i] = take_part<DT>(u, v);
+            lo[k & 1][i] = pack_pair<DT>(u, v);
           }
+        };
+        ready(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(hi, c[k & 1][b], y[b]);
+        for (int k = 0; k < kNS; ++k) {
+          if (k + 1 < kNS) ready(k + 1);
 #pragma unroll
-          for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(lo, c[k & 1][b], y[b]);
+          for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(hi[k & 1], c[k & 1][b], k ? y[b] : f16x{});
+#pragma unroll
+          for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(lo[k & 1], c[k & 1][b], y[b]);
+          between<2 * kTB, 24 / (2 * kTB), 1>();
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -429,9 +483,30 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
       };
       from_state(up2);
       read_x();
-      const uint32_t at_m[2] = {opaque(row_m0), opaque(row_m1)};
+      if constexpr (GATED) {
+        const __amdgpu_buffer_rsrc_t bz = make_rsrc(a.Z + t * a.z_row + h * a.z_head + part * 32, kOutOfRange - 1);
 #pragma unroll
-      for (int k = 0; k < kTS; ++k) {
+        for (int b = 0; b < kTB; ++b) {
+          const uint32_t tt = 32 * b + l32, at = tt < n && live ? (tt * (uint32_t)a.z_row + 4 * half) * 2 : kOutOfRange;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) zr[b][i] = __builtin_amdgcn_raw_buffer_load_b64(bz, at + 16 * i, 0, 0);
+        }
+      }
+      // M's fragments are read a step ahead, the state decays between the products.
+      const uint32_t idm = opaque(lane), at_m[2] = {m_place<L>(0, idm & 31u, idm >> 5), m_place<L>(1, idm & 31u, idm >> 5)};
+      constexpr int kSteps = kTB == 2 ? 6 : 2;  // products of 16 earlier tokens: 2 for the first 32 tokens, 4 for the others
+      u4 mf[2][2];
+      auto read_m = [&](int j) __attribute__((always_inline)) {
+        const int b = j < 2 ? 0 : 1, k = j < 2 ? j : j - 2;
+        const unsigned char* const p = m0 + (at_m[b] ^ (uint32_t)(k << 5));
+        mf[j & 1][0] = *reinterpret_cast<const u4*>(p);
+        mf[j & 1][1] = *reinterpret_cast<const u4*>(p + m_bytes<L>());
+      };
+      read_m(0);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const int b = j < 2 ? 0 : 1, k = j < 2 ? j : j - 2;
+        if (j + 1 < kSteps) read_m(j + 1);
         u4 v = x[k], rest = u4{0, 0, 0, 0};
         if constexpr (DT == HQ_DTYPE_F16) {  // 11 bits are two bf16 parts, exactly
 #pragma unroll
@@ -442,157 +517,118 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
             rest[i] = pack_pair<BF>(p, q);
           }
         }
-#pragma unroll
-        for (int b = 0; b < kTB; ++b) {
-          if (k > 2 * b + 1) continue;
-          const unsigned char* const p = m0 + (at_m[b] ^ (uint32_t)(k << 5));
-          const u4 hi = *reinterpret_cast<const u4*>(p), lo = *reinterpret_cast<const u4*>(p + m_bytes<L>());
-          y[b] = mfma32<BF>(v, hi, y[b]);
-          y[b] = mfma32<BF>(v, lo, y[b]);
-          if constexpr (DT == HQ_DTYPE_F16) y[b] = mfma32<BF>(rest, hi, y[b]);
-        }
+        y[b] = mfma32<BF>(v, mf[j & 1][0], y[b]);
+        y[b] = mfma32<BF>(v, mf[j & 1][1], y[b]);
+        if constexpr (DT == HQ_DTYPE_F16) y[b] = mfma32<BF>(rest, mf[j & 1][0], y[b]);
         __builtin_amdgcn_sched_barrier(0);
-      }
-      // An infinite or NaN x_s reaches the tokens before it as 0 times itself. The last tokens' sums hold every x, were
-      // it times 0: where they are not finite and an x is not, once more with the finite ones, and NaN from the others on.
-      float sum = 0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum += y[kTB - 1][r];
-      if (__builtin_expect(__any(!(fabsf(sum) < INFINITY)) && __any(any_odd<DT>(x)), 0)) {
-        from_state(__uint_as_float(opaque(__float_as_uint(up2))));  // (or all parts of the state are kept for this)
-        const uint32_t m_at[2] = {opaque(row_m0), opaque(row_m1)};
-#pragma unroll
-        for (int b = 0; b < kTB; ++b) {
-          f16x odd = {};
-#pragma unroll 1
-          for (int k = 0; k < 2 * b + 2; ++k) {
-            u4 v = tr_read(sX + at_x[0] + k * 16 * kXRow, sX + at_x[1] + k * 16 * kXRow), rest = u4{0, 0, 0, 0}, code, seen;
-            constexpr uint32_t kExp = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;
-            const uint32_t s0 = 16 * k + 8 * half, tt = 32 * b + l32;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool o0 = (v[i] & kExp) == kExp, o1 = (v[i] >> 16 & kExp) == kExp;
-              code[i] = (o0 ? 0x3F80u : 0u) | (o1 ? 0x3F800000u : 0u);  // 1 in bf16
-              seen[i] = (s0 + 2 * i <= tt ? 0x3F80u : 0u) | (s0 + 2 * i + 1 <= tt ? 0x3F800000u : 0u);
-              v[i] &= (o0 ? 0u : 0xFFFFu) | (o1 ? 0u : 0xFFFF0000u);
-              if constexpr (DT == HQ_DTYPE_F16) {
-                float p, q;
-                unpack_pair<DT>(v[i], p, q);
-                v[i] = take_part<BF>(p, q);
-                rest[i] = pack_pair<BF>(p, q);
-              }
-            }
-            const unsigned char* const p = m0 + (m_at[b] ^ (uint32_t)(k << 5));
-            const u4 hi = *reinterpret_cast<const u4*>(p), lo = *reinterpret_cast<const u4*>(p + m_bytes<L>());
-            y[b] = mfma32<BF>(v, hi, y[b]);
-            y[b] = mfma32<BF>(v, lo, y[b]);
-            if constexpr (DT == HQ_DTYPE_F16) y[b] = mfma32<BF>(rest, hi, y[b]);
-            odd = mfma32<BF>(code, seen, odd);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (odd[r] != 0.f) y[b][r] = NAN;
-        }
-        read_x();
-      }
-
-      // Out: this lane's token (and the one 32 on), four channels side by side.
-#pragma unroll
-      for (int b = 0; b < kTB; ++b) {
-        const uint32_t tt = 32 * b + l32;
-        if (tt < n && live) {
-          const uint32_t p0 = part * 32 + 4 * half;
-          uint16_t* const to = a.Y + (t + tt) * a.y_row + h * a.y_head + p0;
-          const uint16_t* const zp = a.Z + (t + tt) * a.z_row + h * a.z_head + p0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v[4];
-#pragma unroll
-            for (int e2 = 0; e2 < 4; ++e2) v[e2] = y[b][4 * i + e2];
-            if (a.Z) {
-              const u2 zw = *reinterpret_cast<const u2*>(zp + 8 * i);
-              float z[4];
-              unpack_pair<DT>(zw[0], z[0], z[1]);
-              unpack_pair<DT>(zw[1], z[2], z[3]);
-#pragma unroll
-              for (int e2 = 0; e2 < 4; ++e2) v[e2] *= silu(z[e2]);
-            }
-            *reinterpret_cast<u2*>(to + 8 * i) = u2{pack_pair<DT>(v[0], v[1]), pack_pair<DT>(v[2], v[3])};
-          }
-        }
       }
     }
 
-    // The state: decayed, and the chunk's terms.
+    if (!CARRY && t + n < run.t1) put_x(odd + (turn ^ 1u));
+
+    // The state decayed, and the chunk's terms; between their products the outputs go out, this lane's token (and the one 32
+    // on), four channels side by side.
+    const __amdgpu_buffer_rsrc_t by = make_rsrc(a.Y + t * a.y_row + h * a.y_head + part * 32, kOutOfRange - 1);
+    uint32_t to[kTB];
+#pragma unroll
+    for (int b = 0; b < kTB; ++b) to[b] = 32 * b + l32 < n && live ? ((32 * b + l32) * (uint32_t)a.y_row + 4 * half) * 2 : kOutOfRange;
+    auto out = [&](int j) __attribute__((always_inline)) {
+      if constexpr (!CARRY) {
+        const int b = j / 4, i = j % 4;
+        float v[4];
+#pragma unroll
+        for (int e2 = 0; e2 < 4; ++e2) v[e2] = y[b][4 * i + e2];
+        if constexpr (GATED) {
+          float z[4];
+          unpack_pair<DT>(zr[b][i][0], z[0], z[1]);
+          unpack_pair<DT>(zr[b][i][1], z[2], z[3]);
+#pragma unroll
+          for (int e2 = 0; e2 < 4; ++e2) v[e2] *= silu(z[e2]);
+        }
+        __builtin_amdgcn_raw_buffer_store_b64(u2{pack_pair<DT>(v[0], v[1]), pack_pair<DT>(v[2], v[3])}, by, to[b] + 16 * i, 0, 0);
+      }
+    };
+    constexpr int kOuts = kTB * 4;
     const float keep = __builtin_amdgcn_exp2f(whole);
     const uint32_t at_b[2] = {opaque(tr_b[0]), opaque(tr_b[1])};
-    if constexpr (DT == HQ_DTYPE_F16) {
-      float m = 0, xw[kTS][8], up3, down3;
+    auto read_b = [&](int k, int i) __attribute__((always_inline)) {
+      return tr_read(sB + (at_b[0] ^ (uint32_t)(i << 6)) + k * 16 * kRow, sB + (at_b[1] ^ (uint32_t)(i << 6)) + k * 16 * kRow);
+    };
+    auto weigh = [&](int k, float (&v)[8]) __attribute__((always_inline)) {
+      const f4 w0 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half), w1 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half + 4);
 #pragma unroll
-      for (int k = 0; k < kTS; ++k) {
-        const f4 w0 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half), w1 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          unpack_pair<DT>(x[k][i], xw[k][2 * i], xw[k][2 * i + 1]);
-          xw[k][2 * i] *= i < 2 ? w0[(2 * i) & 3] : w1[(2 * i) & 3];
-          xw[k][2 * i + 1] *= i < 2 ? w0[(2 * i + 1) & 3] : w1[(2 * i + 1) & 3];
-          m = fmaxf(m, fmaxf(fabsf(xw[k][2 * i]), fabsf(xw[k][2 * i + 1])));
-        }
+      for (int i = 0; i < 4; ++i) {
+        unpack_pair<DT>(x[k][i], v[2 * i], v[2 * i + 1]);
+        v[2 * i] *= i < 2 ? w0[(2 * i) & 3] : w1[(2 * i) & 3];
+        v[2 * i + 1] *= i < 2 ? w0[(2 * i + 1) & 3] : w1[(2 * i + 1) & 3];
       }
-      range_scale(max_of_lanes(m), up3, down3);
+    };
+    if constexpr (DT == HQ_DTYPE_F16) {
       u4 hi[kTS], lo[kTS];
 #pragma unroll
-      for (int k = 0; k < kTS; ++k)
+      for (int k = 0; k < kTS; ++k) {
+        float v[8];
+        weigh(k, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float u = xw[k][2 * i] * up3, v = xw[k][2 * i + 1] * up3;
-          hi[k][i] = take_part<DT>(u, v);
-          lo[k][i] = pack_pair<DT>(u, v);
+          hi[k][i] = take_part<DT>(v[2 * i], v[2 * i + 1]);
+          lo[k][i] = pack_pair<DT>(v[2 * i], v[2 * i + 1]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int i = 0; i < kNT; ++i) {
-        f16x acc = {};
+        f16x acc;
 #pragma unroll
         for (int k = 0; k < kTS; ++k) {
-          const u4 b = tr_read(sB + (at_b[0] ^ (uint32_t)(i << 6)) + k * 16 * kRow, sB + (at_b[1] ^ (uint32_t)(i << 6)) + k * 16 * kRow);
-          acc = mfma32<DT>(b, hi[k], acc);
+          const u4 b = read_b(k, i);
+          acc = mfma32<DT>(b, hi[k], k ? acc : f16x{});
           acc = mfma32<DT>(b, lo[k], acc);
         }
+#pragma unroll
+        for (int j = i * kOuts / kNT; j < (i + 1) * kOuts / kNT; ++j) out(j);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], keep, acc[r] * down3);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
+      u4 part3[2][3];
+      auto ready = [&](int k) __attribute__((always_inline)) {
+        float v[8];
+        weigh(k, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          part3[k & 1][0][i] = take_part<DT>(v[2 * i], v[2 * i + 1]);
+          part3[k & 1][1][i] = take_part<DT>(v[2 * i], v[2 * i + 1]);
+          part3[k & 1][2][i] = pack_pair<DT>(v[2 * i], v[2 * i + 1]);
+        }
+      };
+      ready(0);
 #pragma unroll
       for (int i = 0; i < kNT; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[i][r] *= keep;
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < kTS; ++k) {
-        const f4 w0 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half), w1 = *reinterpret_cast<const f4*>(weights + 16 * k + 8 * half + 4);
-        u4 p0, p1, p2;
+        if (k + 1 < kTS) ready(k + 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float u, v;
-          unpack_pair<DT>(x[k][i], u, v);
-          u *= i < 2 ? w0[(2 * i) & 3] : w1[(2 * i) & 3];
-          v *= i < 2 ? w0[(2 * i + 1) & 3] : w1[(2 * i + 1) & 3];
-          p0[i] = take_part<DT>(u, v);
-          p1[i] = take_part<DT>(u, v);
-          p2[i] = pack_pair<DT>(u, v);
-        }
+        for (int j = k * kOuts / kTS; j < (k + 1) * kOuts / kTS; ++j) out(j);
 #pragma unroll
         for (int i = 0; i < kNT; ++i) {
-          const u4 b = tr_read(sB + (at_b[0] ^ (uint32_t)(i << 6)) + k * 16 * kRow, sB + (at_b[1] ^ (uint32_t)(i << 6)) + k * 16 * kRow);
-          s[i] = mfma32<DT>(b, p0, s[i]);
-          s[i] = mfma32<DT>(b, p1, s[i]);
-          s[i] = mfma32<DT>(b, p2, s[i]);
+          const u4 b = read_b(k, i);
+#pragma unroll
+          for (int e2 = 0; e2 < 3; ++e2) s[i] = mfma32<DT>(b, part3[k & 1][e2], s[i]);
         }
+        between<3 * kNT, CARRY ? 5 : 10, 0>();
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     __syncthreads();
-    if (t + L < run.t1) put();
+    if (t + n < run.t1) {
+      put();
+      if (CARRY) put_x(odd + (turn ^ 1u));
+    }
   }
 
   if constexpr (CARRY) {
@@ -609,10 +645,10 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   }
 }
 
-template <int DT, int P, int N, bool CARRY>
+template <int DT, int P, int N, int KIND>
 hipError_t launch_one(const ScanArgs& a, const ChunkArgs& c, hipStream_t s) {
-  auto k = hq_ssm_chunk_kernel<DT, P, N, CARRY>;
-  constexpr uint32_t lds = chunk_lds<N, CARRY>(kColumns / P);
+  auto k = hq_ssm_chunk_kernel<DT, P, N, KIND>;
+  constexpr uint32_t lds = chunk_lds<N, KIND == kCarry>(kColumns / P);
   static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (set != hipSuccess) return set;
   hipLaunchKernelGGL(k, dim3((c.blocks + 7) / 8 * 8), dim3(kChunkThreads), lds, s, a, c);
@@ -625,10 +661,10 @@ hipError_t launch(const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s)
   if (p.split) {
     c.states = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes);
     c.totals = c.states + (size_t)c.blocks * kColumns * N;
-    const hipError_t e = launch_one<DT, P, N, true>(a, c, s);
+    const hipError_t e = launch_one<DT, P, N, kCarry>(a, c, s);
     if (e != hipSuccess) return e;
   }
-  return launch_one<DT, P, N, false>(a, c, s);
+  return a.Z ? launch_one<DT, P, N, kGated>(a, c, s) : launch_one<DT, P, N, kPlain>(a, c, s);
 }
 
 template <int DT>
