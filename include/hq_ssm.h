@@ -56,7 +56,7 @@ hq_status hq_ssm_conv(const hq_state_cache* cache, uint32_t layer, const void* X
 
 /* Inputs and outputs of a scan, strides in elements: X, Y, Z (NULL: no gate) [tokens][heads][head_dim], B, C
  * [tokens][groups][state_dim], dt [tokens][heads] with its heads side by side, fp32 (dt_f32) or of the activations' type.
- * X, B, C, Y, Z: 16-byte aligned, strides multiples of 8 (rows at most 2^23). A, D (NULL: 0), dt_bias (NULL: 0): fp32 [heads], A not
+ * X, B, C, Y, Z: 16-byte aligned, strides multiples of 8 (rows at most 2^22, dt's too). A, D (NULL: 0), dt_bias (NULL: 0): fp32 [heads], A not
  * positive. heads: a multiple of groups. Y may be Z with the same strides (in place), else it is apart from all inputs. */
 typedef struct hq_ssm_io {
     const void* X;

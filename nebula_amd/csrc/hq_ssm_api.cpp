@@ -13,7 +13,8 @@ namespace {
 
 using namespace hq::checks;
 
-constexpr int64_t kMaxRow = (int64_t)1 << 23;
+// Rows of a scan's operands at most 2^22 elements apart: the kernels multiply their bytes by a chunk's tokens in 24 bits.
+constexpr int64_t kMaxRow = (int64_t)1 << 22;
 
 hq_status check_sizes(uint32_t heads, uint32_t head_dim, uint32_t state_dim) {
   if (head_dim != 64 && head_dim != 128) return fail(HQ_ERR_UNSUPPORTED, "head_dim=%u must be 64 or 128", head_dim);
@@ -155,13 +156,12 @@ hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_
       (st = check_strides("C", io->c_row, io->c_group, T, G, N)) != HQ_OK || (st = check_strides("Y", io->y_row, io->y_head, T, H, P)) != HQ_OK ||
       (io->Z && (st = check_strides("Z", io->z_row, io->z_head, T, H, P)) != HQ_OK))
     return st;
-  // The chunk kernel reaches 64 tokens with 32-bit offsets.
   if (io->x_row > kMaxRow || io->b_row > kMaxRow || io->c_row > kMaxRow || io->y_row > kMaxRow || (io->Z && io->z_row > kMaxRow))
     return fail(HQ_ERR_SHAPE, "X, B, C, Y, Z: row strides %lld, %lld, %lld, %lld, %lld above %lld elements", (long long)io->x_row,
                 (long long)io->b_row, (long long)io->c_row, (long long)io->y_row, (long long)io->z_row, (long long)kMaxRow);
   if (overlaps(io->y_row, io->y_head, T, H, P)) return fail(HQ_ERR_SHAPE, "Y: strides %lld, %lld make rows or heads overlap", (long long)io->y_row, (long long)io->y_head);
   if (io->Y == io->Z && ((T > 1 && io->y_row != io->z_row) || (H > 1 && io->y_head != io->z_head))) return fail(HQ_ERR_SHAPE, "Y is Z with other strides");
-  if (io->dt_row < 0 || io->dt_row > kMaxSpan || (T > 1 && io->dt_row < (int64_t)H) || (double)io->dt_row * T > (double)kMaxSpan)
+  if (io->dt_row < 0 || io->dt_row > kMaxRow || (T > 1 && io->dt_row < (int64_t)H))
     return fail(HQ_ERR_SHAPE, "dt: stride %lld out of range (heads=%u)", (long long)io->dt_row, H);
   a.X = static_cast<const uint16_t*>(io->X);
   a.B = static_cast<const uint16_t*>(io->B);

@@ -41,6 +41,7 @@ __device__ __forceinline__ f16x mfma32(u4 a, u4 b, f16x c) {
 
 constexpr int BF = HQ_DTYPE_BF16;
 constexpr uint32_t kChunkThreads = 256;
+constexpr uint32_t kOwnBytes = 4096;  // of LDS for a wavefront: a chunk's x of 32 channels, then 32 tokens' fp32 outputs
 constexpr uint32_t kColumns = 128;  // channels of a workgroup, four wavefronts of 32
 
 // Tokens of a chunk: the state of 256 leaves registers and LDS for 32.
@@ -105,14 +106,20 @@ __device__ __forceinline__ void range_scale(float m, float& up, float& down) {
   down = __uint_as_float((254u - k) << 23);
 }
 
-// The rest that one rounding of two values leaves, and the rounded ones.
+// The rest that one rounding of two values leaves, exactly, and the rounded ones. (For fp16 one instruction each, with a half
+// of w as an operand. bf16 has such a one, a dot product of two, but its result is waited for: 8% slower.)
 template <int DT>
 __device__ __forceinline__ uint32_t take_part(float& a, float& b) {
   const uint32_t w = pack_pair<DT>(a, b);
-  float x, y;
-  unpack_pair<DT>(w, x, y);
-  a -= x;
-  b -= y;
+  if constexpr (DT == HQ_DTYPE_F16) {
+    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel_hi:[1,0,0]" : "+v"(a) : "v"(w));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(b) : "v"(w));
+  } else {
+    float x, y;
+    unpack_pair<DT>(w, x, y);
+    a -= x;
+    b -= y;
+  }
   return w;
 }
 
@@ -145,6 +152,13 @@ __device__ __forceinline__ void between() {
     if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
     __builtin_amdgcn_sched_group_barrier(0x2, VALU, 0);
   }
+}
+
+// A uniform value that stays in its scalar registers.
+template <class T>
+__device__ __forceinline__ T held(T v) {
+  asm volatile("" : "+s"(v));
+  return v;
 }
 
 // Which run of chunks a workgroup works on.
@@ -189,12 +203,12 @@ struct ChunkArgs {
 
 template <int N>
 constexpr uint32_t vec_bytes() {
-  return 4 * 4 * chunk_tokens<N>() * 4;
+  return 4 * 2 * 3 * chunk_tokens<N>() * 4;
 }
 template <int N, bool CARRY>
 constexpr uint32_t chunk_lds(uint32_t heads) {
   constexpr uint32_t L = chunk_tokens<N>();
-  return (CARRY ? 1 : 2) * L * N * 2 + L * kColumns * 2 + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>()) + 16;
+  return (CARRY ? 1 : 2) * L * N * 2 + 4 * kOwnBytes + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>()) + 16;
 }
 
 // What a launch computes: outputs, outputs through a gate, or the state alone, of all runs but a sequence's last, for the runs
@@ -210,7 +224,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   extern __shared__ __align__(16) unsigned char smem[];
   unsigned char* const sB = smem;
   unsigned char* const sX = sB + L * kRow;
-  float* const vec = reinterpret_cast<float*>(sX + 4 * L * kXRow);
+  float* const vec = reinterpret_cast<float*>(sX + 4 * kOwnBytes);
   unsigned char* const sC = reinterpret_cast<unsigned char*>(vec) + vec_bytes<N>();
   unsigned char* const sM = sC + L * kRow;
 
@@ -238,26 +252,46 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   // ---- a chunk's inputs, on their way in registers ----
   constexpr int kPieces = N / 8, kRows = kChunkThreads / kPieces, kLoads = L / kRows, kXLoads = L / 16;
   u4 rb[kLoads], rc[CARRY ? 1 : kLoads], rx[kXLoads];
-  float rdt = 0;
-  // 32-bit offsets from the chunk's first token, made anew for each chunk; a place past any operand reads as 0 without
-  // touching memory.
-  auto load = [&](uint32_t t) __attribute__((always_inline)) {  // of the chunk at token t; zeros from the run's end on
-    const uint32_t id = opaque(tid), row = id / kPieces, piece = id % kPieces, xrow = (id & 63u) / 4, xpiece = id % 4;  // x: the wavefront's channels
-    const uint32_t b_off = (row * (uint32_t)a.b_row + piece * 8) * 2, c_off = (row * (uint32_t)a.c_row + piece * 8) * 2;
-    const uint32_t x_off = (xrow * (uint32_t)a.x_row + xpiece * 8) * 2;
-    const uint32_t n = run.t1 - t;
-    const __amdgpu_buffer_rsrc_t bb = make_rsrc(a.B + t * a.b_row + g * a.b_group, kOutOfRange - 1);
-    const __amdgpu_buffer_rsrc_t bc = make_rsrc(a.C + t * a.c_row + g * a.c_group, kOutOfRange - 1);
-    const __amdgpu_buffer_rsrc_t bx = make_rsrc(a.X + t * a.x_row + h * a.x_head + part * 32, kOutOfRange - 1);
-    auto place = [&](uint32_t off, uint32_t r) __attribute__((always_inline)) { return off | (r < n ? 0u : kOutOfRange); };
+  uint32_t rdt = 0;  // as it is in memory: turned into a number here, it would be waited for
+  // Addresses of the chunk that is loaded, and strides in bytes, kept in scalar registers (from the arguments anew, they
+  // were 2 us of a chunk's loads). Lanes' offsets from them are 32-bit; a place past any operand reads as 0 without touching
+  // memory: from the run's end on (`left` tokens), and for a chunk that there is none of, so that what is in flight is the
+  // same on every way.
+  const bool dt_f32 = a.dt_f32;
+  const uint32_t b_step = held((uint32_t)a.b_row * 2), c_step = held((uint32_t)a.c_row * 2), x_step = held((uint32_t)a.x_row * 2);
+  const uint32_t y_step = held((uint32_t)a.y_row * 2), z_step = held((uint32_t)a.z_row * 2), dt_size = dt_f32 ? 4 : 2;
+  const uint32_t dt_step = held((uint32_t)a.dt_row * dt_size);
+  uint64_t b_at = held(reinterpret_cast<uint64_t>(a.B + run.t0 * a.b_row + g * a.b_group));
+  uint64_t c_at = held(reinterpret_cast<uint64_t>(a.C + run.t0 * a.c_row + g * a.c_group));
+  uint64_t x_at = held(reinterpret_cast<uint64_t>(a.X + run.t0 * a.x_row + h * a.x_head + part * 32));
+  uint64_t dt_at = held(reinterpret_cast<uint64_t>(a.dt) + (run.t0 * a.dt_row + h) * dt_size);
+  uint64_t y_at = held(reinterpret_cast<uint64_t>(a.Y + run.t0 * a.y_row + h * a.y_head + part * 32));
+  uint64_t z_at = held(reinterpret_cast<uint64_t>(a.Z + run.t0 * a.z_row + h * a.z_head + part * 32));
+  auto rsrc = [](uint64_t at) __attribute__((always_inline)) { return make_rsrc(reinterpret_cast<const void*>(at), kOutOfRange - 1); };
+  auto past = [](uint32_t off, bool there) __attribute__((always_inline)) { return there ? off : kOutOfRange; };
+  auto load_x = [&](uint32_t left) __attribute__((always_inline)) {
+    const uint32_t id = opaque(lane), xrow = id / 4, x_off = __umul24(xrow, x_step) + id % 4 * 16;  // the wavefront's channels
+    const __amdgpu_buffer_rsrc_t bx = rsrc(x_at), bd = rsrc(dt_at);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      rb[i] = __builtin_amdgcn_raw_buffer_load_b128(bb, place(b_off + i * kRows * (uint32_t)a.b_row * 2, row + i * kRows), 0, 0);
-      if constexpr (!CARRY) rc[i] = __builtin_amdgcn_raw_buffer_load_b128(bc, place(c_off + i * kRows * (uint32_t)a.c_row * 2, row + i * kRows), 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < kXLoads; ++i) rx[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, place(x_off + i * 16 * (uint32_t)a.x_row * 2, xrow + i * 16), 0, 0);
-    rdt = lane < min(n, (uint32_t)L) ? load_dt(a, t + lane, h, DT) : 0.f;
+    for (int i = 0; i < kXLoads; ++i) rx[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, past(x_off, xrow + i * 16 < left), i * 16 * x_step, 0);
+    const uint32_t dt_off = past(__umul24(id, dt_step), id < left);
+    if (dt_f32) rdt = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(bd, dt_off, 0, 0);
+    else rdt = __builtin_amdgcn_raw_buffer_load_b16(bd, dt_off, 0, 0);
+  };
+  // B and C in kBCLoads steps, so that they go out between other work.
+  constexpr int kBCLoads = (CARRY ? 1 : 2) * kLoads;
+  uint32_t b_off, c_off, bc_row;
+  auto place_bc = [&]() __attribute__((always_inline)) {
+    const uint32_t id = opaque(tid);
+    bc_row = id / kPieces;
+    b_off = __umul24(bc_row, b_step) + id % kPieces * 16;
+    c_off = __umul24(bc_row, c_step) + id % kPieces * 16;
+  };
+  auto load_bc = [&](uint32_t left, int j) __attribute__((always_inline)) {
+    const int i = CARRY ? j : j / 2;
+    const bool is_c = !CARRY && j % 2, there = bc_row + i * kRows < left;
+    if (is_c) rc[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(c_at), past(c_off, there), i * kRows * c_step, 0);
+    else rb[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(b_at), past(b_off, there), i * kRows * b_step, 0);
   };
   auto put = [&]() __attribute__((always_inline)) {
     const uint32_t id = opaque(tid);
@@ -269,11 +303,19 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     }
   };
   // x goes through LDS for its order alone, to the wavefront that brought it.
-  unsigned char* const own = sX + wave * L * kXRow;
+  unsigned char* const own = sX + wave * kOwnBytes;
   constexpr uint32_t kOdd = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;  // the exponent of infinities and NaN
-  float x_most = 0;  // fp16: a power of two above the next chunk's x
+  float x_most = 0;  // fp16: a power of two above the x that have come
+  uint32_t most = 0;
+  auto look_x = [&]() __attribute__((always_inline)) {
+    most = exponents<DT>(rx);
+    if constexpr (DT == HQ_DTYPE_F16) {
+      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)scan(most, 0, [](uint32_t p, uint32_t q) { return max(p, q); }), 63);
+      x_most = __uint_as_float(((all >> 10) + 113u) << 23);  // 2^(e - 15 + 1), for exponent e
+    }
+  };
   auto put_x = [&](uint32_t* odd) __attribute__((always_inline)) {
-    const uint32_t id = opaque(lane), xrow = id / 4, at = piece_at<kXRow>(xrow, id % 4), most = exponents<DT>(rx);
+    const uint32_t id = opaque(lane), xrow = id / 4, at = piece_at<kXRow>(xrow, id % 4);
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) *reinterpret_cast<u4*>(own + at + i * 16 * kXRow) = rx[i];
     if (__builtin_expect(most == kOdd, 0)) {
@@ -283,21 +325,16 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         if (exponents<DT>(one) == kOdd) atomicMin(odd, xrow + i * 16);
       }
     }
-    if constexpr (DT == HQ_DTYPE_F16) {
-      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)scan(most, 0, [](uint32_t p, uint32_t q) { return max(p, q); }), 63);
-      x_most = __uint_as_float(((all >> 10) + 113u) << 23);  // 2^(e - 15 + 1), for exponent e
-    }
   };
-  load(run.t0);
+  load_x(run.t1 - run.t0);
+  place_bc();
+#pragma unroll
+  for (int j = 0; j < kBCLoads; ++j) load_bc(run.t1 - run.t0, j);
 
   // ---- the state: s[nt][r] is channel l32, state 32 nt + 16 (r / 8) + 8 half + r % 8 ----
   f16x s[kNT];
   float* const kept = a.state + run.q.row * a.row_stride + ((size_t)h * P + part * 32 + l32) * N + 8 * half;
   auto place = [&](uint32_t i) { return pl.states + (((size_t)i * pl.units + unit) * (kNT * 4) * kChunkThreads + tid) * 4; };
-  auto fetch = [&](const float* p, size_t quad, f4 (&v)[kNT * 4]) {
-#pragma unroll
-    for (int i = 0; i < kNT * 4; ++i) v[i] = *reinterpret_cast<const f4*>(p + i * quad);
-  };
 #pragma unroll
   for (int i = 0; i < kNT; ++i) s[i] = f16x{};
   if (CARRY ? run.idx == run.first : run.first == run.last) {
@@ -309,8 +346,8 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         for (int e = 0; e < 4; ++e) s[i / 4][(i & 3) * 4 + e] = v[e];
       }
     }
-    // A sequence's first run reads its state here for both launches: its last one, whose place is free, will have
-    // replaced it when the second launch's first one begins.
+    // A sequence's first run reads its state here, for itself and, in the place of the last one, which has nothing to leave,
+    // for the run of the outputs: by then the last of those may have replaced it.
     if constexpr (CARRY) {
       float* const p = place(run.last);
 #pragma unroll
@@ -318,20 +355,33 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         *reinterpret_cast<f4*>(p + i * 4 * kChunkThreads) = f4{s[i / 4][(i & 3) * 4], s[i / 4][(i & 3) * 4 + 1], s[i / 4][(i & 3) * 4 + 2], s[i / 4][(i & 3) * 4 + 3]};
     }
   } else if constexpr (!CARRY) {
-    // What the runs before this one leave: each adds its own to what it decays.
-    for (uint32_t i = run.first; i < max(run.idx, run.first + 1); ++i) {
-      f4 v[kNT * 4];
-      fetch(place(run.idx == run.first ? run.last : i), 4 * kChunkThreads, v);
-      const float d = i == run.first ? 0.f : __builtin_amdgcn_exp2f(pl.totals[(size_t)i * a.H + h]);
+    const float* const p = place(run.idx);
 #pragma unroll
-      for (int j = 0; j < kNT * 4; ++j)
+    for (int i = 0; i < kNT * 4; ++i) {
+      const f4 v = *reinterpret_cast<const f4*>(p + i * 4 * kChunkThreads);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j / 4][(j & 3) * 4 + e] = i == run.first ? v[j][e] : fmaf(s[j / 4][(j & 3) * 4 + e], d, v[j][e]);
+      for (int e = 0; e < 4; ++e) s[i / 4][(i & 3) * 4 + e] = v[e];
     }
   }
 
-  float* const cum = vec + wave * 4 * L;  // of this wavefront's head: exponents (of 2), steps, weights, decays
-  float *const steps = cum + L, *const weights = steps + L, *const decays = weights + L;
+  // Of a chunk of n tokens, for this wavefront's head: steps and their sums, a token a lane, from the chunk's beginning and
+  // from its end. Computed during the chunk before it, between products.
+  float whole = 0, down3 = 1.f;  // the whole chunk's exponent; fp16: what the state's terms are scaled down by
+  auto sums = [&](uint32_t to, uint32_t n, float x_most) __attribute__((always_inline)) {
+    const float dt = lane < n ? step_of((dt_f32 ? __uint_as_float(rdt) : to_f32<DT>((uint16_t)rdt)) + dt0, a.softplus) : 0.f;
+    // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it.)
+    const float e = lane < n ? fmaxf(dt * A, -200.f) : 0.f;
+    const float up = scan_add(e), back = scan_add(__shfl(e, 63 - lane)), after = __shfl(back, (62 - lane) & 63);
+    float weight = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt, up3 = 1.f;
+    if constexpr (DT == HQ_DTYPE_F16) range_scale(max_of_lanes(fabsf(weight)) * x_most, up3, down3);
+    float* const cum = vec + (wave * 2 + to) * 3 * L;
+    if (lane < L) {
+      cum[lane] = up;
+      cum[L + lane] = dt;
+      cum[2 * L + lane] = weight * up3;
+    }
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(up), 63));
+  };
   unsigned char* const m0 = sM + mine * 2 * m_bytes<L>();  // M's parts
   if constexpr (!CARRY) {
     // The tiles of 16 x 16 right of the diagonal that products of 32 tokens take in stay zero.
@@ -347,8 +397,9 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   if (tid < 2) odd[tid] = L;
   __syncthreads();
   put();
+  look_x();
   put_x(odd);
-  float total = 0;
+  float total = 0, next_whole = sums(0, min(run.t1 - run.t0, (uint32_t)L), x_most), next_down = down3;
   uint32_t n, turn = 0;
   for (uint32_t t = run.t0; t < run.t1; t += n, turn ^= 1u) {
     __syncthreads();
@@ -358,30 +409,36 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     const uint32_t first = uni(odd[turn]);
     if (__builtin_expect(first < n, 0)) {
       n = max(first, 1u);
+      next_whole = sums(turn, n, x_most);
+      next_down = down3;
       for (uint32_t i = tid; i < (L - n) * kPieces; i += kChunkThreads) *reinterpret_cast<u4*>(sB + n * kRow + i * 16) = u4{0, 0, 0, 0};
       for (uint32_t i = lane; i < (L - n) * 4; i += 64) *reinterpret_cast<u4*>(own + n * kXRow + i * 16) = u4{0, 0, 0, 0};
       __syncthreads();
     }
     if (tid == 0) odd[turn ^ 1u] = L;
-    // Steps and their sums, a token a lane: from the chunk's beginning, and from its end for the state's weights.
-    const float dt = lane < n ? step_of(rdt + dt0, a.softplus) : 0.f;
-    // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it.)
-    const float e = lane < n ? fmaxf(dt * A, -200.f) : 0.f;
-    const float up = scan_add(e);
-    const float back = scan_add(__shfl(e, 63 - lane));
-    const float after = __shfl(back, (62 - lane) & 63);
-    const float whole = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(up), 63));
-    const float weight = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt;
-    float up3 = 1.f, down3 = 1.f;
-    if constexpr (DT == HQ_DTYPE_F16) range_scale(max_of_lanes(fabsf(weight)) * x_most, up3, down3);
-    if (lane < L) {
-      cum[lane] = up;
-      steps[lane] = dt;
-      weights[lane] = weight * up3;
-      decays[lane] = __builtin_amdgcn_exp2f(up);
-    }
+    whole = next_whole;
     total += whole;
-    if (t + n < run.t1) load(t + n);
+    const float scale_down = next_down;
+    float* const cum = vec + (wave * 2 + turn) * 3 * L;  // of this chunk: exponents (of 2), steps, weights of the state's terms
+    const float *const steps = cum + L, *const weights = steps + L;
+    // Outputs leave as 16-byte pieces, four lanes a token: token lane / 4 + 16 i, channels 8 (lane % 4) ..
+    u4 zr[kTB * 2];
+    uint32_t out_at[kTB * 2];
+    if constexpr (!CARRY) {
+#pragma unroll
+      for (int i = 0; i < kTB * 2; ++i) out_at[i] = 16 * i + lane / 4 < n && live ? 0u : kOutOfRange;
+      if constexpr (GATED) {
+        const uint32_t z_off = __umul24(lane / 4, z_step) + lane % 4 * 16;
+#pragma unroll
+        for (int i = 0; i < kTB * 2; ++i) zr[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(z_at), out_at[i] | z_off, i * 16 * z_step, 0);
+      }
+    }
+    const uint32_t left = run.t1 - t - n;  // (none: 0)
+    b_at += (uint64_t)n * b_step;
+    c_at += (uint64_t)n * c_step;
+    x_at += (uint64_t)n * x_step;
+    dt_at += (uint64_t)n * dt_step;
+    load_x(left);
     __builtin_amdgcn_sched_barrier(0);
 
     u4 x[kTS];  // x^T: channel l32, tokens 16 i + 8 half ..
@@ -392,45 +449,50 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     if constexpr (CARRY) read_x();
 
     f16x y[kTB];
-    u2 zr[kTB][4];  // the gates
     if constexpr (!CARRY) {
       // M in tiles of 16 x 16, dealt to the head's wavefronts: B_s . C_t, a lane one t and four s.
-      constexpr int kT16 = L / 16, kTiles = kT16 * (kT16 + 1) / 2;
+      // Those on the diagonal come first.
+      constexpr int kT16 = L / 16, kTiles = kT16 * (kT16 + 1) / 2, kMine = (kTiles + kWaves - 1) / kWaves;
+      const uint32_t id = opaque(lane), l16 = id & 15u, quad = id >> 4, at = piece_at<kRow>(l16, quad);
+      uint32_t ti[kMine], si[kMine];
+      f4 m[kMine];
 #pragma unroll
-      for (int k = 0; k < (kTiles + kWaves - 1) / kWaves; ++k) {
-        const uint32_t tile = k * kWaves + part;
-        if (tile < kTiles) {
-          const uint32_t ti = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, si = tile - ti * (ti + 1) / 2;
-          // (Opaque: places and masks of all tiles are not to be kept from chunk to chunk.)
-          const uint32_t id = opaque(lane), l16 = id & 15u, quad = id >> 4, at = piece_at<kRow>(l16, quad);
-          f4 m = {0, 0, 0, 0};
+      for (int k = 0; k < kMine; ++k) {
+        const uint32_t tile = min(k * kWaves + part, kTiles - 1u), o = tile - kT16;  // (a wavefront without a tile takes the last one)
+        ti[k] = tile < kT16 ? tile : o < 1 ? 1 : o < 3 ? 2 : 3;
+        si[k] = tile < kT16 ? tile : o - ti[k] * (ti[k] - 1) / 2;
+        m[k] = f4{0, 0, 0, 0};
+      }
 #pragma unroll
-          for (int j = 0; j < N / 32; ++j) {
-            const u4 fb = *reinterpret_cast<const u4*>(sB + 16 * si * kRow + (at ^ (uint32_t)(j << 6)));
-            const u4 fc = *reinterpret_cast<const u4*>(sC + 16 * ti * kRow + (at ^ (uint32_t)(j << 6)));
-            m = mfma16x16x32<DT>(fb, fc, m);
-          }
-          const uint32_t tt = 16 * ti + l16, ss = 16 * si + 4 * quad;
-          const float ct = cum[tt];
-          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
-          float w[4];
+      for (int j = 0; j < N / 32; ++j)
 #pragma unroll
-          for (int v = 0; v < 4; ++v) w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[v];
-          if (ti == si) {
-            const int32_t past = (int32_t)l16 - 4 * (int32_t)quad;  // tokens from the lane's first one to its own
-#pragma unroll
-            for (int v = 0; v < 4; ++v) w[v] = v < past ? w[v] : v == past ? w[v] + D : 0.f;
-          }
-          const uint32_t to = m_place<L>(ti / 2, tt & 31u, ss / 8) + (ss & 4u) * 2;
-          u2 hi, lo;
-          hi[0] = take_part<BF>(w[0], w[1]);
-          hi[1] = take_part<BF>(w[2], w[3]);
-          lo[0] = pack_pair<BF>(w[0], w[1]);
-          lo[1] = pack_pair<BF>(w[2], w[3]);
-          *reinterpret_cast<u2*>(m0 + to) = hi;
-          *reinterpret_cast<u2*>(m0 + m_bytes<L>() + to) = lo;
+        for (int k = 0; k < kMine; ++k) {
+          const u4 fb = *reinterpret_cast<const u4*>(sB + 16 * si[k] * kRow + (at ^ (uint32_t)(j << 6)));
+          const u4 fc = *reinterpret_cast<const u4*>(sC + 16 * ti[k] * kRow + (at ^ (uint32_t)(j << 6)));
+          m[k] = mfma16x16x32<DT>(fb, fc, m[k]);
         }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < kMine; ++k) {
+        const uint32_t tt = 16 * ti[k] + l16, ss = 16 * si[k] + 4 * quad;
+        const float ct = cum[tt];
+        const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
+        float w[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[k][v];
+          if (k * kWaves < kT16) {
+            const int32_t back = (int32_t)(tt - ss);  // tokens from the lane's first one to its own
+            w[v] = v < back ? w[v] : v == back ? w[v] + D : 0.f;
+          }
+        }
+        const uint32_t to = m_place<L>(ti[k] / 2, tt & 31u, ss / 8) + (ss & 4u) * 2;
+        u2 hi, lo;
+        hi[0] = take_part<BF>(w[0], w[1]);
+        hi[1] = take_part<BF>(w[2], w[3]);
+        lo[0] = pack_pair<BF>(w[0], w[1]);
+        lo[1] = pack_pair<BF>(w[2], w[3]);
+        *reinterpret_cast<u2*>(m0 + to) = hi;
+        *reinterpret_cast<u2*>(m0 + m_bytes<L>() + to) = lo;
       }
       __syncthreads();
 
@@ -463,10 +525,13 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
           }
         };
         ready(0);
+        place_bc();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < kNS; ++k) {
           if (k + 1 < kNS) ready(k + 1);
+#pragma unroll
+          for (int j = k * kBCLoads / kNS; j < (k + 1) * kBCLoads / kNS; ++j) load_bc(left, j);
 #pragma unroll
           for (int b = 0; b < kTB; ++b) y[b] = mfma32<DT>(hi[k & 1], c[k & 1][b], k ? y[b] : f16x{});
 #pragma unroll
@@ -476,23 +541,17 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         }
 #pragma unroll
         for (int b = 0; b < kTB; ++b) {
-          const float d = decays[32 * b + l32] * down2;
+          const float d = __builtin_amdgcn_exp2f(cum[32 * b + l32]) * down2;
 #pragma unroll
           for (int r = 0; r < 16; ++r) y[b][r] *= d;
         }
       };
       from_state(up2);
       read_x();
-      if constexpr (GATED) {
-        const __amdgpu_buffer_rsrc_t bz = make_rsrc(a.Z + t * a.z_row + h * a.z_head + part * 32, kOutOfRange - 1);
-#pragma unroll
-        for (int b = 0; b < kTB; ++b) {
-          const uint32_t tt = 32 * b + l32, at = tt < n && live ? (tt * (uint32_t)a.z_row + 4 * half) * 2 : kOutOfRange;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) zr[b][i] = __builtin_amdgcn_raw_buffer_load_b64(bz, at + 16 * i, 0, 0);
-        }
-      }
-      // M's fragments are read a step ahead, the state decays between the products.
+      // M's fragments are read a step ahead; between the products, the next chunk's sums.
+      look_x();
+      next_whole = sums(turn ^ 1u, min(left, (uint32_t)L), x_most);
+      next_down = down3;
       const uint32_t idm = opaque(lane), at_m[2] = {m_place<L>(0, idm & 31u, idm >> 5), m_place<L>(1, idm & 31u, idm >> 5)};
       constexpr int kSteps = kTB == 2 ? 6 : 2;  // products of 16 earlier tokens: 2 for the first 32 tokens, 4 for the others
       u4 mf[2][2];
@@ -520,35 +579,54 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         y[b] = mfma32<BF>(v, mf[j & 1][0], y[b]);
         y[b] = mfma32<BF>(v, mf[j & 1][1], y[b]);
         if constexpr (DT == HQ_DTYPE_F16) y[b] = mfma32<BF>(rest, mf[j & 1][0], y[b]);
-        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      // Through the wavefront's own LDS, whose x is in registers, 32 tokens at a time.
+      const uint32_t idy = opaque(lane);
+#pragma unroll
+      for (int b = 0; b < kTB; ++b) {
+        const uint32_t tt = idy & 31u, put_at = tt * 128 + ((idy >> 5 ^ (tt >> 1 & 7u)) << 4), get_t = idy / 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f4*>(own + (put_at ^ (uint32_t)(i << 5))) = f4{y[b][4 * i], y[b][4 * i + 1], y[b][4 * i + 2], y[b][4 * i + 3]};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e2 = 0; e2 < 2; ++e2) {
+            const uint32_t r = get_t + 16 * i;
+            const f4 v = *reinterpret_cast<const f4*>(own + r * 128 + (((2 * (idy & 3u) + e2) ^ (r >> 1 & 7u)) << 4));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[b][8 * i + 4 * e2 + c] = v[c];
+          }
       }
     }
 
-    if (!CARRY && t + n < run.t1) put_x(odd + (turn ^ 1u));
+    if constexpr (!CARRY) put_x(odd + (turn ^ 1u));
 
-    // The state decayed, and the chunk's terms; between their products the outputs go out, this lane's token (and the one 32
-    // on), four channels side by side.
-    const __amdgpu_buffer_rsrc_t by = make_rsrc(a.Y + t * a.y_row + h * a.y_head + part * 32, kOutOfRange - 1);
-    uint32_t to[kTB];
-#pragma unroll
-    for (int b = 0; b < kTB; ++b) to[b] = 32 * b + l32 < n && live ? ((32 * b + l32) * (uint32_t)a.y_row + 4 * half) * 2 : kOutOfRange;
+    // The state decayed, and the chunk's terms; between their products the outputs go out.
+    const __amdgpu_buffer_rsrc_t by = rsrc(y_at);
+    const uint32_t y_off = __umul24(lane / 4, y_step) + lane % 4 * 16;
+    y_at += (uint64_t)n * y_step;
+    z_at += (uint64_t)n * z_step;
     auto out = [&](int j) __attribute__((always_inline)) {
       if constexpr (!CARRY) {
-        const int b = j / 4, i = j % 4;
-        float v[4];
+        u4 w;
 #pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2) v[e2] = y[b][4 * i + e2];
-        if constexpr (GATED) {
-          float z[4];
-          unpack_pair<DT>(zr[b][i][0], z[0], z[1]);
-          unpack_pair<DT>(zr[b][i][1], z[2], z[3]);
-#pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) v[e2] *= silu(z[e2]);
+        for (int i = 0; i < 4; ++i) {
+          float u = y[j / 2][8 * (j & 1) + 2 * i], v = y[j / 2][8 * (j & 1) + 2 * i + 1];
+          if constexpr (GATED) {
+            float z0, z1;
+            unpack_pair<DT>(zr[j][i], z0, z1);
+            u *= silu(z0);
+            v *= silu(z1);
+          }
+          w[i] = pack_pair<DT>(u, v);
         }
-        __builtin_amdgcn_raw_buffer_store_b64(u2{pack_pair<DT>(v[0], v[1]), pack_pair<DT>(v[2], v[3])}, by, to[b] + 16 * i, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(w, by, out_at[j] | y_off, j * 16 * y_step, 0);
       }
     };
-    constexpr int kOuts = kTB * 4;
+    constexpr int kOuts = kTB * 2;
     const float keep = __builtin_amdgcn_exp2f(whole);
     const uint32_t at_b[2] = {opaque(tr_b[0]), opaque(tr_b[1])};
     auto read_b = [&](int k, int i) __attribute__((always_inline)) {
@@ -563,6 +641,12 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         v[2 * i + 1] *= i < 2 ? w0[(2 * i + 1) & 3] : w1[(2 * i + 1) & 3];
       }
     };
+    if constexpr (CARRY) {
+      place_bc();
+#pragma unroll
+      for (int j = 0; j < kBCLoads; ++j) load_bc(left, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (DT == HQ_DTYPE_F16) {
       u4 hi[kTS], lo[kTS];
 #pragma unroll
@@ -588,7 +672,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
 #pragma unroll
         for (int j = i * kOuts / kNT; j < (i + 1) * kOuts / kNT; ++j) out(j);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], keep, acc[r] * down3);
+        for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], keep, acc[r] * scale_down);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -625,10 +709,13 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
       }
     }
     __syncthreads();
-    if (t + n < run.t1) {
-      put();
-      if (CARRY) put_x(odd + (turn ^ 1u));
+    if constexpr (CARRY) {
+      look_x();
+      next_whole = sums(turn ^ 1u, min(left, (uint32_t)L), x_most);
+      next_down = down3;
     }
+    put();
+    if constexpr (CARRY) put_x(odd + (turn ^ 1u));
   }
 
   if constexpr (CARRY) {
@@ -642,6 +729,47 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     for (int i = 0; i < kNT * 4; ++i)
       *reinterpret_cast<f4*>(kept + 16 * (i / 2) + 4 * (i & 1)) =
           f4{s[i / 4][(i & 3) * 4], s[i / 4][(i & 3) * 4 + 1], s[i / 4][(i & 3) * 4 + 2], s[i / 4][(i & 3) * 4 + 3]};
+  }
+}
+
+// Between the two launches: what enters each run of sequence blockIdx.y in place of what it leaves, the first one's own state,
+// then S <- S times the run's decay + what the run adds. Workgroup x: 16 bytes a thread of a unit's state.
+template <int P, int N>
+__global__ __launch_bounds__(kChunkThreads) void hq_ssm_join_kernel(ScanArgs a, ChunkArgs pl) {
+  constexpr uint32_t kQuads = N / 8, kHeads = kColumns / P, kWaves = P / 32;
+  const uint32_t unit = blockIdx.x / kQuads, quad = blockIdx.x - unit * kQuads, b = blockIdx.y, lane = threadIdx.x & 63u;
+  uint32_t first = 0, runs = 0;
+  for (uint32_t i = 0; i <= b; i += 64) {
+    const uint32_t j = min(i + lane, b), s0 = clamp_to(a.s.cu[j], a.s.T), s1 = clamp_to(a.s.cu[j + 1], a.s.T);
+    const uint32_t mine = i + lane <= b && s1 > s0 ? (s1 - s0 + pl.run_tokens - 1) / pl.run_tokens : 0u, upto = scan_sum(mine);
+    runs = (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)(b & 63u));
+    first += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  }
+  first -= runs;
+  if (runs < 2 || first + runs > pl.runs) return;
+  const uint32_t of_group = a.H / a.G, per_group = (of_group + kHeads - 1) / kHeads, g = unit / per_group;
+  const uint32_t h = g * of_group + min((unit - g * per_group) * kHeads + uni(threadIdx.x >> 6) / kWaves, of_group - 1);
+  const size_t step = (size_t)pl.units * kQuads * kChunkThreads;  // pieces of a run
+  f4* const p = reinterpret_cast<f4*>(pl.states) + first * step + ((size_t)unit * kQuads + quad) * kChunkThreads + threadIdx.x;
+  const float* const totals = pl.totals + (size_t)first * a.H + h;
+  f4 s = p[(runs - 1) * step];
+  constexpr uint32_t kAhead = 8;  // runs whose loads are in flight together
+  for (uint32_t i0 = 0; i0 < runs; i0 += kAhead) {
+    f4 v[kAhead];
+    float d[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) {
+      const uint32_t r = min(i0 + i, runs - 2);
+      v[i] = p[r * step];
+      d[i] = __builtin_amdgcn_exp2f(totals[(size_t)r * a.H]);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) {
+      if (i0 + i >= runs) break;
+      p[(i0 + i) * step] = s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = i0 + i ? fmaf(s[e], d[i], v[i][e]) : v[i][e];  // (the first run has begun with its state)
+    }
   }
 }
 
@@ -661,8 +789,10 @@ hipError_t launch(const ScanArgs& a, const ScanPlan& p, void* ws, hipStream_t s)
   if (p.split) {
     c.states = reinterpret_cast<float*>(static_cast<unsigned char*>(ws) + kCounterBytes);
     c.totals = c.states + (size_t)c.blocks * kColumns * N;
-    const hipError_t e = launch_one<DT, P, N, kCarry>(a, c, s);
+    hipError_t e = launch_one<DT, P, N, kCarry>(a, c, s);
     if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((hq_ssm_join_kernel<P, N>), dim3(p.units * (N / 8), a.s.n), dim3(kChunkThreads), 0, s, a, c);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return a.Z ? launch_one<DT, P, N, kGated>(a, c, s) : launch_one<DT, P, N, kPlain>(a, c, s);
 }

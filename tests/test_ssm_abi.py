@@ -98,7 +98,7 @@ def test_bad_scan(kw, status):
     (dict(x_head=64), hq.HQ_ERR_SHAPE), (dict(b_group=64), hq.HQ_ERR_SHAPE), (dict(c_row=-8), hq.HQ_ERR_SHAPE), (dict(y_row=256), hq.HQ_ERR_SHAPE),
     (dict(Z=P, z_head=100), hq.HQ_ERR_ALIGNMENT), (dict(Z=P + 4096, z_row=1024), hq.HQ_ERR_SHAPE), (dict(dt_row=3), hq.HQ_ERR_SHAPE),
     (dict(dt_row=-4), hq.HQ_ERR_SHAPE), (dict(dt_row=1 << 50), hq.HQ_ERR_SHAPE), (dict(tokens=0), hq.HQ_ERR_SHAPE), (dict(tokens=5), hq.HQ_ERR_SHAPE),
-    (dict(y_row=128, y_head=256), hq.HQ_ERR_SHAPE), (dict(x_row=(1 << 23) + 8), hq.HQ_ERR_SHAPE), (dict(b_row=1 << 24), hq.HQ_ERR_SHAPE)])
+    (dict(y_row=128, y_head=256), hq.HQ_ERR_SHAPE), (dict(x_row=(1 << 22) + 8), hq.HQ_ERR_SHAPE), (dict(b_row=1 << 23), hq.HQ_ERR_SHAPE), (dict(dt_row=(1 << 22) + 1), hq.HQ_ERR_SHAPE)])
 def test_bad_io(kw, status):
     assert scan(i=io(**kw)) == status
 
