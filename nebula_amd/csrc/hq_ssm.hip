@@ -11,18 +11,80 @@ namespace hq {
 namespace {
 
 // ---- the convolution ----
-// Bound by the bytes moved, inputs and outputs once. A lane holds 8 channels of a run of TT tokens: the run's inputs and the
-// W - 1 before it are loaded side by side, and each is W products' operand in registers.
+// Bound by the bytes moved, inputs and outputs once, and the arithmetic beside them (half the time alone: a product needs its
+// exponential and reciprocal). A lane holds 8 channels of a run of TT tokens: the run's inputs and the W - 1 before it are
+// loaded side by side, and each is W products' operand in registers. 2046 tokens of 10240 channels: 22 us, 3.8 TB/s of
+// inputs and outputs; runs of 4, 6 and 16 tokens 23.9, 22.2 and 23.5.
 //
 // A sequence's first W - 1 tokens read the row's kept inputs, and its last ones replace them: whoever reads them
 // writes them. So those first tokens are all the work of the run that the sequence begins in, up to W - 2 tokens past
 // its end, and a run leaves out the first tokens of a sequence that begins before it.
 constexpr uint32_t kRuns = 4;  // wavefronts, and runs, of a workgroup
+constexpr uint32_t kRunTokens = 8;
 
 template <int DT>
 __device__ __forceinline__ void unpack8(u4 v, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) unpack_pair<DT>(v[i], f[2 * i], f[2 * i + 1]);
+}
+
+template <int DT>
+__device__ __forceinline__ u4 pack8(const float (&y)[8]) {
+  return u4{pack_pair<DT>(y[0], y[1]), pack_pair<DT>(y[2], y[3]), pack_pair<DT>(y[4], y[5]), pack_pair<DT>(y[6], y[7])};
+}
+
+// Weights, channel by channel, and biases of channels [c, c + 8).
+template <int W>
+__device__ __forceinline__ void load_weights(const ConvArgs& a, uint32_t c, float (&w)[8 * W], float (&bias)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2 * W; ++i) {
+    const f4 v = *reinterpret_cast<const f4*>(a.W + (size_t)c * W + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bias[i] = a.bias ? a.bias[c + i] : 0.f;
+}
+
+// One token a sequence: bound by the wait for the row's number and then for its kept inputs, so everything else is loaded
+// before them. 64 sequences of 10240 channels: 5.2 us (9.2 MB); 8.5 with the kernel below.
+template <int DT, int W>
+__global__ __launch_bounds__(64) void hq_ssm_conv_step_kernel(ConvArgs a) {
+  const uint32_t c = (blockIdx.x * 64 + threadIdx.x) * 8, b = blockIdx.y;
+  const bool some = c < a.C;
+  const uint32_t cc = some ? c : 0u;
+  const u4 x = *reinterpret_cast<const u4*>(a.X + b * a.ldx + cc);
+  float w[8 * W], bias[8];
+  load_weights<W>(a, cc, w, bias);
+  const Seq q = find_seq(a.s, b, blockIdx.x == 0);
+  uint16_t* kept = a.state + q.row * a.row_stride + cc;
+  u4 in[W];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) {
+    in[j] = u4{0, 0, 0, 0};
+    if (q.read) in[j] = *reinterpret_cast<const u4*>(kept + (size_t)j * a.C);
+  }
+  in[W - 1] = x;
+  if (!some) return;
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = bias[e];
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    float f[8];
+    unpack8<DT>(in[j], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = fmaf(w[e * W + j], f[e], y[e]);
+  }
+  if (a.silu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = silu(y[e]);
+  }
+  *reinterpret_cast<u4*>(a.Y + b * a.ldy + c) = pack8<DT>(y);
+  if (q.keep) {
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) *reinterpret_cast<u4*>(kept + (size_t)j * a.C) = in[j + 1];
+  }
 }
 
 template <int DT, int W, int TT>
@@ -41,17 +103,33 @@ __global__ __launch_bounds__(64 * kRuns) void hq_ssm_conv_kernel(ConvArgs a) {
     if (t >= 0 && t < a.s.T) x[i] = *reinterpret_cast<const u4*>(a.X + t * a.ldx + cc);
   }
   float w[8 * W], bias[8];
-#pragma unroll
-  for (int i = 0; i < 2 * W; ++i) {
-    const f4 v = *reinterpret_cast<const f4*>(a.W + (size_t)cc * W + 4 * i);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[4 * i + e] = v[e];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bias[i] = a.bias ? a.bias[cc + i] : 0.f;
+  load_weights<W>(a, cc, w, bias);
 
   uint32_t b = uni(seq_of(a.s, t0));
   uint32_t begin = a.s.cu ? clamp_to(a.s.cu[b], a.s.T) : b, end = a.s.cu ? clamp_to(a.s.cu[b + 1], a.s.T) : b + 1;
+  // Most runs lie in one sequence, its first tokens not among them: every input is unpacked once.
+  if (t0 >= (uint64_t)begin + (W - 1) && end >= (uint64_t)t0 + TT) {
+    float in[W][8];  // token t's in place t % W
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) unpack8<DT>(x[i], in[i]);
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      unpack8<DT>(x[i + W - 1], in[(i + W - 1) % W]);
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = bias[e];
+#pragma unroll
+        for (int j = 0; j < W; ++j) y[e] = fmaf(w[e * W + j], in[(i + j) % W][e], y[e]);
+      }
+      if (a.silu) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = silu(y[e]);
+      }
+      if (some) *reinterpret_cast<u4*>(a.Y + (int64_t)(t0 + i) * a.ldy + c) = pack8<DT>(y);
+    }
+    return;
+  }
   u4 old[W - 1];  // the kept inputs of the sequence that begins in this run
 #pragma unroll
   for (int i = 0; i < W - 1; ++i) old[i] = u4{0, 0, 0, 0};
@@ -116,19 +194,22 @@ __global__ __launch_bounds__(64 * kRuns) void hq_ssm_conv_kernel(ConvArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = silu(y[e]);
       }
-      if (some) *reinterpret_cast<u4*>(a.Y + t * a.ldy + c) = u4{pack_pair<DT>(y[0], y[1]), pack_pair<DT>(y[2], y[3]), pack_pair<DT>(y[4], y[5]), pack_pair<DT>(y[6], y[7])};
+      if (some) *reinterpret_cast<u4*>(a.Y + t * a.ldy + c) = pack8<DT>(y);
     }
   }
 }
 
 template <int DT, int W>
 hipError_t launch_conv(const ConvArgs& a, hipStream_t s) {
-  // Runs of 16 tokens read 1.3 times what they write; single tokens and short sequences, whose runs would wait for one row of
-  // the states after the other, go one a wavefront.
-  const bool run = a.s.cu && a.s.T >= 32ull * a.s.n;
-  const uint32_t tile = run ? 16 : 1, per = tile * kRuns;
+  if (!a.s.cu) {
+    hipLaunchKernelGGL((hq_ssm_conv_step_kernel<DT, W>), dim3((a.C / 8 + 63) / 64, a.s.n), dim3(64), 0, s, a);
+    return hipGetLastError();
+  }
+  // Short sequences, whose runs would wait for one row of the states after the other, go one token a wavefront.
+  const bool run = a.s.T >= 32ull * a.s.n;
+  const uint32_t tile = run ? kRunTokens : 1, per = tile * kRuns;
   const dim3 grid((a.C / 8 + 63) / 64, (a.s.T + per - 1) / per);
-  if (run) hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, 16>), grid, dim3(64 * kRuns), 0, s, a);
+  if (run) hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, kRunTokens>), grid, dim3(64 * kRuns), 0, s, a);
   else hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, 1>), grid, dim3(64 * kRuns), 0, s, a);
   return hipGetLastError();
 }
@@ -246,10 +327,12 @@ hipError_t launch_ssm_conv(int dtype, const ConvArgs& a, hipStream_t s) {
 ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim, uint32_t max_len) {
   ScanPlan p;
   p.largest = (uint64_t)heads * (head_dim / kStepRows) * n;
-  if (!cu || tokens < 8ull * n) return p;
-  p.chunk = true;
   const uint32_t L = state_dim == 256 ? 32 : 64, two = 128 / head_dim, slots = (uint32_t)cu_count() * (state_dim == 256 ? 1 : 2);
   p.units = groups * ((heads / groups + two - 1) / two);
+  // Few tokens a sequence go one by one. 48 heads of 128x128: 8 sequences of 6 and 8 tokens 18.3 and 23.9 us, in a chunk
+  // 20.9; where there are more than workgroups at once, as 64 sequences are, of 4 and 6 tokens 93 and 116 us, in a chunk 96.
+  if (!cu || tokens < ((uint64_t)n * p.units > slots ? 5ull : 8ull) * n) return p;
+  p.chunk = true;
   const uint32_t longest = ((max_len && max_len < tokens ? max_len : tokens) + L - 1) / L;
   // Runs there may be: two rounds of workgroups and one a sequence.
   const uint32_t most = 2 * slots / p.units + n;
@@ -260,7 +343,11 @@ ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_
       const uint32_t c = (longest + k - 1) / k, runs = tokens / (c * L) + n;
       if (k > 1 && runs > most) break;
       const uint64_t groups_of = (uint64_t)(k == 1 ? n : runs) * p.units, rounds = (groups_of + slots - 1) / slots;
-      const float cost = rounds * c * (groups_of * 2 > slots ? 4.f : 2.5f) * (k > 1 ? 1.6f : 1.f) + (k > 1 ? 8.f + k : 0.f);
+      // In us: a chunk of one workgroup a compute unit 5.0, of two at once 9.5; a carry is 0.45 of one; a launch about a chunk
+      // before the first, and 3 or 18 apart. 512 tokens of 48 heads of 128x128: whole 48.5, runs of 2 chunks 42.8, of 1 48.5;
+      // 1024: whole 88, of 4 56.6, of 2 59; 8192: whole 670, of 13 191, of 26 238.
+      const float one = state_dim != 256 && groups_of * 2 > slots ? 9.5f : 5.f;
+      const float cost = rounds * (c + 1) * one * (k > 1 ? 1.45f : 1.f) + (k > 1 ? 18.f : 3.f);
       if (k == 1 || cost < best) {
         best = cost;
         chunks = c;
