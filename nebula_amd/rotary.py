@@ -140,29 +140,42 @@ def _weight(name: str, w, D: int, dev: int) -> int:
     """Address of a norm's weight (None: 0)."""
     if w is None:
         return 0
-    if not (w.get_device() == dev and w.dtype == (hq._torch or hq._load()).float32 and w.is_contiguous() and w.numel() == D):
+    if w.get_device() != dev or w.dtype != (hq._torch or hq._load()).float32 or not w.is_contiguous() or w.numel() != D:
         raise ValueError(f"{name} must be a contiguous float32 tensor of {D} entries on the call's device, got {w.dtype} {tuple(w.shape)} on {w.device}")
     return w.data_ptr()
 
 
-def _heads(name: str, x, out, weight, eps: float, dev: int) -> bytes:
-    T, H, D = x.shape
-    row, head = attn._strides(x)
-    if out is None:
-        return _HEADS.pack(x.data_ptr(), 0, row, head, 0, 0, _weight(name + "_weight", weight, D, dev), H, eps)
-    orow, ohead = attn._strides(out)
-    return _HEADS.pack(x.data_ptr(), out.data_ptr(), row, head, orow, ohead, _weight(name + "_weight", weight, D, dev), H, eps)
+def _heads(name: str, x, shape, out, weight, eps: float, dev: int) -> bytes:
+    """hq_rotary_heads of a tensor that is checked."""
+    T, H, D = shape
+    row, head, _ = x.stride()
+    op = orow = ohead = 0
+    if out is not None:
+        op = out.data_ptr()
+        orow, ohead, _ = out.stride()
+        if H == 1:
+            ohead = 0
+    if T == 1:
+        row = orow = 0
+    return _HEADS.pack(x.data_ptr(), op, row, head if H > 1 else 0, orow, ohead, 0 if weight is None else _weight(name, weight, D, dev), H, eps)
 
 
-def _output(name: str, x, out):
+def _check_heads(name: str, x, shape, dtype, dev: int) -> None:
+    if len(shape) != 3 or x.dtype != dtype or x.get_device() != dev or dev < 0:
+        raise ValueError(f"{name} must be a {dtype} tensor [tokens, heads, head_dim] on the call's GPU, got {x.dtype} {tuple(shape)} on {x.device}")
+    if x.stride()[2] != 1:
+        raise ValueError(f"{name} must have unit stride along its last dimension, got strides {x.stride()}")
+
+
+def _output(name: str, x, shape, out):
     """The output tensor for x, checked or made."""
     if out is None:
-        if attn._i32t is None:
+        if attn._empty_like is None:
             attn._int32()
         return attn._empty_like(x, memory_format=attn._dense)
-    attn._check_heads(name, out, x, x.dtype)
-    if out.shape != x.shape:
-        raise ValueError(f"{name} has shape {tuple(out.shape)}, expected {tuple(x.shape)}")
+    if out.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(out.shape)}, expected {tuple(shape)}")
+    _check_heads(name, out, shape, x.dtype, x.get_device())
     return out
 
 
@@ -175,19 +188,20 @@ def rotate(q, k, rotary: Rotary, positions, q_weight=None, k_weight=None, eps: f
     """q and k (None: q alone) [tokens, heads, head_dim], each head normed (with a weight: x * weight / sqrt(mean(x^2) + eps))
     and rotated by its token's position; positions: int32 [tokens]. Returns (q', k'), or q' without k. out_q may be q
     and out_k k (in place)."""
-    attn._check_heads("q", q)
-    dev = q.get_device()
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    _check_heads("q", q, shape, dtype, dev)
     _check_rotary(rotary, dev)
-    out_q = _output("out_q", q, out_q)
-    T, _, D = q.shape
+    T, _, D = shape
+    out_q = _output("out_q", q, shape, out_q)
     kb = None
     if k is not None:
-        attn._check_heads("k", k, q, q.dtype)
-        if k.shape[0] != T or k.shape[2] != D:
-            raise ValueError(f"k has shape {tuple(k.shape)}, q {tuple(q.shape)}: the same tokens and head_dim are needed")
-        out_k = _output("out_k", k, out_k)
-        kb = _heads("k", k, out_k, k_weight, eps, dev)
-    st = (_bound or _lib()).hq_rotate(rotary._ref, _heads("q", q, out_q, q_weight, eps, dev), kb, T, D, hq._dt(q),
+        ks = k.shape
+        _check_heads("k", k, ks, dtype, dev)
+        if ks[0] != T or ks[2] != D:
+            raise ValueError(f"k has shape {tuple(ks)}, q {tuple(shape)}: the same tokens and head_dim are needed")
+        out_k = _output("out_k", k, ks, out_k)
+        kb = _heads("k_weight", k, ks, out_k, k_weight, eps, dev)
+    st = (_bound or _lib()).hq_rotate(rotary._ref, _heads("q_weight", q, shape, out_q, q_weight, eps, dev), kb, T, D, hq._dt(q),
                                       attn._ints("positions", positions, T, dev) or None, hq._stream_ptr(stream))
     if st:
         hq.check(st)
@@ -197,21 +211,28 @@ def rotate(q, k, rotary: Rotary, positions, q_weight=None, k_weight=None, eps: f
 def append(cache, layer: int, rotary: Rotary, q, k, v, rows, cu_seqlens=None, q_weight=None, k_weight=None, eps: float = 1e-6, out=None,
            stream=None):
     """KVCache.append_rotated."""
-    cache._new("k", k)
-    cache._new("v", v, k.shape[0])
-    dev, T = cache.device_index, k.shape[0]
+    shape, dtype, dev, D = k.shape, cache.k.dtype, cache.device_index, cache.head_dim
+    _check_heads("k", k, shape, dtype, dev)
+    T, H, _ = shape
+    if shape != (T, cache.kv_heads, D):
+        raise ValueError(f"k has shape {tuple(shape)}, the cache holds {cache.kv_heads} heads of {D}")
+    if v.shape != shape:
+        raise ValueError(f"v has shape {tuple(v.shape)}, k {tuple(shape)}")
+    _check_heads("v", v, shape, dtype, dev)
     _check_rotary(rotary, dev)
     qb = None
     if q is not None:
-        attn._check_heads("q", q, cache.k, cache.k.dtype)
-        if q.shape[0] != T or q.shape[2] != cache.head_dim:
-            raise ValueError(f"q has shape {tuple(q.shape)}: {T} tokens with head_dim {cache.head_dim} are needed")
-        out = _output("out", q, out)
-        qb = _heads("q", q, out, q_weight, eps, dev)
+        qs = q.shape
+        _check_heads("q", q, qs, dtype, dev)
+        if qs[0] != T or qs[2] != D:
+            raise ValueError(f"q has shape {tuple(qs)}: {T} tokens with head_dim {D} are needed")
+        out = _output("out", q, qs, out)
+        qb = _heads("q_weight", q, qs, out, q_weight, eps, dev)
     n = rows.numel()
-    vr, vh = attn._strides(v)
-    st = (_bound or _lib()).hq_cache_append_rotated(cache._ref, layer, rotary._ref, qb, _heads("k", k, None, k_weight, eps, dev), v.data_ptr(), vr, vh, T,
-                                                    cache._list("rows", rows), attn._ints("cu_seqlens", cu_seqlens, n + 1, dev) or None, n,
+    vr, vh, _ = v.stride()
+    st = (_bound or _lib()).hq_cache_append_rotated(cache._ref, layer, rotary._ref, qb, _heads("k_weight", k, shape, None, k_weight, eps, dev), v.data_ptr(),
+                                                    vr if T > 1 else 0, vh if H > 1 else 0, T, cache._list("rows", rows),
+                                                    None if cu_seqlens is None else attn._ints("cu_seqlens", cu_seqlens, n + 1, dev), n,
                                                     hq._stream_ptr(stream))
     if st:
         hq.check(st)

@@ -72,9 +72,34 @@ def _floats(name: str, t, n: int, dev: int) -> int:
     """Address of a contiguous float32 tensor of n entries on GPU dev (None: 0)."""
     if t is None:
         return 0
-    if not (t.get_device() == dev and t.dtype == (hq._torch or hq._load()).float32 and t.is_contiguous() and t.numel() == n):
+    if t.get_device() != dev or t.dtype != (hq._torch or hq._load()).float32 or not t.is_contiguous() or t.numel() != n:
         raise ValueError(f"{name} must be a contiguous float32 tensor of {n} entries on the call's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
+
+
+def _heads(name: str, t, shape, dtype, dev: int):
+    """(address, row stride, head stride) of a [tokens, heads, dim] operand; an axis of one entry may have any stride: 0 stands for it."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on device {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    row, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{name} must have unit stride along its last dimension, got strides {t.stride()}")
+    return t.data_ptr(), row if shape[0] > 1 else 0, head if shape[1] > 1 else 0
+
+
+def _rows(name: str, t, shape, dtype, dev: int):
+    """(address, row stride) of a [tokens, channels] operand; that of one token is the channels."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on device {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    row, one = t.stride()
+    if one != 1 or (shape[0] > 1 and row < shape[1]):
+        raise ValueError(f"{name} must have unit stride along its channels and rows apart, got strides {t.stride()}")
+    return t.data_ptr(), row if shape[0] > 1 else shape[1]
+
+
+def _torch_calls():
+    attn._int32()
+    return attn._empty_like
 
 
 class StateCache:
@@ -148,31 +173,27 @@ class StateCache:
 
     def _sequences(self, T: int, rows, cu_seqlens, held):
         """Addresses of the lists, and how many sequences."""
-        dev = self.device_index
-        n = T if cu_seqlens is None else cu_seqlens.numel() - 1
-        return attn._ints("rows", rows, n, dev) or None, attn._ints("held", held, n, dev) or None, \
-            attn._ints("cu_seqlens", cu_seqlens, None, dev) or None, max(n, 0)
+        dev, n, cp = self.device_index, T, None
+        if cu_seqlens is not None:
+            n, cp = max(cu_seqlens.numel() - 1, 0), attn._ints("cu_seqlens", cu_seqlens, None, dev)
+        return None if rows is None else attn._ints("rows", rows, n, dev), None if held is None else attn._ints("held", held, n, dev), cp, n
 
     def conv(self, layer: int, x, weight, rows=None, cu_seqlens=None, bias=None, silu: bool = True, held=None, out=None, stream=None):
         """Causal convolution of each channel of x [tokens, channels] with weight [channels, width] (float32), plus bias
         [channels], through u / (1 + exp(-u)) if silu: tokens [cu_seqlens[i], cu_seqlens[i + 1]) are rows[i]'s next ones
         (cu_seqlens None: one token a row; rows None: row i). The rows' last inputs are kept. Returns out, apart from x."""
-        T, C = x.shape
-        ref = self._refs.get(x.dtype)
+        T, C = shape = x.shape
+        dtype, dev = x.dtype, self.device_index
+        ref = self._refs.get(dtype)
         if ref is None or self.conv_state is None or C != self.channels:
-            raise ValueError(f"x is {x.dtype} of {C} channels, the states {self.dtype} of {self.channels}")
-        if not hq._rows_ok(x, T, C, x.dtype) or x.get_device() != self.device_index:
-            hq._check_rows("x", x, T, C, x.dtype)
-            raise ValueError(f"x is on {x.device}, the states on device {self.device_index}")
+            raise ValueError(f"x is {dtype} of {C} channels, the states {self.dtype} of {self.channels}")
+        xp, ldx = _rows("x", x, shape, dtype, dev)
         if out is None:
-            out = x.new_empty((T, C))
-        elif out.shape != x.shape or not hq._rows_ok(out, T, C, x.dtype) or out.get_device() != self.device_index:
-            raise ValueError(f"out must be a {x.dtype} tensor of shape {(T, C)} with unit column stride on x's device")
-        dev = self.device_index
+            out = (attn._empty_like or _torch_calls())(x, memory_format=attn._dense)
+        yp, ldy = _rows("out", out, shape, dtype, dev)
         rp, hp, cp, n = self._sequences(T, rows, cu_seqlens, held)
-        st = (_bound or _lib()).hq_ssm_conv(ref, layer, x.data_ptr(), x.stride(0) if T > 1 else C, out.data_ptr(), out.stride(0) if T > 1 else C,
-                                            _floats("weight", weight, C * self.width, dev), _floats("bias", bias, C, dev) or None, int(silu), T, rp, hp,
-                                            cp, n, hq._stream_ptr(stream))
+        st = (_bound or _lib()).hq_ssm_conv(ref, layer, xp, ldx, yp, ldy, _floats("weight", weight, C * self.width, dev),
+                                            None if bias is None else _floats("bias", bias, C, dev), silu, T, rp, hp, cp, n, hq._stream_ptr(stream))
         if st:
             hq.check(st)
         return out
@@ -184,30 +205,36 @@ class StateCache:
         x, z and out [tokens, heads, head_dim], B and C [tokens, groups, state_dim], dt [tokens, heads] float32 or x's type; A (not
         positive), D and dt_bias float32 [heads]. Sequences as in conv(); their states S are kept. max_len: no sequence has more
         new tokens (a hint for the split). Single tokens and a long chunk are faster as two calls. out may be z."""
-        ref = self._refs.get(x.dtype)
+        dtype = x.dtype
+        ref = self._refs.get(dtype)
         if ref is None or self.ssm_state is None:
-            raise ValueError(f"x is {x.dtype}, the states {self.dtype}")
-        dev, H, P, N = self.device_index, self.heads, self.head_dim, self.state_dim
-        for name, t in (("x", x), ("B", B), ("C", C)) if z is None else (("x", x), ("B", B), ("C", C), ("z", z)):
-            attn._check_heads(name, t, self.ssm_state, x.dtype)
-        T, G = x.shape[0], B.shape[1]
-        if x.shape[1:] != (H, P) or (z is not None and z.shape != x.shape) or B.shape != (T, G, N) or C.shape != B.shape:
-            raise ValueError(f"x {tuple(x.shape)}, z {None if z is None else tuple(z.shape)}, B {tuple(B.shape)}, C {tuple(C.shape)}: need [tokens, {H}, {P}] "
-                             f"and [tokens, groups, {N}]")
-        f32 = dt.dtype == (hq._torch or hq._load()).float32
-        if dt.get_device() != dev or dt.shape != (T, H) or (H > 1 and dt.stride(1) != 1) or not (f32 or dt.dtype == x.dtype):
-            raise ValueError(f"dt must be [{T}, {H}] float32 or {x.dtype} with unit stride along the heads, got {dt.dtype} {tuple(dt.shape)} on {dt.device}")
-        out, _ = attn._outputs(x, out, None, False)
-        rp, hp, cp, n = self._sequences(T, rows, cu_seqlens, held)
-        wp, wb = hq._ws(workspace)
-        zr, zh = (0, 0) if z is None else attn._strides(z)
-        io = _IO.pack(x.data_ptr(), B.data_ptr(), C.data_ptr(), dt.data_ptr(), 0 if z is None else z.data_ptr(), out.data_ptr(), _floats("A", A, H, dev),
-                      _floats("D", D, H, dev), _floats("dt_bias", dt_bias, H, dev), *attn._strides(x), *attn._strides(B), *attn._strides(C),
-                      dt.stride(0) if T > 1 else H, zr, zh, *attn._strides(out), T, G, f32, softplus)
-        st = (_bound or _lib()).hq_ssm_scan(ref, layer, io, rp, hp, cp, n, max_len, wp, wb, hq._stream_ptr(stream))
+            raise ValueError(f"x is {dtype}, the states {self.dtype}")
+        dev, H, xs, bs = self.device_index, self.heads, x.shape, B.shape
+        if len(xs) != 3 or len(bs) != 3 or xs != (xs[0], H, self.head_dim) or bs != (xs[0], bs[1], self.state_dim):
+            raise self._shapes(x, B, C, z)
+        xp, xr, xh = _heads("x", x, xs, dtype, dev)
+        bp, br, bh = _heads("B", B, bs, dtype, dev)
+        cp, cr, ch = _heads("C", C, bs, dtype, dev)
+        zp, zr, zh = (0, 0, 0) if z is None else _heads("z", z, xs, dtype, dev)
+        T, f32 = xs[0], dt.dtype
+        f32 = f32 == (hq._torch or hq._load()).float32 or (None if f32 != dtype else False)
+        if f32 is None or dt.get_device() != dev or dt.shape != (T, H) or (H > 1 and dt.stride(1) != 1):
+            raise ValueError(f"dt must be [{T}, {H}] float32 or {dtype} with unit stride along the heads, got {dt.dtype} {tuple(dt.shape)} on {dt.device}")
+        if out is None:
+            out = (attn._empty_like or _torch_calls())(x, memory_format=attn._dense)
+        yp, yr, yh = _heads("out", out, xs, dtype, dev)
+        rp, hp, cup, n = self._sequences(T, rows, cu_seqlens, held)
+        wp, wb = (None, 0) if workspace is None else hq._ws(workspace)
+        io = _IO.pack(xp, bp, cp, dt.data_ptr(), zp, yp, _floats("A", A, H, dev), _floats("D", D, H, dev), _floats("dt_bias", dt_bias, H, dev),
+                      xr, xh, br, bh, cr, ch, dt.stride(0) if T > 1 else H, zr, zh, yr, yh, T, bs[1], f32, softplus)
+        st = (_bound or _lib()).hq_ssm_scan(ref, layer, io, rp, hp, cup, n, max_len, wp, wb, hq._stream_ptr(stream))
         if st:
             hq.check(st)
         return out
+
+    def _shapes(self, x, B, C, z):
+        return ValueError(f"x {tuple(x.shape)}, z or out {None if z is None else tuple(z.shape)}, B {tuple(B.shape)}, C {tuple(C.shape)}: need "
+                          f"[tokens, {self.heads}, {self.head_dim}] and [tokens, groups, {self.state_dim}]")
 
     def check(self) -> None:
         """Waits for the device, all its streams, and raises HQError if a call met a fault there since the last check."""
