@@ -19,8 +19,10 @@ tokens first, then one prefill chunk); the library picks its streaming (decode) 
 up to 80 rows and its prefill kernels above. `StepRows` builds such a batch's activation
 matrix and splits the outputs back per chunk. Between q | k | v and attn_output, `LayerProjections.attend`
 keeps the keys and values in a paged cache and computes the attention (nebula_amd.attn) of the step's
-decode tokens, over a shared prefix where they have one, and of its prefill chunk; `StepCache` holds what
-a step's layers have in common. Normalisation, rotation and gating of the query, the SSM step and SwiGLU stay
+decode tokens, over a shared prefix where they have one, and of its prefill chunk; with a `rotary` the heads are normed
+and rotated on their way into the cache (nebula_amd.rotary). Between gate | qkv and ssm_out, `LayerProjections.mix` runs
+the short convolution and the state space scan over the sequences' states (nebula_amd.ssm). `StepCache` holds
+what a step's layers have in common. The layer norms, the gating of attention's output, the scan's step widths and SwiGLU stay
 with the caller.
 
 Activations are fp16 or bf16 (the reference's are fp32); the ternary weights and their
@@ -31,7 +33,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple
 
-from . import attn, hq
+from . import attn, hq, ssm
 
 # Dimensions of the reference's 27B model (hydrogen/include/native_decoder.hpp:180-188).
 EMBEDDING = 5120
@@ -42,6 +44,7 @@ MIXER_IN = 6144      # attn_output / ssm_out input width
 HEADS, KV_HEADS, HEAD_DIM = 24, 4, 256   # MIXER_IN = 24 x 256, KV_OUT = 4 x 256; q holds the query and its gate
 SSM_GATE = 6144
 SSM_QKV = 10240
+SSM_HEADS, SSM_HEAD_DIM, SSM_GROUPS, SSM_STATE = 48, 128, 16, 128   # qkv: x of 48 x 128, B and C of 16 x 128 each
 TQ1_GROUP = 256
 
 # Projection name -> (K, N), as the reference launches them.
@@ -101,7 +104,8 @@ class LayerProjections:
         """attn_output or ssm_out (6144 -> 5120)."""
         return self._fused(FUSED_GROUPS[self.kind][1], y, None if out is None else [out], stream)[0]
 
-    def attend(self, x_norm, cache: "attn.KVCache", cache_layer: int, step: "StepCache", prepare=None, gate=None, stream=None):
+    def attend(self, x_norm, cache: "attn.KVCache", cache_layer: int, step: "StepCache", prepare=None, gate=None, stream=None,
+               rotary=None, q_weight=None, k_weight=None, eps: float = 1e-6):
         """The attention mixer of one layer over a step's rows: mixer_in, the new keys and values to layer
         cache_layer of the cache, attention of the decode rows and of the prefill chunks, mixer_out.
 
@@ -110,6 +114,9 @@ class LayerProjections:
         (default: the first half of q_out, k and v as they are). gate(y, q_out) is what goes to mixer_out in
         y's place (default: y, [M, 6144]). step.reserve(cache) comes first, once for all layers.
 
+        With a rotary (nebula_amd.rotary.Rotary), q and k are as prepare gives them still to be normed (each with its
+        weight, if there is one) and rotated by their tokens' places: one launch does it and appends.
+
         With a stream (torch's), everything runs on it, prepare and gate too, and it is the current one while
         they do: the layer's tensors are its own. The caller orders it after what made x_norm, and orders
         others after it."""
@@ -117,7 +124,7 @@ class LayerProjections:
             import torch
 
             with torch.cuda.stream(stream):
-                return self.attend(x_norm, cache, cache_layer, step, prepare, gate)
+                return self.attend(x_norm, cache, cache_layer, step, prepare, gate, None, rotary, q_weight, k_weight, eps)
         if self.kind != "attention":
             raise ValueError(f"attend() is the attention mixer's, the layer's kind is {self.kind!r}")
         M = step.M
@@ -129,7 +136,12 @@ class LayerProjections:
             k, v = (t.unflatten(1, (KV_HEADS, HEAD_DIM)) for t in (k, v))
         else:
             q, k, v = prepare(q_out, k, v)
-        cache.append(cache_layer, k, v, step.rows, step.cu)
+        if rotary is not None:
+            q = cache.append_rotated(cache_layer, rotary, q, k, v, step.rows, step.cu, q_weight=q_weight, k_weight=k_weight, eps=eps)
+        elif q_weight is not None or k_weight is not None:
+            raise ValueError("q_weight and k_weight need a rotary")
+        else:
+            cache.append(cache_layer, k, v, step.rows, step.cu)
         y = q.new_empty((M, HEADS, HEAD_DIM))
         n = step.decodes
         if n and step.prefix is not None and step.prefix[2] >= cache.page_tokens:  # whole pages are shared
@@ -141,6 +153,36 @@ class LayerProjections:
         y = y.flatten(1)
         return self.mixer_out(y if gate is None else gate(y, q_out))
 
+    def mix(self, x_norm, dt, mixer: "StateMixer", states: "ssm.StateCache", states_layer: int, step: "StepCache", stream=None):
+        """The state space mixer of one layer over a step's rows: mixer_in, the short convolution of qkv, the scan
+        of its x, B and C gated by gate, mixer_out. dt: the tokens' step widths [M, 48], float32 or x_norm's type, before
+        bias and softplus. The step's requests hold rows of layer states_layer of the states, the same ones as of the
+        cache (states.refused = cache.refused: a step that step.reserve(cache) was refused for leaves them too); a
+        request whose chunk starts at token 0 begins with zero states. A stream is taken as attend() does."""
+        if stream is not None:
+            import torch
+
+            with torch.cuda.stream(stream):
+                return self.mix(x_norm, dt, mixer, states, states_layer, step)
+        if self.kind != "ssm":
+            raise ValueError(f"mix() is the state space mixer's, the layer's kind is {self.kind!r}")
+        M, n = step.M, step.decodes
+        if x_norm.shape[0] != M or dt.shape[0] != M:
+            raise ValueError(f"x_norm has {x_norm.shape[0]} rows, dt {dt.shape[0]}, the step {M}")
+        gate, qkv = self.mixer_in(x_norm)
+        xbc, y = qkv.new_empty(qkv.shape), gate.new_empty((M, SSM_HEADS, SSM_HEAD_DIM))
+        x, B, C = (t.unflatten(1, (-1, SSM_HEAD_DIM)) for t in xbc.split([SSM_GATE, SSM_GROUPS * SSM_STATE, SSM_GROUPS * SSM_STATE], 1))
+        z = gate.unflatten(1, (SSM_HEADS, SSM_HEAD_DIM))
+        # Single tokens and chunks are faster apart: (tokens, rows, offsets, held, most tokens of a sequence).
+        parts = [(slice(0, n), step.decode_rows, None, step.decode_held, 1)] if n else []
+        if M > n:
+            parts.append((slice(n, M), step.chunk_rows, step.chunk_cu, step.chunk_held, step.max_new))
+        for at, rows, cu, held, most in parts:
+            states.conv(states_layer, qkv[at], mixer.conv_weight, rows, cu, bias=mixer.conv_bias, held=held, out=xbc[at])
+            states.scan(states_layer, x[at], dt[at], mixer.A, B[at], C[at], rows, cu, D=mixer.D, z=z[at], dt_bias=mixer.dt_bias, held=held,
+                        max_len=most, out=y[at])
+        return self.mixer_out(y.flatten(1))
+
     def ffn_in(self, x_norm, outs=None, stream=None) -> List:
         """[gate, up] — one fused call."""
         return self._fused(FUSED_GROUPS["ffn"][0], x_norm, outs, stream)
@@ -148,6 +190,17 @@ class LayerProjections:
     def ffn_out(self, act, out=None, stream=None):
         """down (17408 -> 5120)."""
         return self._fused(FUSED_GROUPS["ffn"][1], act, None if out is None else [out], stream)[0]
+
+
+@dataclass
+class StateMixer:
+    """A state space layer's own weights, float32 (nebula_amd.ssm): conv_weight [10240, width], conv_bias [10240] or None, A (not
+    positive), D and dt_bias [48], the last two or None."""
+    conv_weight: object
+    A: object
+    conv_bias: object = None
+    D: object = None
+    dt_bias: object = None
 
 
 @dataclass
@@ -198,7 +251,7 @@ class StepCache:
     """The cache rows of a step, made once and used by each of its layers. row_of[request_id] is a request's
     row of the cache. groups: lists of the step's decode requests, in its order and all of them, with the
     number of first tokens that each list's rows share (as cache.fork leaves them): [([request_id, ..],
-    prefix), ..]."""
+    prefix), ..]. held: the tokens that each request holds before the step (its chunk's start_token)."""
 
     def __init__(self, rows: StepRows, row_of: Dict[int, int], groups=None, device="cuda"):
         import torch
@@ -210,6 +263,7 @@ class StepCache:
             raise ValueError(f"two chunks of a step have the same cache row: {held}")
         cu = rows.offsets + [rows.M]
         self.max_len = max((c.start_token + c.num_tokens for c in rows.chunks), default=0)
+        self.max_new = max((c.num_tokens for c in rows.chunks), default=0)
         self.prefix = None
         starts, lens = [0], []
         if groups is not None:
@@ -221,10 +275,11 @@ class StepCache:
                 lens.append(n)
         # One copy to the device for all lists.
         chunk_cu = [c - self.decodes for c in cu[self.decodes:]]
-        parts = [held, counts, cu, chunk_cu, starts, lens]
+        parts = [held, counts, cu, chunk_cu, [c.start_token for c in rows.chunks], starts, lens]
         both = torch.tensor([x for p in parts for x in p], dtype=torch.int32).to(device)
-        self.rows, self.counts, self.cu, self.chunk_cu, starts_t, lens_t = both.split([len(p) for p in parts])
+        self.rows, self.counts, self.cu, self.chunk_cu, self.held, starts_t, lens_t = both.split([len(p) for p in parts])
         self.decode_rows, self.chunk_rows = self.rows[:self.decodes], self.rows[self.decodes:]
+        self.decode_held, self.chunk_held = self.held[:self.decodes], self.held[self.decodes:]
         if lens:
             self.prefix = (starts_t, lens_t, max(lens))
 
