@@ -90,6 +90,7 @@ hq_status hq_ssm_conv(const hq_state_cache* cache, uint32_t layer, const void* X
   if (misaligned(cache->conv, 16)) return fail(HQ_ERR_ALIGNMENT, "cache: conv must be 16-byte aligned");
   if (w < 2 || w > 4) return fail(HQ_ERR_UNSUPPORTED, "width=%u must be 2, 3 or 4", w);
   if (C == 0 || C % 8 || C > (1u << 20)) return fail(HQ_ERR_SHAPE, "channels=%u must be a positive multiple of 8, at most %u", C, 1u << 20);
+  if ((uint64_t)tokens * C > (1ull << 37)) return fail(HQ_ERR_SHAPE, "tokens=%u of %u channels: too many for one call", tokens, C);
   if ((st = check_pool("conv", cache->conv_layer, cache->conv_row, cache->layers, cache->rows, (int64_t)(w - 1) * C, 8)) != HQ_OK) return st;
   if (!X || !Y || !W) return fail(HQ_ERR_INVALID_ARG, "X, Y or W is null");
   if (X == Y) return fail(HQ_ERR_INVALID_ARG, "Y is X: a convolution needs its inputs");

@@ -274,7 +274,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     const __amdgpu_buffer_rsrc_t bx = rsrc(x_at), bd = rsrc(dt_at);
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) rx[i] = __builtin_amdgcn_raw_buffer_load_b128(bx, past(x_off, xrow + i * 16 < left), i * 16 * x_step, 0);
-    const uint32_t dt_off = past(__umul24(id, dt_step), id < left);
+    const uint32_t dt_off = past(id * dt_step, id < left);  // (up to 2^24 bytes: not in 24 bits)
     if (dt_f32) rdt = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(bd, dt_off, 0, 0);
     else rdt = __builtin_amdgcn_raw_buffer_load_b16(bd, dt_off, 0, 0);
   };
