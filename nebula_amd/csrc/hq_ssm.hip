@@ -228,7 +228,8 @@ hipError_t launch_conv_type(const ConvArgs& a, hipStream_t s) {
 // ---- the scan, token by token ----
 // Bound by the states' bytes, read and written once: a wavefront holds 8 rows of a head's state (32 a workgroup), every lane
 // 4 elements of a row as one 16-byte piece, so that a load is 1 KB of memory in one piece. The sum over a row is
-// one over the lanes that hold it, by moves between lanes.
+// one over the lanes that hold it, by moves between lanes. 64 sequences of 48 heads of 128x128: 89 us, 4.56 TB/s of states, inputs and
+// outputs; one sequence 4.8, its launch and chain of loads.
 constexpr uint32_t kColumnsOfRun = 128;  // channels of a workgroup of the chunk kernel
 constexpr uint32_t kStepRows = 32;  // of a workgroup of four wavefronts
 
