@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <cstdio>
+#include <type_traits>
 
 #include "hq_internal.hpp"
 #include "hq_ssm_device.hpp"
@@ -81,6 +82,21 @@ constexpr uint32_t m_bytes() {
 template <int L>
 __device__ __forceinline__ uint32_t m_place(uint32_t block, uint32_t r, uint32_t c) {
   return L == 64 && block ? 32 * 64 + piece_at<128>(r, c) : piece_at<64>(r, c);
+}
+
+// The tiles of M, 16 tokens t with 16 earlier ones s, of a head's wavefront `part` of 4 or 2.
+struct MTiles {
+  int n, t[5], s[5];
+};
+constexpr MTiles m_tiles(int L, int waves, int part) {
+  if (L == 32) {
+    if (waves == 2) return part == 0 ? MTiles{2, {1, 1}, {0, 1}} : MTiles{1, {0}, {0}};
+    return part == 0 ? MTiles{1, {1}, {0}} : part == 1 ? MTiles{1, {1}, {1}} : MTiles{1, {0}, {0}};
+  }
+  if (waves == 2) return part == 0 ? MTiles{5, {3, 3, 3, 3, 2}, {3, 0, 1, 2, 2}} : MTiles{5, {2, 2, 1, 1, 0}, {0, 1, 0, 1, 0}};
+  if (part == 0) return {3, {3, 3, 3}, {0, 1, 2}};
+  if (part == 1) return {3, {2, 2, 1}, {0, 1, 0}};
+  return part == 2 ? MTiles{2, {0, 1}, {0, 1}} : MTiles{2, {2, 3}, {2, 3}};
 }
 
 // A fragment of the transposed tile [tokens][columns]: columns 32 c32 .., tokens 16 ks ..; lane: column (SWAP: the middle
@@ -429,6 +445,9 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     whole = next_whole;
     total += whole;
     const float scale_down = next_down;
+    // Of two wavefronts on a SIMD, the one that makes outputs goes first: its chain is the longer one, and the other's products of the
+    // state's sums fill what it leaves (8 prompts of 512 tokens 82 -> 77 us, one of 8192 197 -> 192).
+    if constexpr (!CARRY) __builtin_amdgcn_s_setprio(2);
     float* const cum = vec + (wave * 2 + turn) * 3 * L;  // of this chunk: exponents (of 2), steps, weights of the state's terms
     const float *const steps = cum + L, *const weights = steps + L;
     // Outputs leave as 16-byte pieces, four lanes a token: token lane / 4 + 16 i, channels 8 (lane % 4) ..
@@ -460,49 +479,51 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
 
     f16x y[kTB];
     if constexpr (!CARRY) {
-      // M in tiles of 16 x 16, dealt to the head's wavefronts: B_s . C_t, a lane one t and four s.
-      // Those on the diagonal come first.
-      constexpr int kT16 = L / 16, kTiles = kT16 * (kT16 + 1) / 2, kMine = (kTiles + kWaves - 1) / kWaves;
+      // M in tiles of 16 x 16, dealt to the head's wavefronts so that each has few rows of B and C to read: B_s . C_t, a lane one t
+      // and four s.
       const uint32_t id = opaque(lane), l16 = id & 15u, quad = id >> 4, at = piece_at<kRow>(l16, quad);
-      uint32_t ti[kMine], si[kMine];
-      f4 m[kMine];
+      auto weights_of = [&](auto which) __attribute__((always_inline)) {
+        constexpr MTiles kMine = m_tiles(L, kWaves, decltype(which)::value);
+        f4 m[kMine.n];
 #pragma unroll
-      for (int k = 0; k < kMine; ++k) {
-        const uint32_t tile = min(k * kWaves + part, kTiles - 1u), o = tile - kT16;  // (a wavefront without a tile takes the last one)
-        ti[k] = tile < kT16 ? tile : o < 1 ? 1 : o < 3 ? 2 : 3;
-        si[k] = tile < kT16 ? tile : o - ti[k] * (ti[k] - 1) / 2;
-        m[k] = f4{0, 0, 0, 0};
-      }
+        for (int k = 0; k < kMine.n; ++k) m[k] = f4{0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < N / 32; ++j)
+        for (int j = 0; j < N / 32; ++j)
 #pragma unroll
-        for (int k = 0; k < kMine; ++k) {
-          const u4 fb = *reinterpret_cast<const u4*>(sB + 16 * si[k] * kRow + (at ^ (uint32_t)(j << 6)));
-          const u4 fc = *reinterpret_cast<const u4*>(sC + 16 * ti[k] * kRow + (at ^ (uint32_t)(j << 6)));
-          m[k] = mfma16x16x32<DT>(fb, fc, m[k]);
-        }
-#pragma unroll
-      for (int k = 0; k < kMine; ++k) {
-        const uint32_t tt = 16 * ti[k] + l16, ss = 16 * si[k] + 4 * quad;
-        const float ct = cum[tt];
-        const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
-        float w[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[k][v];
-          if (k * kWaves < kT16) {
-            const int32_t back = (int32_t)(tt - ss);  // tokens from the lane's first one to its own
-            w[v] = v < back ? w[v] : v == back ? w[v] + D : 0.f;
+          for (int k = 0; k < kMine.n; ++k) {
+            const u4 fb = *reinterpret_cast<const u4*>(sB + 16 * kMine.s[k] * kRow + (at ^ (uint32_t)(j << 6)));
+            const u4 fc = *reinterpret_cast<const u4*>(sC + 16 * kMine.t[k] * kRow + (at ^ (uint32_t)(j << 6)));
+            m[k] = mfma16x16x32<DT>(fb, fc, m[k]);
           }
+#pragma unroll
+        for (int k = 0; k < kMine.n; ++k) {
+          const uint32_t tt = 16 * kMine.t[k] + l16, ss = 16 * kMine.s[k] + 4 * quad;
+          const float ct = cum[tt];
+          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
+          float w[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[k][v];
+            if (kMine.t[k] == kMine.s[k]) {
+              const int32_t back = (int32_t)(tt - ss);  // tokens from the lane's first one to its own
+              w[v] = v < back ? w[v] : v == back ? w[v] + D : 0.f;
+            }
+          }
+          const uint32_t to = m_place<L>(kMine.t[k] / 2, tt & 31u, ss / 8) + (ss & 4u) * 2;
+          u2 hi, lo;
+          hi[0] = take_part<BF>(w[0], w[1]);
+          hi[1] = take_part<BF>(w[2], w[3]);
+          lo[0] = pack_pair<BF>(w[0], w[1]);
+          lo[1] = pack_pair<BF>(w[2], w[3]);
+          *reinterpret_cast<u2*>(m0 + to) = hi;
+          *reinterpret_cast<u2*>(m0 + m_bytes<L>() + to) = lo;
         }
-        const uint32_t to = m_place<L>(ti[k] / 2, tt & 31u, ss / 8) + (ss & 4u) * 2;
-        u2 hi, lo;
-        hi[0] = take_part<BF>(w[0], w[1]);
-        hi[1] = take_part<BF>(w[2], w[3]);
-        lo[0] = pack_pair<BF>(w[0], w[1]);
-        lo[1] = pack_pair<BF>(w[2], w[3]);
-        *reinterpret_cast<u2*>(m0 + to) = hi;
-        *reinterpret_cast<u2*>(m0 + m_bytes<L>() + to) = lo;
+      };
+      if (part == 0) weights_of(std::integral_constant<int, 0>{});
+      else if (part == 1) weights_of(std::integral_constant<int, 1>{});
+      else if constexpr (kWaves == 4) {
+        if (part == 2) weights_of(std::integral_constant<int, 2>{});
+        else if constexpr (L == 64) weights_of(std::integral_constant<int, 3>{});
       }
       __syncthreads();
 
@@ -614,6 +635,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
 
     if constexpr (!CARRY) put_x(odd + (turn ^ 1u));
 
+    if constexpr (!CARRY) __builtin_amdgcn_s_setprio(0);
     // The state decayed, and the chunk's terms; between their products the outputs go out.
     const __amdgpu_buffer_rsrc_t by = rsrc(y_at);
     const uint32_t y_off = __umul24(lane / 4, y_step) + lane % 4 * 16;
