@@ -343,17 +343,22 @@ ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_
   if ((uint64_t)n * p.units < 2 * slots && longest > 1) {
     float best = 0;
     for (uint32_t k = 1; k <= std::min(longest, 64u); ++k) {
-      const uint32_t c = (longest + k - 1) / k, runs = tokens / (c * L) + n;
-      if (k > 1 && runs > most) break;
-      const uint64_t groups_of = (uint64_t)(k == 1 ? n : runs) * p.units, rounds = (groups_of + slots - 1) / slots;
-      // In us: a chunk of one workgroup a compute unit 5.0, of two at once 9.5; a carry is 0.45 of one; a launch about a chunk
-      // before the first, and 3 or 18 apart. 512 tokens of 48 heads of 128x128: whole 48.5, runs of 2 chunks 42.8, of 1 48.5;
-      // 1024: whole 88, of 4 56.6, of 2 59; 8192: whole 670, of 13 191, of 26 238.
-      const float one = state_dim != 256 && groups_of * 2 > slots ? 9.5f : 5.f;
-      const float cost = rounds * (c + 1) * one * (k > 1 ? 1.45f : 1.f) + (k > 1 ? 18.f : 3.f);
-      if (k == 1 || cost < best) {
-        best = cost;
-        chunks = c;
+      const uint32_t even = (longest + k - 1) / k;  // the longest sequence in k even runs, and, for the others' sake, a chunk more
+      if (k > 1 && tokens / ((even + 1) * L) + n > most) break;
+      for (uint32_t c = even; c <= even + (k > 1); ++c) {
+        const uint32_t runs = tokens / (c * L) + n;
+        if (k > 1 && (runs > most || c >= longest)) continue;
+        const uint64_t groups_of = (uint64_t)(k == 1 ? n : runs) * p.units, rounds = (groups_of + slots - 1) / slots;
+        // In us: a chunk of one workgroup a compute unit 5.15, of two at once 8.3; a carry is 0.45 of one; a launch about a chunk
+        // before the first, and 3 or 18 apart. 48 heads of 128x128, 512 tokens: whole 45.6, runs of 2 chunks 42.8, of 1 47; 1024: whole
+        // 83, of 4 55.2, of 2 57.7; 4096: of 13 119, of 7 110; 8192: of 26 215, of 13 186. 80 heads of 64x128, 1 to 1008 tokens: whole 90,
+        // of 5 86 (fp16: 99, 88).
+        const float one = state_dim != 256 && groups_of * 2 > slots ? 8.3f : 5.15f;
+        const float cost = rounds * (c + 1) * one * (k > 1 ? 1.45f : 1.f) + (k > 1 ? 18.f : 3.f);
+        if (k == 1 || cost < best) {
+          best = cost;
+          chunks = c;
+        }
       }
     }
     const size_t run_bytes = (size_t)p.units * (kColumnsOfRun * state_dim + two) * 4;

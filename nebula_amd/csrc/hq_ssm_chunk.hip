@@ -487,6 +487,15 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         f4 m[kMine.n];
 #pragma unroll
         for (int k = 0; k < kMine.n; ++k) m[k] = f4{0, 0, 0, 0};
+        f4 f[kMine.n];  // the decays and steps, while rows are on their way
+#pragma unroll
+        for (int k = 0; k < kMine.n; ++k) {
+          const uint32_t tt = 16 * kMine.t[k] + l16, ss = 16 * kMine.s[k] + 4 * quad;
+          const float ct = cum[tt];
+          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) f[k][v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v];
+        }
 #pragma unroll
         for (int j = 0; j < N / 32; ++j)
 #pragma unroll
@@ -498,12 +507,10 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
 #pragma unroll
         for (int k = 0; k < kMine.n; ++k) {
           const uint32_t tt = 16 * kMine.t[k] + l16, ss = 16 * kMine.s[k] + 4 * quad;
-          const float ct = cum[tt];
-          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
           float w[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            w[v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v] * m[k][v];
+            w[v] = f[k][v] * m[k][v];
             if (kMine.t[k] == kMine.s[k]) {
               const int32_t back = (int32_t)(tt - ss);  // tokens from the lane's first one to its own
               w[v] = v < back ? w[v] : v == back ? w[v] + D : 0.f;
