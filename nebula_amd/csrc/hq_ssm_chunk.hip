@@ -15,9 +15,9 @@
 // Few sequences are dealt to several workgroups in runs of chunks: a launch of this kernel sums what each run adds to the state
 // (kCarry), hq_ssm_join_kernel turns that into what enters each run, and a second launch computes the outputs from there.
 //
-// Bound by the vector pipe (parts of operands, decays, the gate) and the matrix pipe together: 54% and 29% busy at 8192 tokens of 48
-// heads of 128x128, where a wavefront has 1350 vector instructions and 104 products a chunk and a SIMD two wavefronts: 59 us of carries,
-// 11 of joins, 132 of outputs, 373 MB of operands (78 us at a copy's rate). One workgroup a CU: 5 us a chunk, bound by its own chain.
+// Bound by the vector pipe (parts of operands, decays, the gate) and the matrix pipe together: 58% and 33% busy at 8192 tokens of 48
+// heads of 128x128, where a wavefront has 1300 vector instructions and 102 products a chunk and a SIMD two wavefronts: 59 us of carries,
+// 11 of joins, 122 of outputs, 373 MB of operands (78 us at a copy's rate). One workgroup a CU: 5 us a chunk, bound by its own chain.
 //
 // Sums are fp32 throughout. What a matrix product's operands round away:
 //   the state's terms w x (fp32 times 16 bits) are kept as three bf16 parts, or in fp16 as two parts of values scaled by a
