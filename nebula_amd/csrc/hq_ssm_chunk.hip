@@ -395,8 +395,9 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   float whole = 0, down3 = 1.f;  // the whole chunk's exponent; fp16: what the state's terms are scaled down by
   auto sums = [&](uint32_t to, uint32_t n, float x_most) __attribute__((always_inline)) {
     const float dt = lane < n ? step_of((dt_f32 ? __uint_as_float(rdt) : to_f32<DT>((uint16_t)rdt)) + dt0, a.softplus) : 0.f;
-    // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it.)
-    const float e = lane < n ? fmaxf(dt * A, -200.f) : 0.f;
+    // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it. Compared, not a maximum,
+    // which would make a number of NaN.)
+    const float forgets = dt * A, e = lane < n ? (forgets < -200.f ? -200.f : forgets) : 0.f;
     const float up = scan_add(e), back = scan_add(__shfl(e, 63 - lane)), after = __shfl(back, (62 - lane) & 63);
     float weight = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt, up3 = 1.f;
     if constexpr (DT == HQ_DTYPE_F16) range_scale(max_of_lanes(fabsf(weight)) * x_most, up3, down3);
