@@ -201,17 +201,19 @@ __global__ __launch_bounds__(64 * kRuns) void hq_ssm_conv_kernel(ConvArgs a) {
   }
 }
 
+// Workgroups along the channels, and tokens of a wavefront: short sequences, whose runs would wait for one row of the states after
+// the other, go one token a wavefront.
+uint32_t conv_across(const ConvArgs& a) { return (a.C / 8 + 63) / 64; }
+uint32_t conv_tile(const ConvArgs& a) { return a.s.T >= 32ull * a.s.n ? kRunTokens : 1; }
+
 template <int DT, int W>
 hipError_t launch_conv(const ConvArgs& a, hipStream_t s) {
   if (!a.s.cu) {
-    hipLaunchKernelGGL((hq_ssm_conv_step_kernel<DT, W>), dim3((a.C / 8 + 63) / 64, a.s.n), dim3(64), 0, s, a);
+    hipLaunchKernelGGL((hq_ssm_conv_step_kernel<DT, W>), dim3(conv_across(a), a.s.n), dim3(64), 0, s, a);
     return hipGetLastError();
   }
-  // Short sequences, whose runs would wait for one row of the states after the other, go one token a wavefront.
-  const bool run = a.s.T >= 32ull * a.s.n;
-  const uint32_t tile = run ? kRunTokens : 1, per = tile * kRuns;
-  const dim3 grid((a.s.T + per - 1) / per * ((a.C / 8 + 63) / 64));
-  if (run) hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, kRunTokens>), grid, dim3(64 * kRuns), 0, s, a);
+  const dim3 grid((uint32_t)conv_workgroups(a));
+  if (conv_tile(a) > 1) hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, kRunTokens>), grid, dim3(64 * kRuns), 0, s, a);
   else hipLaunchKernelGGL((hq_ssm_conv_kernel<DT, W, 1>), grid, dim3(64 * kRuns), 0, s, a);
   return hipGetLastError();
 }
@@ -321,6 +323,12 @@ hipError_t launch_step(const ScanArgs& a, hipStream_t s) {
 }
 
 }  // namespace
+
+uint64_t conv_workgroups(const ConvArgs& a) {
+  if (!a.s.cu) return (uint64_t)conv_across(a) * a.s.n;
+  const uint32_t per = conv_tile(a) * kRuns;
+  return (uint64_t)((a.s.T + per - 1) / per) * conv_across(a);
+}
 
 hipError_t launch_ssm_conv(int dtype, const ConvArgs& a, hipStream_t s) {
   return dtype == HQ_DTYPE_F16 ? launch_conv_type<HQ_DTYPE_F16>(a, s) : launch_conv_type<HQ_DTYPE_BF16>(a, s);

@@ -30,6 +30,7 @@ struct ConvArgs {
   uint32_t C, width;
   uint32_t silu;
 };
+uint64_t conv_workgroups(const ConvArgs& a);  // of its launch
 hipError_t launch_ssm_conv(int dtype, const ConvArgs& a, hipStream_t s);
 
 struct ScanArgs {

@@ -108,6 +108,8 @@ hq_status hq_ssm_conv(const hq_state_cache* cache, uint32_t layer, const void* X
   a.C = C;
   a.width = w;
   a.silu = silu != 0;
+  if (hq::conv_workgroups(a) > hq::kMaxGrid)
+    return fail(HQ_ERR_SHAPE, "%llu workgroups: too many tokens and channels for one call", (unsigned long long)hq::conv_workgroups(a));
   return from_hip(hq::launch_ssm_conv(cache->dtype, a, reinterpret_cast<hipStream_t>(stream)), "convolution launch");
 }
 
