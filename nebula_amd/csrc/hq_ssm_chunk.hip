@@ -54,6 +54,7 @@ constexpr int BF = HQ_DTYPE_BF16;
 constexpr uint32_t kChunkThreads = 256;
 constexpr uint32_t kOwnBytes = 4096;  // of LDS for a wavefront: a chunk's x of 32 channels, then 32 tokens' fp32 outputs
 constexpr uint32_t kColumns = 128;  // channels of a workgroup, four wavefronts of 32
+constexpr uint32_t kScaleBytes = kColumns * 4;  // of LDS for their scales
 
 // Tokens of a chunk: the state of 256 leaves registers and LDS for 32.
 template <int N>
@@ -121,6 +122,12 @@ __device__ __forceinline__ float scan_add(float x) {
 __device__ __forceinline__ float max_of_lanes(float x) {
   return __int_as_float(__builtin_amdgcn_readlane(
       (int)scan(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }), 63));
+}
+
+// Of the two lanes that hold a channel.
+__device__ __forceinline__ float max_of_halves(float x) {
+  const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
 }
 
 // 2^k that brings a maximum m to 2^14..2^15, and 2^-k: fp16 then holds 11 bits of a value and as many of the rest, down to
@@ -234,7 +241,7 @@ constexpr uint32_t vec_bytes() {
 template <int N, bool CARRY>
 constexpr uint32_t chunk_lds(uint32_t heads) {
   constexpr uint32_t L = chunk_tokens<N>();
-  return (CARRY ? 1 : 2) * L * N * 2 + 4 * kOwnBytes + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>()) + 16;
+  return (CARRY ? 1 : 2) * L * N * 2 + 4 * kOwnBytes + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>() + kScaleBytes) + 16;
 }
 
 // What a launch computes: outputs, outputs through a gate, or the state alone, of all runs but a sequence's last, for the runs
@@ -536,14 +543,18 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
       __syncthreads();
 
       // y^T: what the state gives, decayed, and the chunk's own.
-      float up2 = 1.f, down2 = 1.f;
+      // fp16: a channel's states have a scale of their own, so that what another channel holds, infinite or far larger, takes no
+      // digits from them. Two lanes hold a channel as an operand, all of them as outputs: the way back goes through LDS.
+      float up2 = 1.f;
+      float* const downs = reinterpret_cast<float*>(smem + chunk_lds<N, CARRY>(kHeads) - 16 - kScaleBytes) + wave * 32;
       if constexpr (DT == HQ_DTYPE_F16) {
-        float m = 0;
+        float m = 0, down2;
 #pragma unroll
         for (int i = 0; i < kNT; ++i)
 #pragma unroll
           for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(s[i][r]));
-        range_scale(max_of_lanes(m), up2, down2);
+        range_scale(max_of_halves(m), up2, down2);
+        if (lane < 32) downs[lane] = down2;
       }
       auto from_state = [&](float up) __attribute__((always_inline)) {
         const uint32_t id = opaque(lane), at_c = piece_at<kRow>(id & 31u, id >> 5);
@@ -580,9 +591,14 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
         }
 #pragma unroll
         for (int b = 0; b < kTB; ++b) {
-          const float d = __builtin_amdgcn_exp2f(cum[32 * b + l32]) * down2;
+          const float d = __builtin_amdgcn_exp2f(cum[32 * b + l32]);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) y[b][r] *= d;
+          for (int i = 0; i < 4; ++i) {
+            f4 down = {1.f, 1.f, 1.f, 1.f};
+            if constexpr (DT == HQ_DTYPE_F16) down = *reinterpret_cast<const f4*>(downs + 8 * i + 4 * half);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) y[b][4 * i + v] *= d * down[v];
+          }
         }
       };
       from_state(up2);
