@@ -21,9 +21,10 @@
 //
 // Sums are fp32 throughout. What a matrix product's operands round away:
 //   the state's terms w x (fp32 times 16 bits) are kept as three bf16 parts, or in fp16 as two parts of values scaled by a
-//   power of two (22 bits of them either way), because the state is fp32 and goes on for the whole sequence;
-//   S as an operand, and M, are kept as two parts (16 bits, fp16: 22 of S): with one, outputs would be off by 1.4
-//   times their own rounding.
+//   power of two of their channel and chunk, because the state is fp32 and goes on for the whole sequence: 22 bits of them either
+//   way (fp16: of those above 2^-17 of their channel's largest in the chunk, and 2^-39 of that of the others);
+//   S as an operand, and M, are kept as two parts (16 bits, fp16: 22 of S, scaled as the terms are): with one, outputs would be
+//   off by 1.4 times their own rounding.
 //
 // A product adds 0 x_s for tokens s behind t, which is no 0 for an infinite x_s or NaN. A chunk therefore ends before such an x and the
 // next one begins with it; the exponents of a chunk's x are looked at on their way to LDS, so that a prompt without any pays a maximum.
@@ -119,11 +120,6 @@ __device__ __forceinline__ u4 tr_read(const unsigned char* p0, const unsigned ch
 __device__ __forceinline__ float scan_add(float x) {
   return __uint_as_float(scan(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
-__device__ __forceinline__ float max_of_lanes(float x) {
-  return __int_as_float(__builtin_amdgcn_readlane(
-      (int)scan(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }), 63));
-}
-
 // Of the two lanes that hold a channel.
 __device__ __forceinline__ float max_of_halves(float x) {
   const auto v = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -338,15 +334,8 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   // x goes through LDS for its order alone, to the wavefront that brought it.
   unsigned char* const own = sX + wave * kOwnBytes;
   constexpr uint32_t kOdd = DT == HQ_DTYPE_F16 ? 0x7C00u : 0x7F80u;  // the exponent of infinities and NaN
-  float x_most = 0;  // fp16: a power of two above the x that have come
   uint32_t most = 0;
-  auto look_x = [&]() __attribute__((always_inline)) {
-    most = exponents<DT>(rx);
-    if constexpr (DT == HQ_DTYPE_F16) {
-      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)scan(most, 0, [](uint32_t p, uint32_t q) { return max(p, q); }), 63);
-      x_most = __uint_as_float(((all >> 10) + 113u) << 23);  // 2^(e - 15 + 1), for exponent e
-    }
-  };
+  auto look_x = [&]() __attribute__((always_inline)) { most = exponents<DT>(rx); };
   auto put_x = [&](uint32_t* odd) __attribute__((always_inline)) {
     const uint32_t id = opaque(lane), xrow = id / 4, at = piece_at<kXRow>(xrow, id % 4);
 #pragma unroll
@@ -399,20 +388,18 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
 
   // Of a chunk of n tokens, for this wavefront's head: steps and their sums, a token a lane, from the chunk's beginning and
   // from its end. Computed during the chunk before it, between products.
-  float whole = 0, down3 = 1.f;  // the whole chunk's exponent; fp16: what the state's terms are scaled down by
-  auto sums = [&](uint32_t to, uint32_t n, float x_most) __attribute__((always_inline)) {
+  float whole = 0;  // the whole chunk's exponent
+  auto sums = [&](uint32_t to, uint32_t n) __attribute__((always_inline)) {
     const float dt = lane < n ? step_of((dt_f32 ? __uint_as_float(rdt) : to_f32<DT>((uint16_t)rdt)) + dt0, a.softplus) : 0.f;
     // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it. Compared, not a maximum,
     // which would make a number of NaN.)
     const float forgets = dt * A, e = lane < n ? (forgets < -200.f ? -200.f : forgets) : 0.f;
     const float up = scan_add(e), back = scan_add(__shfl(e, 63 - lane)), after = __shfl(back, (62 - lane) & 63);
-    float weight = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt, up3 = 1.f;
-    if constexpr (DT == HQ_DTYPE_F16) range_scale(max_of_lanes(fabsf(weight)) * x_most, up3, down3);
     float* const cum = vec + (wave * 2 + to) * 3 * L;
     if (lane < L) {
       cum[lane] = up;
       cum[L + lane] = dt;
-      cum[2 * L + lane] = weight * up3;
+      cum[2 * L + lane] = __builtin_amdgcn_exp2f(lane == 63 ? 0.f : after) * dt;
     }
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(up), 63));
   };
@@ -433,7 +420,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   put();
   look_x();
   put_x(odd);
-  float total = 0, next_whole = sums(0, min(run.t1 - run.t0, (uint32_t)L), x_most), next_down = down3;
+  float total = 0, next_whole = sums(0, min(run.t1 - run.t0, (uint32_t)L));
   uint32_t n, turn = 0;
   for (uint32_t t = run.t0; t < run.t1; t += n, turn ^= 1u) {
     __syncthreads();
@@ -443,8 +430,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     const uint32_t first = uni(odd[turn]);
     if (__builtin_expect(first < n, 0)) {
       n = max(first, 1u);
-      next_whole = sums(turn, n, x_most);
-      next_down = down3;
+      next_whole = sums(turn, n);
       for (uint32_t i = tid; i < (L - n) * kPieces; i += kChunkThreads) *reinterpret_cast<u4*>(sB + n * kRow + i * 16) = u4{0, 0, 0, 0};
       for (uint32_t i = lane; i < (L - n) * 4; i += 64) *reinterpret_cast<u4*>(own + n * kXRow + i * 16) = u4{0, 0, 0, 0};
       __syncthreads();
@@ -452,7 +438,6 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     if (tid == 0) odd[turn ^ 1u] = L;
     whole = next_whole;
     total += whole;
-    const float scale_down = next_down;
     // Of two wavefronts on a SIMD, the one that makes outputs goes first: its chain is the longer one, and the other's products of the
     // state's sums fill what it leaves (8 prompts of 512 tokens 82 -> 77 us, one of 8192 197 -> 192).
     if constexpr (!CARRY) __builtin_amdgcn_s_setprio(2);
@@ -605,8 +590,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
       read_x();
       // M's fragments are read a step ahead; between the products, the next chunk's sums.
       look_x();
-      next_whole = sums(turn ^ 1u, min(left, (uint32_t)L), x_most);
-      next_down = down3;
+      next_whole = sums(turn ^ 1u, min(left, (uint32_t)L));
       const uint32_t idm = opaque(lane), at_m[2] = {m_place<L>(0, idm & 31u, idm >> 5), m_place<L>(1, idm & 31u, idm >> 5)};
       constexpr int kSteps = kTB == 2 ? 6 : 2;  // products of 16 earlier tokens: 2 for the first 32 tokens, 4 for the others
       u4 mf[2][2];
@@ -704,15 +688,24 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (DT == HQ_DTYPE_F16) {
+      // Each channel's terms, two lanes', have a scale of their own.
+      float v[kTS][8], up, scale_down, m = 0;
+#pragma unroll
+      for (int k = 0; k < kTS; ++k) {
+        weigh(k, v[k]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[k][i]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      range_scale(max_of_halves(m), up, scale_down);
       u4 hi[kTS], lo[kTS];
 #pragma unroll
       for (int k = 0; k < kTS; ++k) {
-        float v[8];
-        weigh(k, v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          hi[k][i] = take_part<DT>(v[2 * i], v[2 * i + 1]);
-          lo[k][i] = pack_pair<DT>(v[2 * i], v[2 * i + 1]);
+          float p = v[k][2 * i] * up, q = v[k][2 * i + 1] * up;
+          hi[k][i] = take_part<DT>(p, q);
+          lo[k][i] = pack_pair<DT>(p, q);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -767,8 +760,7 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
     __syncthreads();
     if constexpr (CARRY) {
       look_x();
-      next_whole = sums(turn ^ 1u, min(left, (uint32_t)L), x_most);
-      next_down = down3;
+      next_whole = sums(turn ^ 1u, min(left, (uint32_t)L));
     }
     put();
     if constexpr (CARRY) put_x(odd + (turn ^ 1u));
