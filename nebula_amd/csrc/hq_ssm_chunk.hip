@@ -56,6 +56,7 @@ constexpr uint32_t kChunkThreads = 256;
 constexpr uint32_t kOwnBytes = 4096;  // of LDS for a wavefront: a chunk's x of 32 channels, then 32 tokens' fp32 outputs
 constexpr uint32_t kColumns = 128;  // channels of a workgroup, four wavefronts of 32
 constexpr uint32_t kScaleBytes = kColumns * 4;  // of LDS for their scales
+constexpr uint32_t kLowBytes = 4 * 64 * 4;      // of LDS for the low parts of four wavefronts' sums
 
 // Tokens of a chunk: the state of 256 leaves registers and LDS for 32.
 template <int N>
@@ -119,6 +120,24 @@ __device__ __forceinline__ u4 tr_read(const unsigned char* p0, const unsigned ch
 
 __device__ __forceinline__ float scan_add(float x) {
   return __uint_as_float(scan(__float_as_uint(x), 0, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+// The same in 64 bits.
+__device__ __forceinline__ double scan_add(double x) {
+#define HQ_ADD(CTRL, ROWS)                                                                                                         \
+  {                                                                                                                                \
+    const uint64_t v = __builtin_bit_cast(uint64_t, x);                                                                            \
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);                        \
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);                \
+    x += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);                                                                      \
+  }
+  HQ_ADD(0x111, 0xF)  // as in scan()
+  HQ_ADD(0x112, 0xF)
+  HQ_ADD(0x114, 0xF)
+  HQ_ADD(0x118, 0xF)
+  HQ_ADD(0x142, 0xA)
+  HQ_ADD(0x143, 0xC)
+#undef HQ_ADD
+  return x;
 }
 // Of the two lanes that hold a channel.
 __device__ __forceinline__ float max_of_halves(float x) {
@@ -237,7 +256,7 @@ constexpr uint32_t vec_bytes() {
 template <int N, bool CARRY>
 constexpr uint32_t chunk_lds(uint32_t heads) {
   constexpr uint32_t L = chunk_tokens<N>();
-  return (CARRY ? 1 : 2) * L * N * 2 + 4 * kOwnBytes + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>() + kScaleBytes) + 16;
+  return (CARRY ? 1 : 2) * L * N * 2 + 4 * kOwnBytes + vec_bytes<N>() + (CARRY ? 0 : heads * 2 * m_bytes<L>() + kLowBytes + kScaleBytes) + 16;
 }
 
 // What a launch computes: outputs, outputs through a gate, or the state alone, of all runs but a sequence's last, for the runs
@@ -389,12 +408,24 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
   // Of a chunk of n tokens, for this wavefront's head: steps and their sums, a token a lane, from the chunk's beginning and
   // from its end. Computed during the chunk before it, between products.
   float whole = 0;  // the whole chunk's exponent
+  float* const lows = reinterpret_cast<float*>(smem + chunk_lds<N, CARRY>(kHeads) - 16 - kScaleBytes - kLowBytes) + wave * 64;
   auto sums = [&](uint32_t to, uint32_t n) __attribute__((always_inline)) {
     const float dt = lane < n ? step_of((dt_f32 ? __uint_as_float(rdt) : to_f32<DT>((uint16_t)rdt)) + dt0, a.softplus) : 0.f;
     // (2^-200 is 0 already: what one token forgets is no reason to lose the digits of the tokens behind it. Compared, not a maximum,
     // which would make a number of NaN.)
     const float forgets = dt * A, e = lane < n ? (forgets < -200.f ? -200.f : forgets) : 0.f;
-    const float up = scan_add(e), back = scan_add(__shfl(e, 63 - lane)), after = __shfl(back, (62 - lane) & 63);
+    const float back = scan_add(__shfl(e, 63 - lane)), after = __shfl(back, (62 - lane) & 63);
+    // The weights M take differences of two sums: what tokens before both of them forgot goes out again, and so must its
+    // rounding. The sums are made in 64 bits and kept in two parts. (In fp32, steps of -115 in half a chunk took the digits of
+    // fp16 outputs behind them.)
+    float up;
+    if constexpr (CARRY) {
+      up = scan_add(e);
+    } else {
+      const double both = scan_add((double)e);
+      up = (float)both;
+      if (lane < L) lows[lane] = (float)(both - (double)up);
+    }
     float* const cum = vec + (wave * 2 + to) * 3 * L;
     if (lane < L) {
       cum[lane] = up;
@@ -484,10 +515,10 @@ __global__ __launch_bounds__(kChunkThreads, N == 256 ? 1 : 2) void hq_ssm_chunk_
 #pragma unroll
         for (int k = 0; k < kMine.n; ++k) {
           const uint32_t tt = 16 * kMine.t[k] + l16, ss = 16 * kMine.s[k] + 4 * quad;
-          const float ct = cum[tt];
-          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
+          const float ct = cum[tt], lt = lows[tt];
+          const f4 cs = *reinterpret_cast<const f4*>(cum + ss), ls = *reinterpret_cast<const f4*>(lows + ss), ds = *reinterpret_cast<const f4*>(steps + ss);
 #pragma unroll
-          for (int v = 0; v < 4; ++v) f[k][v] = __builtin_amdgcn_exp2f(ct - cs[v]) * ds[v];
+          for (int v = 0; v < 4; ++v) f[k][v] = __builtin_amdgcn_exp2f((ct - cs[v]) + (lt - ls[v])) * ds[v];
         }
 #pragma unroll
         for (int j = 0; j < N / 32; ++j)
