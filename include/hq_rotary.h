@@ -35,7 +35,8 @@ typedef struct hq_rotary {
 
 /* Heads of a call: element (t, h, d) of In at t * in_row + h * in_head + d, of Out likewise, no two of Out in one place.
  * Strides are in elements and multiples of 8, In and Out 16-byte aligned. Out may be In with the same strides
- * (in place), else they are apart. weight: fp32 [head_dim], 16-byte aligned, or NULL: no norm. eps: not negative, finite. */
+ * (in place), else they are apart; q's Out is apart from k's In and Out and from V, k's Out from q's In. weight: fp32 [head_dim],
+ * 16-byte aligned, or NULL: no norm. eps: not negative, finite. */
 typedef struct hq_rotary_heads {
     const void* In;
     void* Out;

@@ -419,6 +419,8 @@ hq_status hq_rotate(const hq_rotary* rotary, const hq_rotary_heads* q, const hq_
   a.all = a.q.heads + a.k.heads;
   a.pos = positions;
   if ((st = check_rotated(tokens, a)) != HQ_OK) return st;
+  if (k && (q->Out == k->Out || q->Out == k->In || k->Out == q->In))
+    return fail(HQ_ERR_INVALID_ARG, "an Out of q or k is the other's: heads are written while others read them");
   return from_hip(hq::launch_rotate(dtype, rotary->layout, a, nullptr, reinterpret_cast<hipStream_t>(stream)), "rotation launch");
 }
 
@@ -450,6 +452,7 @@ hq_status hq_cache_append_rotated(const hq_kv_cache* cache, uint32_t layer, cons
   a.cu = cu;
   a.n = n;
   if ((st = check_rotated(tokens, a)) != HQ_OK) return st;
+  if (q && (q->Out == k->In || q->Out == V)) return fail(HQ_ERR_INVALID_ARG, "q's Out is k or V: heads are written while others read them");
   c.K += layer * c.layer_stride;
   c.V += layer * c.layer_stride;
   return from_hip(hq::launch_rotate(cache->dtype, rotary->layout, a, &c, reinterpret_cast<hipStream_t>(stream)), "rotated append launch");
