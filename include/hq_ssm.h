@@ -20,7 +20,13 @@
  *   dt = dt_raw[t, h] + dt_bias[h], or log(1 + exp(that))
  *   S = exp(A[h] dt) S + dt x[t, h, :] B[t, g, :]^T
  *   y[t, h, :] = S C[t, g, :] + D[h] x[t, h, :],   times z / (1 + exp(-z)) with a gate z
- * States, decays and sums are kept in fp32; outputs are rounded once.
+ * States, decays and sums are kept in fp32 (sums of a chunk's exponents in 64 bits); outputs are rounded once. Calls of a few
+ * tokens a sequence are computed so throughout. Longer ones go in chunks of tokens as products of 16-bit operands
+ * (hq_describe_ssm says which), into which fp32 values enter as two or three parts: a state's terms with 22 bits (fp16: or to 2^-39
+ * of the largest term of their channel and chunk), the state with 16 (fp16: 22, or to 2^-39 of its channel's largest), the
+ * weights of a chunk's own tokens with 16.
+ * Values that are not finite: tokens before one, other sequences, heads (another group's, for B and C) and, for an x or a state,
+ * other channels are as without it. What it enters is not finite; whether an infinity or NaN depends on the kernel.
  */
 #ifndef HQ_SSM_H
 #define HQ_SSM_H
@@ -80,8 +86,9 @@ hq_status hq_ssm_workspace_bytes(uint32_t tokens, uint32_t n, int cu, uint32_t h
 /* The kernels that such a call runs and the workspace that it uses, as text. */
 hq_status hq_describe_ssm(uint32_t tokens, uint32_t n, int cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim,
                           uint32_t max_len, char* buf, size_t buf_len);
-/* Scan. max_len: no sequence has more new tokens (0: tokens); it only chooses how the work is split, as does the mean
- * number of tokens: single tokens and a long chunk are faster as two calls. */
+/* Scan. max_len: no sequence has more new tokens (0: tokens); it only chooses how the work is split (several prompts of one
+ * length take up to twice as long without it), as does the mean number of tokens, which alone chooses between the kernels:
+ * single tokens and a long chunk are faster as two calls. */
 hq_status hq_ssm_scan(const hq_state_cache* cache, uint32_t layer, const hq_ssm_io* io, const int32_t* rows, const int32_t* held,
                       const int32_t* cu, uint32_t n, uint32_t max_len, void* workspace, size_t workspace_bytes, hq_stream stream);
 

@@ -5,8 +5,8 @@
 // pieces, both members of its 8 pairs among them (pieces of the head R / 2 apart, or neighbours), so a rotation
 // needs no exchange and a norm one sum over the D / 16 lanes of the head, by moves inside rows of 16 lanes. The
 // angles of a token are the same for all its heads: a workgroup computes them once for its tokens and heads
-// (64-bit turns, whole turns off, then fp32 sine and cosine) and keeps them in LDS. 4096 tokens of 24 + 4 heads of 256: 24.0 us
-// for 117 MB, 4.9 TB/s; 16 tokens 3.4, 80 appended ones 4.4, 1008 of 48 + 8 heads of 128 8.1 (33 MB).
+// (64-bit turns, whole turns off, then fp32 sine and cosine) and keeps them in LDS. 4096 tokens of 24 + 4 heads of 256: 23.9 us
+// for 117 MB, 4.9 TB/s; 16 tokens 3.3, 80 appended ones 4.4, 1008 of 48 + 8 heads of 128 8.2 (33 MB).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -338,6 +338,8 @@ hipError_t launch_ssm_conv(int dtype, const ConvArgs& a, hipStream_t s) {
 ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_t groups, uint32_t head_dim, uint32_t state_dim, uint32_t max_len) {
   ScanPlan p;
   p.largest = (uint64_t)heads * (head_dim / kStepRows) * n;
+  // States of 256 are counted with one workgroup a CU, as fp16 has it (registers past 256); bf16 (at most 254) lets a second one in,
+  // and is split as fp16 is.
   const uint32_t L = state_dim == 256 ? 32 : 64, two = 128 / head_dim, slots = (uint32_t)cu_count() * (state_dim == 256 ? 1 : 2);
   p.units = groups * ((heads / groups + two - 1) / two);
   // Few tokens a sequence go one by one. 48 heads of 128x128: 8 sequences of 6 and 8 tokens 18.3 and 23.9 us, in a chunk
@@ -357,9 +359,9 @@ ScanPlan plan_scan(uint32_t tokens, uint32_t n, bool cu, uint32_t heads, uint32_
         const uint32_t runs = tokens / (c * L) + n;
         if (k > 1 && (runs > most || c >= longest)) continue;
         const uint64_t groups_of = (uint64_t)(k == 1 ? n : runs) * p.units, rounds = (groups_of + slots - 1) / slots;
-        // In us: a chunk of one workgroup a compute unit 5.15, of two at once 8.3; a carry is 0.45 of one; a launch about a chunk
+        // In us, of states of 128, which stand for those of 64 and 256 too: a chunk of one workgroup a compute unit 5.15, of two at once 8.3; a carry is 0.45 of one; a launch about a chunk
         // before the first, and 3 or 18 apart. 48 heads of 128x128, 512 tokens: whole 45.6, runs of 2 chunks 42.8, of 1 47; 1024: whole
-        // 83, of 4 55.2, of 2 57.7; 4096: of 13 119, of 7 110; 8192: of 26 215, of 13 186. 80 heads of 64x128, 1 to 1008 tokens: whole 90,
+        // 83, of 4 55.2, of 2 57.7; 4096: of 13 119, of 7 110; 8192: of 26 215, of 13 191. 80 heads of 64x128, 1 to 1008 tokens: whole 90,
         // of 5 86 (fp16: 99, 88).
         const float one = state_dim != 256 && groups_of * 2 > slots ? 8.3f : 5.15f;
         const float cost = rounds * (c + 1) * one * (k > 1 ? 1.45f : 1.f) + (k > 1 ? 18.f : 3.f);

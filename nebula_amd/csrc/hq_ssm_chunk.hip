@@ -15,11 +15,12 @@
 // Few sequences are dealt to several workgroups in runs of chunks: a launch of this kernel sums what each run adds to the state
 // (kCarry), hq_ssm_join_kernel turns that into what enters each run, and a second launch computes the outputs from there.
 //
-// Bound by the vector pipe (parts of operands, decays, the gate) and the matrix pipe together: 58% and 33% busy at 8192 tokens of 48
-// heads of 128x128, where a wavefront has 1300 vector instructions and 102 products a chunk and a SIMD two wavefronts: 59 us of carries,
-// 11 of joins, 122 of outputs, 373 MB of operands (78 us at a copy's rate). One workgroup a CU: 5 us a chunk, bound by its own chain.
+// Bound by the vector pipe (parts of operands, decays, the gate) and the matrix pipe together: 59% and 32% busy at 8192 tokens of 48
+// heads of 128x128, where a wavefront has 1350 vector instructions and 102 products a chunk and a SIMD two wavefronts: 191 us, of which
+// carries, joins and outputs have 58, 11 and 122, for 373 MB of operands (78 us at a copy's rate). One workgroup a CU: 5 us a chunk,
+// bound by its own chain.
 //
-// Sums are fp32 throughout. What a matrix product's operands round away:
+// Sums are fp32, those of a chunk's exponents in 64 bits. What a matrix product's operands round away:
 //   the state's terms w x (fp32 times 16 bits) are kept as three bf16 parts, or in fp16 as two parts of values scaled by a
 //   power of two of their channel and chunk, because the state is fp32 and goes on for the whole sequence: 22 bits of them either
 //   way (fp16: of those above 2^-17 of their channel's largest in the chunk, and 2^-39 of that of the others);
@@ -28,6 +29,7 @@
 //
 // A product adds 0 x_s for tokens s behind t, which is no 0 for an infinite x_s or NaN. A chunk therefore ends before such an x and the
 // next one begins with it; the exponents of a chunk's x are looked at on their way to LDS, so that a prompt without any pays a maximum.
+// An infinite operand leaves NaN as the rest of its first part: its channel is lost either way, as an infinity or NaN.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

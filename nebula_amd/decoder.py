@@ -158,7 +158,9 @@ class LayerProjections:
         of its x, B and C gated by gate, mixer_out. dt: the tokens' step widths [M, 48], float32 or x_norm's type, before
         bias and softplus. The step's requests hold rows of layer states_layer of the states, the same ones as of the
         cache (states.refused = cache.refused: a step that step.reserve(cache) was refused for leaves them too); a
-        request whose chunk starts at token 0 begins with zero states. A stream is taken as attend() does."""
+        request whose chunk starts at token 0 begins with zero states. qkv's columns are x (48 heads of 128), then B, then C (16
+        groups of 128 each). What goes to mixer_out is the gated scan as it is: a layer that norms it first calls mixer_in,
+        states.conv, states.scan and mixer_out itself. A stream is taken as attend() does."""
         if stream is not None:
             import torch
 

@@ -187,7 +187,7 @@ def _check_rotary(rotary: Rotary, dev: int) -> None:
 def rotate(q, k, rotary: Rotary, positions, q_weight=None, k_weight=None, eps: float = 1e-6, out_q=None, out_k=None, stream=None):
     """q and k (None: q alone) [tokens, heads, head_dim], each head normed (with a weight: x * weight / sqrt(mean(x^2) + eps))
     and rotated by its token's position; positions: int32 [tokens]. Returns (q', k'), or q' without k. out_q may be q
-    and out_k k (in place)."""
+    and out_k k (in place), neither the other's."""
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
     _check_heads("q", q, shape, dtype, dev)
     _check_rotary(rotary, dev)

@@ -204,7 +204,8 @@ class StateCache:
             S = exp(A s) S + s x B^T;  y = S C + D x,  times z / (1 + exp(-z)) with a gate z.
         x, z and out [tokens, heads, head_dim], B and C [tokens, groups, state_dim], dt [tokens, heads] float32 or x's type; A (not
         positive), D and dt_bias float32 [heads]. Sequences as in conv(); their states S are kept. max_len: no sequence has more
-        new tokens (a hint for the split). Single tokens and a long chunk are faster as two calls. out may be z."""
+        new tokens (a hint for the split: several prompts of one length take up to twice as long without it). Single tokens and a
+        long chunk are faster as two calls. out may be z."""
         dtype = x.dtype
         ref = self._refs.get(dtype)
         if ref is None or self.ssm_state is None:
